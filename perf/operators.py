@@ -262,8 +262,7 @@ def run(state):
         dx = s["rstd"][:, None] * (g - g.mean(-1, keepdim=True) - hat * (g * hat).mean(-1, keepdim=True))
         return {"dx": dx.to(s["x"].dtype), "dweight": (dy * hat).sum(0), "dbias": dy.sum(0)}
     if op == "layer_norm_quantize":  # 64 bits: a value may lie next to the border of two codes
-        y = _round_bf16(_norm(s["x"].double(), s["weight"].double(), s["bias"].double())[0])
-        codes, scales = _quantize(y, s["dtype"], s["sub"])
+        codes, scales = _quantize(_norm(s["x"].double(), s["weight"].double(), s["bias"].double())[0], s["dtype"], s["sub"])
         return {"codes": codes, "scales": scales}
     if op == "quantize_tokens":
         codes, scales = _quantize(s["x"], s["dtype"], s["sub"])
@@ -365,5 +364,5 @@ def exact(case, seed):
     y = torch.addcmul(s["bias"].double(), (x - mean[:, None]) * rstd[:, None], w)
     if op == "layer_norm":
         return {"y": y, "mean": mean, "rstd": rstd}
-    codes, scales = _exact_row_codes(_exact_bf16(y), TOP_CODE[s["dtype"]], s["sub"])
+    codes, scales = _exact_row_codes(y, TOP_CODE[s["dtype"]], s["sub"])
     return {"codes": codes.to(torch.int8), "scales": scales if s["sub"] else scales[:, 0]}
