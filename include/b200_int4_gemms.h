@@ -341,6 +341,42 @@ int b200_int4_gemms_quantize(int device_index, uintptr_t stream_handle, const vo
 int b200_int4_gemms_repack_tokens(int device_index, uintptr_t stream_handle, const void* src, void* dst,
                                   int64_t rows, int64_t cols);
 
+/* ---- Around the quantised products: norms and scales for each token ---------------------------- */
+
+/* Quantises every row with a scale of its own (subchannel = 0) or one for each `subchannel` values (32, 64,
+ * 128, 256; the last group may be shorter):  scale = bf16(max|x| / top), top = 7 (bits 4) or 127 (bits 8);
+ * code = round_half_even(x / scale).  A scale that rounds to zero becomes one (all codes are then zero); a
+ * group that is not finite gets that scale (infinity or NaN) and codes of zero.
+ *   src    bf16 [rows, cols];   codes  u8 [rows, ceil(cols/2)] packed as everywhere, or int8 [rows, cols]
+ *   scales bf16 [rows] or [rows, ceil(cols/subchannel)]: the a_scale of the products
+ * No reference counterpart (its quantiser takes one constant scale, quant.py:14-29). */
+int b200_int4_gemms_quantize_tokens(int device_index, uintptr_t stream_handle, const void* src_bf16, void* codes,
+                                    void* scales_bf16, int64_t rows, int64_t cols, int32_t bits, int32_t subchannel);
+
+/* Layer norm over the last axis: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps).
+ *   x, y [rows, cols] of x_type; weight, bias [cols] of weight_type (B200_OUT_BF16 or B200_OUT_F32); bias may be NULL
+ *   mean, rstd  f32 [rows], for the backward pass.  Statistics in fp32. */
+int b200_int4_gemms_layer_norm(int device_index, uintptr_t stream_handle, const void* x, const void* weight,
+                               const void* bias, void* y, float* mean, float* rstd, int64_t rows, int64_t cols,
+                               int32_t x_type, int32_t weight_type, double eps);
+
+/* Layer norm and b200_int4_gemms_quantize_tokens of its unrounded result in one pass: statistics in fp64, every
+ * code and scale as the exactly computed norm has it. */
+int b200_int4_gemms_layer_norm_quantize(int device_index, uintptr_t stream_handle, const void* x, const void* weight,
+                                        const void* bias, void* codes, void* scales_bf16, int64_t rows, int64_t cols,
+                                        int32_t x_type, int32_t weight_type, double eps, int32_t bits,
+                                        int32_t subchannel);
+
+/* Backward pass of b200_int4_gemms_layer_norm.  dy, x, dx [rows, cols] of x_type; mean, rstd as the forward pass
+ * wrote them; dweight, dbias f32 [cols] (zero for rows = 0).  Sums over rows in a fixed order: the same bits on
+ * every run.  workspace: float32-aligned scratch of ..._workspace_bytes (0 for cols > 16384); calls that may
+ * overlap need their own. */
+size_t b200_int4_gemms_layer_norm_bwd_workspace_bytes(int device_index, int64_t rows, int64_t cols);
+int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream_handle, const void* dy, const void* x,
+                                   const void* weight, const float* mean, const float* rstd, void* dx, float* dweight,
+                                   float* dbias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t cols,
+                                   int32_t x_type, int32_t weight_type);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,12 +50,14 @@ from .native import (
     native_library_path,
     unpack_int4_on_device,
 )
+from .norm import layer_norm, layer_norm_bwd, layer_norm_quantize
 from .quant import (
     fake_quant_int,
     pack_int4_k_major,
     pack_ragged_rhs_subchannel_scales,
     pack_rhs_subchannel_scales,
     quantize_int_cuda,
+    quantize_tokens,
     repack_int4_tokens,
     unpack_int4_k_major,
 )
@@ -74,7 +76,11 @@ from .torch_ops import TORCH_GEMM_OP, TORCH_OP_NAMESPACE, register_torch_ops, to
 
 __all__ = [
     "calculate_group_info_on_device",
+    "layer_norm",
+    "layer_norm_bwd",
+    "layer_norm_quantize",
     "quantize_int_cuda",
+    "quantize_tokens",
     "ragged_dot_int4_bwd_flat",
     "repack_int4_tokens",
     "ACC_DTYPE",

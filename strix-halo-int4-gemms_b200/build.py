@@ -28,8 +28,10 @@ LIB_NAME = "libb200_int4_gemms.so"
 HOST_SOURCE = "b200_int4_gemms.cu"
 KERNEL_SOURCE = "tc_kernels.cu"
 TC_PARTS = 8  # kTcParts of csrc/tc_table.h
-SOURCES = (HOST_SOURCE, KERNEL_SOURCE)
-HEADERS = ("ptx.cuh", "gemm_kernel.cuh", "simt_kernel.cuh", "prep_kernels.cuh", "tc_table.h")
+# operators beside the GEMM family: (source, defines), one translation unit each
+OPERATOR_UNITS = (("norm_quantize.cu", ("B200_NORM_X_F32=0",)), ("norm_quantize.cu", ("B200_NORM_X_F32=1",)), ("row_ops.cu", ()))
+SOURCES = (HOST_SOURCE, KERNEL_SOURCE, *sorted({source for source, _ in OPERATOR_UNITS}))
+HEADERS = ("host_common.h", "row_common.cuh", "row_kernels.cuh", "row_launch.h", "ptx.cuh", "gemm_kernel.cuh", "simt_kernel.cuh", "prep_kernels.cuh", "tc_table.h")
 GENCODE = "arch=compute_100a,code=sm_100a"
 # the build of the bounded-wait test: a short wait limit and an MMA warp that never signals "accumulator full"
 # (see csrc/ptx.cuh); tests/test_gpu_wait_timeout.py loads it from TEST_LIB_NAME, nothing else does
@@ -91,6 +93,8 @@ def build_native(*, force: bool = False, verbose: bool = False, defines: tuple[s
         common += ["-Xptxas", "-v"]
     with tempfile.TemporaryDirectory(prefix="b200_build_") as tmp:
         units = [(HOST_SOURCE, [], Path(tmp) / "host.o")]
+        units += [(source, [f"-D{item}" for item in unit_defines], Path(tmp) / f"operator_{index}.o")
+                  for index, (source, unit_defines) in enumerate(OPERATOR_UNITS)]
         units += [(KERNEL_SOURCE, [f"-DB200_TC_PART={part}"], Path(tmp) / f"tc_part_{part}.o") for part in range(TC_PARTS)]
 
         def compile_unit(unit):

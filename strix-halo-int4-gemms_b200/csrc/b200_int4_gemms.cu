@@ -14,6 +14,7 @@
 #include "../../include/b200_int4_gemms.h"
 #include <vector>
 
+#include "host_common.h"
 #include "tc_table.h"
 #include "simt_kernel.cuh"
 #include "prep_kernels.cuh"
@@ -315,6 +316,42 @@ bool workspace_seen_before(const void* ptr, size_t bytes, int device) {
   return false;
 }
 }  // namespace
+
+namespace b200 {
+
+int host_fail(std::string msg) { return fail(std::move(msg)); }
+int host_fail_cuda(const char* what, cudaError_t err) { return fail_cuda(what, err); }
+void host_clear_error() { g_last_error.clear(); }
+
+int DeviceScope::enter(int device_index, int* sm_count) {
+  if (device_index < 0 || device_index >= kMaxDevices) return fail("device_index out of range");
+  static std::mutex mutex;
+  static int sms[kMaxDevices] = {};
+  cudaError_t err = cudaGetDevice(&previous_);
+  if (err != cudaSuccess) return fail_cuda("cudaGetDevice", err);
+  if (previous_ != device_index) {
+    err = cudaSetDevice(device_index);
+    if (err != cudaSuccess) return fail_cuda("cudaSetDevice", err);
+    changed_ = true;
+  }
+  std::lock_guard<std::mutex> lock(mutex);
+  if (sms[device_index] == 0) {
+    int major = 0, count = 0;
+    err = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device_index);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device_index);
+    if (err != cudaSuccess) return fail_cuda("cudaDeviceGetAttribute", err);
+    if (major != 10) return fail("this library holds sm_100a kernels only");
+    sms[device_index] = count;
+  }
+  *sm_count = sms[device_index];
+  return 0;
+}
+
+DeviceScope::~DeviceScope() {
+  if (changed_) (void)cudaSetDevice(previous_);
+}
+
+}  // namespace b200
 
 extern "C" int b200_int4_gemms_dispatch_version(void) { return 1; }
 

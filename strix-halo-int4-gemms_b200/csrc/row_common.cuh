@@ -1,0 +1,252 @@
+// Pieces of the kernels that work on rows of values: 8-value loads and stores, reductions over the threads of a
+// row, and the two quantisers (of exactly known bf16 values, and of values known to within a small error).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cstdint>
+
+namespace b200 {
+
+using bf16 = __nv_bfloat16;
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+
+// Eight consecutive values of a row, kept as they were read (4 registers of bf16, 8 of fp32).  Values past the
+// end of the row are zero.
+template <typename T>
+struct Raw8;
+
+template <>
+struct Raw8<bf16> {
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const { return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]); }
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0u; }
+  template <bool kAligned>
+  __device__ __forceinline__ void load(const bf16* row, long long at, long long cols) {
+    if (kAligned) {
+      if (at < cols) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + at));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
+        zero();
+      }
+    } else {
+      const unsigned short* src = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = at + 2 * i < cols ? __ldg(src + at + 2 * i) : 0u;
+        const uint32_t b = at + 2 * i + 1 < cols ? __ldg(src + at + 2 * i + 1) : 0u;
+        w[i] = a | (b << 16);
+      }
+    }
+  }
+};
+
+template <>
+struct Raw8<float> {
+  float f[8];
+  __device__ __forceinline__ float get(int i) const { return f[i]; }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  }
+  template <bool kAligned>
+  __device__ __forceinline__ void load(const float* row, long long at, long long cols) {
+    if (kAligned) {
+      if (at < cols) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(row + at));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(row + at + 4));
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+      } else {
+        zero();
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = at + i < cols ? __ldg(row + at + i) : 0.f;
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+template <bool kAligned>
+__device__ __forceinline__ void store8(bf16* row, long long at, long long cols, const float (&v)[8]) {
+  if (kAligned) {
+    if (at < cols)
+      *reinterpret_cast<uint4*>(row + at) =
+          make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i < cols) row[at + i] = __float2bfloat16_rn(v[i]);
+  }
+}
+
+template <bool kAligned>
+__device__ __forceinline__ void store8(float* row, long long at, long long cols, const float (&v)[8]) {
+  if (kAligned) {
+    if (at < cols) {
+      *reinterpret_cast<float4*>(row + at) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(row + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i < cols) row[at + i] = v[i];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// reductions over the threads of a row: one warp (TPR == 32) or one block (TPR threads)
+// ---------------------------------------------------------------------------------------------------------------
+struct SumOp {
+  template <typename V>
+  __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct MaxOp {
+  template <typename V>
+  __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
+};
+
+template <typename V, typename Op>
+__device__ __forceinline__ V warp_reduce(V v, Op op, int width = 32) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < width) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+
+// Two values at once; every thread of the row gets both results.  `scratch` holds 2 * TPR / 32 values and is not
+// shared by consecutive reductions, so one barrier is enough; the caller has a barrier between two uses of it.
+template <int TPR, typename A, typename B, typename OpA, typename OpB>
+__device__ __forceinline__ void row_reduce2(A& a, B& b, OpA op_a, OpB op_b, void* scratch) {
+  a = warp_reduce(a, op_a);
+  b = warp_reduce(b, op_b);
+  if (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    A* sa = static_cast<A*>(scratch);
+    B* sb = reinterpret_cast<B*>(sa + kWarps);
+    if ((threadIdx.x & 31) == 0) {
+      sa[threadIdx.x >> 5] = a;
+      sb[threadIdx.x >> 5] = b;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & (kWarps - 1);
+    a = sa[lane];
+    b = sb[lane];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      a = op_a(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+      b = op_b(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+    }
+  }
+}
+
+template <int TPR, typename A, typename OpA>
+__device__ __forceinline__ A row_reduce(A a, OpA op_a, void* scratch) {
+  a = warp_reduce(a, op_a);
+  if (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    A* sa = static_cast<A*>(scratch);
+    if ((threadIdx.x & 31) == 0) sa[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = sa[threadIdx.x & (kWarps - 1)];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) a = op_a(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+  }
+  return a;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// quantisation
+// ---------------------------------------------------------------------------------------------------------------
+// float64 -> bf16 with one rounding: to odd in fp32 (16 more bits than bf16 keeps), then to nearest even.
+__device__ __forceinline__ float bf16_from_double(double v) {
+  float f = __double2float_rz(v);
+  if (static_cast<double>(f) != v) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return __bfloat162float(__float2bfloat16_rn(f));
+}
+
+// A scale that rounds to zero (a row of zeros, or of numbers below the least bf16) counts as one: every code is
+// then zero, and the scale stays a positive number as the rest of the library asks.
+__device__ __forceinline__ float nonzero_scale(float s) { return s == 0.f ? 1.f : s; }
+
+// bf16(amax / top) of a bf16 amax given by its bit pattern (NaN patterns are above infinity's, so that a row with
+// a NaN gets a NaN scale).  The quotient of an 8-bit significand and 7 or 127 is never close to a tie of two bf16
+// numbers without being one, so rounding it to fp32 first changes nothing.
+template <int BITS>
+__device__ __forceinline__ float scale_of_bf16(uint32_t amax_bits) {
+  const float top = BITS == 4 ? 7.f : 127.f;
+  return nonzero_scale(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(amax_bits << 16), top))));
+}
+
+constexpr float kRoundMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to the nearest even integer, left in the low bits
+
+// A scale for which 1 / s and the products below are normal numbers.
+__device__ __forceinline__ bool scale_is_ordinary(float s) { return s >= 7.9e-31f && s <= 1.3e30f; }
+
+// round_half_even(x / s) of bf16 x and s, by multiplication.  x / s = (mx / ms) 2^j with significands below 256:
+// it is a tie n + 1/2 or, |2^(j+1) mx - (2n+1) ms| being a whole number from j = -1 on and ms < 256, at least 1 / 1020 away
+// from every tie, and it is at most 128.  The products with 1 / s made 2^-20 smaller and larger (1.3e-4 at 128) therefore round to one integer, which is the answer, or, at a tie, to
+// its two neighbours, of which the even one is.  Two multiply-adds instead of a division (which needs about nine
+// instructions): the loop is bound by instructions otherwise.
+struct ExactQuotient {
+  float low, high;
+  __device__ __forceinline__ explicit ExactQuotient(float s) {
+    const float inv = __frcp_rn(s);
+    low = inv * (1.f - 9.5367431640625e-7f);
+    high = inv * (1.f + 9.5367431640625e-7f);
+  }
+  __device__ __forceinline__ uint32_t code(float x) const {
+    const uint32_t a = __float_as_uint(__fmaf_rn(x, low, kRoundMagic));
+    const uint32_t b = __float_as_uint(__fmaf_rn(x, high, kRoundMagic));
+    return (a & 1u) ? b : a;
+  }
+};
+
+// The same by division, for scales outside the ordinary range (and codes of 0 where the scale is not finite).
+template <int BITS>
+__device__ __forceinline__ uint32_t code_by_division(float x, float s) {
+  const float top = BITS == 4 ? 7.f : 127.f;
+  const float q = rintf(__fdiv_rn(x, s));
+  if (!(q == q) || !(s < __int_as_float(0x7F800000))) return 0u;
+  return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(q, -top), top)));
+}
+
+// Eight codes (low bits of each word) to memory: 4 bytes of nibbles or 8 bytes.
+template <int BITS, bool kAligned>
+__device__ __forceinline__ void store_codes(uint8_t* row, long long at, long long cols, const uint32_t (&c)[8]) {
+  if (at >= cols) return;
+  if (BITS == 4) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= (c[i] & 0xFu) << (4 * i);
+    if (kAligned) {
+      *reinterpret_cast<uint32_t*>(row + at / 2) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at + 2 * i < cols) row[at / 2 + i] = static_cast<uint8_t>(w >> (8 * i));
+    }
+  } else {
+    if (kAligned) {
+      uint2 w;
+      w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+      w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+      *reinterpret_cast<uint2*>(row + at) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (at + i < cols) row[at + i] = static_cast<uint8_t>(c[i]);
+    }
+  }
+}
+
+}  // namespace b200

@@ -82,6 +82,11 @@ EXPORTED_SYMBOLS = (
     "b200_int4_gemms_launch_ragged_bwd_flat_static",
     "b200_int4_gemms_quantize",
     "b200_int4_gemms_repack_tokens",
+    "b200_int4_gemms_quantize_tokens",
+    "b200_int4_gemms_layer_norm",
+    "b200_int4_gemms_layer_norm_quantize",
+    "b200_int4_gemms_layer_norm_bwd_workspace_bytes",
+    "b200_int4_gemms_layer_norm_bwd",
 )
 
 
@@ -195,6 +200,17 @@ def _declare(library: ctypes.CDLL) -> None:
     library.b200_int4_gemms_quantize.argtypes = [ctypes.c_int, size_t, void_p, void_p, i64, i64, i32, ctypes.c_float]
     library.b200_int4_gemms_repack_tokens.restype = ctypes.c_int
     library.b200_int4_gemms_repack_tokens.argtypes = [ctypes.c_int, size_t, void_p, void_p, i64, i64]
+    library.b200_int4_gemms_quantize_tokens.restype = ctypes.c_int
+    library.b200_int4_gemms_quantize_tokens.argtypes = [ctypes.c_int, size_t] + [void_p] * 3 + [i64, i64, i32, i32]
+    library.b200_int4_gemms_layer_norm.restype = ctypes.c_int
+    library.b200_int4_gemms_layer_norm.argtypes = [ctypes.c_int, size_t] + [void_p] * 6 + [i64, i64, i32, i32, ctypes.c_double]
+    library.b200_int4_gemms_layer_norm_quantize.restype = ctypes.c_int
+    library.b200_int4_gemms_layer_norm_quantize.argtypes = (
+        [ctypes.c_int, size_t] + [void_p] * 5 + [i64, i64, i32, i32, ctypes.c_double, i32, i32])
+    library.b200_int4_gemms_layer_norm_bwd_workspace_bytes.restype = size_t
+    library.b200_int4_gemms_layer_norm_bwd_workspace_bytes.argtypes = [ctypes.c_int, i64, i64]
+    library.b200_int4_gemms_layer_norm_bwd.restype = ctypes.c_int
+    library.b200_int4_gemms_layer_norm_bwd.argtypes = [ctypes.c_int, size_t] + [void_p] * 9 + [size_t, i64, i64, i32, i32]
 
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:
@@ -862,3 +878,90 @@ def repack_tokens_on_device(packed: Any, *, library_path: str | Path | None = No
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
     return out
+
+
+def quantize_tokens_on_device(x: Any, *, bits: int, subchannel: int = 0, library_path: str | Path | None = None,
+                              stream: Any | None = None) -> tuple[Any, Any]:
+    """bf16 ``[..., cols]`` -> codes (packed uint8 or int8) and bf16 scales, one for each row or ``subchannel`` values."""
+    torch = _torch()
+    if not getattr(x, "is_cuda", False) or x.dtype is not torch.bfloat16:
+        raise RuntimeError("quantize_tokens_on_device requires a CUDA bfloat16 tensor")
+    x = _require_contiguous("x", x)
+    codes, scales, rows, cols = _token_code_outputs(torch, x, bits, subchannel)
+    library = load_dispatch_library(library_path)
+    rc = library.b200_int4_gemms_quantize_tokens(
+        _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols,
+        int(bits), int(subchannel))
+    if rc != 0:
+        raise RuntimeError(_library_last_error(library))
+    return codes, scales
+
+
+def _token_code_outputs(torch: Any, x: Any, bits: int, subchannel: int) -> tuple[Any, Any, int, int]:
+    lead, cols = x.shape[:-1], int(x.shape[-1])
+    rows = x.numel() // cols if cols else 0
+    if bits == 4:
+        codes = torch.empty((*lead, (cols + 1) // 2), device=x.device, dtype=torch.uint8)
+    else:
+        codes = torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    scales = torch.empty((*lead, -(-cols // subchannel)) if subchannel else lead, device=x.device, dtype=torch.bfloat16)
+    return codes, scales, rows, cols
+
+
+def _type_code(torch: Any, tensor: Any) -> int:
+    return OUT_F32 if tensor.dtype is torch.float32 else OUT_BF16
+
+
+def layer_norm_on_device(x: Any, weight: Any, bias: Any | None, *, eps: float, library_path: str | Path | None = None,
+                         stream: Any | None = None) -> tuple[Any, Any, Any]:
+    """(y, mean, rstd) of checked CUDA operands; see :func:`norm.layer_norm`."""
+    torch = _torch()
+    cols = int(x.shape[-1])
+    y = torch.empty_like(x)
+    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32)
+    mean, rstd = stats[0], stats[1]
+    library = load_dispatch_library(library_path)
+    rc = library.b200_int4_gemms_layer_norm(
+        _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x.numel() // cols, cols, _type_code(torch, x), _type_code(torch, weight), eps)
+    if rc != 0:
+        raise RuntimeError(_library_last_error(library))
+    return y, mean, rstd
+
+
+def layer_norm_quantize_on_device(x: Any, weight: Any, bias: Any | None, *, eps: float, bits: int, subchannel: int,
+                                  library_path: str | Path | None = None, stream: Any | None = None) -> tuple[Any, Any]:
+    """(codes, scales) of checked CUDA operands; see :func:`norm.layer_norm_quantize`."""
+    torch = _torch()
+    codes, scales, rows, cols = _token_code_outputs(torch, x, bits, subchannel)
+    library = load_dispatch_library(library_path)
+    rc = library.b200_int4_gemms_layer_norm_quantize(
+        _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        codes.data_ptr(), scales.data_ptr(), rows, cols, _type_code(torch, x), _type_code(torch, weight), eps, int(bits), int(subchannel))
+    if rc != 0:
+        raise RuntimeError(_library_last_error(library))
+    return codes, scales
+
+
+def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any, *, library_path: str | Path | None = None,
+                             stream: Any | None = None) -> tuple[Any, Any, Any]:
+    """(dx, dweight, dbias) of checked CUDA operands; see :func:`norm.layer_norm_bwd`.
+
+    The scratch is allocated for the call: the caching allocator keeps it apart from other streams' and, under
+    capture, inside the graph's own pool."""
+    torch = _torch()
+    cols = int(x.shape[-1])
+    rows = x.numel() // cols
+    library = load_dispatch_library(library_path)
+    index = _device_index(x)
+    need = int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(index, rows, cols))
+    dx = torch.empty_like(x)
+    sums = torch.empty((2, cols), device=x.device, dtype=torch.float32)
+    workspace = torch.empty(need // 4, device=x.device, dtype=torch.float32)
+    rc = library.b200_int4_gemms_layer_norm_bwd(
+        index, _stream_handle(torch, x, stream), dy.data_ptr(), x.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+        dx.data_ptr(), sums[0].data_ptr(), sums[1].data_ptr(), workspace.data_ptr(), need, rows, cols, _type_code(torch, x),
+        _type_code(torch, weight))
+    if rc != 0:
+        raise RuntimeError(_library_last_error(library))
+    return dx, sums[0], sums[1]

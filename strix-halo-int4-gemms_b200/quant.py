@@ -12,6 +12,8 @@ from __future__ import annotations
 
 from typing import Any
 
+from .metadata import OperandDType, ScaleMode, ScaleSpec
+
 
 def _torch() -> Any:
     try:
@@ -95,6 +97,35 @@ def quantize_int_cuda(x: Any, *, bits: int, scale: float) -> Any:
     from .native import quantize_on_device
 
     return quantize_on_device(x, bits=bits, scale=float(scale))
+
+
+def _code_bits(dtype: Any) -> int:
+    if type(dtype) is not OperandDType:
+        raise TypeError(f"dtype must be an OperandDType, got {type(dtype).__name__}")
+    return 4 if dtype is OperandDType.INT4 else 8
+
+
+def quantize_tokens(
+    x: Any, *, dtype: OperandDType = OperandDType.INT4, scale: ScaleSpec = ScaleSpec(ScaleMode.PER_CHANNEL)
+) -> tuple[Any, Any]:
+    """Quantise each token (row) of ``x`` with scales of its own: the A operand and ``a_scale`` of the products.
+
+    ``x``: CUDA bfloat16 ``[..., K]``, contiguous.  Per-channel: one scale a row, ``scales [...]``; subchannel
+    ``S``: one for every ``S`` values along K, ``scales [..., ceil(K/S)]``.  ``scale = bf16(max|x| / top)`` with
+    ``top`` 7 (INT4) or 127 (INT8) and ``code = round_half_even(x / scale)``, both exactly.  Codes are packed uint8
+    ``[..., ceil(K/2)]`` (an odd K is padded with a zero code) or int8 ``[..., K]``.  A scale that rounds to zero is
+    stored as one, with codes of zero; values that are not finite give their group that scale and codes of zero, so
+    that a product with them is not finite either.  No rows: empty results.  No autograd.
+    """
+    torch = _torch()
+    bits = _code_bits(dtype)
+    if not torch.is_tensor(x):
+        raise TypeError("x must be a torch.Tensor")
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have at least one value a row; got shape {tuple(x.shape)}")
+    from .native import quantize_tokens_on_device
+
+    return quantize_tokens_on_device(x, bits=bits, subchannel=scale.subchannel_size or 0)
 
 
 def repack_int4_tokens(x_packed: Any) -> Any:
