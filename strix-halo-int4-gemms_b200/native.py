@@ -156,6 +156,7 @@ def native_library_path(*, root: str | Path | None = None) -> Path:
 
 _LIBRARIES: dict[str, ctypes.CDLL] = {}
 _LIBRARIES_LOCK = threading.Lock()
+_DEFAULT_LIBRARY: ctypes.CDLL | None = None   # once loaded: resolving its path again costs a call about 20 us
 
 
 def _declare(library: ctypes.CDLL) -> None:
@@ -215,11 +216,16 @@ def _declare(library: ctypes.CDLL) -> None:
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:
     """dlopen the CUDA library (once per path) and declare its prototypes."""
+    global _DEFAULT_LIBRARY
+    if path is None and _DEFAULT_LIBRARY is not None:
+        return _DEFAULT_LIBRARY
     library_path = Path(path) if path is not None else native_library_path()
     key = str(library_path)
     with _LIBRARIES_LOCK:
         cached = _LIBRARIES.get(key)
         if cached is not None:
+            if path is None:
+                _DEFAULT_LIBRARY = cached
             return cached
         if not library_path.exists():
             raise RuntimeError(
@@ -229,6 +235,8 @@ def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:
         library = ctypes.CDLL(key)
         _declare(library)
         _LIBRARIES[key] = library
+        if path is None:
+            _DEFAULT_LIBRARY = library
         return library
 
 
