@@ -377,6 +377,47 @@ int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream_handle, co
                                    float* dbias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t cols,
                                    int32_t x_type, int32_t weight_type);
 
+/* ---- A whole mixture-of-experts layer for a few tokens ------------------------------------------ */
+
+#define B200_MOE_MAX_TOKENS 64
+#define B200_MOE_MAX_TOP_K 16
+#define B200_MOE_MAX_EXPERTS 1024
+
+typedef struct b200_moe_problem {
+  int32_t dtype;       /* B200_DTYPE_*: of the weights and of the quantised activations */
+  int32_t layout;      /* B200_LAYOUT_NN: w_up_gate [experts, hidden bytes, 2 inner], w_down [experts, inner bytes, hidden];
+                          B200_LAYOUT_NT: w_up_gate [experts, 2 inner, hidden bytes], w_down [experts, hidden, inner bytes] */
+  int32_t subchannel;  /* 0: per-channel scales; 32, 64, 128, 256: one for each that many values of K */
+  int32_t tokens;      /* 0 .. B200_MOE_MAX_TOKENS */
+  int32_t hidden;      /* multiples of 32 below 131072 */
+  int32_t inner;
+  int32_t experts;     /* 1 .. B200_MOE_MAX_EXPERTS */
+  int32_t top_k;       /* 1 .. B200_MOE_MAX_TOP_K */
+  int32_t router_type; /* B200_OUT_BF16 or B200_OUT_F32 */
+  int32_t renormalize; /* softmax over the chosen experts (1) or over all (0) */
+  int32_t ids_bits;    /* 32 or 64: type of topk_ids where they are given */
+} b200_moe_problem;
+
+/* out[t] = sum_j p_tj down_e(a_tj), e = the token's j-th expert:
+ *   logits = x router^T; the top_k largest (ties to the lowest expert) and p = softmax, in fp64;
+ *   x is quantised for each token as b200_int4_gemms_quantize_tokens does; [up | gate] = product with w_up_gate[e],
+ *   scaled; a = up * gate / (1 + exp(-gate)), quantised in the same way from its unrounded value; the product with
+ *   w_down[e], scaled and weighted with p, is added up in fp32 in the order of j and rounded to bf16 once.
+ * Integer sums are exact; the same bits on every run.
+ *   x [tokens, hidden] bf16, out [tokens, hidden] bf16
+ *   router_weight [experts, hidden], or NULL: then topk_ids [tokens, top_k] and topk_weights f32 [tokens, top_k] are
+ *     the routing; an id outside [0, experts) stands for no expert and adds nothing.  With router_weight, topk_ids
+ *     (int32) and topk_weights receive the routing, or are NULL.
+ *   up_gate_scale bf16 [experts, 2 inner] or [experts, ceil(hidden/S), 2 inner]; down_scale [experts, hidden] or
+ *     [experts, ceil(inner/S), hidden]
+ *   workspace: 256-byte aligned scratch of ..._workspace_bytes; calls that may overlap need their own.
+ * No reference counterpart: its grouped dot takes rows sorted by expert (ragged.py:1008-1229). */
+size_t b200_int4_gemms_moe_swiglu_workspace_bytes(const b200_moe_problem* problem);
+int b200_int4_gemms_moe_swiglu(const b200_moe_problem* problem, int device_index, uintptr_t stream_handle,
+                               const void* x_bf16, const void* router_weight, void* topk_ids, float* topk_weights,
+                               const void* w_up_gate, const void* up_gate_scale, const void* w_down,
+                               const void* down_scale, void* out_bf16, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -39,6 +39,7 @@ from .metadata import (
     ScaleSpec,
     TileConfig,
 )
+from .moe import moe_swiglu
 from .native import (
     NativeRuntimeStatus,
     accumulation_order,
@@ -79,6 +80,7 @@ __all__ = [
     "layer_norm",
     "layer_norm_bwd",
     "layer_norm_quantize",
+    "moe_swiglu",
     "quantize_int_cuda",
     "quantize_tokens",
     "ragged_dot_int4_bwd_flat",

@@ -29,9 +29,12 @@ HOST_SOURCE = "b200_int4_gemms.cu"
 KERNEL_SOURCE = "tc_kernels.cu"
 TC_PARTS = 8  # kTcParts of csrc/tc_table.h
 # operators beside the GEMM family: (source, defines), one translation unit each
-OPERATOR_UNITS = (("norm_quantize.cu", ("B200_NORM_X_F32=0",)), ("norm_quantize.cu", ("B200_NORM_X_F32=1",)), ("row_ops.cu", ()))
+OPERATOR_UNITS = (
+    ("norm_quantize.cu", ("B200_NORM_X_F32=0",)), ("norm_quantize.cu", ("B200_NORM_X_F32=1",)), ("row_ops.cu", ()),
+    ("moe_product.cu", ("B200_MOE_BITS=4",)), ("moe_product.cu", ("B200_MOE_BITS=8",)), ("moe_ops.cu", ()),
+)
 SOURCES = (HOST_SOURCE, KERNEL_SOURCE, *sorted({source for source, _ in OPERATOR_UNITS}))
-HEADERS = ("host_common.h", "row_common.cuh", "row_kernels.cuh", "row_launch.h", "ptx.cuh", "gemm_kernel.cuh", "simt_kernel.cuh", "prep_kernels.cuh", "tc_table.h")
+HEADERS = ("host_common.h", "row_common.cuh", "row_kernels.cuh", "row_launch.h", "moe_kernels.cuh", "moe_launch.h", "ptx.cuh", "gemm_kernel.cuh", "simt_kernel.cuh", "prep_kernels.cuh", "tc_table.h")
 GENCODE = "arch=compute_100a,code=sm_100a"
 # the build of the bounded-wait test: a short wait limit and an MMA warp that never signals "accumulator full"
 # (see csrc/ptx.cuh); tests/test_gpu_wait_timeout.py loads it from TEST_LIB_NAME, nothing else does

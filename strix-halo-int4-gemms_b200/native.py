@@ -87,6 +87,8 @@ EXPORTED_SYMBOLS = (
     "b200_int4_gemms_layer_norm_quantize",
     "b200_int4_gemms_layer_norm_bwd_workspace_bytes",
     "b200_int4_gemms_layer_norm_bwd",
+    "b200_int4_gemms_moe_swiglu_workspace_bytes",
+    "b200_int4_gemms_moe_swiglu",
 )
 
 
@@ -129,6 +131,24 @@ class DensePlan(ctypes.Structure):
 
     def as_tuple(self) -> tuple[int, int, int, int, int, int]:
         return (int(self.path), int(self.grid), int(self.tile_rows), int(self.tile_cols), int(self.group_m), int(self.split_k))
+
+
+class MoeProblem(ctypes.Structure):
+    """``b200_moe_problem`` of include/b200_int4_gemms.h."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("subchannel", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("inner", ctypes.c_int32),
+        ("experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("router_type", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("ids_bits", ctypes.c_int32),
+    ]
 
 
 @dataclass(frozen=True, slots=True)
@@ -212,6 +232,10 @@ def _declare(library: ctypes.CDLL) -> None:
     library.b200_int4_gemms_layer_norm_bwd_workspace_bytes.argtypes = [ctypes.c_int, i64, i64]
     library.b200_int4_gemms_layer_norm_bwd.restype = ctypes.c_int
     library.b200_int4_gemms_layer_norm_bwd.argtypes = [ctypes.c_int, size_t] + [void_p] * 9 + [size_t, i64, i64, i32, i32]
+    library.b200_int4_gemms_moe_swiglu_workspace_bytes.restype = size_t
+    library.b200_int4_gemms_moe_swiglu_workspace_bytes.argtypes = [ctypes.POINTER(MoeProblem)]
+    library.b200_int4_gemms_moe_swiglu.restype = ctypes.c_int
+    library.b200_int4_gemms_moe_swiglu.argtypes = [ctypes.POINTER(MoeProblem), ctypes.c_int, size_t] + [void_p] * 10 + [size_t]
 
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:
@@ -973,3 +997,26 @@ def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any,
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
     return dx, sums[0], sums[1]
+
+
+def moe_swiglu_on_device(
+    problem: MoeProblem, x: Any, *, router_weight: Any | None, topk_ids: Any | None, topk_weights: Any | None, w_up_gate: Any,
+    up_gate_scale: Any, w_down: Any, down_scale: Any, library_path: str | Path | None = None, stream: Any | None = None,
+) -> Any:
+    """The layer's output for checked CUDA operands; see :func:`moe.moe_swiglu`.
+
+    The scratch is allocated for the call: the caching allocator keeps it apart from other streams' and, under
+    capture, inside the graph's own pool."""
+    torch = _torch()
+    library = load_dispatch_library(library_path)
+    out = torch.empty_like(x)
+    need = int(library.b200_int4_gemms_moe_swiglu_workspace_bytes(ctypes.byref(problem)))
+    workspace = torch.empty(need, device=x.device, dtype=torch.uint8)
+    rc = library.b200_int4_gemms_moe_swiglu(
+        ctypes.byref(problem), _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(),
+        0 if router_weight is None else router_weight.data_ptr(), 0 if topk_ids is None else topk_ids.data_ptr(),
+        0 if topk_weights is None else topk_weights.data_ptr(), w_up_gate.data_ptr(), up_gate_scale.data_ptr(), w_down.data_ptr(),
+        down_scale.data_ptr(), out.data_ptr(), workspace.data_ptr(), need)
+    if rc != 0:
+        raise RuntimeError(_library_last_error(library))
+    return out
