@@ -1,14 +1,19 @@
 // A whole mixture-of-experts layer for a few tokens:
 //   moe_route_kernel     router logits (fp64 sums), the tokens' codes and scales, counters set to zero
 //   moe_select_kernel    top-k, softmax, and for each expert in use the list of its (token, choice) pairs
-//   moe_product_kernel   up/gate product, SwiGLU; the last block of an expert quantises the activations
+//   moe_product_kernel   up/gate product, SwiGLU
+//   moe_quantize_kernel  the activations' codes and scales
 //   moe_product_kernel   down product; the last block of a column range adds the experts' shares for every token
+// Each kernel is launched while the one before it still runs (programmatic dependent launch) and waits for it where
+// it needs its results.
 //
 // At a few tokens each weight is used by a handful of rows, so the layer is bound by reading the weights of the
 // experts in use once from HBM.  The products therefore run on mma.sync.m16n8k32 (int8, exact int32 sums) with the
-// WEIGHTS as the 16-row operand and up to eight tokens as the other: the weights go from global memory straight
-// into the registers that feed the matrix instruction, with no stop in shared memory and no barrier in the loop.
-// tcgen05 would want 128-row tiles of unpacked weights in shared memory; its rate is of no use here.
+// WEIGHTS as the 16-row operand and eight tokens at a time as the other.  Every warp copies its share of the weights
+// into a ring of its own in shared memory (cp.async), several steps ahead and on into the next columns while the sums
+// of the last ones are finished: some 100 KB an SM in flight, which is what HBM's latency asks for.  tcgen05 would
+// want 128-row tiles of unpacked weights in shared memory; its rate is of no use here (measured on this part:
+// m16n8k32 every 2 clocks an SM, 256 weights a clock for eight tokens, where HBM delivers 46).
 //
 // Operand order.  A lane (g = lane / 4, q = lane % 4) supplies rows g and g + 8 of the 16 x 32 operand and, for
 // each, K values that a quad of lanes divides up.  Which K a lane holds does not matter as long as both operands
@@ -17,7 +22,7 @@
 // shifted right at the end, exactly.
 #pragma once
 
-#include <climits>
+#include <type_traits>
 
 #include "row_common.cuh"
 
@@ -44,7 +49,7 @@ struct MoeParams {
   int router_f32, ids_64, renormalize;
   // scratch
   uint8_t* xq;              // [tokens, hidden bytes]
-  bf16* xs;                 // [tokens, groups of hidden]
+  float* xs;                // [tokens, groups of hidden]
   double* logits;           // [tokens, experts]
   int* pair_expert;         // [pairs], -1: no expert
   float* pair_weight;       // [pairs]
@@ -52,44 +57,67 @@ struct MoeParams {
   int* pair_list;           // [pairs], by expert
   double* act;              // [pairs, inner]
   uint8_t* aq;              // [pairs, inner bytes]
-  bf16* as;                 // [pairs, groups of inner]
+  float* as;                // [pairs, groups of inner]
   float* part;              // [pairs, hidden]
-  int* done_up;             // [slots]
   int* done_down;           // [column ranges]
-  int slots, down_ranges;
+  int slots, up_ranges, down_ranges;
 };
 
 template <int DT>
 __device__ __forceinline__ long long code_bytes(long long k) { return DT == 4 ? k / 2 : k; }
 
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------------------------------------
+// Logits of four experts for up to eight tokens: 12 values converted to fp64 (16 a clock and SM) for 32 products (64 a
+// clock), the eight warps divide K between them.
 template <typename W>
 __device__ __forceinline__ void route_logits(const MoeParams& p, int block) {
-  const int expert_blocks = (p.experts + 7) / 8;
-  const int e = (block % expert_blocks) * 8 + (threadIdx.x >> 5), t0 = (block / expert_blocks) * 8;
-  if (e >= p.experts) return;
-  const W* row = static_cast<const W*>(p.router) + static_cast<long long>(e) * p.hidden;
-  const int lane = threadIdx.x & 31, count = min(8, p.tokens - t0);
-  double acc[8];
+  __shared__ double part[8][32];
+  const int expert_blocks = (p.experts + 3) / 4;
+  const int e0 = (block % expert_blocks) * 4, t0 = (block / expert_blocks) * 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, count = min(8, p.tokens - t0), last_e = p.experts - 1;
+  double acc[32];  // [expert][token]
 #pragma unroll
-  for (int t = 0; t < 8; ++t) acc[t] = 0.0;
-  for (int at = lane * 8; at < p.hidden; at += 256) {
-    Raw8<W> w;
-    w.template load<true>(row, at, p.hidden);
+  for (int i = 0; i < 32; ++i) acc[i] = 0.0;
+  for (int at = threadIdx.x * 8; at < p.hidden; at += 2048) {
+    Raw8<W> w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // beyond the last expert: the last one again, not stored
+      w[e].template load<true>(static_cast<const W*>(p.router) + static_cast<long long>(min(e0 + e, last_e)) * p.hidden, at, p.hidden);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      if (t >= count) break;
-      Raw8<bf16> x;
-      x.load<true>(p.x + static_cast<long long>(t0 + t) * p.hidden, at, p.hidden);
+      if (t < count) {
+        Raw8<bf16> x;
+        x.load<true>(p.x + static_cast<long long>(t0 + t) * p.hidden, at, p.hidden);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[t] = fma(static_cast<double>(x.get(i)), static_cast<double>(w.get(i)), acc[t]);
+        for (int i = 0; i < 8; ++i) {
+          const double v = static_cast<double>(x.get(i));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e * 8 + t] = fma(v, static_cast<double>(w[e].get(i)), acc[e * 8 + t]);
+        }
+      }
     }
   }
+  // sum of 32 values over 32 lanes; lane i is left with value i
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    if (t >= count) break;
-    const double sum = warp_reduce(acc[t], SumOp());
-    if (lane == 0) p.logits[static_cast<long long>(t0 + t) * p.experts + e] = sum;
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const bool upper = (lane & o) != 0;
+      const double send = upper ? acc[j] : acc[j + o], keep = upper ? acc[j + o] : acc[j];
+      acc[j] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, o);
+    }
+  }
+  part[warp][lane] = acc[0];
+  __syncthreads();
+  if (warp == 0) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part[i][lane];
+    const int e = e0 + lane / 8, t = t0 + lane % 8;
+    if (e <= last_e && t < p.tokens) p.logits[static_cast<long long>(t) * p.experts + e] = sum;
   }
 }
 
@@ -110,7 +138,7 @@ __device__ __forceinline__ void route_quantize(const MoeParams& p, int token) {
       for (int i = 0; i < 4; ++i) m = __vmaxu2(m, raw.w[i] & 0x7FFF7FFFu);
     }
     s = scale_of_bf16<DT>(row_reduce<256>(max(m & 0xFFFFu, m >> 16), MaxOp(), scratch));
-    if (threadIdx.x == 0) p.xs[token] = __float2bfloat16_rn(s);
+    if (threadIdx.x == 0) p.xs[token] = s;
   }
   for (int base = 0; base < p.hidden; base += 2048) {
     const int at = base + threadIdx.x * 8;
@@ -121,7 +149,7 @@ __device__ __forceinline__ void route_quantize(const MoeParams& p, int token) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = __vmaxu2(m, raw.w[i] & 0x7FFF7FFFu);
       s = scale_of_bf16<DT>(warp_reduce(max(m & 0xFFFFu, m >> 16), MaxOp(), lanes));
-      if ((threadIdx.x & (lanes - 1)) == 0 && at < p.hidden) p.xs[token * groups + at / p.sub] = __float2bfloat16_rn(s);
+      if ((threadIdx.x & (lanes - 1)) == 0 && at < p.hidden) p.xs[token * groups + at / p.sub] = s;
     }
     uint32_t c[8];
     if (scale_is_ordinary(s)) {
@@ -136,15 +164,15 @@ __device__ __forceinline__ void route_quantize(const MoeParams& p, int token) {
   }
 }
 
-// Blocks [0, tokens): a token's codes.  Block `tokens`: counters.  The others: logits of eight experts for up to
+// Blocks [0, tokens): a token's codes.  Block `tokens`: counters.  The others: logits of four experts for up to
 // eight tokens.  The sums are in fp64, so that the choice of experts does not hang on the order of a sum.
 template <int DT>
 __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
+  grid_release();
   const int b = blockIdx.x;
   if (b < p.tokens) {
     route_quantize<DT>(p, b);
   } else if (b == p.tokens) {
-    for (int i = threadIdx.x; i < p.slots; i += 256) p.done_up[i] = 0;
     for (int i = threadIdx.x; i < p.down_ranges; i += 256) p.done_down[i] = 0;
   } else if (p.router_f32) {
     route_logits<float>(p, b - p.tokens - 1);
@@ -153,57 +181,70 @@ __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
   }
 }
 
+// fp64 numbers as whole numbers in the same order: 0 stands for "taken", 1 for NaN, which is below everything.
+__device__ __forceinline__ unsigned long long logit_key(double v) {
+  if (!(v == v)) return 1ull;
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));  // -0 becomes 0
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double logit_of_key(unsigned long long k) {
+  if (k == 1ull) return __longlong_as_double(0x7FF8000000000000LL);
+  return __longlong_as_double(static_cast<long long>((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
+}
+
 // One block of 1024 threads.  A warp picks a token's experts one after the other: the largest logit that is left,
-// ties to the lowest index, NaN below everything (a token with such logits gets weights of NaN).
-static __global__ void __launch_bounds__(1024) moe_select_kernel(const MoeParams p) {
+// ties to the lowest index (a token whose logits are NaN gets the first experts and weights of NaN).  A lane keeps
+// PER logits, of experts lane, lane + 32, ...
+template <int PER>
+__global__ void __launch_bounds__(1024) moe_select_kernel(const MoeParams p) {
   __shared__ int chosen[kMoeMaxPairs];
   __shared__ int count[kMoeMaxExperts];
   __shared__ int first[kMoeMaxExperts];
   __shared__ int warp_sums[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = p.tokens * p.top_k;
+  grid_wait();
+  grid_release();
   if (p.router != nullptr) {
     for (int t = warp; t < p.tokens; t += 32) {
-      const double* row = p.logits + static_cast<long long>(t) * p.experts;
-      uint32_t taken = 0;  // of this lane's experts lane, lane + 32, ...
-      double mine = 0.0;   // lane j: the logit of choice j
+      unsigned long long key[PER], mine = 0;  // lane j: the key of choice j
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = e < p.experts ? logit_key(__ldcg(p.logits + static_cast<long long>(t) * p.experts + e)) : 0ull;
+      }
+      double all = 0.0;
       int mine_id = -1;
       for (int j = 0; j < p.top_k; ++j) {
-        double best = 0.0;
-        int best_id = INT_MAX;
-        for (int i = 0, e = lane; e < p.experts; ++i, e += 32) {
-          if ((taken >> i) & 1u) continue;
-          double v = row[e];
-          if (!(v == v)) v = -__longlong_as_double(0x7FF0000000000000LL);
-          if (best_id == INT_MAX || v > best) {
-            best = v;
-            best_id = e;
+        unsigned long long best = 0;
+        unsigned best_id = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (key[i] > best) {
+            best = key[i];
+            best_id = lane + 32 * i;
           }
+        const unsigned hi = static_cast<unsigned>(best >> 32), lo = static_cast<unsigned>(best);
+        const unsigned top_hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+        const unsigned top_lo = __reduce_max_sync(0xFFFFFFFFu, hi == top_hi ? lo : 0u);
+        const unsigned id = __reduce_min_sync(0xFFFFFFFFu, hi == top_hi && lo == top_lo ? best_id : 0xFFFFFFFFu);
+        if (lane == j) {
+          mine = (static_cast<unsigned long long>(top_hi) << 32) | top_lo;
+          mine_id = static_cast<int>(id);
+        }
+        if (j == 0 && !p.renormalize) {
+          const double top = logit_of_key((static_cast<unsigned long long>(top_hi) << 32) | top_lo);
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (key[i] != 0) all += exp(logit_of_key(key[i]) - top);
+          all = warp_reduce(all, SumOp());
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const double v = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-          const int id = __shfl_xor_sync(0xFFFFFFFFu, best_id, o);
-          if (id != INT_MAX && (best_id == INT_MAX || v > best || (v == best && id < best_id))) {
-            best = v;
-            best_id = id;
-          }
-        }
-        if ((best_id & 31) == lane) taken |= 1u << (best_id >> 5);
-        if (lane == j) {
-          mine = row[best_id];
-          mine_id = best_id;
-        }
+        for (int i = 0; i < PER; ++i)
+          if (id == static_cast<unsigned>(lane + 32 * i)) key[i] = 0;
       }
-      const double top = __shfl_sync(0xFFFFFFFFu, mine, 0);
-      const double e = lane < p.top_k ? exp(mine - top) : 0.0;
-      double total;
-      if (p.renormalize) {
-        total = warp_reduce(e, SumOp());
-      } else {
-        total = 0.0;
-        for (int i = lane; i < p.experts; i += 32) total += exp(row[i] - top);
-        total = warp_reduce(total, SumOp());
-      }
+      const double logit = logit_of_key(mine), top = __shfl_sync(0xFFFFFFFFu, logit, 0);
+      const double e = lane < p.top_k ? exp(logit - top) : 0.0;
+      const double total = p.renormalize ? warp_reduce(e, SumOp()) : all;
       if (lane < p.top_k) {
         chosen[t * p.top_k + lane] = mine_id;
         p.pair_weight[t * p.top_k + lane] = static_cast<float>(e / total);
@@ -271,25 +312,23 @@ __device__ __forceinline__ void mma_i8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Weights: read once, kept out of L1.
-template <int WORDS>
-__device__ __forceinline__ void load_weight_words(uint32_t (&w)[4], const uint8_t* p, bool valid) {
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) w[i] = 0u;
-  if (!valid) return;
-  if (WORDS == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
-  else if (WORDS == 2)
-    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+// BYTES of global memory to shared memory, or zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool valid) {
+  const int size = valid ? BYTES : 0;
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
   else
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
 template <int WORDS>
-__device__ __forceinline__ void load_code_words(uint32_t (&w)[4], const uint8_t* p, bool valid) {
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) w[i] = 0u;
-  if (!valid) return;
+__device__ __forceinline__ void read_words(uint32_t (&w)[4], const uint8_t* p) {
   if (WORDS == 4) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
@@ -304,245 +343,338 @@ __device__ __forceinline__ void load_code_words(uint32_t (&w)[4], const uint8_t*
 __device__ __forceinline__ uint32_t even_codes(uint32_t w) { return (w << 4) & 0xF0F0F0F0u; }
 __device__ __forceinline__ uint32_t odd_codes(uint32_t w) { return w & 0xF0F0F0F0u; }
 
-// 4 x 4 bytes: r[i] holds row i of four columns; the result w[c] holds column c of four rows.
-__device__ __forceinline__ void transpose_bytes(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t (&w)[4]) {
-  const uint32_t a = __byte_perm(r0, r1, 0x5140), b = __byte_perm(r0, r1, 0x7362);  // columns 0,1 and 2,3 of rows 0,1
-  const uint32_t c = __byte_perm(r2, r3, 0x5140), d = __byte_perm(r2, r3, 0x7362);
-  w[0] = __byte_perm(a, c, 0x5410);
-  w[1] = __byte_perm(a, c, 0x7632);
-  w[2] = __byte_perm(b, d, 0x5410);
-  w[3] = __byte_perm(b, d, 0x7632);
+// Two 16 x 16 byte matrices, transposed: lane (g, q) gets bytes 4 q .. 4 q + 3 of columns g and g + 8 of each.
+__device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
 }
 
-// What a block knows of its product: rows of weight codes times the codes of `count` pairs.
+constexpr int kMoeThreads = 256;
+constexpr int kMoeWarps = kMoeThreads / 32;
+
+// What a block knows of its product: columns of weight codes times the codes of some tokens or pairs.
 struct MoeTile {
   const uint8_t* w;       // the expert's matrix
   const bf16* w_scale;    // the expert's scales: [N] or [groups, N]
-  const uint8_t* codes;   // of all rows; row index given by rows_of
-  const bf16* scales;
+  const uint8_t* codes;   // of all tokens or pairs
+  const float* scales;
   int k, n;               // K, and N of the matrix (2 * inner for up/gate)
   int groups;
 };
 
-// Accumulators of one lane: kFrags fragments of 16 rows, kN groups of eight tokens.
-template <bool SC>
-struct MoeSum {
-  using type = int;
-};
-template <>
-struct MoeSum<true> {
-  using type = double;
+// A block works on a range of columns at a time: 32 (K-major weights, NT) or 128 (N-major, NN), for up/gate half of
+// them up columns and half the same columns of the gate.  Its eight warps divide K into shares and, for NN, the
+// columns into halves; a warp has kFrags fragments of 16 columns.
+// NT: a lane takes WORDS words of a column at a time, the quad 4 * WORDS: a step of 4 * WORDS * (8 or 4) values of K.
+// NN: a step is 32 values of K: 16 rows of packed pairs or 32 of int8, 64 columns each, transposed by ldmatrix.
+// One stage of a warp's ring: weights, token codes, and (SC) the scales of the step's group of K.
+template <int DT, bool NN, bool SC, int WORDS, int kN>
+struct MoeStage {
+  static constexpr int kCols = NN ? 128 : 32, kFrags = NN ? 4 : 2, kHalves = NN ? 2 : 1, kShares = kMoeWarps / kHalves;
+  static constexpr int kStepK = NN ? 32 : 4 * WORDS * (DT == 4 ? 8 : 4);
+  static constexpr int kRows = DT == 4 ? 16 : 32;                            // NN: rows of a step
+  static constexpr int kWeights = NN ? kRows * 64 : 4 * 32 * 4 * WORDS;      // bytes
+  static constexpr int kCodeBytes = NN ? (DT == 4 ? 4 : 8) : 4 * WORDS;      // of a token, by a lane
+  static constexpr int kScalesAt = kWeights + kN * 32 * kCodeBytes;
+  static constexpr int kRowScalesAt = kScalesAt + (SC ? kFrags * 32 : 0);
+  static constexpr int kBytes = kRowScalesAt + (SC ? kN * 8 * 4 : 0);
+  // about 8 KB a warp, so that three blocks fit an SM where their registers do
+  static constexpr int kStages = 8192 / kBytes < 3 ? 3 : (8192 / kBytes > 8 ? 8 : 8192 / kBytes);
+  using Sum = typename std::conditional<SC, double, int>::type;
+  static constexpr int kRingBytes = kMoeWarps * kStages * kBytes;
+  // integers are added in place; fp64 numbers are kept by share, to be added in order
+  static constexpr int kSums = kFrags * kHalves * kN * 4 * 32 * (SC ? kShares : 1);
+  static constexpr int kSmemBytes = kRingBytes + kSums * static_cast<int>(sizeof(Sum));
 };
 
-// `columns`: kTileCols weight columns (rows of the transposed matrix) a block works on.
-// K-major weights (NT): 32 columns, warps = 2 fragments x 4 shares of K.
-// N-major weights (NN): 128 columns in 8 fragments, 8 shares of K; lane group g holds columns 16 g .. 16 g + 15, of
-// which fragment f takes the two at 2 f.
-template <bool NN>
-struct MoeShape {
-  static constexpr int kCols = NN ? 128 : 32;
-  static constexpr int kFrags = NN ? 8 : 1;
-  static constexpr int kShares = NN ? 8 : 4;
-};
+// Where the sum of fragment `frag` (of the block), token group n and result j of a lane lies: spread over the banks.
+template <int kN>
+__device__ __forceinline__ int sum_place(int frag, int n, int j, int lane) {
+  return (((frag * kN + n) * 4 + j) << 5) + (lane ^ ((frag * 4 + j) & 31));
+}
 
-constexpr int kMoeThreads = 256;
-
-template <int DT, bool NN, bool SC, int WORDS, int TOKENS, bool kDown>
-__device__ __forceinline__ void moe_product(const MoeParams& p, const MoeTile& tile, int tile_index, const int* row_of, int count,
-                                            typename MoeSum<SC>::type* red) {
-  using Sum = typename MoeSum<SC>::type;
-  constexpr int kN = TOKENS / 8, kFrags = MoeShape<NN>::kFrags, kCols = MoeShape<NN>::kCols;
+// Column ranges [range0, range1) of one expert for the `count` <= 8 kN tokens in `rows`.  `before_codes` runs between
+// the first weight copies and the first use of `rows` and the codes; `finish(range, sum)` is called by all threads with
+// the sums of a range at hand: sum(c, t, gate) for its column c and token t.
+template <int DT, bool NN, bool SC, int WORDS, int kN, bool kDown, typename Before, typename Finish>
+__device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile, int range0, int range1, const int* rows, int count,
+                                         uint8_t* smem, Before&& before_codes, Finish&& finish) {
+  using Stage = MoeStage<DT, NN, SC, WORDS, kN>;
+  using Sum = typename Stage::Sum;
+  constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int half_n = tile.n / 2;  // up/gate: the gate columns start here
-  int acc[kFrags][kN][4];
-  double sum[SC ? kFrags : 1][SC ? kN : 1][4];
-#pragma unroll
-  for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-    for (int n = 0; n < kN; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[f][n][i] = 0;
-        if (SC) sum[f][n][i] = 0.0;
-      }
-  // rows of the token operand that this lane reads, and (for the scales) the rows its results belong to
+  const int half = NN ? warp & 1 : 0, share = NN ? warp >> 1 : warp;
+  const int gate = tile.n / 2;  // where the gate columns start
+  const int steps = (tile.k + Stage::kStepK - 1) / Stage::kStepK;
+  // NN: consecutive steps (whole groups of K as far as it goes); NT: every eighth
+  const int per_share = (steps + kShares - 1) / kShares;
+  const int begin = NN ? share * per_share : share, by = NN ? 1 : kShares;
+  const int mine = NN ? max(0, min(steps - begin, per_share)) : (steps - share + kShares - 1) / kShares;
+  uint8_t* ring = smem + warp * kStages * Stage::kBytes;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  Sum* sums = reinterpret_cast<Sum*>(smem + Stage::kRingBytes);
   const long long code_pitch = code_bytes<DT>(tile.k);
-  const uint8_t* codes[kN];
-#pragma unroll
-  for (int n = 0; n < kN; ++n) codes[n] = n * 8 + g < count ? tile.codes + row_of[n * 8 + g] * code_pitch : nullptr;
 
-  if constexpr (!NN) {
-    // a lane takes 4 * WORDS consecutive bytes of a row, a quad 16 * WORDS: `chunk` values of K
-    constexpr int kPerLane = WORDS * (DT == 4 ? 8 : 4), chunk = 4 * kPerLane;
-    const int frag = warp & 1, share = warp >> 1;
-    const int col0 = kDown ? tile_index * 32 + frag * 16 : frag * half_n + tile_index * 16;
-    const uint8_t* row_a = tile.w + (col0 + g) * code_pitch;
-    const uint8_t* row_b = row_a + 8 * code_pitch;
-    const int chunks = (tile.k + chunk - 1) / chunk;
-#pragma unroll 2
-    for (int c = share; c < chunks; c += MoeShape<false>::kShares) {
-      const int k0 = c * chunk + q * kPerLane;
+  // first column of a fragment of this warp in a range; NN: whether the matrix has it (16 columns at a time)
+  auto column_of = [&](int range, int f) {
+    const int frag = half * kFrags + f;
+    if (kDown) return range * Stage::kCols + frag * 16;
+    return frag < kAllFrags / 2 ? range * (Stage::kCols / 2) + frag * 16 : gate + range * (Stage::kCols / 2) + (frag - kAllFrags / 2) * 16;
+  };
+  auto column_valid = [&](int range, int f) {
+    if (!NN) return true;
+    if (kDown) return column_of(range, f) < tile.n;
+    return range * (Stage::kCols / 2) + (half * kFrags + f) % (kAllFrags / 2) * 16 < gate;
+  };
+
+  auto copy_weights = [&](int range, int i, int slot) {
+    const int step = begin + i * by;
+    const uint32_t at = ring_at + slot * Stage::kBytes;
+    if constexpr (NN) {
+      // 16 bytes of row r and fragment f to place r * 4 + (f ^ (r / 2 % 4)): eight rows of a fragment on eight banks
+      const int f = lane & 3;
+      const bool valid = column_valid(range, f);
+      const uint8_t* src = tile.w + (valid ? column_of(range, f) : 0) + (static_cast<long long>(step) * Stage::kRows + (lane >> 2)) * tile.n;
+#pragma unroll
+      for (int l = 0; l < Stage::kRows / 8; ++l) {
+        const int r = l * 8 + (lane >> 2);
+        copy_async<16>(at + (r * 4 + (f ^ ((r >> 1) & 3))) * 16, src + static_cast<long long>(l) * 8 * tile.n, valid);
+      }
+      if constexpr (SC) {  // two columns a lane
+        const bool scale_valid = column_valid(range, lane >> 3);
+        const bf16* scale = tile.w_scale + static_cast<long long>(step * 32 / p.sub) * tile.n + (scale_valid ? column_of(range, lane >> 3) + (lane & 7) * 2 : 0);
+        copy_async<4>(at + Stage::kScalesAt + lane * 4, scale, scale_valid);
+      }
+    } else {
+      const int k0 = step * Stage::kStepK + q * (Stage::kStepK / 4);
       const bool valid = k0 < tile.k;
-      const long long at = code_bytes<DT>(k0);
-      uint32_t wa[4], wb[4], x[kN][4];
-      load_weight_words<WORDS>(wa, row_a + at, valid);
-      load_weight_words<WORDS>(wb, row_b + at, valid);
 #pragma unroll
-      for (int n = 0; n < kN; ++n) load_code_words<WORDS>(x[n], codes[n] + at, valid && codes[n] != nullptr);
-      if constexpr (DT == 4) {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i)
-#pragma unroll
-          for (int n = 0; n < kN; ++n)
-            mma_i8(acc[0][n], even_codes(wa[i]), even_codes(wb[i]), odd_codes(wa[i]), odd_codes(wb[i]), even_codes(x[n][i]), odd_codes(x[n][i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < WORDS; i += 2)
-#pragma unroll
-          for (int n = 0; n < kN; ++n) mma_i8(acc[0][n], wa[i], wb[i], wa[i + 1], wb[i + 1], x[n][i], x[n][i + 1]);
-      }
-      if constexpr (SC) {  // the chunk lies in one group of K
-        const int kg = c * chunk / p.sub;
-        const double sa = to_f32(tile.w_scale[static_cast<long long>(kg) * tile.n + col0 + g]);
-        const double sb = to_f32(tile.w_scale[static_cast<long long>(kg) * tile.n + col0 + g + 8]);
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int token = n * 8 + 2 * q + (i & 1);
-            const double st = token < count ? to_f32(tile.scales[row_of[token] * tile.groups + kg]) : 0.f;
-            sum[0][n][i] = fma(static_cast<double>(DT == 4 ? acc[0][n][i] >> 8 : acc[0][n][i]), st * (i < 2 ? sa : sb), sum[0][n][i]);
-            acc[0][n][i] = 0;
-          }
-      }
-    }
-  } else {
-    // a step is 32 values of K: a lane takes 4 (packed) or 8 rows of K, 16 columns each
-    const int block = kDown ? tile_index * 128 + g * 16 : (g < 4 ? tile_index * 64 + g * 16 : half_n + tile_index * 64 + (g - 4) * 16);
-    const bool col_valid = kDown ? block < tile.n : (g < 4 ? block < half_n : block < tile.n);
-    const int steps = tile.k / 32, share_steps = (steps + 7) / 8;
-    const int begin = warp * share_steps, end = min(steps, begin + share_steps);
-    constexpr int kRows = DT == 4 ? 4 : 8;
-    const uint8_t* base = tile.w + block + static_cast<long long>(q * kRows) * tile.n;
-    for (int s = begin; s < end; ++s) {
-      uint32_t r[kRows][4], x[kN][4];
-      const uint8_t* at = base + static_cast<long long>(s) * 4 * kRows * tile.n;
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) load_weight_words<4>(r[i], at + static_cast<long long>(i) * tile.n, col_valid);
-#pragma unroll
-      for (int n = 0; n < kN; ++n)
-        load_code_words<DT == 4 ? 1 : 2>(x[n], codes[n] + code_bytes<DT>(s * 32 + q * 8), codes[n] != nullptr);
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4) {  // four columns at a time: fragments 2 c4 and 2 c4 + 1
-        uint32_t lo[4], hi[4];
-        transpose_bytes(r[0][c4], r[1][c4], r[2][c4], r[3][c4], lo);
-        if constexpr (DT == 8) transpose_bytes(r[4][c4], r[5][c4], r[6][c4], r[7][c4], hi);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            if constexpr (DT == 4)
-              mma_i8(acc[2 * c4 + h][n], even_codes(lo[2 * h]), even_codes(lo[2 * h + 1]), odd_codes(lo[2 * h]), odd_codes(lo[2 * h + 1]),
-                     even_codes(x[n][0]), odd_codes(x[n][0]));
-            else
-              mma_i8(acc[2 * c4 + h][n], lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1], x[n][0], x[n][1]);
-          }
+      for (int l = 0; l < 4; ++l) {  // fragment l / 2, rows g and g + 8
+        const uint8_t* src = tile.w + (column_of(range, l >> 1) + g + (l & 1) * 8) * code_pitch + (valid ? code_bytes<DT>(k0) : 0);
+        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, src, valid);
       }
       if constexpr (SC) {
-        const bool last = s + 1 == end || ((s + 1) * 32) % p.sub == 0;
-        if (last) {
-          const int kg = s * 32 / p.sub;
-          const bf16* ws = tile.w_scale + static_cast<long long>(kg) * tile.n + block;
-#pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            double st[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int token = n * 8 + 2 * q + i;
-              st[i] = token < count ? to_f32(tile.scales[row_of[token] * tile.groups + kg]) : 0.f;
-            }
-#pragma unroll
-            for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const double sw = col_valid ? to_f32(ws[2 * f + (i >> 1)]) : 0.f;
-                sum[f][n][i] = fma(static_cast<double>(DT == 4 ? acc[f][n][i] >> 8 : acc[f][n][i]), st[i & 1] * sw, sum[f][n][i]);
-                acc[f][n][i] = 0;
-              }
-          }
+        if (lane < 16) {
+          const bf16* scale = tile.w_scale + static_cast<long long>(step * Stage::kStepK / p.sub) * tile.n + column_of(range, lane >> 3) + (lane & 7) * 2;
+          copy_async<4>(at + Stage::kScalesAt + lane * 4, scale, true);
         }
       }
     }
+  };
+  auto copy_codes = [&](int i, int slot) {
+    const int step = begin + i * by;
+    const uint32_t at = ring_at + slot * Stage::kBytes + Stage::kWeights;
+    // NN int8: two words 16 K apart, one for each half of the instruction's K
+    const int k0 = step * Stage::kStepK + q * (NN && DT == 8 ? 4 : Stage::kStepK / 4);
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const bool valid = n * 8 + g < count && k0 < tile.k;
+      const uint8_t* src = tile.codes + (valid ? rows[n * 8 + g] * code_pitch + code_bytes<DT>(k0) : 0);
+      const uint32_t to = at + (n * 32 + lane) * Stage::kCodeBytes;
+      if constexpr (NN && DT == 8) {
+        copy_async<4>(to, src, valid);
+        copy_async<4>(to + 4, src + (valid ? 16 : 0), valid);
+      } else {
+        copy_async<Stage::kCodeBytes>(to, src, valid);
+      }
+    }
+    if constexpr (SC) {
+      if (lane < kN * 8) {
+        const bool valid = lane < count;
+        const float* scale = tile.scales + (valid ? static_cast<long long>(rows[lane]) * tile.groups + step * Stage::kStepK / p.sub : 0);
+        copy_async<4>(ring_at + slot * Stage::kBytes + Stage::kRowScalesAt + lane * 4, scale, valid);
+      }
+    }
+  };
+
+  // the next step to copy
+  int ahead_range = range0, ahead_step = 0, ahead_slot = 0;
+  auto advance = [&]() {
+    if (++ahead_slot == kStages) ahead_slot = 0;
+    if (++ahead_step == mine) {
+      ahead_step = 0;
+      ++ahead_range;
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (mine > 0 && ahead_range < range1) copy_weights(ahead_range, ahead_step, ahead_slot);
+    advance();
+  }
+  if constexpr (!SC)  // integers are added to what lies here
+    for (int i = threadIdx.x; i < Stage::kSums; i += kMoeThreads) sums[i] = 0;
+  before_codes();  // holds a barrier
+  ahead_range = range0, ahead_step = 0, ahead_slot = 0;
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (mine > 0 && ahead_range < range1) copy_codes(ahead_step, ahead_slot);
+    copy_commit();
+    advance();
   }
 
-  // the shares of K: exact integers in any order, or fp64 numbers one warp after the other
-  for (int i = threadIdx.x; i < kCols * TOKENS; i += kMoeThreads) red[i] = 0;
-  __syncthreads();
-  auto column = [&](int f, int i) { return NN ? g * 16 + 2 * f + (i >> 1) : (warp & 1) * 16 + g + (i >> 1) * 8; };
-  if constexpr (!SC) {
+  int slot = 0;
+  for (int range = range0; range < range1; ++range) {
+    int acc[kFrags][kN][4];
+    double sum[SC ? kFrags : 1][SC ? kN : 1][4];
 #pragma unroll
     for (int f = 0; f < kFrags; ++f)
 #pragma unroll
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int token = n * 8 + 2 * q + (i & 1);
-          if (token < count) atomicAdd(&red[column(f, i) * TOKENS + token], DT == 4 ? acc[f][n][i] >> 8 : acc[f][n][i]);
+          acc[f][n][i] = 0;
+          if (SC) sum[f][n][i] = 0.0;
         }
-    __syncthreads();
-  } else {
-    for (int turn = 0; turn < MoeShape<NN>::kShares; ++turn) {
-      if ((NN ? warp : warp >> 1) == turn) {
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      copy_wait<kStages - 2>();
+      __syncwarp();  // what the other lanes have copied
+      const uint8_t* stage = ring + slot * Stage::kBytes;
+      uint32_t x[kN][4];
 #pragma unroll
-        for (int f = 0; f < kFrags; ++f)
+      for (int n = 0; n < kN; ++n) read_words<Stage::kCodeBytes / 4>(x[n], stage + Stage::kWeights + (n * 32 + lane) * Stage::kCodeBytes);
+      if constexpr (NN) {
+        // lanes 0 .. 15 name the rows of one matrix, 16 .. 31 those of the other: two fragments (packed), or the two
+        // halves of K of one (int8)
+        const uint32_t at = ring_at + slot * Stage::kBytes;
 #pragma unroll
-          for (int n = 0; n < kN; ++n)
+        for (int l = 0; l < (DT == 4 ? kFrags / 2 : kFrags); ++l) {
+          const int r = DT == 4 ? lane & 15 : lane, f = DT == 4 ? 2 * l + (lane >> 4) : l;
+          uint32_t m[4];
+          load_transposed(m, at + (r * 4 + (f ^ ((r >> 1) & 3))) * 16);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) red[column(f, i) * TOKENS + n * 8 + 2 * q + (i & 1)] += sum[f][n][i];
+          for (int n = 0; n < kN; ++n) {
+            if constexpr (DT == 4) {
+              mma_i8(acc[2 * l][n], even_codes(m[0]), even_codes(m[1]), odd_codes(m[0]), odd_codes(m[1]), even_codes(x[n][0]), odd_codes(x[n][0]));
+              mma_i8(acc[2 * l + 1][n], even_codes(m[2]), even_codes(m[3]), odd_codes(m[2]), odd_codes(m[3]), even_codes(x[n][0]), odd_codes(x[n][0]));
+            } else {
+              mma_i8(acc[l][n], m[0], m[1], m[2], m[3], x[n][0], x[n][1]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f) {
+          uint32_t wa[4], wb[4];
+          read_words<WORDS>(wa, stage + (2 * f * 32 + lane) * 4 * WORDS);
+          read_words<WORDS>(wb, stage + ((2 * f + 1) * 32 + lane) * 4 * WORDS);
+          if constexpr (DT == 4) {
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j)
+#pragma unroll
+              for (int n = 0; n < kN; ++n)
+                mma_i8(acc[f][n], even_codes(wa[j]), even_codes(wb[j]), odd_codes(wa[j]), odd_codes(wb[j]), even_codes(x[n][j]), odd_codes(x[n][j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < WORDS; j += 2)
+#pragma unroll
+              for (int n = 0; n < kN; ++n) mma_i8(acc[f][n], wa[j], wb[j], wa[j + 1], wb[j + 1], x[n][j], x[n][j + 1]);
+          }
+        }
       }
-      __syncthreads();
+      if constexpr (SC) {
+        // the integers of a group of K end here: scaled and added up in fp64 (NT: a step lies in one group)
+        if (!NN || i + 1 == mine || ((begin + i + 1) * 32) % p.sub == 0) {
+          const bf16* w_scales = reinterpret_cast<const bf16*>(stage + Stage::kScalesAt);
+          const float* row_scales = reinterpret_cast<const float*>(stage + Stage::kRowScalesAt);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            const float2 st = *reinterpret_cast<const float2*>(row_scales + n * 8 + 2 * q);
+#pragma unroll
+            for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float sw = to_f32(w_scales[f * 16 + g + (j >> 1) * 8]);
+                // a product of two bf16 numbers is exact in fp32
+                sum[f][n][j] = fma(static_cast<double>(DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]), static_cast<double>(((j & 1) ? st.y : st.x) * sw), sum[f][n][j]);
+                acc[f][n][j] = 0;
+              }
+          }
+        }
+      }
+      __syncwarp();  // before the stage that was read a step ago is written again
+      if (ahead_range < range1) {
+        copy_weights(ahead_range, ahead_step, ahead_slot);
+        copy_codes(ahead_step, ahead_slot);
+        advance();
+      }
+      copy_commit();
+      if (++slot == kStages) slot = 0;
     }
+    if constexpr (!SC) {
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) atomicAdd(sums + sum_place<kN>(half * kFrags + f, n, j, lane), DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]);
+    } else {
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sums[share * (kAllFrags * kN * 128) + sum_place<kN>(half * kFrags + f, n, j, lane)] = sum[f][n][j];
+    }
+    __syncthreads();
+    finish(range, [&](int c, int t, bool gate_part) -> Sum {
+      const int column = c + (gate_part ? Stage::kCols / 2 : 0);
+      const int place = sum_place<kN>(column >> 4, t >> 3, ((column >> 3) & 1) * 2 + (t & 1), (column & 7) * 4 + ((t & 7) >> 1));
+      Sum total = sums[place];
+      if constexpr (SC) {
+#pragma unroll
+        for (int w = 1; w < kShares; ++w) total += sums[w * (kAllFrags * kN * 128) + place];
+      } else {
+        sums[place] = 0;  // for the next range
+      }
+      return total;
+    });
+    __syncthreads();
   }
+  copy_wait<0>();
 }
 
-// Quantises the activations of one expert's pairs (fp64 in, as they were computed): what quantize_tokens does, with
-// values that are not exactly known in fp32, so that each code is settled against them where it has to be.
+// Quantises the activations of one pair (fp64 in, as they were computed): what quantize_tokens does, with values that
+// are not exactly known in fp32, so that a code is settled against them where it has to be.
+constexpr int kMoeQuantThreads = 512;
+
 template <int DT>
-__device__ __forceinline__ void quantize_activations(const MoeParams& p, const int* list, int count) {
+__global__ void __launch_bounds__(kMoeQuantThreads) moe_quantize_kernel(const MoeParams p) {
   constexpr double kTop = DT == 4 ? 7.0 : 127.0;
-  __shared__ unsigned long long warp_max[8];
+  constexpr int kWarps = kMoeQuantThreads / 32;
+  __shared__ unsigned long long warp_max[kWarps];
+  grid_wait();
+  grid_release();
+  const int pair = blockIdx.x;
+  if (p.pair_expert[pair] < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int length = p.sub ? p.sub : p.inner, groups = p.sub ? (p.inner + p.sub - 1) / p.sub : 1;
-  // a row by all warps, by four, two or one; a group of values by one
-  const int per_row = p.sub ? 1 : (count == 1 ? 8 : count == 2 ? 4 : count <= 4 ? 2 : 1);
-  const int items = count * groups, step = 8 / per_row;
-  for (int base = 0; base < items; base += step) {
-    const int item = base + warp / per_row;
-    const bool live = item < items;
-    const int pair = live ? list[item / groups] : 0, c0 = live ? (item % groups) * length : 0;
-    const int c1 = live ? min(c0 + length, p.inner) : 0;
-    const double* row = p.act + static_cast<long long>(pair) * p.inner;
-    const int begin = c0 + ((warp % per_row) * 32 + lane) * 2, stride = per_row * 64;
+  const double* row = p.act + static_cast<long long>(pair) * p.inner;
+  uint8_t* codes = p.aq + static_cast<long long>(pair) * code_bytes<DT>(p.inner);
+  // the row by all warps, or a group of values by one
+  const int length = p.sub ? p.sub : p.inner, groups = p.sub ? (p.inner + p.sub - 1) / p.sub : 1, per_group = p.sub ? 1 : kWarps;
+  for (int group = p.sub ? warp : 0; group < groups; group += kWarps) {
+    const int c0 = group * length, c1 = min(c0 + length, p.inner);
+    const int begin = c0 + ((warp % per_group) * 32 + lane) * 2, stride = per_group * 64;
     unsigned long long most = 0;
+#pragma unroll 4
     for (int c = begin; c < c1; c += stride) {
-      const double2 v = __ldcg(reinterpret_cast<const double2*>(row + c));
+      const double2 v = *reinterpret_cast<const double2*>(row + c);
       const unsigned long long a = __double_as_longlong(v.x) & 0x7FFFFFFFFFFFFFFFLL, b = __double_as_longlong(v.y) & 0x7FFFFFFFFFFFFFFFLL;
       most = max(most, max(a, b));
     }
     most = warp_reduce(most, MaxOp());
-    if (per_row > 1) {
+    if (per_group > 1) {  // one group: the barrier is met by all
       if (lane == 0) warp_max[warp] = most;
       __syncthreads();
-      for (int i = 0; i < per_row; ++i) most = max(most, warp_max[warp / per_row * per_row + i]);
-      __syncthreads();
+      most = warp_reduce(warp_max[lane % kWarps], MaxOp());
     }
     const float s = nonzero_scale(bf16_from_double(__longlong_as_double(most) / kTop));
-    if (live && begin == c0) p.as[static_cast<long long>(pair) * groups + item % groups] = __float2bfloat16_rn(s);
+    if (begin == c0) p.as[static_cast<long long>(pair) * groups + group] = s;
     const bool ordinary = scale_is_ordinary(s);
     const float inv = __frcp_rn(s), delta = static_cast<float>(kTop) * 4.76837158203125e-7f;  // fp32 value, product: 3 roundings
-    uint8_t* codes = p.aq + static_cast<long long>(pair) * code_bytes<DT>(p.inner);
+#pragma unroll 4
     for (int c = begin; c < c1; c += stride) {
-      const double2 v = __ldcg(reinterpret_cast<const double2*>(row + c));
+      const double2 v = *reinterpret_cast<const double2*>(row + c);
       uint32_t code[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -561,86 +693,114 @@ __device__ __forceinline__ void quantize_activations(const MoeParams& p, const i
   }
 }
 
-// True in the whole block for the last of `total` blocks that count up `counter`: what the others wrote before is
-// then visible to it (through L2: read with __ldcg).
-__device__ __forceinline__ bool last_block(int* counter, int total) {
-  __shared__ int is_last;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    is_last = atomicAdd(counter, 1) == total - 1;
-    __threadfence();
+// The grid is as large as the device holds at once; the (expert, column range) units of the experts in use, whose
+// number only the device knows, are divided evenly among its blocks, consecutive ones to a block.
+// kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
+template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
+__global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_product_kernel(const MoeParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int rows[kMaxN * 8];
+  constexpr int kCols = NN ? 128 : 32, out_cols = kDown ? kCols : kCols / 2;
+  if (!kDown) {
+    grid_wait();
+    grid_release();
   }
-  __syncthreads();
-  return is_last != 0;
-}
-
-template <int DT, bool NN, bool SC, int WORDS, bool kDown>
-__global__ void __launch_bounds__(kMoeThreads) moe_product_kernel(const MoeParams p) {
-  using Sum = typename MoeSum<SC>::type;
-  constexpr int kCols = MoeShape<NN>::kCols;
-  constexpr int kMaxTokens = SC ? 8 : 16;  // of one pass over the weights: what the accumulators leave room for
-  __shared__ Sum red[kCols * kMaxTokens];
-  __shared__ int rows[kMaxTokens];
-  const int out_cols = kDown ? kCols : kCols / 2;
-  const int ranges = ((kDown ? p.hidden : p.inner) + out_cols - 1) / out_cols;
-  const int slot = blockIdx.x / ranges, range = blockIdx.x % ranges, col0 = range * out_cols;
-  const int in_use = p.active[0];
-  if (slot >= in_use) {
-    if (kDown && in_use == 0 && slot == 0)  // no pair has an expert: nothing is added up
-      for (int i = threadIdx.x; i < p.tokens * kCols; i += kMoeThreads)
-        if (col0 + i % kCols < p.hidden) p.out[static_cast<long long>(i / kCols) * p.hidden + col0 + i % kCols] = __float2bfloat16_rn(0.f);
+  const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges;
+  // written by the select kernel, which had ended before the up/gate product let the next kernels start
+  const int in_use = __ldcg(p.active);
+  if (kDown && in_use == 0) {  // no pair has an expert: nothing is added up
+    grid_wait();
+    for (long long i = blockIdx.x * kMoeThreads + threadIdx.x; i < static_cast<long long>(p.tokens) * p.hidden; i += gridDim.x * kMoeThreads)
+      p.out[i] = __float2bfloat16_rn(0.f);
     return;
   }
-  const int expert = p.active[1 + 3 * slot], first = p.active[2 + 3 * slot], count = p.active[3 + 3 * slot];
-  const int* list = p.pair_list + first;
+  const long long units = static_cast<long long>(in_use) * ranges;
+  const long long unit0 = units * blockIdx.x / gridDim.x, unit1 = units * (blockIdx.x + 1) / gridDim.x;
+  bool waited = !kDown;
   MoeTile tile;
   tile.k = kDown ? p.inner : p.hidden;
   tile.n = kDown ? p.hidden : 2 * p.inner;
   tile.groups = SC ? (tile.k + p.sub - 1) / p.sub : 1;
-  tile.w = (kDown ? p.w_down : p.w_up_gate) + static_cast<long long>(expert) * tile.n * code_bytes<DT>(tile.k);
-  tile.w_scale = (kDown ? p.s_down : p.s_up_gate) + static_cast<long long>(expert) * tile.n * tile.groups;
   tile.codes = kDown ? p.aq : p.xq;
   tile.scales = kDown ? p.as : p.xs;
-
-  for (int done = 0; done < count; done += kMaxTokens) {
-    const int here = min(kMaxTokens, count - done);
-    __syncthreads();
-    if (threadIdx.x < kMaxTokens) rows[threadIdx.x] = threadIdx.x < here ? (kDown ? list[done + threadIdx.x] : list[done + threadIdx.x] / p.top_k) : 0;
-    __syncthreads();
-    if (SC || here <= 8) moe_product<DT, NN, SC, WORDS, 8, kDown>(p, tile, range, rows, here, red);
-    else moe_product<DT, NN, SC, WORDS, kMaxTokens, kDown>(p, tile, range, rows, here, red);
-    const int width = SC || here <= 8 ? 8 : kMaxTokens;
-    for (int i = threadIdx.x; i < here * out_cols; i += kMoeThreads) {
-      const int token = i / out_cols, c = i % out_cols, col = col0 + c, pair = list[done + token];
-      if (col >= (kDown ? p.hidden : p.inner)) continue;
-      if (kDown) {
-        double y = static_cast<double>(red[c * width + token]);
-        if (!SC) y *= static_cast<double>(to_f32(tile.scales[rows[token]])) * static_cast<double>(to_f32(tile.w_scale[col]));
-        p.part[static_cast<long long>(pair) * p.hidden + col] = static_cast<float>(y) * p.pair_weight[pair];
-      } else {
-        double up = static_cast<double>(red[c * width + token]), gate = static_cast<double>(red[(c + out_cols) * width + token]);
-        if (!SC) {
-          const double s = to_f32(tile.scales[rows[token]]);
-          up *= s * static_cast<double>(to_f32(tile.w_scale[col]));
-          gate *= s * static_cast<double>(to_f32(tile.w_scale[p.inner + col]));
+  const int c = threadIdx.x % out_cols;  // a thread's outputs are all of one column of a range
+  for (long long unit = unit0; unit < unit1;) {
+    const int slot = static_cast<int>(unit / ranges), range0 = static_cast<int>(unit % ranges);
+    const int range1 = static_cast<int>(min(static_cast<long long>(ranges), range0 + (unit1 - unit)));
+    unit += range1 - range0;
+    const int expert = __ldcg(p.active + 1 + 3 * slot), first = __ldcg(p.active + 2 + 3 * slot), count = __ldcg(p.active + 3 + 3 * slot);
+    const int* list = p.pair_list + first;
+    tile.w = (kDown ? p.w_down : p.w_up_gate) + static_cast<long long>(expert) * tile.n * code_bytes<DT>(tile.k);
+    tile.w_scale = (kDown ? p.s_down : p.s_up_gate) + static_cast<long long>(expert) * tile.n * tile.groups;
+    for (int done = 0; done < count; done += kMaxN * 8) {
+      const int here = min(kMaxN * 8, count - done);
+      auto before_codes = [&]() {
+        if (!waited) grid_wait();
+        waited = true;
+        if (threadIdx.x < here) {
+          const int pair = __ldcg(list + done + threadIdx.x);
+          rows[threadIdx.x] = kDown ? pair : pair / p.top_k;
         }
-        p.act[static_cast<long long>(pair) * p.inner + col] = up * gate / (1.0 + exp(-gate));
-      }
+        __syncthreads();
+      };
+      auto finish = [&](int range, auto sum) {
+        const int col = range * out_cols + c;
+        if (col >= out_n) return;
+        const float scale = SC ? 1.f : to_f32(tile.w_scale[col]), gate_scale = SC || kDown ? 1.f : to_f32(tile.w_scale[p.inner + col]);
+        for (int t = threadIdx.x / out_cols; t < here; t += kMoeThreads / out_cols) {
+          const int pair = kDown ? rows[t] : __ldcg(list + done + t);
+          const double s = SC ? 1.0 : static_cast<double>(__ldcg(tile.scales + rows[t]));
+          if (kDown) {
+            double y = static_cast<double>(sum(c, t, false));
+            if (!SC) y *= s * static_cast<double>(scale);
+            p.part[static_cast<long long>(pair) * p.hidden + col] = static_cast<float>(y) * __ldcg(p.pair_weight + pair);
+          } else {
+            double up = static_cast<double>(sum(c, t, false)), gate = static_cast<double>(sum(c, t, true));
+            if (!SC) {
+              up *= s * static_cast<double>(scale);
+              gate *= s * static_cast<double>(gate_scale);
+            }
+            p.act[static_cast<long long>(pair) * p.inner + col] = up * gate / (1.0 + exp(-gate));
+          }
+        }
+      };
+      auto pass = [&](auto n) {
+        moe_pass<DT, NN, SC, WORDS, decltype(n)::value, kDown>(p, tile, range0, range1, rows, here, smem, before_codes, finish);
+      };
+      if (kMaxN == 1 || here <= 8) pass(std::integral_constant<int, 1>());
+      else if (kMaxN == 2 || here <= 16) pass(std::integral_constant<int, kMaxN < 2 ? kMaxN : 2>());
+      else pass(std::integral_constant<int, kMaxN>());
     }
   }
-  if (!kDown) {
-    if (last_block(p.done_up + slot, ranges)) quantize_activations<DT>(p, list, count);
-  } else if (last_block(p.done_down + range, in_use)) {
-    for (int i = threadIdx.x; i < p.tokens * kCols; i += kMoeThreads) {
-      const int token = i / kCols, col = col0 + i % kCols;
-      if (col >= p.hidden) continue;
-      float y = 0.f;
-      for (int j = 0; j < p.top_k; ++j) {
-        const int pair = token * p.top_k + j;
-        if (p.pair_expert[pair] >= 0) y += __ldcg(p.part + static_cast<long long>(pair) * p.hidden + col);
+  if (!waited) grid_wait();  // no kernel of the call ends before those in front of it
+  if constexpr (kDown) {
+    // The last block to finish a column range adds up the experts' shares for all tokens, in the order of the choices.
+    __shared__ int full[kMoeThreads];
+    __shared__ int full_count;
+    __threadfence();
+    for (long long base = unit0; base < unit1; base += kMoeThreads) {
+      __syncthreads();
+      if (threadIdx.x == 0) full_count = 0;
+      __syncthreads();
+      if (base + threadIdx.x < unit1) {
+        const int range = static_cast<int>((base + threadIdx.x) % ranges);
+        if (atomicAdd(p.done_down + range, 1) == in_use - 1) full[atomicAdd(&full_count, 1)] = range;
+        __threadfence();
       }
-      p.out[static_cast<long long>(token) * p.hidden + col] = __float2bfloat16_rn(y);
+      __syncthreads();
+      for (int f = 0; f < full_count; ++f) {
+        const int col0 = full[f] * kCols;
+        for (int i = threadIdx.x; i < p.tokens * kCols; i += kMoeThreads) {
+          const int token = i / kCols, col = col0 + i % kCols;
+          if (col >= p.hidden) continue;
+          float y = 0.f;
+          for (int j = 0; j < p.top_k; ++j) {
+            const int pair = token * p.top_k + j;
+            if (__ldcg(p.pair_expert + pair) >= 0) y += __ldcg(p.part + static_cast<long long>(pair) * p.hidden + col);
+          }
+          p.out[static_cast<long long>(token) * p.hidden + col] = __float2bfloat16_rn(y);
+        }
+      }
     }
   }
 }

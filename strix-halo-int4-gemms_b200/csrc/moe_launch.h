@@ -6,7 +6,7 @@
 
 namespace b200 {
 
-int launch_moe_int4(const MoeParams& params, bool n_major, cudaStream_t stream);
-int launch_moe_int8(const MoeParams& params, bool n_major, cudaStream_t stream);
+int launch_moe_int4(const MoeParams& params, bool n_major, int sm_count, cudaStream_t stream);
+int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStream_t stream);
 
 }  // namespace b200

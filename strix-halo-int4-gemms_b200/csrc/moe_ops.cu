@@ -38,11 +38,12 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   const size_t per_byte = m.dtype == B200_DTYPE_INT4 ? 2 : 1;
   const size_t x_groups = m.subchannel ? (m.hidden + m.subchannel - 1) / m.subchannel : 1;
   const size_t a_groups = m.subchannel ? (m.inner + m.subchannel - 1) / m.subchannel : 1;
-  const int down_cols = m.layout == B200_LAYOUT_NN ? MoeShape<true>::kCols : MoeShape<false>::kCols;
+  const int down_cols = m.layout == B200_LAYOUT_NN ? 128 : 32;  // of one block
   p->slots = static_cast<int>(pairs < static_cast<size_t>(m.experts) ? pairs : m.experts);
+  p->up_ranges = (m.inner + down_cols / 2 - 1) / (down_cols / 2);
   p->down_ranges = (m.hidden + down_cols - 1) / down_cols;
   p->xq = reinterpret_cast<uint8_t*>(take(static_cast<size_t>(m.tokens) * m.hidden / per_byte));
-  p->xs = reinterpret_cast<bf16*>(take(m.tokens * x_groups * 2));
+  p->xs = reinterpret_cast<float*>(take(m.tokens * x_groups * 4));
   p->logits = reinterpret_cast<double*>(take(static_cast<size_t>(m.tokens) * m.experts * 8));
   p->pair_expert = reinterpret_cast<int*>(take(pairs * 4));
   p->pair_weight = reinterpret_cast<float*>(take(pairs * 4));
@@ -50,9 +51,8 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->pair_list = reinterpret_cast<int*>(take(pairs * 4));
   p->act = reinterpret_cast<double*>(take(pairs * m.inner * 8));
   p->aq = reinterpret_cast<uint8_t*>(take(pairs * m.inner / per_byte));
-  p->as = reinterpret_cast<bf16*>(take(pairs * a_groups * 2));
+  p->as = reinterpret_cast<float*>(take(pairs * a_groups * 4));
   p->part = reinterpret_cast<float*>(take(pairs * m.hidden * 4));
-  p->done_up = reinterpret_cast<int*>(take(static_cast<size_t>(p->slots) * 4));
   p->done_down = reinterpret_cast<int*>(take(static_cast<size_t>(p->down_ranges) * 4));
   return at;
 }
@@ -83,11 +83,10 @@ extern "C" int b200_int4_gemms_moe_swiglu(const b200_moe_problem* problem, int d
     if (router_weight == nullptr && (topk_ids == nullptr || topk_weights == nullptr))
       return host_fail("either router weights or topk_ids and topk_weights must be given");
     if (router_weight != nullptr && topk_ids != nullptr && m.ids_bits != 32) return host_fail("topk_ids are written as int32");
-    for (const void* ptr : {x_bf16, router_weight, w_up_gate, w_down})
-      if (!is_aligned(ptr, 16)) return host_fail("x and weight pointers must be 16-byte aligned");
-    if (!is_aligned(up_gate_scale, 2) || !is_aligned(down_scale, 2) || !is_aligned(out_bf16, 2) || !is_aligned(topk_weights, 4) ||
-        !is_aligned(topk_ids, m.ids_bits / 8))
-      return host_fail("scale, out, topk_ids and topk_weights pointers must be aligned to their element size");
+    for (const void* ptr : {x_bf16, router_weight, w_up_gate, w_down, up_gate_scale, down_scale})
+      if (!is_aligned(ptr, 16)) return host_fail("x, weight and scale pointers must be 16-byte aligned");
+    if (!is_aligned(out_bf16, 2) || !is_aligned(topk_weights, 4) || !is_aligned(topk_ids, m.ids_bits / 8))
+      return host_fail("out, topk_ids and topk_weights pointers must be aligned to their element size");
     DeviceScope device;
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
@@ -117,6 +116,6 @@ extern "C" int b200_int4_gemms_moe_swiglu(const b200_moe_problem* problem, int d
     p.renormalize = m.renormalize;
     const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
     const bool n_major = m.layout == B200_LAYOUT_NN;
-    return m.dtype == B200_DTYPE_INT4 ? launch_moe_int4(p, n_major, stream) : launch_moe_int8(p, n_major, stream);
+    return m.dtype == B200_DTYPE_INT4 ? launch_moe_int4(p, n_major, sms, stream) : launch_moe_int8(p, n_major, sms, stream);
   });
 }

@@ -1,50 +1,81 @@
 // The expert layer's kernels for one code type: compiled with B200_MOE_BITS 4 and 8.
 #include "moe_launch.h"
 
-#include <type_traits>
-
 namespace b200 {
 namespace {
 
 constexpr int kBits = B200_MOE_BITS;
 
+// A launch that may start while the kernel before it on the stream still runs (it waits for it by itself).
+template <typename... Args>
+int launch_dependent(void (*kernel)(Args...), int blocks, int threads, int smem_bytes, cudaStream_t stream, const MoeParams& p) {
+  if (smem_bytes > 48 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+    if (err != cudaSuccess) return host_fail_cuda("cudaFuncSetAttribute(max dynamic shared memory)", err);
+  }
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
+  config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
+  return err == cudaSuccess ? 0 : host_fail_cuda("moe_swiglu launch", err);
+}
+
+template <bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
+int launch_product(const MoeParams& p, int sm_count, cudaStream_t stream) {
+  using Stage = MoeStage<kBits, NN, SC, WORDS, kMaxN>;
+  // the most that any number of token groups up to kMaxN asks for
+  using One = MoeStage<kBits, NN, SC, WORDS, 1>;
+  using Two = MoeStage<kBits, NN, SC, WORDS, kMaxN < 2 ? kMaxN : 2>;
+  int smem = Stage::kSmemBytes > One::kSmemBytes ? Stage::kSmemBytes : One::kSmemBytes;
+  smem = smem > Two::kSmemBytes ? smem : Two::kSmemBytes;
+  auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kDown>;
+  const long long units = static_cast<long long>(p.slots) * (kDown ? p.down_ranges : p.up_ranges);
+  const int resident = smem <= 74 * 1024 && !SC && kMaxN != 4 ? 3 : smem <= 112 * 1024 ? 2 : 1;  // by shared memory and launch bounds
+  const long long blocks = units < static_cast<long long>(resident) * sm_count ? units : static_cast<long long>(resident) * sm_count;
+  return launch_dependent(kernel, static_cast<int>(blocks), kMoeThreads, smem, stream, p);
+}
+
+// An expert can have at most as many rows as there are tokens (times the same expert given twice to a token, which
+// only takes more passes): the fewer rows a pass has to be ready for, the more registers are left for other blocks.
 template <bool NN, bool SC, int WORDS>
-void launch_products(const MoeParams& p, cudaStream_t stream) {
-  const int cols = MoeShape<NN>::kCols;
-  const int up_ranges = (p.inner + cols / 2 - 1) / (cols / 2);
-  moe_product_kernel<kBits, NN, SC, WORDS, false><<<p.slots * up_ranges, kMoeThreads, 0, stream>>>(p);
-  moe_product_kernel<kBits, NN, SC, WORDS, true><<<p.slots * p.down_ranges, kMoeThreads, 0, stream>>>(p);
+int launch_for_tokens(const MoeParams& p, int sm_count, cudaStream_t stream) {
+  auto products = [&](auto max_n) {
+    constexpr int kMaxN = decltype(max_n)::value;
+    if (int rc = launch_product<NN, SC, WORDS, kMaxN, false>(p, sm_count, stream); rc != 0) return rc;
+    if (int rc = launch_dependent(moe_quantize_kernel<kBits>, p.tokens * p.top_k, kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
+    return launch_product<NN, SC, WORDS, kMaxN, true>(p, sm_count, stream);
+  };
+  if (p.tokens <= 8) return products(std::integral_constant<int, 1>());
+  if (p.tokens <= 16 || SC) return products(std::integral_constant<int, 2>());
+  return products(std::integral_constant<int, SC ? 2 : 4>());
 }
 
 }  // namespace
 
 #if B200_MOE_BITS == 4
-int launch_moe_int4(const MoeParams& p, bool n_major, cudaStream_t stream) {
+int launch_moe_int4(const MoeParams& p, bool n_major, int sm_count, cudaStream_t stream) {
 #else
-int launch_moe_int8(const MoeParams& p, bool n_major, cudaStream_t stream) {
+int launch_moe_int8(const MoeParams& p, bool n_major, int sm_count, cudaStream_t stream) {
 #endif
-  const int logit_blocks = p.router != nullptr ? (p.experts + 7) / 8 * ((p.tokens + 7) / 8) : 0;
+  const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 7) / 8) : 0;
   moe_route_kernel<kBits><<<p.tokens + 1 + logit_blocks, 256, 0, stream>>>(p);
-  moe_select_kernel<<<1, 1024, 0, stream>>>(p);
-  // K-major weights with scales for groups of K: a warp's load stays within one group (32 K a word of nibbles, 16 a
-  // word of bytes)
+  if (const cudaError_t err = cudaGetLastError(); err != cudaSuccess) return host_fail_cuda("moe_swiglu launch", err);
+  auto select = p.experts <= 64 ? moe_select_kernel<2> : p.experts <= 256 ? moe_select_kernel<8> : moe_select_kernel<32>;
+  if (int rc = launch_dependent(select, 1, 1024, 0, stream, p); rc != 0) return rc;
+  if (n_major) return p.sub ? launch_for_tokens<true, true, 4>(p, sm_count, stream) : launch_for_tokens<true, false, 4>(p, sm_count, stream);
+  if (!p.sub) return launch_for_tokens<false, false, 4>(p, sm_count, stream);
+  // K-major weights with scales for groups of K: a step stays within one group (32 K a word of nibbles, 16 a word of bytes)
   constexpr int kWord = kBits == 4 ? 32 : 16;
-  if (n_major) {
-    if (p.sub) launch_products<true, true, 4>(p, stream);
-    else launch_products<true, false, 4>(p, stream);
-  } else if (!p.sub) {
-    launch_products<false, false, 4>(p, stream);
-  } else if (p.sub >= 4 * kWord) {
-    launch_products<false, true, 4>(p, stream);
-  } else if (p.sub == 2 * kWord) {
-    launch_products<false, true, 2>(p, stream);
-#if B200_MOE_BITS == 4
-  } else {
-    launch_products<false, true, 1>(p, stream);
-#endif
-  }
-  const cudaError_t err = cudaGetLastError();
-  return err == cudaSuccess ? 0 : host_fail_cuda("moe_swiglu launch", err);
+  if (p.sub >= 4 * kWord) return launch_for_tokens<false, true, 4>(p, sm_count, stream);
+  if (kBits == 8 || p.sub == 2 * kWord) return launch_for_tokens<false, true, 2>(p, sm_count, stream);
+  return launch_for_tokens<false, true, kBits == 4 ? 1 : 2>(p, sm_count, stream);
 }
 
 }  // namespace b200

@@ -132,7 +132,8 @@ def moe_swiglu(
         top_k = int(topk_ids.shape[1])
     if not 0 < top_k <= min(MOE_MAX_TOP_K, experts):
         raise ValueError(f"top_k must be in [1, {min(MOE_MAX_TOP_K, experts)}]; got {top_k}")
-    for name, tensor in (("x", x), ("router_weight", router_weight), ("w_up_gate", w_up_gate), ("w_down", w_down)):
+    for name, tensor in (("x", x), ("router_weight", router_weight), ("w_up_gate", w_up_gate), ("w_down", w_down),
+                         ("up_gate_scale", up_gate_scale), ("down_scale", down_scale)):
         if tensor is not None and tensor.data_ptr() % 16:
             raise ValueError(f"{name} must start on a multiple of 16 bytes")
 

@@ -70,7 +70,7 @@ def test_c_entry_point_checks_arguments(pkg, native_lib):
     assert "either router weights or" in said(problem(), pointers)[1]
     pointers = [4096] * 9
     pointers[4] = 4100
-    assert said(problem(), pointers)[1] == "x and weight pointers must be 16-byte aligned"
+    assert said(problem(), pointers)[1] == "x, weight and scale pointers must be 16-byte aligned"
     assert "written as int32" in said(problem(ids_bits=64))[1]
     assert said(problem(tokens=0), [None] * 9, (None, 0))[0] == 0
     # scratch of the documented size: everything a pair and a token need, each part rounded up to 256 bytes
