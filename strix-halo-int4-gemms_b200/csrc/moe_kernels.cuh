@@ -1,9 +1,10 @@
 // A whole mixture-of-experts layer for a few tokens:
-//   moe_route_kernel     router logits (fp64 sums), the tokens' codes and scales, counters set to zero
+//   moe_route_kernel     router logits (fp64 sums), the tokens' codes and scales
 //   moe_select_kernel    top-k, softmax, and for each expert in use the list of its (token, choice) pairs
 //   moe_product_kernel   up/gate product, SwiGLU
 //   moe_quantize_kernel  the activations' codes and scales
-//   moe_product_kernel   down product; the last block of a column range adds the experts' shares for every token
+//   moe_product_kernel   down product
+//   moe_combine_kernel   the experts' shares of every token added up
 // Each kernel is launched while the one before it still runs (programmatic dependent launch) and waits for it where
 // it needs its results.
 //
@@ -58,9 +59,8 @@ struct MoeParams {
   double* act;              // [pairs, inner]
   uint8_t* aq;              // [pairs, inner bytes]
   float* as;                // [pairs, groups of inner]
-  float* part;              // [pairs, hidden]
-  int* done_down;           // [column ranges]
-  int slots, up_ranges, down_ranges;
+  void* part;               // [down_splits, pairs, hidden]: sums of the codes' products (int32), or scaled ones (fp64)
+  int slots, up_ranges, down_ranges, down_splits;
 };
 
 template <int DT>
@@ -164,20 +164,17 @@ __device__ __forceinline__ void route_quantize(const MoeParams& p, int token) {
   }
 }
 
-// Blocks [0, tokens): a token's codes.  Block `tokens`: counters.  The others: logits of four experts for up to
-// eight tokens.  The sums are in fp64, so that the choice of experts does not hang on the order of a sum.
+// Blocks [0, tokens): a token's codes.  The others: logits of four experts for up to eight tokens.  The sums are in fp64, so that the choice of experts does not hang on the order of a sum.
 template <int DT>
 __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
   grid_release();
   const int b = blockIdx.x;
   if (b < p.tokens) {
     route_quantize<DT>(p, b);
-  } else if (b == p.tokens) {
-    for (int i = threadIdx.x; i < p.down_ranges; i += 256) p.done_down[i] = 0;
   } else if (p.router_f32) {
-    route_logits<float>(p, b - p.tokens - 1);
+    route_logits<float>(p, b - p.tokens);
   } else {
-    route_logits<bf16>(p, b - p.tokens - 1);
+    route_logits<bf16>(p, b - p.tokens);
   }
 }
 
@@ -349,6 +346,16 @@ __device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t addre
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
 }
 
+// Sums over K: exact integers, or (a scale for each group of K) scaled ones.
+template <bool SC>
+struct MoeSum {
+  using type = int;
+};
+template <>
+struct MoeSum<true> {
+  using type = double;
+};
+
 constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
 
@@ -365,27 +372,32 @@ struct MoeTile {
 // A block works on a range of columns at a time: 32 (K-major weights, NT) or 128 (N-major, NN), for up/gate half of
 // them up columns and half the same columns of the gate.  Its eight warps divide K into shares and, for NN, the
 // columns into halves; a warp has kFrags fragments of 16 columns.
-// NT: a lane takes WORDS words of a column at a time, the quad 4 * WORDS: a step of 4 * WORDS * (8 or 4) values of K.
-// NN: a step is 32 values of K: 16 rows of packed pairs or 32 of int8, 64 columns each, transposed by ldmatrix.
+// A step is 4 * WORDS * (8 or 4) values of K, of which lane q of a quad has WORDS consecutive words of the token codes.
+// NT: and the same words of each column.  NN: rows of 64 columns, which ldmatrix transposes; the row that a lane names
+// for it puts the right values of K into each quad's words.
 // One stage of a warp's ring: weights, token codes, and (SC) the scales of the step's group of K.
 template <int DT, bool NN, bool SC, int WORDS, int kN>
 struct MoeStage {
   static constexpr int kCols = NN ? 128 : 32, kFrags = NN ? 4 : 2, kHalves = NN ? 2 : 1, kShares = kMoeWarps / kHalves;
-  static constexpr int kStepK = NN ? 32 : 4 * WORDS * (DT == 4 ? 8 : 4);
-  static constexpr int kRows = DT == 4 ? 16 : 32;                            // NN: rows of a step
-  static constexpr int kWeights = NN ? kRows * 64 : 4 * 32 * 4 * WORDS;      // bytes
-  static constexpr int kCodeBytes = NN ? (DT == 4 ? 4 : 8) : 4 * WORDS;      // of a token, by a lane
+  static constexpr int kStepK = 4 * WORDS * (DT == 4 ? 8 : 4), kStepBytes = 16 * WORDS;  // of a column
+  static constexpr int kWeights = kFrags * 16 * kStepBytes;                              // bytes
+  static constexpr int kCodeBytes = 4 * WORDS;                                           // of a token, by a lane
   static constexpr int kScalesAt = kWeights + kN * 32 * kCodeBytes;
   static constexpr int kRowScalesAt = kScalesAt + (SC ? kFrags * 32 : 0);
   static constexpr int kBytes = kRowScalesAt + (SC ? kN * 8 * 4 : 0);
   // about 8 KB a warp, so that three blocks fit an SM where their registers do
-  static constexpr int kStages = 8192 / kBytes < 3 ? 3 : (8192 / kBytes > 8 ? 8 : 8192 / kBytes);
-  using Sum = typename std::conditional<SC, double, int>::type;
+  static constexpr int kStages = 8448 / kBytes < 3 ? 3 : (8448 / kBytes > 8 ? 8 : 8448 / kBytes);
+  using Sum = typename MoeSum<SC>::type;
   static constexpr int kRingBytes = kMoeWarps * kStages * kBytes;
-  // integers are added in place; fp64 numbers are kept by share, to be added in order
-  static constexpr int kSums = kFrags * kHalves * kN * 4 * 32 * (SC ? kShares : 1);
+  static constexpr int kSums = kFrags * kHalves * kN * 4 * 32;
   static constexpr int kSmemBytes = kRingBytes + kSums * static_cast<int>(sizeof(Sum));
 };
+
+// int32 -> fp64 without a conversion instruction (16 a clock and SM; the subtraction runs at 64): 2^52 + 2^31 + v, bit
+// by bit, minus 2^52 + 2^31.
+__device__ __forceinline__ double exact_double(int v) {
+  return __hiloint2double(0x43300000, v ^ 0x80000000) - 4503601774854144.0;
+}
 
 // Where the sum of fragment `frag` (of the block), token group n and result j of a lane lies: spread over the banks.
 template <int kN>
@@ -393,25 +405,25 @@ __device__ __forceinline__ int sum_place(int frag, int n, int j, int lane) {
   return (((frag * kN + n) * 4 + j) << 5) + (lane ^ ((frag * 4 + j) & 31));
 }
 
-// Column ranges [range0, range1) of one expert for the `count` <= 8 kN tokens in `rows`.  `before_codes` runs between
-// the first weight copies and the first use of `rows` and the codes; `finish(range, sum)` is called by all threads with
-// the sums of a range at hand: sum(c, t, gate) for its column c and token t.
+// Column ranges [range0, range1) and steps [step0, step1) of K of one expert for the `count` <= 8 kN tokens in `rows`.
+// `before_codes` runs between the first weight copies and the first use of `rows` and the codes; `finish(range, sum)` is
+// called by all threads with the sums of a range at hand: sum(c, t, gate) for its column c and token t.
 template <int DT, bool NN, bool SC, int WORDS, int kN, bool kDown, typename Before, typename Finish>
-__device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile, int range0, int range1, const int* rows, int count,
-                                         uint8_t* smem, Before&& before_codes, Finish&& finish) {
+__device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile, int range0, int range1, int step0, int step1,
+                                         const int* rows, int count, uint8_t* smem, Before&& before_codes, Finish&& finish) {
   using Stage = MoeStage<DT, NN, SC, WORDS, kN>;
   using Sum = typename Stage::Sum;
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
+  constexpr int kStepBytes = Stage::kStepBytes;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int half = NN ? warp & 1 : 0, share = NN ? warp >> 1 : warp;
   const int gate = tile.n / 2;  // where the gate columns start
-  const int steps = (tile.k + Stage::kStepK - 1) / Stage::kStepK;
   // NN: consecutive steps (whole groups of K as far as it goes); NT: every eighth
-  const int per_share = (steps + kShares - 1) / kShares;
-  const int begin = NN ? share * per_share : share, by = NN ? 1 : kShares;
-  const int mine = NN ? max(0, min(steps - begin, per_share)) : (steps - share + kShares - 1) / kShares;
-  uint8_t* ring = smem + warp * kStages * Stage::kBytes;
-  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const int steps = step1 - step0, per_share = (steps + kShares - 1) / kShares;
+  const int begin = step0 + (NN ? share * per_share : share), by = NN ? 1 : kShares;
+  const int mine = NN ? max(0, min(steps - share * per_share, per_share)) : max(0, (steps - share + kShares - 1) / kShares);
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kStages * Stage::kBytes;
+  const uint8_t* ring = smem + warp * kStages * Stage::kBytes;
   Sum* sums = reinterpret_cast<Sum*>(smem + Stage::kRingBytes);
   const long long code_pitch = code_bytes<DT>(tile.k);
 
@@ -427,89 +439,113 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
     return range * (Stage::kCols / 2) + (half * kFrags + f) % (kAllFrags / 2) * 16 < gate;
   };
 
-  auto copy_weights = [&](int range, int i, int slot) {
-    const int step = begin + i * by;
-    const uint32_t at = ring_at + slot * Stage::kBytes;
+  // What is copied next: step `i` of `range` into the stage at `to`.  The weight pointer moves on by additions.
+  struct Cursor {
+    int range, i, slot;
+    const uint8_t* w;   // of this lane at step i
+    const bf16* scale;  // of this lane's columns in the first group of K
+    bool valid, scale_valid;
+  } next;
+  const long long w_step = NN ? static_cast<long long>(by) * kStepBytes * tile.n : static_cast<long long>(by) * kStepBytes;
+  const long long w_rows = NN ? 8LL * tile.n : 8 * code_pitch;                                     // to the next of a lane's loads
+  const long long w_frag = NN ? 0 : (kDown ? 16LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its second fragment
+  auto enter_range = [&]() {
+    if (next.range >= range1) return;
     if constexpr (NN) {
-      // 16 bytes of row r and fragment f to place r * 4 + (f ^ (r / 2 % 4)): eight rows of a fragment on eight banks
-      const int f = lane & 3;
-      const bool valid = column_valid(range, f);
-      const uint8_t* src = tile.w + (valid ? column_of(range, f) : 0) + (static_cast<long long>(step) * Stage::kRows + (lane >> 2)) * tile.n;
-#pragma unroll
-      for (int l = 0; l < Stage::kRows / 8; ++l) {
-        const int r = l * 8 + (lane >> 2);
-        copy_async<16>(at + (r * 4 + (f ^ ((r >> 1) & 3))) * 16, src + static_cast<long long>(l) * 8 * tile.n, valid);
-      }
-      if constexpr (SC) {  // two columns a lane
-        const bool scale_valid = column_valid(range, lane >> 3);
-        const bf16* scale = tile.w_scale + static_cast<long long>(step * 32 / p.sub) * tile.n + (scale_valid ? column_of(range, lane >> 3) + (lane & 7) * 2 : 0);
-        copy_async<4>(at + Stage::kScalesAt + lane * 4, scale, scale_valid);
+      next.valid = column_valid(next.range, lane & 3);
+      next.w = tile.w + (next.valid ? column_of(next.range, lane & 3) : 0) + (static_cast<long long>(begin) * kStepBytes + (lane >> 2)) * tile.n;
+      if (SC) {
+        next.scale_valid = column_valid(next.range, lane >> 3);
+        next.scale = tile.w_scale + (next.scale_valid ? column_of(next.range, lane >> 3) + (lane & 7) * 2 : 0);
       }
     } else {
-      const int k0 = step * Stage::kStepK + q * (Stage::kStepK / 4);
-      const bool valid = k0 < tile.k;
-#pragma unroll
-      for (int l = 0; l < 4; ++l) {  // fragment l / 2, rows g and g + 8
-        const uint8_t* src = tile.w + (column_of(range, l >> 1) + g + (l & 1) * 8) * code_pitch + (valid ? code_bytes<DT>(k0) : 0);
-        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, src, valid);
-      }
-      if constexpr (SC) {
-        if (lane < 16) {
-          const bf16* scale = tile.w_scale + static_cast<long long>(step * Stage::kStepK / p.sub) * tile.n + column_of(range, lane >> 3) + (lane & 7) * 2;
-          copy_async<4>(at + Stage::kScalesAt + lane * 4, scale, true);
-        }
-      }
+      next.w = tile.w + (column_of(next.range, 0) + g) * code_pitch + static_cast<long long>(begin) * kStepBytes + q * 4 * WORDS;
+      if (SC) next.scale = tile.w_scale + column_of(next.range, (lane >> 3) & 1) + (lane & 7) * 2;
     }
   };
-  auto copy_codes = [&](int i, int slot) {
-    const int step = begin + i * by;
-    const uint32_t at = ring_at + slot * Stage::kBytes + Stage::kWeights;
-    // NN int8: two words 16 K apart, one for each half of the instruction's K
-    const int k0 = step * Stage::kStepK + q * (NN && DT == 8 ? 4 : Stage::kStepK / 4);
+  auto start = [&]() {
+    next.range = range0;
+    next.i = next.slot = 0;
+    enter_range();
+  };
+  auto advance = [&]() {
+    if (++next.slot == kStages) next.slot = 0;
+    next.w += w_step;
+    if (++next.i == mine) {
+      next.i = 0;
+      ++next.range;
+      enter_range();
+    }
+  };
+  auto copy_weights = [&]() {
+    const uint32_t at = ring_at + next.slot * Stage::kBytes;
+    if constexpr (NN) {
+      // 16 bytes of row r and fragment f to place r * 4 + (f ^ (r / 2 % 4)): eight rows of a fragment on eight banks
+      const uint8_t* src = next.w;
+      const uint32_t to = at + ((lane >> 2) * 4 + ((lane & 3) ^ ((lane >> 3) & 3))) * 16;
+      // the last step may reach beyond K, which is a multiple of 32: by whole groups of eight rows
+      const int rows_left = static_cast<int>(code_pitch) - (begin + next.i * by) * kStepBytes;
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const bool valid = n * 8 + g < count && k0 < tile.k;
-      const uint8_t* src = tile.codes + (valid ? rows[n * 8 + g] * code_pitch + code_bytes<DT>(k0) : 0);
-      const uint32_t to = at + (n * 32 + lane) * Stage::kCodeBytes;
-      if constexpr (NN && DT == 8) {
-        copy_async<4>(to, src, valid);
-        copy_async<4>(to + 4, src + (valid ? 16 : 0), valid);
-      } else {
-        copy_async<Stage::kCodeBytes>(to, src, valid);
+      for (int l = 0; l < kStepBytes / 8; ++l, src += w_rows) {
+        const bool valid = next.valid && l * 8 < rows_left;
+        copy_async<16>(to + l * 512, valid ? src : tile.w, valid);
       }
+    } else {
+      const bool valid = (begin + next.i * by) * Stage::kStepK + q * (Stage::kStepK / 4) < tile.k;
+#pragma unroll
+      for (int l = 0; l < 4; ++l)  // fragment l / 2, rows g and g + 8
+        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, valid ? next.w + ((l & 1) ? w_rows : 0) + ((l & 2) ? w_frag : 0) : tile.w, valid);
     }
     if constexpr (SC) {
-      if (lane < kN * 8) {
-        const bool valid = lane < count;
-        const float* scale = tile.scales + (valid ? static_cast<long long>(rows[lane]) * tile.groups + step * Stage::kStepK / p.sub : 0);
-        copy_async<4>(ring_at + slot * Stage::kBytes + Stage::kRowScalesAt + lane * 4, scale, valid);
-      }
+      const long long group = static_cast<long long>((begin + next.i * by) * Stage::kStepK / p.sub) * tile.n;
+      if (NN || lane < 16) copy_async<4>(at + Stage::kScalesAt + lane * 4, next.scale + group, !NN || next.scale_valid);
+    }
+  };
+  const uint8_t* codes[kN];  // of this lane's tokens, at its first step
+  bool has_token[kN];
+  const float* row_scale = tile.scales;
+  auto enter_rows = [&]() {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      has_token[n] = n * 8 + g < count;
+      codes[n] = tile.codes + (has_token[n] ? rows[n * 8 + g] * code_pitch : 0) + static_cast<long long>(begin) * kStepBytes + q * 4 * WORDS;
+    }
+    if (SC && lane < count && lane < kN * 8) row_scale = tile.scales + static_cast<long long>(rows[lane]) * tile.groups;
+  };
+  auto copy_codes = [&]() {
+    const uint32_t at = ring_at + next.slot * Stage::kBytes;
+    const int step = begin + next.i * by, offset = next.i * by * kStepBytes;
+    const bool in_k = step * Stage::kStepK + q * (Stage::kStepK / 4) < tile.k;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const bool valid = in_k && has_token[n];
+      copy_async<4 * WORDS>(at + Stage::kWeights + (n * 32 + lane) * 4 * WORDS, valid ? codes[n] + offset : tile.codes, valid);
+    }
+    if constexpr (SC) {
+      if (lane < kN * 8) copy_async<4>(at + Stage::kRowScalesAt + lane * 4, row_scale + step * Stage::kStepK / p.sub, lane < count);
     }
   };
 
-  // the next step to copy
-  int ahead_range = range0, ahead_step = 0, ahead_slot = 0;
-  auto advance = [&]() {
-    if (++ahead_slot == kStages) ahead_slot = 0;
-    if (++ahead_step == mine) {
-      ahead_step = 0;
-      ++ahead_range;
-    }
-  };
+  start();
 #pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) {
-    if (mine > 0 && ahead_range < range1) copy_weights(ahead_range, ahead_step, ahead_slot);
-    advance();
+    if (mine > 0 && next.range < range1) {
+      copy_weights();
+      advance();
+    }
   }
   if constexpr (!SC)  // integers are added to what lies here
     for (int i = threadIdx.x; i < Stage::kSums; i += kMoeThreads) sums[i] = 0;
   before_codes();  // holds a barrier
-  ahead_range = range0, ahead_step = 0, ahead_slot = 0;
+  enter_rows();
+  start();
 #pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) {
-    if (mine > 0 && ahead_range < range1) copy_codes(ahead_step, ahead_slot);
+    if (mine > 0 && next.range < range1) {
+      copy_codes();
+      advance();
+    }
     copy_commit();
-    advance();
   }
 
   int slot = 0;
@@ -532,23 +568,48 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
       const uint8_t* stage = ring + slot * Stage::kBytes;
       uint32_t x[kN][4];
 #pragma unroll
-      for (int n = 0; n < kN; ++n) read_words<Stage::kCodeBytes / 4>(x[n], stage + Stage::kWeights + (n * 32 + lane) * Stage::kCodeBytes);
+      for (int n = 0; n < kN; ++n) read_words<WORDS>(x[n], stage + Stage::kWeights + (n * 32 + lane) * 4 * WORDS);
       if constexpr (NN) {
-        // lanes 0 .. 15 name the rows of one matrix, 16 .. 31 those of the other: two fragments (packed), or the two
-        // halves of K of one (int8)
         const uint32_t at = ring_at + slot * Stage::kBytes;
+        // Row rho = 4 q' + i of a matrix holds byte i of a word of lane q' of each quad, which is row
+        // q' * 4 * WORDS + (4 * word) + i of the stage.  Lanes 0 .. 15 name the rows of the first matrix, the others
+        // those of the second: the same word of two fragments (packed), or two words of one (int8).
+        const int rho = lane & 15, second = lane >> 4;
+        const int row0 = (rho >> 2) * 4 * WORDS + (rho & 3);
+        if constexpr (DT == 4) {
 #pragma unroll
-        for (int l = 0; l < (DT == 4 ? kFrags / 2 : kFrags); ++l) {
-          const int r = DT == 4 ? lane & 15 : lane, f = DT == 4 ? 2 * l + (lane >> 4) : l;
-          uint32_t m[4];
-          load_transposed(m, at + (r * 4 + (f ^ ((r >> 1) & 3))) * 16);
+          for (int word = 0; word < WORDS; ++word) {
+            const int r = row0 + 4 * word;
+            const uint32_t line = at + r * 64;
+            const int flip = (r >> 1) & 3;
+            uint32_t even_x[kN], odd_x[kN];
 #pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            if constexpr (DT == 4) {
-              mma_i8(acc[2 * l][n], even_codes(m[0]), even_codes(m[1]), odd_codes(m[0]), odd_codes(m[1]), even_codes(x[n][0]), odd_codes(x[n][0]));
-              mma_i8(acc[2 * l + 1][n], even_codes(m[2]), even_codes(m[3]), odd_codes(m[2]), odd_codes(m[3]), even_codes(x[n][0]), odd_codes(x[n][0]));
-            } else {
-              mma_i8(acc[l][n], m[0], m[1], m[2], m[3], x[n][0], x[n][1]);
+            for (int n = 0; n < kN; ++n) {
+              even_x[n] = even_codes(x[n][word]);
+              odd_x[n] = odd_codes(x[n][word]);
+            }
+#pragma unroll
+            for (int l = 0; l < kFrags / 2; ++l) {
+              uint32_t m[4];
+              load_transposed(m, line + (((2 * l + second) ^ flip) << 4));
+#pragma unroll
+              for (int n = 0; n < kN; ++n) mma_i8(acc[2 * l][n], even_codes(m[0]), even_codes(m[1]), odd_codes(m[0]), odd_codes(m[1]), even_x[n], odd_x[n]);
+#pragma unroll
+              for (int n = 0; n < kN; ++n) mma_i8(acc[2 * l + 1][n], even_codes(m[2]), even_codes(m[3]), odd_codes(m[2]), odd_codes(m[3]), even_x[n], odd_x[n]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int word = 0; word < WORDS; word += 2) {
+            const int r = row0 + 4 * (word + second);
+            const uint32_t line = at + r * 64;
+            const int flip = (r >> 1) & 3;
+#pragma unroll
+            for (int f = 0; f < kFrags; ++f) {
+              uint32_t m[4];
+              load_transposed(m, line + ((f ^ flip) << 4));
+#pragma unroll
+              for (int n = 0; n < kN; ++n) mma_i8(acc[f][n], m[0], m[1], m[2], m[3], x[n][word], x[n][word + 1]);
             }
           }
         }
@@ -573,60 +634,65 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
         }
       }
       if constexpr (SC) {
-        // the integers of a group of K end here: scaled and added up in fp64 (NT: a step lies in one group)
-        if (!NN || i + 1 == mine || ((begin + i + 1) * 32) % p.sub == 0) {
+        // the integers of a group of K end here: scaled and added up in fp64 (a step lies in one group)
+        if (i + 1 == mine || !NN || ((begin + i + 1) * Stage::kStepK) % p.sub == 0) {
           const bf16* w_scales = reinterpret_cast<const bf16*>(stage + Stage::kScalesAt);
           const float* row_scales = reinterpret_cast<const float*>(stage + Stage::kRowScalesAt);
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
             const float2 st = *reinterpret_cast<const float2*>(row_scales + n * 8 + 2 * q);
+            const double st0 = st.x, st1 = st.y;
 #pragma unroll
             for (int f = 0; f < kFrags; ++f)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float sw = to_f32(w_scales[f * 16 + g + (j >> 1) * 8]);
-                // a product of two bf16 numbers is exact in fp32
-                sum[f][n][j] = fma(static_cast<double>(DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]), static_cast<double>(((j & 1) ? st.y : st.x) * sw), sum[f][n][j]);
-                acc[f][n][j] = 0;
+              for (int h = 0; h < 2; ++h) {
+                const double sw = to_f32(w_scales[f * 16 + g + h * 8]);
+                const int a = acc[f][n][2 * h], b = acc[f][n][2 * h + 1];
+                sum[f][n][2 * h] = fma(exact_double(DT == 4 ? a >> 8 : a), st0 * sw, sum[f][n][2 * h]);
+                sum[f][n][2 * h + 1] = fma(exact_double(DT == 4 ? b >> 8 : b), st1 * sw, sum[f][n][2 * h + 1]);
+                acc[f][n][2 * h] = acc[f][n][2 * h + 1] = 0;
               }
           }
         }
       }
       __syncwarp();  // before the stage that was read a step ago is written again
-      if (ahead_range < range1) {
-        copy_weights(ahead_range, ahead_step, ahead_slot);
-        copy_codes(ahead_step, ahead_slot);
+      if (next.range < range1) {
+        copy_weights();
+        copy_codes();
         advance();
       }
       copy_commit();
       if (++slot == kStages) slot = 0;
     }
-    if constexpr (!SC) {
+    if constexpr (!SC) {  // exact integers, in any order
 #pragma unroll
       for (int f = 0; f < kFrags; ++f)
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) atomicAdd(sums + sum_place<kN>(half * kFrags + f, n, j, lane), DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]);
-    } else {
+      __syncthreads();
+    } else {  // one share after the other
+      for (int turn = 0; turn < kShares; ++turn) {
+        if (share == turn) {
 #pragma unroll
-      for (int f = 0; f < kFrags; ++f)
+          for (int f = 0; f < kFrags; ++f)
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+            for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sums[share * (kAllFrags * kN * 128) + sum_place<kN>(half * kFrags + f, n, j, lane)] = sum[f][n][j];
+              for (int j = 0; j < 4; ++j) {
+                Sum* at = sums + sum_place<kN>(half * kFrags + f, n, j, lane);
+                *at = turn == 0 ? sum[f][n][j] : *at + sum[f][n][j];
+              }
+        }
+        __syncthreads();
+      }
     }
-    __syncthreads();
     finish(range, [&](int c, int t, bool gate_part) -> Sum {
       const int column = c + (gate_part ? Stage::kCols / 2 : 0);
       const int place = sum_place<kN>(column >> 4, t >> 3, ((column >> 3) & 1) * 2 + (t & 1), (column & 7) * 4 + ((t & 7) >> 1));
-      Sum total = sums[place];
-      if constexpr (SC) {
-#pragma unroll
-        for (int w = 1; w < kShares; ++w) total += sums[w * (kAllFrags * kN * 128) + place];
-      } else {
-        sums[place] = 0;  // for the next range
-      }
+      const Sum total = sums[place];
+      if constexpr (!SC) sums[place] = 0;  // for the next range
       return total;
     });
     __syncthreads();
@@ -693,28 +759,24 @@ __global__ void __launch_bounds__(kMoeQuantThreads) moe_quantize_kernel(const Mo
   }
 }
 
-// The grid is as large as the device holds at once; the (expert, column range) units of the experts in use, whose
+// The grid is as large as the device holds at once; the units of work, (expert in use, part of K, column range), whose
 // number only the device knows, are divided evenly among its blocks, consecutive ones to a block.
 // kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
 template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
 __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_product_kernel(const MoeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int rows[kMaxN * 8];
+  using Sum = typename MoeSum<SC>::type;
   constexpr int kCols = NN ? 128 : 32, out_cols = kDown ? kCols : kCols / 2;
+  constexpr int kStepK = 4 * WORDS * (DT == 4 ? 8 : 4);
   if (!kDown) {
     grid_wait();
     grid_release();
   }
-  const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges;
+  const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges, splits = kDown ? p.down_splits : 1;
   // written by the select kernel, which had ended before the up/gate product let the next kernels start
   const int in_use = __ldcg(p.active);
-  if (kDown && in_use == 0) {  // no pair has an expert: nothing is added up
-    grid_wait();
-    for (long long i = blockIdx.x * kMoeThreads + threadIdx.x; i < static_cast<long long>(p.tokens) * p.hidden; i += gridDim.x * kMoeThreads)
-      p.out[i] = __float2bfloat16_rn(0.f);
-    return;
-  }
-  const long long units = static_cast<long long>(in_use) * ranges;
+  const long long units = static_cast<long long>(in_use) * splits * ranges;
   const long long unit0 = units * blockIdx.x / gridDim.x, unit1 = units * (blockIdx.x + 1) / gridDim.x;
   bool waited = !kDown;
   MoeTile tile;
@@ -723,11 +785,15 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   tile.groups = SC ? (tile.k + p.sub - 1) / p.sub : 1;
   tile.codes = kDown ? p.aq : p.xq;
   tile.scales = kDown ? p.as : p.xs;
+  const int steps = (tile.k + kStepK - 1) / kStepK;
+  const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
   const int c = threadIdx.x % out_cols;  // a thread's outputs are all of one column of a range
   for (long long unit = unit0; unit < unit1;) {
-    const int slot = static_cast<int>(unit / ranges), range0 = static_cast<int>(unit % ranges);
+    const int slot = static_cast<int>(unit / (static_cast<long long>(splits) * ranges)), split = static_cast<int>(unit / ranges % splits);
+    const int range0 = static_cast<int>(unit % ranges);
     const int range1 = static_cast<int>(min(static_cast<long long>(ranges), range0 + (unit1 - unit)));
     unit += range1 - range0;
+    const int step0 = static_cast<int>(static_cast<long long>(steps) * split / splits), step1 = static_cast<int>(static_cast<long long>(steps) * (split + 1) / splits);
     const int expert = __ldcg(p.active + 1 + 3 * slot), first = __ldcg(p.active + 2 + 3 * slot), count = __ldcg(p.active + 3 + 3 * slot);
     const int* list = p.pair_list + first;
     tile.w = (kDown ? p.w_down : p.w_up_gate) + static_cast<long long>(expert) * tile.n * code_bytes<DT>(tile.k);
@@ -746,17 +812,15 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
       auto finish = [&](int range, auto sum) {
         const int col = range * out_cols + c;
         if (col >= out_n) return;
-        const float scale = SC ? 1.f : to_f32(tile.w_scale[col]), gate_scale = SC || kDown ? 1.f : to_f32(tile.w_scale[p.inner + col]);
+        const float scale = SC || kDown ? 1.f : to_f32(tile.w_scale[col]), gate_scale = SC || kDown ? 1.f : to_f32(tile.w_scale[p.inner + col]);
         for (int t = threadIdx.x / out_cols; t < here; t += kMoeThreads / out_cols) {
-          const int pair = kDown ? rows[t] : __ldcg(list + done + t);
-          const double s = SC ? 1.0 : static_cast<double>(__ldcg(tile.scales + rows[t]));
           if (kDown) {
-            double y = static_cast<double>(sum(c, t, false));
-            if (!SC) y *= s * static_cast<double>(scale);
-            p.part[static_cast<long long>(pair) * p.hidden + col] = static_cast<float>(y) * __ldcg(p.pair_weight + pair);
+            static_cast<Sum*>(p.part)[(split * pairs + rows[t]) * p.hidden + col] = sum(c, t, false);
           } else {
+            const int pair = __ldcg(list + done + t);
             double up = static_cast<double>(sum(c, t, false)), gate = static_cast<double>(sum(c, t, true));
             if (!SC) {
+              const double s = static_cast<double>(__ldcg(tile.scales + rows[t]));
               up *= s * static_cast<double>(scale);
               gate *= s * static_cast<double>(gate_scale);
             }
@@ -765,7 +829,7 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         }
       };
       auto pass = [&](auto n) {
-        moe_pass<DT, NN, SC, WORDS, decltype(n)::value, kDown>(p, tile, range0, range1, rows, here, smem, before_codes, finish);
+        moe_pass<DT, NN, SC, WORDS, decltype(n)::value, kDown>(p, tile, range0, range1, step0, step1, rows, here, smem, before_codes, finish);
       };
       if (kMaxN == 1 || here <= 8) pass(std::integral_constant<int, 1>());
       else if (kMaxN == 2 || here <= 16) pass(std::integral_constant<int, kMaxN < 2 ? kMaxN : 2>());
@@ -773,36 +837,51 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     }
   }
   if (!waited) grid_wait();  // no kernel of the call ends before those in front of it
-  if constexpr (kDown) {
-    // The last block to finish a column range adds up the experts' shares for all tokens, in the order of the choices.
-    __shared__ int full[kMoeThreads];
-    __shared__ int full_count;
-    __threadfence();
-    for (long long base = unit0; base < unit1; base += kMoeThreads) {
-      __syncthreads();
-      if (threadIdx.x == 0) full_count = 0;
-      __syncthreads();
-      if (base + threadIdx.x < unit1) {
-        const int range = static_cast<int>((base + threadIdx.x) % ranges);
-        if (atomicAdd(p.done_down + range, 1) == in_use - 1) full[atomicAdd(&full_count, 1)] = range;
-        __threadfence();
-      }
-      __syncthreads();
-      for (int f = 0; f < full_count; ++f) {
-        const int col0 = full[f] * kCols;
-        for (int i = threadIdx.x; i < p.tokens * kCols; i += kMoeThreads) {
-          const int token = i / kCols, col = col0 + i % kCols;
-          if (col >= p.hidden) continue;
-          float y = 0.f;
-          for (int j = 0; j < p.top_k; ++j) {
-            const int pair = token * p.top_k + j;
-            if (__ldcg(p.pair_expert + pair) >= 0) y += __ldcg(p.part + static_cast<long long>(pair) * p.hidden + col);
-          }
-          p.out[static_cast<long long>(token) * p.hidden + col] = __float2bfloat16_rn(y);
-        }
-      }
-    }
+  if (kDown) grid_release();
+}
+
+// Adds up the parts of K, scales, and adds up the experts' shares of a token in the order of its choices.  A thread has
+// two columns of one token; what depends on the pair alone is read once a block.
+template <bool SC>
+__global__ void __launch_bounds__(128) moe_combine_kernel(const MoeParams p) {
+  using Sum = typename MoeSum<SC>::type;
+  using Sum2 = typename std::conditional<SC, double2, int2>::type;
+  __shared__ int expert[kMoeMaxTopK];
+  __shared__ float weight[kMoeMaxTopK], scale[kMoeMaxTopK];
+  const int token = blockIdx.y, col = (blockIdx.x * 128 + threadIdx.x) * 2;
+  grid_wait();
+  if (threadIdx.x < p.top_k) {
+    const int pair = token * p.top_k + threadIdx.x;
+    expert[threadIdx.x] = p.pair_expert[pair];
+    weight[threadIdx.x] = p.pair_weight[pair];
+    scale[threadIdx.x] = !SC && p.pair_expert[pair] >= 0 ? p.as[pair] : 1.f;
   }
+  __syncthreads();
+  if (col >= p.hidden) return;
+  const long long plane = static_cast<long long>(p.tokens) * p.top_k * p.hidden;
+  float total[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int j = 0; j < p.top_k; ++j) {
+    if (expert[j] < 0) continue;
+    const Sum* part = static_cast<const Sum*>(p.part) + static_cast<long long>(token * p.top_k + j) * p.hidden + col;
+    Sum2 sum = *reinterpret_cast<const Sum2*>(part);
+    for (int s = 1; s < p.down_splits; ++s) {
+      const Sum2 more = *reinterpret_cast<const Sum2*>(part + s * plane);
+      sum.x += more.x;
+      sum.y += more.y;
+    }
+    double y0 = static_cast<double>(sum.x), y1 = static_cast<double>(sum.y);
+    if (!SC) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[j]) * p.hidden + col);
+      y0 *= static_cast<double>(scale[j] * bf16_lo(w));  // a product of two bf16 numbers is exact in fp32
+      y1 *= static_cast<double>(scale[j] * bf16_hi(w));
+    }
+    total[0] += static_cast<float>(y0) * weight[j];
+    total[1] += static_cast<float>(y1) * weight[j];
+  }
+  bf16* out = p.out + static_cast<long long>(token) * p.hidden + col;
+  out[0] = __float2bfloat16_rn(total[0]);
+  out[1] = __float2bfloat16_rn(total[1]);
 }
 
 }  // namespace b200

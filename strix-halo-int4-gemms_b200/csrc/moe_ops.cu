@@ -42,6 +42,14 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->slots = static_cast<int>(pairs < static_cast<size_t>(m.experts) ? pairs : m.experts);
   p->up_ranges = (m.inner + down_cols / 2 - 1) / (down_cols / 2);
   p->down_ranges = (m.hidden + down_cols - 1) / down_cols;
+  // The down product divides K between blocks where there are fewer (expert, column range) units than would keep the
+  // blocks that the device holds (2 or 3 an SM) evenly busy, as long as each of a block's warps has four steps left.
+  const int step = m.layout == B200_LAYOUT_NN ? (m.dtype == B200_DTYPE_INT4 ? 64 : 32) : (m.dtype == B200_DTYPE_INT4 ? 128 : 64);
+  const int shares = m.layout == B200_LAYOUT_NN ? 4 : 8;
+  p->down_splits = 1;
+  while (p->down_splits < 8 && static_cast<long long>(p->slots) * p->down_ranges * p->down_splits < 1024 &&
+         m.inner >= static_cast<long long>(step) * shares * p->down_splits * 2 * 4)
+    p->down_splits *= 2;
   p->xq = reinterpret_cast<uint8_t*>(take(static_cast<size_t>(m.tokens) * m.hidden / per_byte));
   p->xs = reinterpret_cast<float*>(take(m.tokens * x_groups * 4));
   p->logits = reinterpret_cast<double*>(take(static_cast<size_t>(m.tokens) * m.experts * 8));
@@ -52,8 +60,7 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->act = reinterpret_cast<double*>(take(pairs * m.inner * 8));
   p->aq = reinterpret_cast<uint8_t*>(take(pairs * m.inner / per_byte));
   p->as = reinterpret_cast<float*>(take(pairs * a_groups * 4));
-  p->part = reinterpret_cast<float*>(take(pairs * m.hidden * 4));
-  p->done_down = reinterpret_cast<int*>(take(static_cast<size_t>(p->down_ranges) * 4));
+  p->part = take(pairs * p->down_splits * m.hidden * (m.subchannel ? 8 : 4));
   return at;
 }
 

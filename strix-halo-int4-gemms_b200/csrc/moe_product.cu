@@ -1,20 +1,33 @@
 // The expert layer's kernels for one code type: compiled with B200_MOE_BITS 4 and 8.
 #include "moe_launch.h"
 
+#include <atomic>
+
 namespace b200 {
 namespace {
 
 constexpr int kBits = B200_MOE_BITS;
 
+// Allows a kernel its dynamic shared memory (with the static part it may pass the 48 KB that need no permission), once
+// for each device: the attribute stays with the device's context.
+template <auto Kernel>
+int allow_shared_memory(int smem_bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (const cudaError_t err = cudaGetDevice(&device); err != cudaSuccess) return host_fail_cuda("cudaGetDevice", err);
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return 0;
+  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+  if (err != cudaSuccess) return host_fail_cuda("cudaFuncSetAttribute(max dynamic shared memory)", err);
+  done.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
 // A launch that may start while the kernel before it on the stream still runs (it waits for it by itself).
 template <typename... Args>
-int launch_dependent(void (*kernel)(Args...), int blocks, int threads, int smem_bytes, cudaStream_t stream, const MoeParams& p) {
-  if (smem_bytes > 48 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
-    if (err != cudaSuccess) return host_fail_cuda("cudaFuncSetAttribute(max dynamic shared memory)", err);
-  }
+int launch_dependent(void (*kernel)(Args...), dim3 blocks, int threads, int smem_bytes, cudaStream_t stream, const MoeParams& p) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.gridDim = blocks;
   config.blockDim = dim3(static_cast<unsigned>(threads));
   config.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
   config.stream = stream;
@@ -35,11 +48,12 @@ int launch_product(const MoeParams& p, int sm_count, cudaStream_t stream) {
   using Two = MoeStage<kBits, NN, SC, WORDS, kMaxN < 2 ? kMaxN : 2>;
   int smem = Stage::kSmemBytes > One::kSmemBytes ? Stage::kSmemBytes : One::kSmemBytes;
   smem = smem > Two::kSmemBytes ? smem : Two::kSmemBytes;
-  auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kDown>;
-  const long long units = static_cast<long long>(p.slots) * (kDown ? p.down_ranges : p.up_ranges);
+  constexpr auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kDown>;
+  if (int rc = allow_shared_memory<kernel>(smem); rc != 0) return rc;
+  const long long units = static_cast<long long>(p.slots) * (kDown ? p.down_ranges * p.down_splits : p.up_ranges);
   const int resident = smem <= 74 * 1024 && !SC && kMaxN != 4 ? 3 : smem <= 112 * 1024 ? 2 : 1;  // by shared memory and launch bounds
   const long long blocks = units < static_cast<long long>(resident) * sm_count ? units : static_cast<long long>(resident) * sm_count;
-  return launch_dependent(kernel, static_cast<int>(blocks), kMoeThreads, smem, stream, p);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), kMoeThreads, smem, stream, p);
 }
 
 // An expert can have at most as many rows as there are tokens (times the same expert given twice to a token, which
@@ -49,8 +63,9 @@ int launch_for_tokens(const MoeParams& p, int sm_count, cudaStream_t stream) {
   auto products = [&](auto max_n) {
     constexpr int kMaxN = decltype(max_n)::value;
     if (int rc = launch_product<NN, SC, WORDS, kMaxN, false>(p, sm_count, stream); rc != 0) return rc;
-    if (int rc = launch_dependent(moe_quantize_kernel<kBits>, p.tokens * p.top_k, kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
-    return launch_product<NN, SC, WORDS, kMaxN, true>(p, sm_count, stream);
+    if (int rc = launch_dependent(moe_quantize_kernel<kBits>, dim3(p.tokens * p.top_k), kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
+    if (int rc = launch_product<NN, SC, WORDS, kMaxN, true>(p, sm_count, stream); rc != 0) return rc;
+    return launch_dependent(moe_combine_kernel<SC>, dim3((p.hidden + 255) / 256, p.tokens), 128, 0, stream, p);
   };
   if (p.tokens <= 8) return products(std::integral_constant<int, 1>());
   if (p.tokens <= 16 || SC) return products(std::integral_constant<int, 2>());
@@ -65,17 +80,22 @@ int launch_moe_int4(const MoeParams& p, bool n_major, int sm_count, cudaStream_t
 int launch_moe_int8(const MoeParams& p, bool n_major, int sm_count, cudaStream_t stream) {
 #endif
   const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 7) / 8) : 0;
-  moe_route_kernel<kBits><<<p.tokens + 1 + logit_blocks, 256, 0, stream>>>(p);
+  moe_route_kernel<kBits><<<p.tokens + logit_blocks, 256, 0, stream>>>(p);
   if (const cudaError_t err = cudaGetLastError(); err != cudaSuccess) return host_fail_cuda("moe_swiglu launch", err);
   auto select = p.experts <= 64 ? moe_select_kernel<2> : p.experts <= 256 ? moe_select_kernel<8> : moe_select_kernel<32>;
-  if (int rc = launch_dependent(select, 1, 1024, 0, stream, p); rc != 0) return rc;
-  if (n_major) return p.sub ? launch_for_tokens<true, true, 4>(p, sm_count, stream) : launch_for_tokens<true, false, 4>(p, sm_count, stream);
+  if (int rc = launch_dependent(select, dim3(1), 1024, 0, stream, p); rc != 0) return rc;
+  // words of token codes that a lane takes at a step: as many as keep a step within a group of K (32 K a word of
+  // nibbles, 16 a word of bytes) and the ring's stages small
+  constexpr int kWord = kBits == 4 ? 32 : 16, kLeast = kBits == 4 ? 1 : 2;
+  if (n_major) {
+    if (!p.sub) return launch_for_tokens<true, false, 2>(p, sm_count, stream);
+    if (p.sub >= 2 * kWord) return launch_for_tokens<true, true, 2>(p, sm_count, stream);
+    return launch_for_tokens<true, true, kLeast>(p, sm_count, stream);
+  }
   if (!p.sub) return launch_for_tokens<false, false, 4>(p, sm_count, stream);
-  // K-major weights with scales for groups of K: a step stays within one group (32 K a word of nibbles, 16 a word of bytes)
-  constexpr int kWord = kBits == 4 ? 32 : 16;
   if (p.sub >= 4 * kWord) return launch_for_tokens<false, true, 4>(p, sm_count, stream);
-  if (kBits == 8 || p.sub == 2 * kWord) return launch_for_tokens<false, true, 2>(p, sm_count, stream);
-  return launch_for_tokens<false, true, kBits == 4 ? 1 : 2>(p, sm_count, stream);
+  if (p.sub >= 2 * kWord) return launch_for_tokens<false, true, 2>(p, sm_count, stream);
+  return launch_for_tokens<false, true, kLeast>(p, sm_count, stream);
 }
 
 }  // namespace b200
