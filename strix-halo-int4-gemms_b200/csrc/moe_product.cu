@@ -79,7 +79,7 @@ int launch_moe_int4(const MoeParams& p, bool n_major, int sm_count, cudaStream_t
 #else
 int launch_moe_int8(const MoeParams& p, bool n_major, int sm_count, cudaStream_t stream) {
 #endif
-  const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 7) / 8) : 0;
+  const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 3) / 4) : 0;
   moe_route_kernel<kBits><<<p.tokens + logit_blocks, 256, 0, stream>>>(p);
   if (const cudaError_t err = cudaGetLastError(); err != cudaSuccess) return host_fail_cuda("moe_swiglu launch", err);
   auto select = p.experts <= 64 ? moe_select_kernel<2> : p.experts <= 256 ? moe_select_kernel<8> : moe_select_kernel<32>;
