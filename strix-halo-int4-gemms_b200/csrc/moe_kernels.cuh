@@ -47,14 +47,14 @@ struct MoeParams {
   const bf16* s_down;
   bf16* out;                // [tokens, hidden]
   int tokens, hidden, inner, experts, top_k, sub;
-  int router_f32, ids_64, renormalize;
+  int router_f32, ids_64, renormalize, rows_a_pass;
   // scratch
   uint8_t* xq;              // [tokens, hidden bytes]
   float* xs;                // [tokens, groups of hidden]
   double* logits;           // [tokens, experts]
   int* pair_expert;         // [pairs], -1: no expert
   float* pair_weight;       // [pairs]
-  int* active;              // [0]: experts in use; then slots of {expert, first, count}
+  int* active;              // {experts in use, total cost}; then slots of {expert, first pair, pairs, cost of those before}
   int* pair_list;           // [pairs], by expert
   double* act;              // [pairs, inner]
   uint8_t* aq;              // [pairs, inner bytes]
@@ -62,6 +62,14 @@ struct MoeParams {
   void* part;               // [down_splits, pairs, hidden]: sums of the codes' products (int32), or scaled ones (fp64)
   int slots, up_ranges, down_ranges, down_splits;
 };
+
+// Relative time of a column range of an expert with `count` rows, by which work is divided among the blocks: a pass for up
+// to 8 rows is bound by the weights' bytes, one for more of them by its matrix instructions.
+__host__ __device__ constexpr int moe_pass_cost(int rows) { return rows <= 8 ? 14 : rows <= 16 ? 17 : rows <= 24 ? 21 : 26; }
+__device__ __forceinline__ int moe_cost(int count, int rows_a_pass) {
+  const int whole = count / rows_a_pass, rest = count - whole * rows_a_pass;
+  return whole * moe_pass_cost(rows_a_pass) + (rest > 0 ? moe_pass_cost(rest) : 0);
+}
 
 template <int DT>
 __device__ __forceinline__ long long code_bytes(long long k) { return DT == 4 ? k / 2 : k; }
@@ -194,17 +202,18 @@ __device__ __forceinline__ double logit_of_key(unsigned long long k) {
 // One block of 1024 threads.  A warp picks a token's experts one after the other: the largest logit that is left,
 // ties to the lowest index (a token whose logits are NaN gets the first experts and weights of NaN).  A lane keeps
 // PER logits, of experts lane, lane + 32, ...
-template <int PER>
-__global__ void __launch_bounds__(1024) moe_select_kernel(const MoeParams p) {
+template <int PER, int THREADS>
+__global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) {
   __shared__ int chosen[kMoeMaxPairs];
-  __shared__ int count[kMoeMaxExperts];
-  __shared__ int first[kMoeMaxExperts];
-  __shared__ int warp_sums[32];
+  __shared__ int count[PER * 32];
+  __shared__ int first[PER * 32];
+  __shared__ int2 warp_sums[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = p.tokens * p.top_k;
+  for (int e = threadIdx.x; e < PER * 32; e += THREADS) count[e] = 0;
   grid_wait();
   grid_release();
   if (p.router != nullptr) {
-    for (int t = warp; t < p.tokens; t += 32) {
+    for (int t = warp; t < p.tokens; t += THREADS / 32) {
       unsigned long long key[PER], mine = 0;  // lane j: the key of choice j
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -241,63 +250,75 @@ __global__ void __launch_bounds__(1024) moe_select_kernel(const MoeParams p) {
         for (int i = 0; i < PER; ++i)
           if (id == static_cast<unsigned>(lane + 32 * i)) key[i] = 0;
       }
+      if (lane < p.top_k) chosen[t * p.top_k + lane] = mine_id;
       const double logit = logit_of_key(mine), top = __shfl_sync(0xFFFFFFFFu, logit, 0);
       const double e = lane < p.top_k ? exp(logit - top) : 0.0;
       const double total = p.renormalize ? warp_reduce(e, SumOp()) : all;
       if (lane < p.top_k) {
-        chosen[t * p.top_k + lane] = mine_id;
-        p.pair_weight[t * p.top_k + lane] = static_cast<float>(e / total);
+        const float weight = static_cast<float>(e / total);
+        p.pair_weight[t * p.top_k + lane] = weight;
+        if (p.weights_out != nullptr) p.weights_out[t * p.top_k + lane] = weight;
       }
     }
   } else {
-    for (int i = threadIdx.x; i < pairs; i += 1024) {
+    for (int i = threadIdx.x; i < pairs; i += THREADS) {
       const long long id = p.ids_64 ? static_cast<const long long*>(p.ids_in)[i] : static_cast<const int*>(p.ids_in)[i];
       chosen[i] = id >= 0 && id < p.experts ? static_cast<int>(id) : -1;  // any other number: no expert
       p.pair_weight[i] = p.weights_in[i];
     }
   }
-  const int e = threadIdx.x;
-  count[e] = 0;
   __syncthreads();
-  int place = 0;
-  const int my_choice = threadIdx.x < pairs ? chosen[threadIdx.x] : -1;  // pairs <= 1024
-  if (my_choice >= 0) place = atomicAdd(&count[my_choice], 1);  // the order within an expert changes no result
-  __syncthreads();
-  // scan over the experts: pairs before (low half) and experts in use before (high half)
-  const int here = count[e] + (count[e] > 0 ? 1 << 16 : 0);
-  int sum = here;
+  constexpr int kPerThread = (kMoeMaxPairs + THREADS - 1) / THREADS;
+  int place[kPerThread];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-    if (lane >= o) sum += v;
+  for (int k = 0; k < kPerThread; ++k) {
+    const int i = threadIdx.x + k * THREADS;
+    place[k] = i < pairs && chosen[i] >= 0 ? atomicAdd(&count[chosen[i]], 1) : 0;  // the order within an expert changes no result
   }
-  if (lane == 31) warp_sums[warp] = sum;
   __syncthreads();
-  if (warp == 0) {
-    int s = warp_sums[lane];
+  // scan over the experts, THREADS at a time: pairs (low half) and experts in use (high half) before, and their cost
+  int2 carry = make_int2(0, 0);
+  for (int base = 0; base < PER * 32; base += THREADS) {
+    const int e = base + threadIdx.x, mine = e < PER * 32 ? count[e] : 0;
+    const int2 here = make_int2(mine + (mine > 0 ? 1 << 16 : 0), mine > 0 ? moe_cost(mine, p.rows_a_pass) : 0);
+    int2 sum = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xFFFFFFFFu, s, o);
-      if (lane >= o) s += v;
+      const int x = __shfl_up_sync(0xFFFFFFFFu, sum.x, o), y = __shfl_up_sync(0xFFFFFFFFu, sum.y, o);
+      if (lane >= o) {
+        sum.x += x;
+        sum.y += y;
+      }
     }
-    warp_sums[lane] = s;
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    int2 total = make_int2(0, 0);
+    for (int w = 0; w < THREADS / 32; ++w) {
+      const int2 other = warp_sums[w];
+      if (w < warp) {
+        sum.x += other.x;
+        sum.y += other.y;
+      }
+      total.x += other.x;
+      total.y += other.y;
+    }
+    if (mine > 0) {
+      const int before = carry.x + sum.x - here.x;
+      first[e] = before & 0xFFFF;
+      *reinterpret_cast<int4*>(p.active + 4 + 4 * (before >> 16)) = make_int4(e, before & 0xFFFF, mine, carry.y + sum.y - here.y);
+    }
+    carry.x += total.x;
+    carry.y += total.y;
+    __syncthreads();
   }
-  __syncthreads();
-  sum += (warp > 0 ? warp_sums[warp - 1] : 0) - here;
-  first[e] = sum & 0xFFFF;
-  if (count[e] > 0) {
-    int* slot = p.active + 1 + 3 * (sum >> 16);
-    slot[0] = e;
-    slot[1] = first[e];
-    slot[2] = count[e];
-  }
-  if (threadIdx.x == 0) p.active[0] = warp_sums[31] >> 16;
-  __syncthreads();
-  if (threadIdx.x < pairs) {
-    p.pair_expert[threadIdx.x] = my_choice;
-    if (my_choice >= 0) p.pair_list[first[my_choice] + place] = threadIdx.x;
-    if (p.ids_out != nullptr) p.ids_out[threadIdx.x] = my_choice;
-    if (p.weights_out != nullptr) p.weights_out[threadIdx.x] = p.pair_weight[threadIdx.x];
+  if (threadIdx.x == 0) *reinterpret_cast<int4*>(p.active) = make_int4(carry.x >> 16, carry.y, 0, 0);
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k) {
+    const int i = threadIdx.x + k * THREADS;
+    if (i >= pairs) break;
+    p.pair_expert[i] = chosen[i];
+    if (chosen[i] >= 0) p.pair_list[first[chosen[i]] + place[k]] = i;
+    if (p.ids_out != nullptr) p.ids_out[i] = chosen[i];
   }
 }
 
@@ -413,9 +434,9 @@ __device__ __forceinline__ int sum_place(int frag, int n, int j, int lane) {
 // Positions whose range does not exist are passed over.
 struct MoeOrder {
   int ranges, run, stride;
-  __device__ __forceinline__ MoeOrder(int n, long long per_block) {
+  __device__ __forceinline__ MoeOrder(int n, int per_block) {
     ranges = n;
-    run = static_cast<int>(max(1ll, min(static_cast<long long>(n), per_block)));
+    run = max(1, min(n, per_block));
     stride = (n + run - 1) / run;
   }
   __device__ __forceinline__ int positions() const { return run * stride; }
@@ -423,11 +444,13 @@ struct MoeOrder {
 };
 
 // Positions [pos0, pos1) and steps [step0, step1) of K of one expert for the `count` <= 8 kN tokens in `rows`.
-// `before_codes` runs between the first weight copies and the first use of `rows` and the codes; `finish(range, sum)` is
-// called by all threads with the sums of a range at hand: sum(c, t, gate) for its column c and token t.
-template <int DT, bool NN, bool SC, int WORDS, int kN, bool kDown, typename Before, typename Finish>
+// `before_codes` runs between the first weight copies and the first use of `rows` and the codes.  For every range all
+// threads call `begin(range)` before the products, `publish()` between them and a barrier, and then
+// `finish(range, begun, sum)` with the sums at hand: sum(c, t, gate) for its column c and token t.
+template <int DT, bool NN, bool SC, int WORDS, int kN, bool kDown, typename Before, typename Begin, typename Publish, typename Finish>
 __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile, const MoeOrder& order, int pos0, int pos1, int step0,
-                                         int step1, const int* rows, int count, uint8_t* smem, Before&& before_codes, Finish&& finish) {
+                                         int step1, const int* rows, int count, uint8_t* smem, Before&& before_codes, Begin&& begin_range,
+                                         Publish&& publish, Finish&& finish) {
   using Stage = MoeStage<DT, NN, SC, WORDS, kN>;
   using Sum = typename Stage::Sum;
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
@@ -573,6 +596,7 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
   for (int pos = pos0; pos < pos1; ++pos) {
     const int range = order.range(pos);
     if (range >= order.ranges) continue;
+    const auto begun = begin_range(range);
     int acc[kFrags][kN][4];
     double sum[SC ? kFrags : 1][SC ? kN : 1][4];
 #pragma unroll
@@ -687,6 +711,7 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
       copy_commit();
       if (++slot == kStages) slot = 0;
     }
+    publish();
     if constexpr (!SC) {  // exact integers, in any order
 #pragma unroll
       for (int f = 0; f < kFrags; ++f)
@@ -711,7 +736,7 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
         __syncthreads();
       }
     }
-    finish(range, [&](int c, int t, bool gate_part) -> Sum {
+    finish(range, begun, [&](int c, int t, bool gate_part) -> Sum {
       const int column = c + (gate_part ? Stage::kCols / 2 : 0);
       const int place = sum_place<kN>(column >> 4, t >> 3, ((column >> 3) & 1) * 2 + (t & 1), (column & 7) * 4 + ((t & 7) >> 1));
       const Sum total = sums[place];
@@ -724,10 +749,11 @@ __device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile
 }
 
 // Quantises the activations of one pair (fp64 in, as they were computed): what quantize_tokens does, with values that
-// are not exactly known in fp32, so that a code is settled against them where it has to be.
+// are not exactly known in fp32, so that a code is settled against them where it has to be.  The row is divided among
+// all threads, V pairs of values each, held in registers (V == 0: read again); or a group of values belongs to a warp.
 constexpr int kMoeQuantThreads = 512;
 
-template <int DT>
+template <int DT, int V>
 __global__ void __launch_bounds__(kMoeQuantThreads) moe_quantize_kernel(const MoeParams p) {
   constexpr double kTop = DT == 4 ? 7.0 : 127.0;
   constexpr int kWarps = kMoeQuantThreads / 32;
@@ -739,56 +765,117 @@ __global__ void __launch_bounds__(kMoeQuantThreads) moe_quantize_kernel(const Mo
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const double* row = p.act + static_cast<long long>(pair) * p.inner;
   uint8_t* codes = p.aq + static_cast<long long>(pair) * code_bytes<DT>(p.inner);
-  // the row by all warps, or a group of values by one
-  const int length = p.sub ? p.sub : p.inner, groups = p.sub ? (p.inner + p.sub - 1) / p.sub : 1, per_group = p.sub ? 1 : kWarps;
-  for (int group = p.sub ? warp : 0; group < groups; group += kWarps) {
-    const int c0 = group * length, c1 = min(c0 + length, p.inner);
-    const int begin = c0 + ((warp % per_group) * 32 + lane) * 2, stride = per_group * 64;
-    unsigned long long most = 0;
-#pragma unroll 4
-    for (int c = begin; c < c1; c += stride) {
-      const double2 v = *reinterpret_cast<const double2*>(row + c);
-      const unsigned long long a = __double_as_longlong(v.x) & 0x7FFFFFFFFFFFFFFFLL, b = __double_as_longlong(v.y) & 0x7FFFFFFFFFFFFFFFLL;
-      most = max(most, max(a, b));
-    }
-    most = warp_reduce(most, MaxOp());
-    if (per_group > 1) {  // one group: the barrier is met by all
-      if (lane == 0) warp_max[warp] = most;
-      __syncthreads();
-      most = warp_reduce(warp_max[lane % kWarps], MaxOp());
-    }
-    const float s = nonzero_scale(bf16_from_double(__longlong_as_double(most) / kTop));
-    if (begin == c0) p.as[static_cast<long long>(pair) * groups + group] = s;
-    const bool ordinary = scale_is_ordinary(s);
-    const float inv = __frcp_rn(s), delta = static_cast<float>(kTop) * 4.76837158203125e-7f;  // fp32 value, product: 3 roundings
-#pragma unroll 4
-    for (int c = begin; c < c1; c += stride) {
-      const double2 v = *reinterpret_cast<const double2*>(row + c);
-      uint32_t code[2];
+  auto largest = [](unsigned long long most, double2 v) {
+    const unsigned long long a = __double_as_longlong(v.x) & 0x7FFFFFFFFFFFFFFFLL, b = __double_as_longlong(v.y) & 0x7FFFFFFFFFFFFFFFLL;
+    return max(most, max(a, b));
+  };
+  auto scale_of = [&](unsigned long long most) { return nonzero_scale(bf16_from_double(__longlong_as_double(most) / kTop)); };
+  // Codes of two values; bit `bit` of `border` is set where one of them has to be settled.  (Settling them here would
+  // put a division into every step of an unrolled loop: code that runs once, and is fetched for longer than it runs.)
+  auto put = [&](int c, double2 v, float inv, uint32_t& border, int bit) {
+    const float delta = static_cast<float>(kTop) * 4.76837158203125e-7f;  // fp32 value, product: 3 roundings
+    const float x = static_cast<float>(v.x), y = static_cast<float>(v.y);
+    const uint32_t a = __float_as_uint(__fadd_rn(__fmaf_rn(x, inv, -delta), kRoundMagic)), b = __float_as_uint(__fadd_rn(__fmaf_rn(y, inv, -delta), kRoundMagic));
+    if (((a ^ __float_as_uint(__fadd_rn(__fmaf_rn(x, inv, delta), kRoundMagic))) | (b ^ __float_as_uint(__fadd_rn(__fmaf_rn(y, inv, delta), kRoundMagic)))) != 0)
+      border |= 1u << bit;
+    if (DT == 4) codes[c / 2] = static_cast<uint8_t>((a & 0xFu) | ((b & 0xFu) << 4));
+    else *reinterpret_cast<uint16_t*>(codes + c) = static_cast<uint16_t>((a & 0xFFu) | ((b & 0xFFu) << 8));
+  };
+  auto settle = [&](int c, float s) {
+    const double2 v = *reinterpret_cast<const double2*>(row + c);
+    uint32_t code[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const double exact = i ? v.y : v.x;
-        const float approx = static_cast<float>(exact);
-        code[i] = __float_as_uint(__fadd_rn(__fmaf_rn(approx, inv, -delta), kRoundMagic));
-        const uint32_t other = __float_as_uint(__fadd_rn(__fmaf_rn(approx, inv, delta), kRoundMagic));
-        if (!ordinary || code[i] != other) {
-          const double quotient = rint(exact / static_cast<double>(s));
-          code[i] = s < __int_as_float(0x7F800000) ? static_cast<uint32_t>(static_cast<int>(fmin(fmax(quotient, -kTop), kTop))) : 0u;
-        }
+    for (int i = 0; i < 2; ++i) {
+      const double quotient = rint((i ? v.y : v.x) / static_cast<double>(s));
+      code[i] = s < __int_as_float(0x7F800000) ? static_cast<uint32_t>(static_cast<int>(fmin(fmax(quotient, -kTop), kTop))) : 0u;
+    }
+    if (DT == 4) codes[c / 2] = static_cast<uint8_t>((code[0] & 0xFu) | ((code[1] & 0xFu) << 4));
+    else *reinterpret_cast<uint16_t*>(codes + c) = static_cast<uint16_t>((code[0] & 0xFFu) | ((code[1] & 0xFFu) << 8));
+  };
+  // the settling of the values c + 2 i stride that `border` names (all of them where the scale is not ordinary)
+  auto settle_all = [&](uint32_t border, int c, int step, int count, float s) {
+    if (!scale_is_ordinary(s)) border = 0xFFFFFFFFu >> (32 - count);
+#pragma unroll 1
+    for (; border != 0; border &= border - 1) {
+      const int i = __ffs(border) - 1;
+      settle(c + i * step, s);
+    }
+  };
+  if (p.sub) {
+    const int groups = (p.inner + p.sub - 1) / p.sub;
+    for (int group = warp; group < groups; group += kWarps) {
+      const int c0 = group * p.sub + lane * 2, c1 = min((group + 1) * p.sub, p.inner);
+      double2 v[4];  // up to 256 values
+      unsigned long long most = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = c0 + 64 * i < c1 ? *reinterpret_cast<const double2*>(row + c0 + 64 * i) : make_double2(0.0, 0.0);
+        most = largest(most, v[i]);
       }
-      if (DT == 4) codes[c / 2] = static_cast<uint8_t>((code[0] & 0xFu) | ((code[1] & 0xFu) << 4));
-      else *reinterpret_cast<uint16_t*>(codes + c) = static_cast<uint16_t>((code[0] & 0xFFu) | ((code[1] & 0xFFu) << 8));
+      const float s = scale_of(warp_reduce(most, MaxOp()));
+      if (lane == 0) p.as[static_cast<long long>(pair) * groups + group] = s;
+      const float inv = __frcp_rn(s);
+      uint32_t border = 0;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + 64 * i < c1) {
+          put(c0 + 64 * i, v[i], inv, border, i);
+          ++count;
+        }
+      if (count > 0) settle_all(border, c0, 64, count, s);
+    }
+    return;
+  }
+  const int c0 = threadIdx.x * 2, stride = kMoeQuantThreads * 2;
+  double2 v[V > 0 ? V : 1];
+  unsigned long long most = 0;
+  if (V > 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[i] = c0 + i * stride < p.inner ? *reinterpret_cast<const double2*>(row + c0 + i * stride) : make_double2(0.0, 0.0);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) most = largest(most, v[i]);
+  } else {
+#pragma unroll 4
+    for (int c = c0; c < p.inner; c += stride) most = largest(most, *reinterpret_cast<const double2*>(row + c));
+  }
+  most = warp_reduce(most, MaxOp());
+  if (lane == 0) warp_max[warp] = most;
+  __syncthreads();
+  const float s = scale_of(warp_reduce(warp_max[lane % kWarps], MaxOp()));
+  if (threadIdx.x == 0) p.as[pair] = s;
+  const float inv = __frcp_rn(s);
+  if (V > 0) {
+    uint32_t border = 0;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c0 + i * stride < p.inner) {
+        put(c0 + i * stride, v[i], inv, border, i);
+        ++count;
+      }
+    if (count > 0) settle_all(border, c0, stride, count, s);
+  } else {
+    for (int c = c0; c < p.inner; c += stride) {
+      uint32_t border = 0;
+      put(c, *reinterpret_cast<const double2*>(row + c), inv, border, 0);
+      settle_all(border, c, stride, 1, s);
     }
   }
 }
 
 // The grid is as large as the device holds at once; the units of work, (expert in use, part of K, column range), whose
-// number only the device knows, are divided evenly among its blocks, consecutive ones to a block.
+// number only the device knows, are divided among its blocks by their cost, consecutive ones to a block.
 // kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
 template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
 __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_product_kernel(const MoeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int rows[kMaxN * 8];
+  constexpr int kHead = 64;  // slots whose records are read at once
+  __shared__ int4 head[1 + kHead];
+  __shared__ int rows[kMaxN * 8], pair_of[kMaxN * 8];
+  __shared__ float row_scale[kMaxN * 8];
   using Sum = typename MoeSum<SC>::type;
   constexpr int kCols = NN ? 128 : 32, out_cols = kDown ? kCols : kCols / 2;
   constexpr int kStepK = 4 * WORDS * (DT == 4 ? 8 : 4);
@@ -798,11 +885,40 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   }
   const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges, splits = kDown ? p.down_splits : 1;
   // written by the select kernel, which had ended before the up/gate product let the next kernels start
-  const int in_use = __ldcg(p.active);
-  const MoeOrder order(ranges, static_cast<long long>(in_use) * splits * ranges / gridDim.x);
-  const int positions = order.positions();
-  const long long units = static_cast<long long>(in_use) * splits * positions;
-  const long long unit0 = units * blockIdx.x / gridDim.x, unit1 = units * (blockIdx.x + 1) / gridDim.x;
+  const int4* records = reinterpret_cast<const int4*>(p.active);
+  if (threadIdx.x < min(1 + kHead, 1 + p.slots)) head[threadIdx.x] = __ldcg(records + threadIdx.x);
+  __syncthreads();
+  auto record = [&](int slot) { return slot < kHead ? head[1 + slot] : __ldcg(records + 1 + slot); };
+  const int in_use = head[0].x, total_cost = head[0].y;
+  const unsigned units = static_cast<unsigned>(in_use) * splits * ranges;
+  const MoeOrder order(ranges, static_cast<int>(units / gridDim.x));
+  const int slot_units = splits * order.positions();
+  // The unit at which block b starts: the first whose cost lies at or behind b / blocks of the whole.
+  auto start_of = [&](unsigned b, int& slot, int& unit) {
+    const unsigned long long target = static_cast<unsigned long long>(total_cost) * slot_units * b / gridDim.x;
+    const unsigned cost = static_cast<unsigned>(target / slot_units);
+    int low = 0, high = in_use;  // the last slot that starts at or before the target
+    while (high - low > 1) {
+      const int middle = (low + high) / 2;
+      if (static_cast<unsigned>(record(middle).w) <= cost) low = middle;
+      else high = middle;
+    }
+    slot = low;
+    if (in_use == 0) {
+      unit = 0;
+      return;
+    }
+    const int4 r = record(low);
+    const unsigned each = moe_cost(r.z, kMaxN * 8);
+    unit = static_cast<int>(min(static_cast<unsigned long long>(slot_units), (target - static_cast<unsigned long long>(r.w) * slot_units + each - 1) / each));
+  };
+  int slot, unit, last_slot, last_unit;
+  start_of(blockIdx.x, slot, unit);
+  start_of(blockIdx.x + 1, last_slot, last_unit);
+  if (blockIdx.x + 1 == gridDim.x) {
+    last_slot = in_use;
+    last_unit = 0;
+  }
   bool waited = !kDown;
   MoeTile tile;
   tile.k = kDown ? p.inner : p.hidden;
@@ -813,51 +929,68 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   const int steps = (tile.k + kStepK - 1) / kStepK;
   const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
   const int c = threadIdx.x % out_cols;  // a thread's outputs are all of one column of a range
-  for (long long unit = unit0; unit < unit1;) {
-    const int slot = static_cast<int>(unit / (static_cast<long long>(splits) * positions)), split = static_cast<int>(unit / positions % splits);
-    const int pos0 = static_cast<int>(unit % positions);
-    const int pos1 = static_cast<int>(min(static_cast<long long>(positions), pos0 + (unit1 - unit)));
-    unit += pos1 - pos0;
+  while (slot < last_slot || (slot == last_slot && unit < last_unit)) {
+    if (unit >= slot_units) {
+      ++slot;
+      unit = 0;
+      continue;
+    }
+    const int split = unit / order.positions(), pos0 = unit % order.positions();
+    const int end = min(slot == last_slot ? last_unit : slot_units, (split + 1) * order.positions());
+    const int pos1 = pos0 + end - unit;
+    unit = end;
     const int step0 = static_cast<int>(static_cast<long long>(steps) * split / splits), step1 = static_cast<int>(static_cast<long long>(steps) * (split + 1) / splits);
-    const int expert = __ldcg(p.active + 1 + 3 * slot), first = __ldcg(p.active + 2 + 3 * slot), count = __ldcg(p.active + 3 + 3 * slot);
-    const int* list = p.pair_list + first;
-    tile.w = (kDown ? p.w_down : p.w_up_gate) + static_cast<long long>(expert) * tile.n * code_bytes<DT>(tile.k);
-    tile.w_scale = (kDown ? p.s_down : p.s_up_gate) + static_cast<long long>(expert) * tile.n * tile.groups;
-    for (int done = 0; done < count; done += kMaxN * 8) {
-      const int here = min(kMaxN * 8, count - done);
+    const int4 r = record(slot);  // {expert, first pair, pairs, ...}
+    const int* list = p.pair_list + r.y;
+    tile.w = (kDown ? p.w_down : p.w_up_gate) + static_cast<long long>(r.x) * tile.n * code_bytes<DT>(tile.k);
+    tile.w_scale = (kDown ? p.s_down : p.s_up_gate) + static_cast<long long>(r.x) * tile.n * tile.groups;
+    for (int done = 0; done < r.z; done += kMaxN * 8) {
+      const int here = min(kMaxN * 8, r.z - done);
+      float my_scale = 1.f;  // of a token; written for the others when a range is finished
       auto before_codes = [&]() {
         if (!waited) grid_wait();
         waited = true;
         if (threadIdx.x < here) {
-          const int pair = __ldcg(list + done + threadIdx.x);
-          rows[threadIdx.x] = kDown ? pair : pair / p.top_k;
+          const int pair = __ldcg(list + done + threadIdx.x), row = kDown ? pair : pair / p.top_k;
+          pair_of[threadIdx.x] = pair;
+          rows[threadIdx.x] = row;
+          if (!SC && !kDown) my_scale = __ldcg(tile.scales + row);
         }
         __syncthreads();
       };
-      auto finish = [&](int range, auto sum) {
+      // what a range needs besides its sums: read before the products
+      auto begin = [&](int range) {
+        const int col = range * out_cols + c;
+        float2 scale = make_float2(0.f, 0.f);
+        if (!SC && !kDown && col < out_n) scale = make_float2(to_f32(tile.w_scale[col]), to_f32(tile.w_scale[p.inner + col]));
+        return scale;
+      };
+      auto publish = [&]() {
+        if (!SC && !kDown && threadIdx.x < here) row_scale[threadIdx.x] = my_scale;
+      };
+      auto finish = [&](int range, float2 scale, auto sum) {
         const int col = range * out_cols + c;
         if (col >= out_n) return;
-        const float scale = SC || kDown ? 1.f : to_f32(tile.w_scale[col]), gate_scale = SC || kDown ? 1.f : to_f32(tile.w_scale[p.inner + col]);
         for (int t = threadIdx.x / out_cols; t < here; t += kMoeThreads / out_cols) {
           if (kDown) {
             static_cast<Sum*>(p.part)[(split * pairs + rows[t]) * p.hidden + col] = sum(c, t, false);
           } else {
-            const int pair = __ldcg(list + done + t);
             double up = static_cast<double>(sum(c, t, false)), gate = static_cast<double>(sum(c, t, true));
             if (!SC) {
-              const double s = static_cast<double>(__ldcg(tile.scales + rows[t]));
-              up *= s * static_cast<double>(scale);
-              gate *= s * static_cast<double>(gate_scale);
+              const float s = row_scale[t];
+              up *= static_cast<double>(s * scale.x);  // a product of two bf16 numbers is exact in fp32
+              gate *= static_cast<double>(s * scale.y);
             }
-            p.act[static_cast<long long>(pair) * p.inner + col] = up * gate / (1.0 + exp(-gate));
+            p.act[static_cast<long long>(pair_of[t]) * p.inner + col] = up * gate / (1.0 + exp(-gate));
           }
         }
       };
       auto pass = [&](auto n) {
-        moe_pass<DT, NN, SC, WORDS, decltype(n)::value, kDown>(p, tile, order, pos0, pos1, step0, step1, rows, here, smem, before_codes, finish);
+        moe_pass<DT, NN, SC, WORDS, decltype(n)::value, kDown>(p, tile, order, pos0, pos1, step0, step1, rows, here, smem, before_codes, begin, publish, finish);
       };
       if (kMaxN == 1 || here <= 8) pass(std::integral_constant<int, 1>());
       else if (kMaxN == 2 || here <= 16) pass(std::integral_constant<int, kMaxN < 2 ? kMaxN : 2>());
+      else if (here <= 24) pass(std::integral_constant<int, kMaxN < 3 ? kMaxN : 3>());
       else pass(std::integral_constant<int, kMaxN>());
     }
   }
@@ -885,24 +1018,43 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(const MoeParams p) {
   if (col >= p.hidden) return;
   const long long plane = static_cast<long long>(p.tokens) * p.top_k * p.hidden;
   float total[2] = {0.f, 0.f};
-#pragma unroll 4
-  for (int j = 0; j < p.top_k; ++j) {
-    if (expert[j] < 0) continue;
-    const Sum* part = static_cast<const Sum*>(p.part) + static_cast<long long>(token * p.top_k + j) * p.hidden + col;
-    Sum2 sum = *reinterpret_cast<const Sum2*>(part);
+  for (int j0 = 0; j0 < p.top_k; j0 += 4) {  // four choices at once
+    Sum2 sum[4];
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = min(j0 + k, p.top_k - 1);
+      const bool valid = j0 + k < p.top_k && expert[j] >= 0;
+      sum[k].x = sum[k].y = 0;
+      w[k] = 0u;
+      if (valid) {
+        sum[k] = *reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + static_cast<long long>(token * p.top_k + j) * p.hidden + col);
+        if (!SC) w[k] = *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[j]) * p.hidden + col);
+      }
+    }
     for (int s = 1; s < p.down_splits; ++s) {
-      const Sum2 more = *reinterpret_cast<const Sum2*>(part + s * plane);
-      sum.x += more.x;
-      sum.y += more.y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = min(j0 + k, p.top_k - 1);
+        if (j0 + k < p.top_k && expert[j] >= 0) {
+          const Sum2 more = *reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + s * plane + static_cast<long long>(token * p.top_k + j) * p.hidden + col);
+          sum[k].x += more.x;
+          sum[k].y += more.y;
+        }
+      }
     }
-    double y0 = static_cast<double>(sum.x), y1 = static_cast<double>(sum.y);
-    if (!SC) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[j]) * p.hidden + col);
-      y0 *= static_cast<double>(scale[j] * bf16_lo(w));  // a product of two bf16 numbers is exact in fp32
-      y1 *= static_cast<double>(scale[j] * bf16_hi(w));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = j0 + k;
+      if (j >= p.top_k || expert[j] < 0) continue;
+      double y0 = static_cast<double>(sum[k].x), y1 = static_cast<double>(sum[k].y);
+      if (!SC) {
+        y0 *= static_cast<double>(scale[j] * bf16_lo(w[k]));  // a product of two bf16 numbers is exact in fp32
+        y1 *= static_cast<double>(scale[j] * bf16_hi(w[k]));
+      }
+      total[0] += static_cast<float>(y0) * weight[j];
+      total[1] += static_cast<float>(y1) * weight[j];
     }
-    total[0] += static_cast<float>(y0) * weight[j];
-    total[1] += static_cast<float>(y1) * weight[j];
   }
   bf16* out = p.out + static_cast<long long>(token) * p.hidden + col;
   out[0] = __float2bfloat16_rn(total[0]);

@@ -55,7 +55,7 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->logits = reinterpret_cast<double*>(take(static_cast<size_t>(m.tokens) * m.experts * 8));
   p->pair_expert = reinterpret_cast<int*>(take(pairs * 4));
   p->pair_weight = reinterpret_cast<float*>(take(pairs * 4));
-  p->active = reinterpret_cast<int*>(take((1 + 3 * static_cast<size_t>(p->slots)) * 4));
+  p->active = reinterpret_cast<int*>(take((1 + static_cast<size_t>(p->slots)) * 16));
   p->pair_list = reinterpret_cast<int*>(take(pairs * 4));
   p->act = reinterpret_cast<double*>(take(pairs * m.inner * 8));
   p->aq = reinterpret_cast<uint8_t*>(take(pairs * m.inner / per_byte));

@@ -1,6 +1,7 @@
 // The expert layer's kernels for one code type: compiled with B200_MOE_BITS 4 and 8.
 #include "moe_launch.h"
 
+#include <algorithm>
 #include <atomic>
 
 namespace b200 {
@@ -46,8 +47,8 @@ int launch_product(const MoeParams& p, int sm_count, cudaStream_t stream) {
   // the most that any number of token groups up to kMaxN asks for
   using One = MoeStage<kBits, NN, SC, WORDS, 1>;
   using Two = MoeStage<kBits, NN, SC, WORDS, kMaxN < 2 ? kMaxN : 2>;
-  int smem = Stage::kSmemBytes > One::kSmemBytes ? Stage::kSmemBytes : One::kSmemBytes;
-  smem = smem > Two::kSmemBytes ? smem : Two::kSmemBytes;
+  using Three = MoeStage<kBits, NN, SC, WORDS, kMaxN < 3 ? kMaxN : 3>;
+  constexpr int smem = std::max({Stage::kSmemBytes, One::kSmemBytes, Two::kSmemBytes, Three::kSmemBytes});
   constexpr auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kDown>;
   if (int rc = allow_shared_memory<kernel>(smem); rc != 0) return rc;
   const long long units = static_cast<long long>(p.slots) * (kDown ? p.down_ranges * p.down_splits : p.up_ranges);
@@ -60,30 +61,38 @@ int launch_product(const MoeParams& p, int sm_count, cudaStream_t stream) {
 // only takes more passes): the fewer rows a pass has to be ready for, the more registers are left for other blocks.
 template <bool NN, bool SC, int WORDS>
 int launch_for_tokens(const MoeParams& p, int sm_count, cudaStream_t stream) {
-  auto products = [&](auto max_n) {
+  auto products = [&](auto max_n) -> int {
     constexpr int kMaxN = decltype(max_n)::value;
     if (int rc = launch_product<NN, SC, WORDS, kMaxN, false>(p, sm_count, stream); rc != 0) return rc;
-    if (int rc = launch_dependent(moe_quantize_kernel<kBits>, dim3(p.tokens * p.top_k), kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
+    constexpr int kRow = kMoeQuantThreads * 2;
+    auto quantize = SC || p.inner <= 2 * kRow ? moe_quantize_kernel<kBits, 2> : p.inner <= 14 * kRow ? moe_quantize_kernel<kBits, 14> : moe_quantize_kernel<kBits, 0>;
+    if (int rc = launch_dependent(quantize, dim3(p.tokens * p.top_k), kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
     if (int rc = launch_product<NN, SC, WORDS, kMaxN, true>(p, sm_count, stream); rc != 0) return rc;
     return launch_dependent(moe_combine_kernel<SC>, dim3((p.hidden + 255) / 256, p.tokens), 128, 0, stream, p);
   };
-  if (p.tokens <= 8) return products(std::integral_constant<int, 1>());
-  if (p.tokens <= 16 || SC) return products(std::integral_constant<int, 2>());
+  if (p.rows_a_pass == 8) return products(std::integral_constant<int, 1>());
+  if (p.rows_a_pass == 16) return products(std::integral_constant<int, 2>());
   return products(std::integral_constant<int, SC ? 2 : 4>());
 }
 
 }  // namespace
 
 #if B200_MOE_BITS == 4
-int launch_moe_int4(const MoeParams& p, bool n_major, int sm_count, cudaStream_t stream) {
+int launch_moe_int4(const MoeParams& params, bool n_major, int sm_count, cudaStream_t stream) {
 #else
-int launch_moe_int8(const MoeParams& p, bool n_major, int sm_count, cudaStream_t stream) {
+int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStream_t stream) {
 #endif
+  MoeParams p = params;
+  p.rows_a_pass = p.tokens <= 8 ? 8 : p.tokens <= 16 || p.sub ? 16 : 32;
   const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 3) / 4) : 0;
   moe_route_kernel<kBits><<<p.tokens + logit_blocks, 256, 0, stream>>>(p);
   if (const cudaError_t err = cudaGetLastError(); err != cudaSuccess) return host_fail_cuda("moe_swiglu launch", err);
-  auto select = p.experts <= 64 ? moe_select_kernel<2> : p.experts <= 256 ? moe_select_kernel<8> : moe_select_kernel<32>;
-  if (int rc = launch_dependent(select, dim3(1), 1024, 0, stream, p); rc != 0) return rc;
+  // experts <= 64, 256, 1024: logits a lane keeps; a warp for each token, as far as 32 go
+  const bool wide = p.tokens > 8 || p.experts > 256;
+  auto select = p.experts <= 64 ? (wide ? moe_select_kernel<2, 1024> : moe_select_kernel<2, 256>)
+                : p.experts <= 256 ? (wide ? moe_select_kernel<8, 1024> : moe_select_kernel<8, 256>)
+                                   : moe_select_kernel<32, 1024>;
+  if (int rc = launch_dependent(select, dim3(1), wide ? 1024 : 256, 0, stream, p); rc != 0) return rc;
   // words of token codes that a lane takes at a step: as many as keep a step within a group of K (32 K a word of
   // nibbles, 16 a word of bytes) and the ring's stages small
   constexpr int kWord = kBits == 4 ? 32 : 16, kLeast = kBits == 4 ? 1 : 2;
