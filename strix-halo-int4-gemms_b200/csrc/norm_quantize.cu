@@ -12,7 +12,7 @@ int launch_norm_quantize_bf16(const NormQuantizeCall& c) {
 #endif
   for_bool(c.weight_f32, [&](auto weight_f32) {
     using W = std::conditional_t<decltype(weight_f32)::value, float, bf16>;
-    for_row_shape(c.cols, c.wide, [&](auto tpr, auto v, auto aligned) {
+    for_row_shape<4>(c.rows, c.cols, c.wide, [&](auto tpr, auto v, auto aligned) {
       constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
       for_bool(c.bits == 4, [&](auto four) {
         layer_norm_quantize_kernel<NormX, W, TPR, V, decltype(four)::value ? 4 : 8, decltype(aligned)::value>

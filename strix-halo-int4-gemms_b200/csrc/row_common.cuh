@@ -24,6 +24,11 @@ struct Raw8<bf16> {
   uint32_t w[4];
   __device__ __forceinline__ float get(int i) const { return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]); }
   __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0u; }
+  __device__ __forceinline__ void set(const bf16 (&e)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = static_cast<uint32_t>(__bfloat16_as_ushort(e[2 * i])) | (static_cast<uint32_t>(__bfloat16_as_ushort(e[2 * i + 1])) << 16);
+  }
   template <bool kAligned>
   __device__ __forceinline__ void load(const bf16* row, long long at, long long cols) {
     if (kAligned) {
@@ -49,6 +54,10 @@ template <>
 struct Raw8<float> {
   float f[8];
   __device__ __forceinline__ float get(int i) const { return f[i]; }
+  __device__ __forceinline__ void set(const float (&e)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = e[i];
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = 0.f;
@@ -103,12 +112,58 @@ __device__ __forceinline__ void store8(float* row, long long at, long long cols,
   }
 }
 
+// Where thread t of the TPR threads of a row has its group v of eight values: at (v * TPR + t) * 8, by wide loads; or,
+// where those cannot be used, at v * 8 * TPR + t and every TPR-th from there, so that narrow loads of a warp are
+// neighbours.
+template <int TPR, bool kAligned>
+struct Columns {
+  int thread;
+  long long cols;
+  __device__ __forceinline__ long long first(int v) const { return (static_cast<long long>(v) * TPR + thread) * 8; }
+  __device__ __forceinline__ long long at(int v, int i) const {
+    return kAligned ? first(v) + i : static_cast<long long>(v) * 8 * TPR + i * TPR + thread;
+  }
+  __device__ __forceinline__ bool has(int v, int i) const { return kAligned ? first(v) < cols : at(v, i) < cols; }
+  template <typename T>
+  __device__ __forceinline__ Raw8<T> load(const T* row, int v) const {
+    Raw8<T> r;
+    if (kAligned) {
+      r.template load<true>(row, first(v), cols);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = has(v, i) ? row[at(v, i)] : T(0.f);
+      r.set(e);
+    }
+    return r;
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int v, const float (&f)[8]) const {
+    if (kAligned) {
+      store8<true>(row, first(v), cols, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (has(v, i)) row[at(v, i)] = static_cast<T>(f[i]);
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------------------
 // reductions over the threads of a row: one warp (TPR == 32) or one block (TPR threads)
 // ---------------------------------------------------------------------------------------------------------------
 struct SumOp {
   template <typename V>
   __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+// NaN if one of the two is; the sizes of both.
+__device__ __forceinline__ float max_size(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+struct MaxSizeOp {
+  __device__ __forceinline__ float operator()(float a, float b) const { return max_size(a, b); }
 };
 struct MaxOp {
   template <typename V>
@@ -179,13 +234,17 @@ __device__ __forceinline__ float bf16_from_double(double v) {
 __device__ __forceinline__ float nonzero_scale(float s) { return s == 0.f ? 1.f : s; }
 
 // bf16(amax / top) of a bf16 amax given by its bit pattern (NaN patterns are above infinity's, so that a row with
-// a NaN gets a NaN scale).  The quotient of an 8-bit significand and 7 or 127 is never close to a tie of two bf16
-// numbers without being one, so rounding it to fp32 first changes nothing.
+// a NaN gets a NaN scale).  A tie of two bf16 numbers is an odd multiple of 2^-9 of a power of two; 7 or 127 times
+// that has more than eight significant bits, so the quotient never is one, and it is at least 2^-17 (relative) away from
+// all of them: a product with the rounded 1 / top rounds to the same bf16 number.
 template <int BITS>
 __device__ __forceinline__ float scale_of_bf16(uint32_t amax_bits) {
-  const float top = BITS == 4 ? 7.f : 127.f;
-  return nonzero_scale(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(amax_bits << 16), top))));
+  const float per_top = BITS == 4 ? 1.f / 7.f : 1.f / 127.f;
+  return nonzero_scale(__bfloat162float(__float2bfloat16_rn(__uint_as_float(amax_bits << 16) * per_top)));
 }
+
+// 1 / s to within 2^-22, for ordinary scales
+__device__ __forceinline__ float about_inverse(float s) { return __fdividef(1.f, s); }
 
 constexpr float kRoundMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to the nearest even integer, left in the low bits
 
@@ -194,20 +253,19 @@ __device__ __forceinline__ bool scale_is_ordinary(float s) { return s >= 7.9e-31
 
 // round_half_even(x / s) of bf16 x and s, by multiplication.  x / s = (mx / ms) 2^j with significands below 256:
 // it is a tie n + 1/2 or, |2^(j+1) mx - (2n+1) ms| being a whole number from j = -1 on and ms < 256, at least 1 / 1020 away
-// from every tie, and it is at most 128.  The products with 1 / s made 2^-20 smaller and larger (1.3e-4 at 128) therefore round to one integer, which is the answer, or, at a tie, to
-// its two neighbours, of which the even one is.  Two multiply-adds instead of a division (which needs about nine
-// instructions): the loop is bound by instructions otherwise.
+// from every tie, and it is at most 128.  The products with 1 / s made 2^-20 smaller and larger (1.5e-4 at 128) therefore
+// round to one integer, which is the answer, or, at a tie, to its two neighbours.  Both carry kRoundMagic; their sum
+// has steps of two, so that it rounds to the even neighbour, and its last bits are the code's.  Three instructions on
+// the multiply-add pipe instead of a division's nine: the kernels are bound by instructions.
 struct ExactQuotient {
   float low, high;
   __device__ __forceinline__ explicit ExactQuotient(float s) {
-    const float inv = __frcp_rn(s);
+    const float inv = about_inverse(s);
     low = inv * (1.f - 9.5367431640625e-7f);
     high = inv * (1.f + 9.5367431640625e-7f);
   }
   __device__ __forceinline__ uint32_t code(float x) const {
-    const uint32_t a = __float_as_uint(__fmaf_rn(x, low, kRoundMagic));
-    const uint32_t b = __float_as_uint(__fmaf_rn(x, high, kRoundMagic));
-    return (a & 1u) ? b : a;
+    return __float_as_uint(__fadd_rn(__fmaf_rn(x, low, kRoundMagic), __fmaf_rn(x, high, kRoundMagic)));
   }
 };
 
@@ -220,33 +278,54 @@ __device__ __forceinline__ uint32_t code_by_division(float x, float s) {
   return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(q, -top), top)));
 }
 
-// Eight codes (low bits of each word) to memory: 4 bytes of nibbles or 8 bytes.
+// Eight codes (low bits of each word), packed: 4 bytes of nibbles or 8 bytes.
+template <int BITS>
+struct CodeWords {
+  using type = uint2;
+  __device__ __forceinline__ static uint2 pack(const uint32_t (&c)[8]) {
+    return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+  }
+};
+template <>
+struct CodeWords<4> {
+  using type = uint32_t;
+  __device__ __forceinline__ static uint32_t pack(const uint32_t (&c)[8]) {
+    // bytes of even and of odd values, then their low nibbles side by side
+    const uint32_t even = __byte_perm(__byte_perm(c[0], c[2], 0x0040), __byte_perm(c[4], c[6], 0x0040), 0x5410);
+    const uint32_t odd = __byte_perm(__byte_perm(c[1], c[3], 0x0040), __byte_perm(c[5], c[7], 0x0040), 0x5410);
+    return (even & 0x0F0F0F0Fu) | ((odd << 4) & 0xF0F0F0F0u);
+  }
+};
+
 template <int BITS, bool kAligned>
-__device__ __forceinline__ void store_codes(uint8_t* row, long long at, long long cols, const uint32_t (&c)[8]) {
+__device__ __forceinline__ void store_packed(uint8_t* row, long long at, long long cols, typename CodeWords<BITS>::type w) {
   if (at >= cols) return;
   if (BITS == 4) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (c[i] & 0xFu) << (4 * i);
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(&w);
     if (kAligned) {
-      *reinterpret_cast<uint32_t*>(row + at / 2) = w;
+      *reinterpret_cast<uint32_t*>(row + at / 2) = v;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (at + 2 * i < cols) row[at / 2 + i] = static_cast<uint8_t>(w >> (8 * i));
+        if (at + 2 * i < cols) row[at / 2 + i] = static_cast<uint8_t>(v >> (8 * i));
     }
   } else {
+    const uint32_t* v = reinterpret_cast<const uint32_t*>(&w);
     if (kAligned) {
-      uint2 w;
-      w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-      w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-      *reinterpret_cast<uint2*>(row + at) = w;
+      *reinterpret_cast<uint2*>(row + at) = make_uint2(v[0], v[BITS == 8 ? 1 : 0]);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (at + i < cols) row[at + i] = static_cast<uint8_t>(c[i]);
+        if (at + i < cols) row[at + i] = static_cast<uint8_t>(v[BITS == 8 ? i >> 2 : 0] >> (8 * (i & 3)));
     }
   }
+}
+
+// Eight codes (low bits of each word) to memory: 4 bytes of nibbles or 8 bytes.
+template <int BITS, bool kAligned>
+__device__ __forceinline__ void store_codes(uint8_t* row, long long at, long long cols, const uint32_t (&c)[8]) {
+  store_packed<BITS, kAligned>(row, at, cols, CodeWords<BITS>::pack(c));
 }
 
 }  // namespace b200

@@ -1,11 +1,16 @@
 // Kernels that go over rows of values once: the quantiser with a scale for each token, layer norm, layer norm
 // with the quantiser behind it, and layer norm's backward pass.  All of them are bound by HBM on large inputs.
 //
-// One row belongs to a warp (TPR == 32, up to 1024 values) or to a block of TPR threads; a thread holds V groups
-// of eight consecutive values in registers, group v of thread t at (v * TPR + t) * 8, so that a row is read once
-// and a warp's load covers consecutive bytes.  V == 0 is the form for rows that no block can hold: the same code,
-// reading the row again (from L2) for every pass over it.
+// One row belongs to a warp (TPR == 32) or to a block of TPR threads; a thread holds V groups of eight values in
+// registers, so that a row is read once.  V == 0 is the form for rows that no block can hold: the same code, reading
+// the row again (from L2) for every pass over it.  What is done once for a row (reductions, scales, addresses) costs some
+// 100 instructions a thread, as much as ten values: many values a thread (V = 8) where rows are many, few (V = 1) where
+// they are too few to fill the device (quantize_tokens of 32768 x 2048: 48 us with 16 values a thread, see below).
 #pragma once
+
+#include <cooperative_groups.h>
+
+#include <cstring>
 
 #include "row_common.cuh"
 
@@ -107,25 +112,33 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, long long cols, float eps) {
   __shared__ float scratch[2][TPR / 32];
   const float inv_cols = 1.f / static_cast<float>(cols);
+  const Columns<TPR, kAligned> column{RowPlace<TPR>::thread(), cols};
+  const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
-    const RowValues<T, TPR, V, kAligned> x(src + r * cols, cols);
+    const T* row = src + r * cols;
+    Raw8<T> held[V > 0 ? V : 1];
+    if (V > 0) {
+#pragma unroll
+      for (int v = 0; v < (V > 0 ? V : 1); ++v) held[v] = column.load(row, v);
+    }
+    auto value = [&](int v) { return V > 0 ? held[V > 0 ? v : 0] : column.load(row, v); };
     float sum = 0.f;
 #pragma unroll
-    for (int v = 0; v < x.count(); ++v) {
-      const Raw8<T> raw = x.get(v);
+    for (int v = 0; v < count; ++v) {
+      const Raw8<T> raw = value(v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += raw.get(i);
     }
     const float mean = row_reduce<TPR>(sum, SumOp(), scratch[0]) * inv_cols;
     float square = 0.f;
 #pragma unroll
-    for (int v = 0; v < x.count(); ++v) {
-      const Raw8<T> raw = x.get(v);
-      const long long at = x.at(v);
+    for (int v = 0; v < count; ++v) {
+      const Raw8<T> raw = value(v);
+      if (kAligned && !column.has(v, 0)) continue;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float d = raw.get(i) - mean;
-        if (at + i < cols) square = __fmaf_rn(d, d, square);
+        if (kAligned || column.has(v, i)) square = __fmaf_rn(d, d, square);
       }
     }
     const float rstd = rsqrtf(row_reduce<TPR>(square, SumOp(), scratch[1]) * inv_cols + eps);
@@ -134,17 +147,16 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
       rstd_out[r] = rstd;
     }
 #pragma unroll
-    for (int v = 0; v < x.count(); ++v) {
-      const Raw8<T> raw = x.get(v);
-      const long long at = x.at(v);
-      Raw8<W> w, b;
-      w.template load<kAligned>(weight, at, cols);
-      if (bias != nullptr) b.template load<kAligned>(bias, at, cols);
+    for (int v = 0; v < count; ++v) {
+      const Raw8<T> raw = value(v);
+      const Raw8<W> w = column.load(weight, v);
+      Raw8<W> b;
+      if (bias != nullptr) b = column.load(bias, v);
       else b.zero();
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = __fmaf_rn((raw.get(i) - mean) * rstd, w.get(i), b.get(i));
-      store8<kAligned>(y + r * cols, at, cols, out);
+      column.store(y + r * cols, v, out);
     }
   }
 }
@@ -156,9 +168,11 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 // would otherwise go to the one or the other with the order of a sum.  The statistics are sums in fp64.  The
 // values are computed in fp32, where they are off by at most E = 2^-21 (|t| + |b|), t = (x - mean) rstd w (four
 // roundings of 2^-24 each, and room); |t| <= amax + |b|, so E <= 2^-21 (amax + 2 max|b|) for a whole group.  If
-// q - E/s and q + E/s round to one integer, that is the code; otherwise (once in some 10^4 values) the value is
-// computed again in fp64.  The scale is settled in the same way: where amax / top is within its error of a tie of
-// two bf16 numbers, the group's maximum is found again in fp64.
+// q - E/s and q + E/s round to one integer, that is the code; otherwise (once in some 10^4 values) the eight values
+// of the thread are computed again in fp64.  The scale is settled in the same way: where amax / top is within its error
+// of a tie of two bf16 numbers, the group's maximum is found again in fp64.  Both are loops that read their values
+// again, out of the way of the code that runs always.
+// The kernel is bound by its instructions, not by HBM.
 // ---------------------------------------------------------------------------------------------------------------
 struct NormExact {
   double mean, rstd;
@@ -173,37 +187,70 @@ __device__ __forceinline__ bool near_bf16_tie(float v, float error) {
   return !(fabsf(v - tie) > error);
 }
 
+// The largest size of up to eight exact values from `at` on.
+template <typename T, typename W>
+__device__ __noinline__ double exact_size(const T* row, const W* weight, const W* bias, long long at, long long cols, const NormExact& exact) {
+  double most = 0.0;
+  for (int i = 0; i < 8 && at + i < cols; ++i)
+    most = fmax(most, fabs(exact.value(to_f32(row[at + i]), to_f32(weight[at + i]), bias != nullptr ? to_f32(bias[at + i]) : 0.f)));
+  return most;
+}
+
+// Eight codes from `at` on, from exact values; zero where the scale is not finite and behind the row.
+template <typename T, typename W, int BITS>
+__device__ __noinline__ unsigned long long exact_codes(const T* row, const W* weight, const W* bias, long long at, long long cols,
+                                                       const NormExact& exact, float s) {
+  const double top = BITS == 4 ? 7.0 : 127.0;
+  unsigned long long packed = 0;
+  if (!(s < __int_as_float(0x7F800000))) return 0;
+  for (int i = 0; i < 8 && at + i < cols; ++i) {
+    const double q = rint(exact.value(to_f32(row[at + i]), to_f32(weight[at + i]), bias != nullptr ? to_f32(bias[at + i]) : 0.f) / static_cast<double>(s));
+    const unsigned long long code = static_cast<unsigned long long>(static_cast<int>(fmin(fmax(q, -top), top))) & (BITS == 4 ? 0xFull : 0xFFull);
+    packed |= code << (BITS * i);
+  }
+  return packed;
+}
+
 template <typename T, typename W, int TPR, int V, int BITS, bool kAligned>
 __global__ void __launch_bounds__(RowPlace<TPR>::kThreads)
 layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias,
                            uint8_t* __restrict__ codes, bf16* __restrict__ scales, long long rows, long long cols, int sub,
                            double inv_cols, double eps) {
-  __shared__ double scratch_d[2 * (TPR / 32)];
-  __shared__ uint32_t scratch_m[2 * (TPR / 32)];
+  __shared__ double scratch_d[2][2 * (TPR / 32)];
+  __shared__ float scratch_m[2 * (TPR / 32)];
   __shared__ double scratch_x[TPR / 32];
+  constexpr int kHeld = V > 0 ? V : 1;
   constexpr float kTop = BITS == 4 ? 7.f : 127.f;
   constexpr float kError = 4.76837158203125e-7f;  // 2^-21
   const long long pitch = BITS == 4 ? (cols + 1) / 2 : cols;
   const int lanes = sub >> 3;
   const long long groups = sub ? (cols + sub - 1) / sub : 1;
-  for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
-    const RowValues<T, TPR, V, kAligned> x(src + r * cols, cols);
+  const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
+  auto place = [&](int v) { return (static_cast<long long>(v) * TPR + RowPlace<TPR>::thread()) * 8; };
+  auto read_affine = [&](int v, Raw8<W>& w, Raw8<W>& b) {
+    w.template load<kAligned>(weight, place(v), cols);
+    if (bias != nullptr) b.template load<kAligned>(bias, place(v), cols);
+    else b.zero();
+  };
+  int turn = 0;
+  for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step(), turn ^= 1) {
+    const T* row = src + r * cols;
+    const RowValues<T, TPR, V, kAligned> x(row, cols);
     // sums of x - shift and of its square; bf16 values need no shift (8 bits of significand against fp64's 53)
-    const float shift = sizeof(T) == 4 ? to_f32(src[r * cols]) : 0.f;
+    const float shift = sizeof(T) == 4 ? to_f32(row[0]) : 0.f;
     double s1 = 0.0, s2 = 0.0;
 #pragma unroll
-    for (int v = 0; v < x.count(); ++v) {
+    for (int v = 0; v < count; ++v) {
       const Raw8<T> raw = x.get(v);
-      const long long at = x.at(v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         double d = static_cast<double>(raw.get(i));
-        if (sizeof(T) == 4) d = at + i < cols ? d - static_cast<double>(shift) : 0.0;
+        if (sizeof(T) == 4) d = place(v) + i < cols ? d - static_cast<double>(shift) : 0.0;
         s1 += d;
         s2 = fma(d, d, s2);
       }
     }
-    row_reduce2<TPR>(s1, s2, SumOp(), SumOp(), scratch_d);
+    row_reduce2<TPR>(s1, s2, SumOp(), SumOp(), scratch_d[turn]);
     NormExact exact;
     // the mean with one step of refinement: a row of equal values has that value as its mean, and no variance
     double off = s1 * inv_cols;
@@ -222,113 +269,86 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
     const float mean_lo = static_cast<float>(exact.mean - static_cast<double>(mean_hi));
     const float rstd = static_cast<float>(exact.rstd);
 
-    // amax (as bits: NaN is above infinity) and max |b|
-    uint32_t amax = 0, bmax = 0;
-    float s = 1.f, delta = 0.f;
-    bool ordinary = false;
-    auto norm8 = [&](const Raw8<T>& raw, long long at, Raw8<W>& w, Raw8<W>& b, float (&out)[8]) {
-      w.template load<kAligned>(weight, at, cols);
-      if (bias != nullptr) b.template load<kAligned>(bias, at, cols);
-      else b.zero();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        out[i] = __fmaf_rn(((raw.get(i) - mean_hi) - mean_lo) * rstd, w.get(i), b.get(i));
-        if (!kAligned && at + i >= cols) out[i] = 0.f;
-        amax = max(amax, __float_as_uint(out[i]) & 0x7FFFFFFFu);
-        bmax = max(bmax, __float_as_uint(b.get(i)) & 0x7FFFFFFFu);
-      }
-    };
-    // bf16(amax / top), and the half-width of the border zones in codes.  `settle`: the scale has to be found from
-    // the exact maximum.
-    auto scale_from = [&](bool& settle) {
-      const float most = __uint_as_float(amax), error = kError * (most + 2.f * __uint_as_float(bmax));
-      const float quotient = __fdiv_rn(most, kTop);
-      s = nonzero_scale(__bfloat162float(__float2bfloat16_rn(quotient)));
-      ordinary = scale_is_ordinary(s);
-      delta = error * __frcp_rn(s) + kTop * kError;
-      settle = most < __int_as_float(0x7F800000) && most > 0.f && near_bf16_tie(quotient, error);
-    };
-
-    if (!lanes) {
-      float out[8];
-      Raw8<W> w, b;
-#pragma unroll
-      for (int v = 0; v < x.count(); ++v)
-        if (x.at(v) < cols) norm8(x.get(v), x.at(v), w, b, out);
-      row_reduce2<TPR>(amax, bmax, MaxOp(), MaxOp(), scratch_m);
-      bool settle;
-      scale_from(settle);
-      if (settle) {  // the same for all threads of the row
-        double most = 0.0;
-        for (int v = 0; v < x.count(); ++v) {
-          const long long at = x.at(v);
-          const Raw8<T> raw = x.get(v);
-          if (at >= cols) continue;
-          w.template load<kAligned>(weight, at, cols);
-          if (bias != nullptr) b.template load<kAligned>(bias, at, cols);
-          else b.zero();
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (at + i < cols) most = fmax(most, fabs(exact.value(raw.get(i), w.get(i), b.get(i))));
-        }
-        most = row_reduce<TPR>(most, MaxOp(), scratch_x);
-        s = nonzero_scale(bf16_from_double(most / static_cast<double>(kTop)));
-        if (TPR > 32) __syncthreads();  // scratch_x may be used again by the next row
-      }
-      if (RowPlace<TPR>::thread() == 0) scales[r] = __float2bfloat16_rn(s);
-    }
-
-    const float inv = __frcp_rn(s);
-#pragma unroll
-    for (int v = 0; v < x.count(); ++v) {
-      const long long at = x.at(v);
+    auto norm8 = [&](int v, float (&out)[8], float& amax, float& bmax) {
       const Raw8<T> raw = x.get(v);
       Raw8<W> w, b;
-      float out[8];
-      w.zero();
-      b.zero();
-      if (lanes) {
-        amax = bmax = 0;
+      read_affine(v, w, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        // behind the row w and b are zero, but a row that is not finite would leave NaN there
+        out[i] = __fmaf_rn(((raw.get(i) - mean_hi) - mean_lo) * rstd, w.get(i), b.get(i));
+        if ((kAligned ? place(v) : place(v) + i) >= cols) out[i] = 0.f;
+        amax = max_size(amax, out[i]);
+        bmax = max_size(bmax, b.get(i));
       }
-      if (at < cols) norm8(raw, at, w, b, out);
-      float inv_group = inv;
-      if (lanes) {
-        amax = warp_reduce(amax, MaxOp(), lanes);
-        bmax = warp_reduce(bmax, MaxOp(), lanes);
-        bool settle;
-        scale_from(settle);
-        if (__any_sync(0xFFFFFFFFu, settle)) {
-          double most = 0.0;
-          if (at < cols)
-            for (int i = 0; i < 8; ++i)
-              if (at + i < cols) most = fmax(most, fabs(exact.value(raw.get(i), w.get(i), b.get(i))));
-          most = warp_reduce(most, MaxOp(), lanes);
-          if (settle) s = nonzero_scale(bf16_from_double(most / static_cast<double>(kTop)));
-        }
-        inv_group = __frcp_rn(s);
-        if ((threadIdx.x & (lanes - 1)) == 0 && at < cols) scales[r * groups + at / sub] = __float2bfloat16_rn(s);
-      }
-      if (at >= cols) continue;
+    };
+    float s = 1.f, delta = 0.f, inv = 1.f;
+    bool ordinary = true;
+    // bf16(amax / top) and the half-width of the border zones in codes; true if the scale has to be found from the
+    // exact maximum
+    auto scale_from = [&](float amax, float bmax) {
+      const float error = kError * (amax + 2.f * bmax), quotient = amax * (1.f / kTop);
+      s = nonzero_scale(__bfloat162float(__float2bfloat16_rn(quotient)));
+      ordinary = scale_is_ordinary(s);
+      inv = about_inverse(s);
+      delta = error * inv + kTop * kError;
+      return amax < __int_as_float(0x7F800000) && amax > 0.f && near_bf16_tie(quotient, error);
+    };
+    auto settled = [&](double most) {
+      s = nonzero_scale(bf16_from_double(most / static_cast<double>(kTop)));
+      inv = about_inverse(s);
+    };
+    auto put = [&](int v, const float (&out)[8]) {
+      const long long at = place(v);
+      if (at >= cols) return;
       uint32_t c[8], border = ordinary ? 0u : 1u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        c[i] = __float_as_uint(__fadd_rn(__fmaf_rn(out[i], inv_group, -delta), kRoundMagic));
-        border |= c[i] ^ __float_as_uint(__fadd_rn(__fmaf_rn(out[i], inv_group, delta), kRoundMagic));
+        c[i] = __float_as_uint(__fadd_rn(__fmaf_rn(out[i], inv, -delta), kRoundMagic));
+        border |= c[i] ^ __float_as_uint(__fadd_rn(__fmaf_rn(out[i], inv, delta), kRoundMagic));
       }
+      typename CodeWords<BITS>::type packed = CodeWords<BITS>::pack(c);
       if (border) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (at + i >= cols || !(s < __int_as_float(0x7F800000))) {
-            c[i] = 0u;  // outside the row, or a row that is not finite
-          } else {
-            const double q = rint(exact.value(raw.get(i), w.get(i), b.get(i)) / static_cast<double>(s));
-            c[i] = static_cast<uint32_t>(static_cast<int>(fmin(fmax(q, -static_cast<double>(kTop)), static_cast<double>(kTop))));
-          }
-        }
+        const unsigned long long exactly = exact_codes<T, W, BITS>(row, weight, bias, at, cols, exact, s);
+        memcpy(&packed, &exactly, sizeof(packed));
       }
-      store_codes<BITS, kAligned>(codes + r * pitch, at, cols, c);
+      store_packed<BITS, kAligned>(codes + r * pitch, at, cols, packed);
+    };
+
+    float out[kHeld][8];
+    if (!lanes) {
+      float amax = 0.f, bmax = 0.f;
+#pragma unroll
+      for (int v = 0; v < count; ++v) norm8(v, out[V > 0 ? v : 0], amax, bmax);
+      row_reduce2<TPR>(amax, bmax, MaxSizeOp(), MaxSizeOp(), scratch_m);
+      if (scale_from(amax, bmax)) {  // the same for all threads of the row
+        double most = 0.0;
+        for (int v = 0; v < count; ++v) most = fmax(most, exact_size<T, W>(row, weight, bias, place(v), cols, exact));
+        most = row_reduce<TPR>(most, MaxOp(), scratch_x);
+        settled(most);
+      }
+      if (RowPlace<TPR>::thread() == 0) scales[r] = __float2bfloat16_rn(s);
+#pragma unroll
+      for (int v = 0; v < count; ++v) {
+        float again = 0.f, unused = 0.f;
+        if (V == 0) norm8(v, out[0], again, unused);
+        put(v, out[V > 0 ? v : 0]);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < count; ++v) {
+        float amax = 0.f, bmax = 0.f;
+        norm8(v, out[0], amax, bmax);
+        amax = warp_reduce(amax, MaxSizeOp(), lanes);
+        bmax = warp_reduce(bmax, MaxSizeOp(), lanes);
+        const bool settle = scale_from(amax, bmax);
+        if (__any_sync(0xFFFFFFFFu, settle)) {
+          const double most = warp_reduce(exact_size<T, W>(row, weight, bias, place(v), cols, exact), MaxOp(), lanes);
+          if (settle) settled(most);
+        }
+        if ((threadIdx.x & (lanes - 1)) == 0 && place(v) < cols) scales[r * groups + place(v) / sub] = __float2bfloat16_rn(s);
+        put(v, out[0]);
+      }
     }
   }
 }
@@ -336,149 +356,159 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
 // ---------------------------------------------------------------------------------------------------------------
 // layer norm's backward pass, with h = (x - mean) rstd and g = dy w:
 //   dx = rstd (g - mean(g) - h mean(g h)),   dw = sum over rows of dy h,   db = sum over rows of dy.
-// A thread keeps its eight columns for all of its block's rows, so the sums over rows stay in registers (or, for
-// wide rows, in shared memory) and x and dy are read once.  Each block leaves one row of partial sums;
-// column_sums_kernel adds those in a fixed order: no atomics, the same bits on every run.
-// The next row is read while the present one is reduced.
+// A thread keeps its columns for all of its rows, so the sums over rows stay in registers and x and dy are read once.
+// A block has several groups of TPR threads, each with rows of its own (and a barrier of its own); the sums of the groups
+// are added up in shared memory, each block leaves one row of partial sums, and column_sums_kernel adds those in a fixed
+// order: no atomics, the same bits on every run.  The next row is read while the present one is reduced.
+// Rows of more than 8192 values belong to a cluster of two blocks, half a row each, which exchange their sums through
+// distributed shared memory.
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, typename W, int TPR, bool kAligned>
-__global__ void __launch_bounds__(RowPlace<TPR>::kThreads, TPR == 1024 ? 1 : (TPR == 32 ? 3 : 768 / TPR))
+template <int TPR, int CLUSTER>
+struct BwdShape {
+  static constexpr int kThreads = TPR < 512 ? 512 : TPR;
+  static constexpr int kGroups = kThreads / TPR;  // rows at once (by half a row for CLUSTER == 2)
+};
+
+// Barrier of one group of a block.
+template <int TPR>
+__device__ __forceinline__ void group_barrier(int group) {
+  if (TPR > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+}
+
+template <typename T, typename W, int TPR, int V, int CLUSTER, bool kAligned>
+__global__ void __launch_bounds__(BwdShape<TPR, CLUSTER>::kThreads)
 layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
                       float* __restrict__ partial, long long rows, long long cols) {
-  __shared__ float scratch[2][2 * (TPR / 32)];
-  __shared__ float across[TPR == 32 ? 8 * 256 : 1];
+  using Shape = BwdShape<TPR, CLUSTER>;
+  constexpr int kWarps = TPR / 32, kGroups = Shape::kGroups, kBlockCols = TPR * V * 8;
+  __shared__ float2 scratch[2][kGroups][kWarps];
+  __shared__ float2 from_peer[2];
+  extern __shared__ float across[];  // [kBlockCols], where there are groups to be added up
+  const int group = threadIdx.x / TPR, thread = threadIdx.x % TPR;
+  const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
+  const long long unit = blockIdx.x / CLUSTER, step = static_cast<long long>(gridDim.x / CLUSTER) * kGroups;
+  // this block's columns: all, or the half `rank` (the first half is kBlockCols wide)
+  const long long col0 = static_cast<long long>(rank) * kBlockCols;
+  const Columns<TPR, kAligned> column{thread, CLUSTER > 1 ? max(0ll, min(cols - col0, static_cast<long long>(kBlockCols))) : cols};
+  src += col0;
+  dy += col0;
+  dx += col0;
   const float inv_cols = 1.f / static_cast<float>(cols);
-  const long long at = RowPlace<TPR>::thread() * 8LL;
-  float w[8], dw[8], db[8];
-  {
-    Raw8<W> raw;
-    raw.template load<kAligned>(weight, at, cols);
+  Raw8<W> w[V];
+  float dw[V][8], db[V][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      w[i] = raw.get(i);
-      dw[i] = db[i] = 0.f;
-    }
+  for (int v = 0; v < V; ++v) {
+    w[v] = column.load(weight + col0, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[v][i] = db[v][i] = 0.f;
   }
-  Raw8<T> next_x, next_dy;
+  Raw8<T> next_x[V], next_dy[V];
   float next_mean = 0.f, next_rstd = 0.f;
-  long long r = RowPlace<TPR>::first();
   auto fetch = [&](long long row) {
-    next_x.template load<kAligned>(src + row * cols, at, cols);
-    next_dy.template load<kAligned>(dy + row * cols, at, cols);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      next_x[v] = column.load(src + row * cols, v);
+      next_dy[v] = column.load(dy + row * cols, v);
+    }
     next_mean = __ldg(mean_in + row);
     next_rstd = __ldg(rstd_in + row);
   };
+  long long r = unit * kGroups + group;
   if (r < rows) fetch(r);
   int turn = 0;
-  for (; r < rows; r += RowPlace<TPR>::step(), turn ^= 1) {
-    const Raw8<T> x = next_x, d = next_dy;
+  for (; r < rows; r += step, turn ^= 1) {
+    Raw8<T> x[V], d[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      x[v] = next_x[v];
+      d[v] = next_dy[v];
+    }
     const float mean = next_mean, rstd = next_rstd;
-    if (r + RowPlace<TPR>::step() < rows) fetch(r + RowPlace<TPR>::step());
-    float sg = 0.f, sgh = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float h = (x.get(i) - mean) * rstd, g = d.get(i) * w[i];
-      sg += g;
-      sgh = __fmaf_rn(g, h, sgh);
-      dw[i] = __fmaf_rn(d.get(i), h, dw[i]);
-      db[i] += d.get(i);
-    }
-    row_reduce2<TPR>(sg, sgh, SumOp(), SumOp(), scratch[turn]);
-    const float mg = sg * inv_cols, mgh = sgh * inv_cols;
-    float out[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float h = (x.get(i) - mean) * rstd;
-      out[i] = rstd * (d.get(i) * w[i] - mg - h * mgh);
-    }
-    store8<kAligned>(dx + r * cols, at, cols, out);
-  }
-  float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * cols;
-  if (TPR == 32) {  // eight warps with the same columns
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int warp = threadIdx.x >> 5;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) across[warp * 256 + i * 32 + (threadIdx.x & 31)] = half ? db[i] : dw[i];
-      __syncthreads();
-      const int col = threadIdx.x;
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum += across[k * 256 + (col & 7) * 32 + (col >> 3)];
-      if (col < cols) mine[half * cols + col] = sum;
-      __syncthreads();
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (at + i < cols) {
-        mine[at + i] = dw[i];
-        mine[cols + at + i] = db[i];
-      }
-    }
-  }
-}
-
-// The same for rows of up to 16384 values: two groups of eight a thread, the sums over rows in shared memory
-// (8 bytes a column), where each thread touches its own columns only.
-template <typename T, typename W, bool kAligned>
-__global__ void __launch_bounds__(1024)
-layer_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
-                           const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
-                           float* __restrict__ partial, long long rows, long long cols) {
-  constexpr int TPR = 1024, V = 2;
-  extern __shared__ float sums[];  // [2][V][8][1024]: value i of group v of thread t at ((v * 8 + i) * 1024 + t)
-  __shared__ float scratch[2][2 * (TPR / 32)];
-  const float inv_cols = 1.f / static_cast<float>(cols);
-  float* sum_w = sums + threadIdx.x;
-  float* sum_b = sums + V * 8 * TPR + threadIdx.x;
-#pragma unroll
-  for (int k = 0; k < V * 8; ++k) sum_w[k * TPR] = sum_b[k * TPR] = 0.f;
-  int turn = 0;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
-    const RowValues<T, TPR, V, kAligned> x(src + r * cols, cols);
-    const RowValues<T, TPR, V, kAligned> d(dy + r * cols, cols);
-    const float mean = __ldg(mean_in + r), rstd = __ldg(rstd_in + r);
+    if (r + step < rows) fetch(r + step);
     float sg = 0.f, sgh = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      Raw8<W> w;
-      w.template load<kAligned>(weight, x.at(v), cols);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = d.held[v].get(i), h = (x.held[v].get(i) - mean) * rstd, g = e * w.get(i);
+        const float e = d[v].get(i), h = (x[v].get(i) - mean) * rstd, g = e * w[v].get(i);
         sg += g;
         sgh = __fmaf_rn(g, h, sgh);
-        sum_w[(v * 8 + i) * TPR] = __fmaf_rn(e, h, sum_w[(v * 8 + i) * TPR]);
-        sum_b[(v * 8 + i) * TPR] += e;
+        dw[v][i] = __fmaf_rn(e, h, dw[v][i]);
+        db[v][i] += e;
       }
     }
-    row_reduce2<TPR>(sg, sgh, SumOp(), SumOp(), scratch[turn]);
+    sg = warp_reduce(sg, SumOp());
+    sgh = warp_reduce(sgh, SumOp());
+    if (TPR > 32) {
+      if ((thread & 31) == 0) scratch[turn][group][thread >> 5] = make_float2(sg, sgh);
+      group_barrier<TPR>(group);
+      const float2 mine = scratch[turn][group][thread & (kWarps - 1)];
+      sg = mine.x;
+      sgh = mine.y;
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) {
+        sg += __shfl_xor_sync(0xFFFFFFFFu, sg, o);
+        sgh += __shfl_xor_sync(0xFFFFFFFFu, sgh, o);
+      }
+    }
+    if constexpr (CLUSTER > 1) {
+      cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+      if (threadIdx.x == 0) *cluster.map_shared_rank(&from_peer[turn], rank ^ 1) = make_float2(sg, sgh);
+      cluster.sync();
+      const float2 other = from_peer[turn];
+      // in the order of the halves, so that both blocks have the same sum
+      sg = rank == 0 ? sg + other.x : other.x + sg;
+      sgh = rank == 0 ? sgh + other.y : other.y + sgh;
+    }
     const float mg = sg * inv_cols, mgh = sgh * inv_cols;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      Raw8<W> w;
-      w.template load<kAligned>(weight, x.at(v), cols);
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float h = (x.held[v].get(i) - mean) * rstd;
-        out[i] = rstd * (d.held[v].get(i) * w.get(i) - mg - h * mgh);
+        const float h = (x[v].get(i) - mean) * rstd;
+        out[i] = rstd * (d[v].get(i) * w[v].get(i) - mg - h * mgh);
       }
-      store8<kAligned>(dx + r * cols, x.at(v), cols, out);
+      column.store(dx + r * cols, v, out);
     }
   }
-  float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * cols;
+  if (CLUSTER > 1) cooperative_groups::this_cluster().sync();  // no block ends while the other may still write to it
+  float* mine = partial + unit * 2 * cols + col0;
+  if (kGroups == 1) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const long long at = (static_cast<long long>(v) * TPR + threadIdx.x) * 8;
+    for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (at + i < cols) {
-        mine[at + i] = sum_w[(v * 8 + i) * TPR];
-        mine[cols + at + i] = sum_b[(v * 8 + i) * TPR];
+      for (int i = 0; i < 8; ++i)
+        if (column.has(v, i)) {
+          mine[column.at(v, i)] = dw[v][i];
+          mine[cols + column.at(v, i)] = db[v][i];
+        }
+    return;
+  }
+  // groups one after the other, in place (i * TPR * V + ...: a warp's lanes on neighbouring words)
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    for (int k = 0; k < kGroups; ++k) {
+      __syncthreads();
+      if (group == k) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float* at = across + (v * 8 + i) * TPR + thread;
+            const float sum = half ? db[v][i] : dw[v][i];
+            *at = k == 0 ? sum : *at + sum;
+          }
       }
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (column.has(v, i)) mine[half * cols + column.at(v, i)] = across[(v * 8 + i) * TPR + thread];
     }
   }
 }

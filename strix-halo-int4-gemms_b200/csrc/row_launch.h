@@ -15,23 +15,33 @@ inline unsigned row_blocks(long long rows) {
   return static_cast<unsigned>(blocks < INT_MAX ? blocks : INT_MAX);
 }
 
-// Threads and values a thread for a row: a warp as far as 32 values a lane go (no barrier), then 16 a thread, so
-// that two 16-byte loads of bf16 are in flight in every thread, and 32 in the longest rows (512 threads have 128
-// registers each, 1024 would have 64 and spill).  Rows that the wide loads cannot take (their length
-// is no multiple of eight, or a tensor does not start on 16 bytes) are bound by their many narrow loads whatever the
-// shape is: they have three.
-template <typename Fn>
-void for_row_shape(long long cols, bool wide, Fn&& fn) {
+// Threads and values a thread for a row.  Many rows: a warp as far as MAX_V groups of eight a lane go, then as few
+// threads as that leaves, since what is done once for a row is done by each of them.  Few rows (fewer than would give
+// each SM four): as many threads as there are groups of eight, since the time is that of one row.
+// Rows that the wide loads cannot take (their length is no multiple of eight, or a tensor does not start on 16 bytes)
+// are bound by their many narrow loads whatever the shape is: they have three.
+constexpr long long kFewRows = 4 * 148;
+
+template <int MAX_V, typename Fn>
+void for_row_shape(long long rows, long long cols, bool wide, Fn&& fn) {
   using std::integral_constant;
+  auto shape = [&](auto tpr, auto v) { fn(tpr, v, std::true_type()); };
   if (wide) {
-    if (cols <= 256) fn(integral_constant<int, 32>(), integral_constant<int, 1>(), std::true_type());
-    else if (cols <= 512) fn(integral_constant<int, 32>(), integral_constant<int, 2>(), std::true_type());
-    else if (cols <= 1024) fn(integral_constant<int, 32>(), integral_constant<int, 4>(), std::true_type());
-    else if (cols <= 2048) fn(integral_constant<int, 128>(), integral_constant<int, 2>(), std::true_type());
-    else if (cols <= 4096) fn(integral_constant<int, 256>(), integral_constant<int, 2>(), std::true_type());
-    else if (cols <= 8192) fn(integral_constant<int, 512>(), integral_constant<int, 2>(), std::true_type());
-    else if (cols <= 16384) fn(integral_constant<int, 512>(), integral_constant<int, 4>(), std::true_type());
-    else fn(integral_constant<int, 512>(), integral_constant<int, 0>(), std::true_type());
+    if (cols <= 256) shape(integral_constant<int, 32>(), integral_constant<int, 1>());
+    else if (cols > 16384) shape(integral_constant<int, 512>(), integral_constant<int, 0>());
+    else if (rows < kFewRows) {
+      if (cols <= 2048) shape(integral_constant<int, 256>(), integral_constant<int, 1>());
+      else if (cols <= 4096) shape(integral_constant<int, 512>(), integral_constant<int, 1>());
+      else if (cols <= 8192) shape(integral_constant<int, 512>(), integral_constant<int, 2>());
+      else shape(integral_constant<int, 512>(), integral_constant<int, 4>());
+    } else {
+      if (cols <= 512) shape(integral_constant<int, 32>(), integral_constant<int, 2>());
+      else if (cols <= 1024) shape(integral_constant<int, 32>(), integral_constant<int, 4>());
+      else if (cols <= 2048) shape(integral_constant<int, 256 / MAX_V>(), integral_constant<int, MAX_V>());
+      else if (cols <= 4096) shape(integral_constant<int, 512 / MAX_V>(), integral_constant<int, MAX_V>());
+      else if (cols <= 8192) shape(integral_constant<int, 1024 / MAX_V>(), integral_constant<int, MAX_V>());
+      else shape(integral_constant<int, 2048 / MAX_V>(), integral_constant<int, MAX_V>());
+    }
   } else {
     if (cols <= 512) fn(integral_constant<int, 32>(), integral_constant<int, 2>(), std::false_type());
     else if (cols <= 4096) fn(integral_constant<int, 256>(), integral_constant<int, 2>(), std::false_type());
@@ -56,7 +66,7 @@ struct NormQuantizeCall {
   void *codes, *scales;
   long long rows, cols;
   bool weight_f32, wide;
-  int bits, subchannel;
+  int bits, subchannel, sm_count;
   double eps;
   cudaStream_t stream;
 };

@@ -45,17 +45,51 @@ int check_alignment(const char* name, const void* p, size_t bytes) {
   return 0;
 }
 
-// Blocks of the backward kernel: as many as are resident at once (its launch bounds), one row of partial sums each.
-int bwd_threads(int64_t cols) {
-  return cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024;
+// The backward kernel's shape: threads of a row (of half of it, above 8192 values) and groups of eight values a thread:
+// two of bf16, one of fp32, whose registers are twice as many.
+struct BwdPlan {
+  int threads, vectors, cluster;
+  int groups() const { return threads < 512 ? 512 / threads : 1; }
+};
+BwdPlan bwd_plan(long long cols, int x_type) {
+  const int v = x_type == B200_OUT_BF16 ? 2 : 1;
+  const int cluster = cols > 8192 ? 2 : 1;
+  int threads = 32;
+  while (static_cast<long long>(threads) * v * 8 * cluster < cols) threads *= 2;
+  return {threads, v, cluster};
 }
 
-long long bwd_blocks(int sm_count, long long rows, long long cols) {
+// As many clusters of its blocks as are resident at once, one row of partial sums each.
+long long bwd_units(int sm_count, long long rows, long long cols, int x_type) {
   if (cols > 16384) return 0;  // no partial sums
-  const int tpr = bwd_threads(cols);
-  const long long resident = static_cast<long long>(sm_count) * (tpr == 32 ? 3 : tpr == 1024 ? 1 : 768 / tpr);
-  const long long needed = tpr == 32 ? (rows + 7) / 8 : rows;
+  const BwdPlan plan = bwd_plan(cols, x_type);
+  // 512 threads: two blocks an SM of bf16 (about 64 registers a thread would allow it), 1024: one
+  const long long resident = static_cast<long long>(sm_count) / plan.cluster;
+  const long long needed = (rows + plan.groups() - 1) / plan.groups();
   return needed < resident ? needed : resident;
+}
+
+template <typename T, typename W, int TPR, int V, int CLUSTER, bool kAligned>
+int launch_bwd(const T* dy, const T* x, const W* weight, const float* mean, const float* rstd, T* dx, float* partial, long long units,
+               long long rows, long long cols, cudaStream_t stream) {
+  auto kernel = layer_norm_bwd_kernel<T, W, TPR, V, CLUSTER, kAligned>;
+  using Shape = BwdShape<TPR, CLUSTER>;
+  constexpr int smem = Shape::kGroups > 1 ? TPR * V * 8 * 4 : 0;
+  static_assert(smem <= 32 * 1024, "fits without permission");
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(units * CLUSTER));
+  config.blockDim = dim3(Shape::kThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = CLUSTER;
+  attribute[0].val.clusterDim.y = 1;
+  attribute[0].val.clusterDim.z = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, dy, x, weight, mean, rstd, dx, partial, rows, cols);
+  return err == cudaSuccess ? 0 : host_fail_cuda("layer_norm_bwd launch", err);
 }
 
 }  // namespace
@@ -74,7 +108,7 @@ extern "C" int b200_int4_gemms_quantize_tokens(int device_index, uintptr_t strea
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
     const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
     const bool wide = cols % 8 == 0 && is_aligned(src_bf16, 16) && is_aligned(codes, 8);
-    for_row_shape(cols, wide, [&](auto tpr, auto v, auto aligned) {
+    for_row_shape<8>(rows, cols, wide, [&](auto tpr, auto v, auto aligned) {
       constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
       for_bool(bits == 4, [&](auto four) {
         quantize_tokens_kernel<TPR, V, decltype(four)::value ? 4 : 8, decltype(aligned)::value>
@@ -110,7 +144,7 @@ extern "C" int b200_int4_gemms_layer_norm(int device_index, uintptr_t stream_han
     for_types(x_type, weight_type, [&](auto xt, auto wt) {
       using T = decltype(xt);
       using W = decltype(wt);
-      for_row_shape(cols, wide, [&](auto tpr, auto v, auto aligned) {
+      for_row_shape<sizeof(T) == 2 ? 8 : 4>(rows, cols, wide, [&](auto tpr, auto v, auto aligned) {
         constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
         layer_norm_kernel<T, W, TPR, V, decltype(aligned)::value><<<row_blocks<TPR>(rows), RowPlace<TPR>::kThreads, 0, stream>>>(
             static_cast<const T*>(x), static_cast<const W*>(weight), static_cast<const W*>(bias), static_cast<T*>(y), mean, rstd, rows,
@@ -144,20 +178,22 @@ extern "C" int b200_int4_gemms_layer_norm_quantize(int device_index, uintptr_t s
     call.wide = cols % 8 == 0 && is_aligned(x, 16) && is_aligned(codes, 8) && is_aligned(weight, 16) && is_aligned(bias, 16);
     call.bits = bits;
     call.subchannel = subchannel;
+    call.sm_count = sms;
     call.eps = eps;
     call.stream = reinterpret_cast<cudaStream_t>(stream_handle);
     return x_type == B200_OUT_F32 ? launch_norm_quantize_f32(call) : launch_norm_quantize_bf16(call);
   });
 }
 
-extern "C" size_t b200_int4_gemms_layer_norm_bwd_workspace_bytes(int device_index, int64_t rows, int64_t cols) {
+extern "C" size_t b200_int4_gemms_layer_norm_bwd_workspace_bytes(int device_index, int64_t rows, int64_t cols, int32_t x_type) {
   size_t bytes = 0;
   guarded([&]() -> int {
     if (int rc = check_rows(rows, cols); rc != 0) return rc;
+    if (int rc = check_types(x_type, x_type); rc != 0) return rc;
     DeviceScope device;
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
-    bytes = static_cast<size_t>(bwd_blocks(sms, rows, cols)) * 2 * static_cast<size_t>(cols) * sizeof(float);
+    bytes = static_cast<size_t>(bwd_units(sms, rows, cols, x_type)) * 2 * static_cast<size_t>(cols) * sizeof(float);
     return 0;
   });
   return bytes;
@@ -184,8 +220,8 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
     const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-    const long long blocks = bwd_blocks(sms, rows, cols);
-    if (blocks > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(blocks) * 2 * cols * sizeof(float)))
+    const long long units = bwd_units(sms, rows, cols, x_type);
+    if (units > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(units) * 2 * cols * sizeof(float)))
       return host_fail("workspace must hold b200_int4_gemms_layer_norm_bwd_workspace_bytes bytes");
     float* partial = static_cast<float*>(workspace);
     const bool wide = cols % 8 == 0 && is_aligned(dy, 16) && is_aligned(x, 16) && is_aligned(dx, 16) && is_aligned(weight, 16);
@@ -201,29 +237,20 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
         T* dx_t = static_cast<T*>(dx);
         for_bool(wide, [&](auto aligned) {
           constexpr bool A = decltype(aligned)::value;
-          auto narrow = [&](auto tpr) {
-            constexpr int TPR = decltype(tpr)::value;
-            layer_norm_bwd_kernel<T, W, TPR, A><<<static_cast<unsigned>(blocks), RowPlace<TPR>::kThreads, 0, stream>>>(
-                dy_t, x_t, w_t, mean, rstd, dx_t, partial, rows, cols);
+          constexpr int V = sizeof(T) == 2 ? 2 : 1;
+          using std::integral_constant;
+          auto rows_of = [&](auto tpr, auto cluster) {
+            rc = launch_bwd<T, W, decltype(tpr)::value, V, decltype(cluster)::value, A>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, units, rows, cols, stream);
           };
-          if (cols <= 256) narrow(std::integral_constant<int, 32>());
-          else if (cols <= 512) narrow(std::integral_constant<int, 64>());
-          else if (cols <= 1024) narrow(std::integral_constant<int, 128>());
-          else if (cols <= 2048) narrow(std::integral_constant<int, 256>());
-          else if (cols <= 4096) narrow(std::integral_constant<int, 512>());
-          else if (cols <= 8192) narrow(std::integral_constant<int, 1024>());
-          else if (cols <= 16384) {
-            constexpr int kSmem = 2 * 2 * 8 * 1024 * 4;
-            const cudaError_t err = cudaFuncSetAttribute(layer_norm_bwd_wide_kernel<T, W, A>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-            if (err != cudaSuccess) {
-              rc = host_fail_cuda("cudaFuncSetAttribute(max dynamic shared memory)", err);
-              return;
-            }
-            layer_norm_bwd_wide_kernel<T, W, A><<<static_cast<unsigned>(blocks), 1024, kSmem, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t,
-                                                                                                     partial, rows, cols);
-          } else {
-            layer_norm_bwd_long_kernel<T, W, A><<<row_blocks<1024>(rows), 1024, 0, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, rows, cols);
-          }
+          const BwdPlan plan = bwd_plan(cols, x_type);
+          if (cols > 16384) layer_norm_bwd_long_kernel<T, W, A><<<row_blocks<1024>(rows), 1024, 0, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, rows, cols);
+          else if (plan.cluster == 2) rows_of(integral_constant<int, 1024 / V>(), integral_constant<int, 2>());
+          else if (plan.threads == 32) rows_of(integral_constant<int, 32>(), integral_constant<int, 1>());
+          else if (plan.threads == 64) rows_of(integral_constant<int, 64>(), integral_constant<int, 1>());
+          else if (plan.threads == 128) rows_of(integral_constant<int, 128>(), integral_constant<int, 1>());
+          else if (plan.threads == 256) rows_of(integral_constant<int, 256>(), integral_constant<int, 1>());
+          else if (plan.threads == 512) rows_of(integral_constant<int, 512>(), integral_constant<int, 1>());
+          else rows_of(integral_constant<int, V == 1 ? 1024 : 512>(), integral_constant<int, 1>());
         });
         if (rc == 0 && cols > 16384)
           layer_norm_bwd_columns_kernel<T><<<column_grid, column_block, 0, stream>>>(dy_t, x_t, mean, rstd, rows, cols, dweight, dbias);
@@ -232,7 +259,7 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
       if (rc = launched("layer_norm_bwd launch"); rc != 0) return rc;
     }
     if (rows == 0 || cols <= 16384)
-      column_sums_kernel<<<column_grid, column_block, 0, stream>>>(partial, static_cast<int>(blocks), cols, dweight, dbias);
+      column_sums_kernel<<<column_grid, column_block, 0, stream>>>(partial, static_cast<int>(units), cols, dweight, dbias);
     return launched("layer_norm_bwd column sums launch");
   });
 }

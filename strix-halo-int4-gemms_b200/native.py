@@ -229,7 +229,7 @@ def _declare(library: ctypes.CDLL) -> None:
     library.b200_int4_gemms_layer_norm_quantize.argtypes = (
         [ctypes.c_int, size_t] + [void_p] * 5 + [i64, i64, i32, i32, ctypes.c_double, i32, i32])
     library.b200_int4_gemms_layer_norm_bwd_workspace_bytes.restype = size_t
-    library.b200_int4_gemms_layer_norm_bwd_workspace_bytes.argtypes = [ctypes.c_int, i64, i64]
+    library.b200_int4_gemms_layer_norm_bwd_workspace_bytes.argtypes = [ctypes.c_int, i64, i64, i32]
     library.b200_int4_gemms_layer_norm_bwd.restype = ctypes.c_int
     library.b200_int4_gemms_layer_norm_bwd.argtypes = [ctypes.c_int, size_t] + [void_p] * 9 + [size_t, i64, i64, i32, i32]
     library.b200_int4_gemms_moe_swiglu_workspace_bytes.restype = size_t
@@ -986,7 +986,7 @@ def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any,
     rows = x.numel() // cols
     library = load_dispatch_library(library_path)
     index = _device_index(x)
-    need = int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(index, rows, cols))
+    need = int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(index, rows, cols, _type_code(torch, x)))
     dx = torch.empty_like(x)
     sums = torch.empty((2, cols), device=x.device, dtype=torch.float32)
     workspace = torch.empty(need // 4, device=x.device, dtype=torch.float32)

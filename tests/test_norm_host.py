@@ -125,4 +125,4 @@ def test_c_entry_points_check_arguments(pkg, native_lib):
     b = lib.b200_int4_gemms_layer_norm_bwd
     assert said(b(0, 0, p, p, p, p, p, p, None, p, p, 8, 1, 8, 0, 0)) == "dweight and dbias pointers must be non-null"
     assert said(b(0, 0, None, p, p, p, p, p, p, p, p, 8, 1, 8, 0, 0)) == "dy, x, weight, mean, rstd and dx pointers must be non-null"
-    assert lib.b200_int4_gemms_layer_norm_bwd_workspace_bytes(99, 1, 8) == 0
+    assert lib.b200_int4_gemms_layer_norm_bwd_workspace_bytes(99, 1, 8, 0) == 0
