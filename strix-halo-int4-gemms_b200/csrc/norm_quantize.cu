@@ -18,7 +18,7 @@ int launch_norm_quantize_bf16(const NormQuantizeCall& c) {
         layer_norm_quantize_kernel<NormX, W, TPR, V, decltype(four)::value ? 4 : 8, decltype(aligned)::value>
             <<<row_blocks<TPR>(c.rows), RowPlace<TPR>::kThreads, 0, c.stream>>>(
                 static_cast<const NormX*>(c.x), static_cast<const W*>(c.weight), static_cast<const W*>(c.bias),
-                static_cast<uint8_t*>(c.codes), static_cast<bf16*>(c.scales), c.rows, c.cols, c.subchannel,
+                static_cast<uint8_t*>(c.codes), static_cast<bf16*>(c.scales), c.rows, c.cols, group_bits(c.subchannel),
                 1.0 / static_cast<double>(c.cols), c.eps);
       });
     });

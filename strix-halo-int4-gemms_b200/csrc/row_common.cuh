@@ -24,6 +24,18 @@ struct Raw8<bf16> {
   uint32_t w[4];
   __device__ __forceinline__ float get(int i) const { return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]); }
   __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0u; }
+  // G values (8 or 4) at place i
+  template <int G>
+  __device__ __forceinline__ void load_chunk(int i, const bf16* p, bool valid) {
+    if constexpr (G == 8) {
+      const uint4 v = valid ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+      const uint2 v = valid ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
+      w[i / 2] = v.x;
+      w[i / 2 + 1] = v.y;
+    }
+  }
   __device__ __forceinline__ void set(const bf16 (&e)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -54,6 +66,14 @@ template <>
 struct Raw8<float> {
   float f[8];
   __device__ __forceinline__ float get(int i) const { return f[i]; }
+  template <int G>
+  __device__ __forceinline__ void load_chunk(int i, const float* p, bool valid) {
+#pragma unroll
+    for (int k = 0; k < G; k += 4) {
+      const float4 v = valid ? __ldg(reinterpret_cast<const float4*>(p + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[i + k] = v.x; f[i + k + 1] = v.y; f[i + k + 2] = v.z; f[i + k + 3] = v.w;
+    }
+  }
   __device__ __forceinline__ void set(const float (&e)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = e[i];
@@ -85,66 +105,49 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <bool kAligned>
-__device__ __forceinline__ void store8(bf16* row, long long at, long long cols, const float (&v)[8]) {
-  if (kAligned) {
-    if (at < cols)
-      *reinterpret_cast<uint4*>(row + at) =
-          make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at + i < cols) row[at + i] = __float2bfloat16_rn(v[i]);
-  }
-}
-
-template <bool kAligned>
-__device__ __forceinline__ void store8(float* row, long long at, long long cols, const float (&v)[8]) {
-  if (kAligned) {
-    if (at < cols) {
-      *reinterpret_cast<float4*>(row + at) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(row + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at + i < cols) row[at + i] = v[i];
-  }
-}
-
-// Where thread t of the TPR threads of a row has its group v of eight values: at (v * TPR + t) * 8, by wide loads; or,
-// where those cannot be used, at v * 8 * TPR + t and every TPR-th from there, so that narrow loads of a warp are
-// neighbours.
-template <int TPR, bool kAligned>
+// Which columns thread t of the TPR threads of a row has: eight values for each v, in chunks of G consecutive ones, G the
+// number of values in 16 bytes (8 of bf16, 4 of fp32), so that a warp's loads are neighbours; or 1 where wide loads
+// cannot be used.
+template <int TPR, int G>
 struct Columns {
   int thread;
   long long cols;
-  __device__ __forceinline__ long long first(int v) const { return (static_cast<long long>(v) * TPR + thread) * 8; }
-  __device__ __forceinline__ long long at(int v, int i) const {
-    return kAligned ? first(v) + i : static_cast<long long>(v) * 8 * TPR + i * TPR + thread;
-  }
-  __device__ __forceinline__ bool has(int v, int i) const { return kAligned ? first(v) < cols : at(v, i) < cols; }
+  __device__ __forceinline__ long long at(int v, int i) const { return (static_cast<long long>(v * (8 / G) + i / G) * TPR + thread) * G + i % G; }
+  __device__ __forceinline__ bool has(int v, int i) const { return at(v, i - i % G) < cols; }  // a chunk is inside or outside
   template <typename T>
   __device__ __forceinline__ Raw8<T> load(const T* row, int v) const {
     Raw8<T> r;
-    if (kAligned) {
-      r.template load<true>(row, first(v), cols);
-    } else {
+    if constexpr (G == 1) {
       T e[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) e[i] = has(v, i) ? row[at(v, i)] : T(0.f);
       r.set(e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += G) r.template load_chunk<G>(i, row + at(v, i), has(v, i));
     }
     return r;
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, int v, const float (&f)[8]) const {
-    if (kAligned) {
-      store8<true>(row, first(v), cols, f);
-    } else {
+    if constexpr (G == 1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (has(v, i)) row[at(v, i)] = static_cast<T>(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += G) {
+        if (!has(v, i)) continue;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int k = 0; k < G; k += 4) *reinterpret_cast<float4*>(row + at(v, i) + k) = make_float4(f[i + k], f[i + k + 1], f[i + k + 2], f[i + k + 3]);
+        } else if constexpr (G == 8) {
+          *reinterpret_cast<uint4*>(row + at(v, i)) =
+              make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+        } else {
+          *reinterpret_cast<uint2*>(row + at(v, i)) = make_uint2(pack_bf16x2(f[i], f[i + 1]), pack_bf16x2(f[i + 2], f[i + 3]));
+        }
+      }
     }
   }
 };

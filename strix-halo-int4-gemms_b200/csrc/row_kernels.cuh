@@ -12,6 +12,7 @@
 
 #include <cstring>
 
+#include "ptx.cuh"
 #include "row_common.cuh"
 
 namespace b200 {
@@ -53,52 +54,64 @@ struct RowValues {
 // quantize_tokens: scale = bf16(amax / top), code = round_half_even(x / scale), for every row (sub == 0) or every
 // `sub` values of it (32, 64, 128 or 256: 4 to 32 lanes of one warp).
 // ---------------------------------------------------------------------------------------------------------------
+// The codes of eight values where the scale is not ordinary: by division, zero where it is not finite.
+template <int BITS>
+__device__ __noinline__ typename CodeWords<BITS>::type divided_codes(Raw8<bf16> raw, float s) {
+  uint32_t c[8];
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    c[2 * i] = code_by_division<BITS>(bf16_lo(raw.w[i]), s);
+    c[2 * i + 1] = code_by_division<BITS>(bf16_hi(raw.w[i]), s);
+  }
+  return CodeWords<BITS>::pack(c);
+}
+
 template <int TPR, int V, int BITS, bool kAligned>
 __global__ void __launch_bounds__(RowPlace<TPR>::kThreads)
 quantize_tokens_kernel(const bf16* __restrict__ src, uint8_t* __restrict__ codes, bf16* __restrict__ scales,
-                       long long rows, long long cols, int sub) {
+                       long long rows, long long cols, int sub_bits) {  // groups of 2^sub_bits values; 0: the row
   __shared__ uint32_t scratch[2][TPR / 32];
   const long long pitch = BITS == 4 ? (cols + 1) / 2 : cols;
-  const int lanes = sub >> 3;  // of a group; 0: one scale a row
-  const long long groups = sub ? (cols + sub - 1) / sub : 1;
+  const int lanes = sub_bits ? 1 << (sub_bits - 3) : 0;  // of a group; 0: one scale a row
+  const long long groups = sub_bits ? (cols + (1 << sub_bits) - 1) >> sub_bits : 1;
+  auto largest = [](uint32_t m, const Raw8<bf16>& raw) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, raw.w[i] & 0x7FFF7FFFu);
+    return m;
+  };
+  auto put = [&](uint8_t* row, long long at, const Raw8<bf16>& raw, float s, bool ordinary, const ExactQuotient& q) {
+    if (ordinary) {
+      uint32_t c[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = q.code(raw.get(i));
+      store_codes<BITS, kAligned>(row, at, cols, c);
+    } else {
+      store_packed<BITS, kAligned>(row, at, cols, divided_codes<BITS>(raw, s));
+    }
+  };
   int turn = 0;
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step(), turn ^= 1) {
     const RowValues<bf16, TPR, V, kAligned> x(src + r * cols, cols);
-    float s = 1.f;
+    uint8_t* out = codes + r * pitch;
     if (!lanes) {
       uint32_t m = 0;
 #pragma unroll
+      for (int v = 0; v < x.count(); ++v) m = largest(m, x.get(v));
+      const float s = scale_of_bf16<BITS>(row_reduce<TPR>(max(m & 0xFFFFu, m >> 16), MaxOp(), scratch[turn]));
+      if (RowPlace<TPR>::thread() == 0) scales[r] = __float2bfloat16_rn(s);
+      const bool ordinary = scale_is_ordinary(s);
+      const ExactQuotient q(s);
+#pragma unroll
+      for (int v = 0; v < x.count(); ++v) put(out, x.at(v), x.get(v), s, ordinary, q);
+    } else {
+#pragma unroll
       for (int v = 0; v < x.count(); ++v) {
         const Raw8<bf16> raw = x.get(v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, raw.w[i] & 0x7FFF7FFFu);
+        const uint32_t m = largest(0u, raw);
+        const float s = scale_of_bf16<BITS>(warp_reduce(max(m & 0xFFFFu, m >> 16), MaxOp(), lanes));
+        if ((threadIdx.x & (lanes - 1)) == 0 && x.at(v) < cols) scales[r * groups + (x.at(v) >> sub_bits)] = __float2bfloat16_rn(s);
+        put(out, x.at(v), raw, s, scale_is_ordinary(s), ExactQuotient(s));
       }
-      m = max(m & 0xFFFFu, m >> 16);
-      s = scale_of_bf16<BITS>(row_reduce<TPR>(m, MaxOp(), scratch[turn]));
-      if (RowPlace<TPR>::thread() == 0) scales[r] = __float2bfloat16_rn(s);
-    }
-#pragma unroll
-    for (int v = 0; v < x.count(); ++v) {
-      const Raw8<bf16> raw = x.get(v);
-      const long long at = x.at(v);
-      if (lanes) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, raw.w[i] & 0x7FFF7FFFu);
-        m = warp_reduce(max(m & 0xFFFFu, m >> 16), MaxOp(), lanes);
-        s = scale_of_bf16<BITS>(m);
-        if ((threadIdx.x & (lanes - 1)) == 0 && at < cols) scales[r * groups + at / sub] = __float2bfloat16_rn(s);
-      }
-      uint32_t c[8];
-      if (scale_is_ordinary(s)) {
-        const ExactQuotient q(s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = q.code(raw.get(i));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = code_by_division<BITS>(raw.get(i), s);
-      }
-      store_codes<BITS, kAligned>(codes + r * pitch, at, cols, c);
     }
   }
 }
@@ -107,12 +120,13 @@ quantize_tokens_kernel(const bf16* __restrict__ src, uint8_t* __restrict__ codes
 // layer norm: y = (x - mean) rstd w + b; mean, then the mean square of the differences, both from registers, in fp32.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, typename W, int TPR, int V, bool kAligned>
-__global__ void __launch_bounds__(RowPlace<TPR>::kThreads)
+__global__ void __launch_bounds__(RowPlace<TPR>::kThreads, 768 / RowPlace<TPR>::kThreads)
 layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias, T* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, long long cols, float eps) {
   __shared__ float scratch[2][TPR / 32];
   const float inv_cols = 1.f / static_cast<float>(cols);
-  const Columns<TPR, kAligned> column{RowPlace<TPR>::thread(), cols};
+  constexpr int G = kAligned ? 16 / sizeof(T) : 1;
+  const Columns<TPR, G> column{RowPlace<TPR>::thread(), cols};
   const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
     const T* row = src + r * cols;
@@ -134,11 +148,10 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 #pragma unroll
     for (int v = 0; v < count; ++v) {
       const Raw8<T> raw = value(v);
-      if (kAligned && !column.has(v, 0)) continue;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float d = raw.get(i) - mean;
-        if (kAligned || column.has(v, i)) square = __fmaf_rn(d, d, square);
+        if (column.has(v, i)) square = __fmaf_rn(d, d, square);
       }
     }
     const float rstd = rsqrtf(row_reduce<TPR>(square, SumOp(), scratch[1]) * inv_cols + eps);
@@ -214,7 +227,7 @@ __device__ __noinline__ unsigned long long exact_codes(const T* row, const W* we
 template <typename T, typename W, int TPR, int V, int BITS, bool kAligned>
 __global__ void __launch_bounds__(RowPlace<TPR>::kThreads)
 layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias,
-                           uint8_t* __restrict__ codes, bf16* __restrict__ scales, long long rows, long long cols, int sub,
+                           uint8_t* __restrict__ codes, bf16* __restrict__ scales, long long rows, long long cols, int sub_bits,
                            double inv_cols, double eps) {
   __shared__ double scratch_d[2][2 * (TPR / 32)];
   __shared__ float scratch_m[2 * (TPR / 32)];
@@ -223,8 +236,8 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
   constexpr float kTop = BITS == 4 ? 7.f : 127.f;
   constexpr float kError = 4.76837158203125e-7f;  // 2^-21
   const long long pitch = BITS == 4 ? (cols + 1) / 2 : cols;
-  const int lanes = sub >> 3;
-  const long long groups = sub ? (cols + sub - 1) / sub : 1;
+  const int lanes = sub_bits ? 1 << (sub_bits - 3) : 0;
+  const long long groups = sub_bits ? (cols + (1 << sub_bits) - 1) >> sub_bits : 1;
   const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   auto place = [&](int v) { return (static_cast<long long>(v) * TPR + RowPlace<TPR>::thread()) * 8; };
   auto read_affine = [&](int v, Raw8<W>& w, Raw8<W>& b) {
@@ -346,7 +359,7 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
           const double most = warp_reduce(exact_size<T, W>(row, weight, bias, place(v), cols, exact), MaxOp(), lanes);
           if (settle) settled(most);
         }
-        if ((threadIdx.x & (lanes - 1)) == 0 && place(v) < cols) scales[r * groups + place(v) / sub] = __float2bfloat16_rn(s);
+        if ((threadIdx.x & (lanes - 1)) == 0 && place(v) < cols) scales[r * groups + (place(v) >> sub_bits)] = __float2bfloat16_rn(s);
         put(v, out[0]);
       }
     }
@@ -369,6 +382,35 @@ struct BwdShape {
   static constexpr int kGroups = kThreads / TPR;  // rows at once (by half a row for CLUSTER == 2)
 };
 
+// Address of this block's shared memory in another block of the cluster.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t address, int rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
+  return there;
+}
+
+// Two floats to another block's shared memory, counted there as eight bytes on its barrier.
+__device__ __forceinline__ void store_async(uint32_t address, uint32_t barrier, float a, float b) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(address), "f"(a), "f"(b), "r"(barrier)
+               : "memory");
+}
+
+// Bounded wait for a barrier: false, and the device's status word, when the time runs out.
+__device__ __forceinline__ bool wait_for_peer(uint32_t barrier, uint32_t parity, volatile int* status) {
+  if (mbar_try_wait(barrier, parity)) return true;
+  const unsigned long long begin = global_timer_ns();
+  while (!mbar_try_wait(barrier, parity)) {
+    if (global_timer_ns() - begin > WAIT_LIMIT_NS) {
+      if (status != nullptr && status[0] == STATUS_OK) {
+        status[1] = static_cast<int>(blockIdx.x);
+        status[0] = STATUS_WAIT_TIMEOUT;
+      }
+      return false;
+    }
+  }
+  return true;
+}
+
 // Barrier of one group of a block.
 template <int TPR>
 __device__ __forceinline__ void group_barrier(int group) {
@@ -379,18 +421,33 @@ template <typename T, typename W, int TPR, int V, int CLUSTER, bool kAligned>
 __global__ void __launch_bounds__(BwdShape<TPR, CLUSTER>::kThreads)
 layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
-                      float* __restrict__ partial, long long rows, long long cols) {
+                      float* __restrict__ partial, long long rows, long long cols, volatile int* status) {
   using Shape = BwdShape<TPR, CLUSTER>;
   constexpr int kWarps = TPR / 32, kGroups = Shape::kGroups, kBlockCols = TPR * V * 8;
   __shared__ float2 scratch[2][kGroups][kWarps];
-  __shared__ float2 from_peer[2];
+  __shared__ __align__(8) float2 from_peer[2];
+  __shared__ __align__(8) uint64_t arrived[2];
+  __shared__ bool go_on;
   extern __shared__ float across[];  // [kBlockCols], where there are groups to be added up
   const int group = threadIdx.x / TPR, thread = threadIdx.x % TPR;
   const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
   const long long unit = blockIdx.x / CLUSTER, step = static_cast<long long>(gridDim.x / CLUSTER) * kGroups;
   // this block's columns: all, or the half `rank` (the first half is kBlockCols wide)
   const long long col0 = static_cast<long long>(rank) * kBlockCols;
-  const Columns<TPR, kAligned> column{thread, CLUSTER > 1 ? max(0ll, min(cols - col0, static_cast<long long>(kBlockCols))) : cols};
+  constexpr int G = kAligned ? 16 / sizeof(T) : 1;
+  const Columns<TPR, G> column{thread, CLUSTER > 1 ? max(0ll, min(cols - col0, static_cast<long long>(kBlockCols))) : cols};
+  uint32_t peer_value = 0, peer_barrier = 0, my_barrier = 0;
+  if constexpr (CLUSTER > 1) {
+    my_barrier = smem_u32(arrived);
+    if (threadIdx.x == 0) {
+      mbar_init(my_barrier, 1);
+      mbar_init(my_barrier + 8, 1);
+      mbar_fence_init();
+    }
+    peer_value = cluster_address(smem_u32(from_peer), rank ^ 1);
+    peer_barrier = cluster_address(my_barrier, rank ^ 1);
+    cooperative_groups::this_cluster().sync();
+  }
   src += col0;
   dy += col0;
   dx += col0;
@@ -417,6 +474,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
   long long r = unit * kGroups + group;
   if (r < rows) fetch(r);
   int turn = 0;
+  uint32_t phase = 0;
   for (; r < rows; r += step, turn ^= 1) {
     Raw8<T> x[V], d[V];
 #pragma unroll
@@ -453,9 +511,20 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
       }
     }
     if constexpr (CLUSTER > 1) {
-      cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-      if (threadIdx.x == 0) *cluster.map_shared_rank(&from_peer[turn], rank ^ 1) = make_float2(sg, sgh);
-      cluster.sync();
+      // One 8-byte store that counts up the other block's barrier; a buffer is written again two rows later, after
+      // the other block has sent its sums of the row between, which it does behind a barrier of all its threads.
+      // (A cluster barrier instead waits for all stores of dx: 517 rows of 14336 took 40 us with it.)
+      if (threadIdx.x == 0) {
+        mbar_arrive_expect_tx(my_barrier + 8 * turn, 8);
+        store_async(peer_value + 8 * turn, peer_barrier + 8 * turn, sg, sgh);
+        go_on = wait_for_peer(my_barrier + 8 * turn, (phase >> turn) & 1u, status);
+      }
+      phase ^= 1u << turn;
+      __syncthreads();
+      if (!go_on) {  // never, unless the device lost the other block: the sums show it
+        dw[0][0] = __int_as_float(0x7FC00000);
+        break;
+      }
       const float2 other = from_peer[turn];
       // in the order of the halves, so that both blocks have the same sum
       sg = rank == 0 ? sg + other.x : other.x + sg;
@@ -473,6 +542,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
       column.store(dx + r * cols, v, out);
     }
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // column_sums_kernel, which waits for this one's end
   if (CLUSTER > 1) cooperative_groups::this_cluster().sync();  // no block ends while the other may still write to it
   float* mine = partial + unit * 2 * cols + col0;
   if (kGroups == 1) {
@@ -519,19 +589,20 @@ __global__ void __launch_bounds__(1024)
 layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
                            const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
                            long long rows, long long cols) {
-  constexpr int TPR = 1024;
+  constexpr int TPR = 1024, G = kAligned ? 16 / sizeof(T) : 1;
   __shared__ float scratch[2][2 * (TPR / 32)];
   const float inv_cols = 1.f / static_cast<float>(cols);
+  const Columns<TPR, G> column{static_cast<int>(threadIdx.x), cols};
+  const int count = static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   int turn = 0;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
-    const RowValues<T, TPR, 0, kAligned> x(src + r * cols, cols);
-    const RowValues<T, TPR, 0, kAligned> d(dy + r * cols, cols);
+    const T* x_row = src + r * cols;
+    const T* d_row = dy + r * cols;
     const float mean = __ldg(mean_in + r), rstd = __ldg(rstd_in + r);
     float sg = 0.f, sgh = 0.f;
-    for (int v = 0; v < x.count(); ++v) {
-      const Raw8<T> xv = x.get(v), dv = d.get(v);
-      Raw8<W> w;
-      w.template load<kAligned>(weight, x.at(v), cols);
+    for (int v = 0; v < count; ++v) {
+      const Raw8<T> xv = column.load(x_row, v), dv = column.load(d_row, v);
+      const Raw8<W> w = column.load(weight, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float g = dv.get(i) * w.get(i);
@@ -541,46 +612,48 @@ layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ src, 
     }
     row_reduce2<TPR>(sg, sgh, SumOp(), SumOp(), scratch[turn]);
     const float mg = sg * inv_cols, mgh = sgh * inv_cols;
-    for (int v = 0; v < x.count(); ++v) {
-      const Raw8<T> xv = x.get(v), dv = d.get(v);
-      Raw8<W> w;
-      w.template load<kAligned>(weight, x.at(v), cols);
+    for (int v = 0; v < count; ++v) {
+      const Raw8<T> xv = column.load(x_row, v), dv = column.load(d_row, v);
+      const Raw8<W> w = column.load(weight, v);
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = rstd * (dv.get(i) * w.get(i) - mg - (xv.get(i) - mean) * rstd * mgh);
-      store8<kAligned>(dx + r * cols, x.at(v), cols, out);
+      column.store(dx + r * cols, v, out);
     }
   }
 }
 
-// Block of 32 columns x 32 rows at a time; the 32 sums of a column are added in a fixed order.
+// Block of 32 columns x ROWS rows at a time; the sums of a column are added in a fixed order.
+template <int ROWS>
 __device__ __forceinline__ void column_finish(float sw, float sb, long long col, long long cols, float* dweight, float* dbias) {
-  __shared__ float tile[2][32][33];
+  __shared__ float tile[2][ROWS][33];
   tile[0][threadIdx.y][threadIdx.x] = sw;
   tile[1][threadIdx.y][threadIdx.x] = sb;
   __syncthreads();
-  // warp y takes column y of the tile
-  const float a = warp_reduce(tile[0][threadIdx.x][threadIdx.y], SumOp());
-  const float b = warp_reduce(tile[1][threadIdx.x][threadIdx.y], SumOp());
-  const long long mine = col - threadIdx.x + threadIdx.y;
-  if (threadIdx.x == 0 && mine < cols) {
-    dweight[mine] = a;
-    dbias[mine] = b;
+  // the first warp adds up dw, the second db, a column a lane
+  if (threadIdx.y < 2 && col < cols) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) sum += tile[threadIdx.y][k][threadIdx.x];
+    (threadIdx.y == 0 ? dweight : dbias)[col] = sum;
   }
 }
 
-static __global__ void __launch_bounds__(1024)
+constexpr int kSumRows = 16;
+
+static __global__ void __launch_bounds__(32 * kSumRows)
 column_sums_kernel(const float* __restrict__ partial, int parts, long long cols, float* __restrict__ dweight, float* __restrict__ dbias) {
   const long long col = static_cast<long long>(blockIdx.x) * 32 + threadIdx.x;
   float sw = 0.f, sb = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (col < cols) {
-#pragma unroll 4
-    for (int p = threadIdx.y; p < parts; p += 32) {
-      sw += __ldg(partial + (2LL * p) * cols + col);
-      sb += __ldg(partial + (2LL * p + 1) * cols + col);
+#pragma unroll 8
+    for (int p = threadIdx.y; p < parts; p += kSumRows) {
+      sw += partial[(2LL * p) * cols + col];
+      sb += partial[(2LL * p + 1) * cols + col];
     }
   }
-  column_finish(sw, sb, col, cols, dweight, dbias);
+  column_finish<kSumRows>(sw, sb, col, cols, dweight, dbias);
 }
 
 template <typename T>
@@ -597,7 +670,7 @@ layer_norm_bwd_columns_kernel(const T* __restrict__ dy, const T* __restrict__ sr
       sb += d;
     }
   }
-  column_finish(sw, sb, col, cols, dweight, dbias);
+  column_finish<32>(sw, sb, col, cols, dweight, dbias);
 }
 
 }  // namespace b200

@@ -9,6 +9,9 @@
 
 namespace b200 {
 
+// log2 of a group's size; 0 for one scale a row
+inline int group_bits(int subchannel) { return subchannel == 32 ? 5 : subchannel == 64 ? 6 : subchannel == 128 ? 7 : subchannel == 256 ? 8 : 0; }
+
 template <int TPR>
 inline unsigned row_blocks(long long rows) {
   const long long blocks = (rows + RowPlace<TPR>::kRows - 1) / RowPlace<TPR>::kRows;

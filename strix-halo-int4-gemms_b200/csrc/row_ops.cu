@@ -71,7 +71,7 @@ long long bwd_units(int sm_count, long long rows, long long cols, int x_type) {
 
 template <typename T, typename W, int TPR, int V, int CLUSTER, bool kAligned>
 int launch_bwd(const T* dy, const T* x, const W* weight, const float* mean, const float* rstd, T* dx, float* partial, long long units,
-               long long rows, long long cols, cudaStream_t stream) {
+               long long rows, long long cols, volatile int* status, cudaStream_t stream) {
   auto kernel = layer_norm_bwd_kernel<T, W, TPR, V, CLUSTER, kAligned>;
   using Shape = BwdShape<TPR, CLUSTER>;
   constexpr int smem = Shape::kGroups > 1 ? TPR * V * 8 * 4 : 0;
@@ -88,7 +88,7 @@ int launch_bwd(const T* dy, const T* x, const W* weight, const float* mean, cons
   attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, dy, x, weight, mean, rstd, dx, partial, rows, cols);
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, dy, x, weight, mean, rstd, dx, partial, rows, cols, status);
   return err == cudaSuccess ? 0 : host_fail_cuda("layer_norm_bwd launch", err);
 }
 
@@ -113,7 +113,7 @@ extern "C" int b200_int4_gemms_quantize_tokens(int device_index, uintptr_t strea
       for_bool(bits == 4, [&](auto four) {
         quantize_tokens_kernel<TPR, V, decltype(four)::value ? 4 : 8, decltype(aligned)::value>
             <<<row_blocks<TPR>(rows), RowPlace<TPR>::kThreads, 0, stream>>>(
-                static_cast<const bf16*>(src_bf16), static_cast<uint8_t*>(codes), static_cast<bf16*>(scales_bf16), rows, cols, subchannel);
+                static_cast<const bf16*>(src_bf16), static_cast<uint8_t*>(codes), static_cast<bf16*>(scales_bf16), rows, cols, group_bits(subchannel));
       });
     });
     return launched("quantize_tokens launch");
@@ -224,6 +224,7 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
     if (units > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(units) * 2 * cols * sizeof(float)))
       return host_fail("workspace must hold b200_int4_gemms_layer_norm_bwd_workspace_bytes bytes");
     float* partial = static_cast<float*>(workspace);
+    volatile int* status = device_status_word(device_index);
     const bool wide = cols % 8 == 0 && is_aligned(dy, 16) && is_aligned(x, 16) && is_aligned(dx, 16) && is_aligned(weight, 16);
     const dim3 column_grid(static_cast<unsigned>((cols + 31) / 32)), column_block(32, 32);
     int rc = 0;
@@ -240,7 +241,7 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
           constexpr int V = sizeof(T) == 2 ? 2 : 1;
           using std::integral_constant;
           auto rows_of = [&](auto tpr, auto cluster) {
-            rc = launch_bwd<T, W, decltype(tpr)::value, V, decltype(cluster)::value, A>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, units, rows, cols, stream);
+            rc = launch_bwd<T, W, decltype(tpr)::value, V, decltype(cluster)::value, A>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, units, rows, cols, status, stream);
           };
           const BwdPlan plan = bwd_plan(cols, x_type);
           if (cols > 16384) layer_norm_bwd_long_kernel<T, W, A><<<row_blocks<1024>(rows), 1024, 0, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, rows, cols);
@@ -258,8 +259,19 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
       if (rc != 0) return rc;
       if (rc = launched("layer_norm_bwd launch"); rc != 0) return rc;
     }
-    if (rows == 0 || cols <= 16384)
-      column_sums_kernel<<<column_grid, column_block, 0, stream>>>(partial, static_cast<int>(units), cols, dweight, dbias);
-    return launched("layer_norm_bwd column sums launch");
+    if (rows > 0 && cols > 16384) return launched("layer_norm_bwd columns launch");
+    // may start while the kernel before it ends: it waits for it by itself
+    cudaLaunchConfig_t config{};
+    config.gridDim = column_grid;
+    config.blockDim = dim3(32, kSumRows);
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = rows > 0 ? 1 : 0;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, column_sums_kernel, static_cast<const float*>(partial), static_cast<int>(units),
+                                               static_cast<long long>(cols), dweight, dbias);
+    return err == cudaSuccess ? 0 : host_fail_cuda("layer_norm_bwd column sums launch", err);
   });
 }
