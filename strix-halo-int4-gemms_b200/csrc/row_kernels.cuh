@@ -180,9 +180,9 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 // A code is decided by the exact value, not by fp32's rounding of it: a value next to the border of two codes
 // would otherwise go to the one or the other with the order of a sum.  The statistics are sums in fp64.  The
 // values are computed in fp32, where they are off by at most E = 2^-21 (|t| + |b|), t = (x - mean) rstd w (four
-// roundings of 2^-24 each, and room); |t| <= amax + |b|, so E <= 2^-21 (amax + 2 max|b|) for a whole group.  If
-// q - E/s and q + E/s round to one integer, that is the code; otherwise (once in some 10^4 values) the eight values
-// of the thread are computed again in fp64.  The scale is settled in the same way: where amax / top is within its error
+// roundings of 2^-24 each, and room); |t| <= amax + |b|, so E <= 2^-21 (amax + 2 max|b|) for a whole group.  A
+// quotient that is further than E/s from every border has its code; otherwise (once in some 10^4 values) the eight
+// values of the thread are computed again in fp64.  The scale is settled in the same way: where amax / top is within its error
 // of a tie of two bf16 numbers, the group's maximum is found again in fp64.  Both are loops that read their values
 // again, out of the way of the code that runs always.
 // The kernel is bound by its instructions, not by HBM.
@@ -225,7 +225,7 @@ __device__ __noinline__ unsigned long long exact_codes(const T* row, const W* we
 }
 
 template <typename T, typename W, int TPR, int V, int BITS, bool kAligned>
-__global__ void __launch_bounds__(RowPlace<TPR>::kThreads)
+__global__ void __launch_bounds__(RowPlace<TPR>::kThreads, (sizeof(T) == 2 ? 768 : 512) / RowPlace<TPR>::kThreads)
 layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias,
                            uint8_t* __restrict__ codes, bf16* __restrict__ scales, long long rows, long long cols, int sub_bits,
                            double inv_cols, double eps) {
@@ -305,7 +305,7 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
       ordinary = scale_is_ordinary(s);
       inv = about_inverse(s);
       delta = error * inv + kTop * kError;
-      return amax < __int_as_float(0x7F800000) && amax > 0.f && near_bf16_tie(quotient, error);
+      return amax < __int_as_float(0x7F800000) && amax > 0.f && near_bf16_tie(quotient, error * (2.f / kTop));
     };
     auto settled = [&](double most) {
       s = nonzero_scale(bf16_from_double(most / static_cast<double>(kTop)));
@@ -314,14 +314,16 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
     auto put = [&](int v, const float (&out)[8]) {
       const long long at = place(v);
       if (at >= cols) return;
-      uint32_t c[8], border = ordinary ? 0u : 1u;
+      uint32_t c[8];
+      float far = 0.f;  // the largest distance of a quotient from its code
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        c[i] = __float_as_uint(__fadd_rn(__fmaf_rn(out[i], inv, -delta), kRoundMagic));
-        border |= c[i] ^ __float_as_uint(__fadd_rn(__fmaf_rn(out[i], inv, delta), kRoundMagic));
+        const float code = __fmaf_rn(out[i], inv, kRoundMagic);
+        far = fmaxf(far, fabsf(__fmaf_rn(out[i], inv, -__fsub_rn(code, kRoundMagic))));
+        c[i] = __float_as_uint(code);
       }
       typename CodeWords<BITS>::type packed = CodeWords<BITS>::pack(c);
-      if (border) {
+      if (!(ordinary && far < 0.5f - delta)) {
         const unsigned long long exactly = exact_codes<T, W, BITS>(row, weight, bias, at, cols, exact, s);
         memcpy(&packed, &exactly, sizeof(packed));
       }
