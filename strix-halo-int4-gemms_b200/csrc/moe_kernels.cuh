@@ -54,7 +54,8 @@ struct MoeParams {
   double* logits;           // [tokens, experts]
   int* pair_expert;         // [pairs], -1: no expert
   float* pair_weight;       // [pairs]
-  int* active;              // {experts in use, total cost}; then slots of {expert, first pair, pairs, cost of those before}
+  int* active;              // {experts in use, passes in all, units handed out by the two products}; then slots of
+                            // {expert, first pair, pairs, passes of those before}
   int* pair_list;           // [pairs], by expert
   double* act;              // [pairs, inner]
   uint8_t* aq;              // [pairs, inner bytes]
@@ -62,14 +63,6 @@ struct MoeParams {
   void* part;               // [down_splits, pairs, hidden]: sums of the codes' products (int32), or scaled ones (fp64)
   int slots, up_ranges, down_ranges, down_splits;
 };
-
-// Relative time of a column range of an expert with `count` rows, by which work is divided among the blocks: a pass for up
-// to 8 rows is bound by the weights' bytes, one for more of them by its matrix instructions.
-__host__ __device__ constexpr int moe_pass_cost(int rows) { return rows <= 8 ? 14 : rows <= 16 ? 17 : rows <= 24 ? 21 : 26; }
-__device__ __forceinline__ int moe_cost(int count, int rows_a_pass) {
-  const int whole = count / rows_a_pass, rest = count - whole * rows_a_pass;
-  return whole * moe_pass_cost(rows_a_pass) + (rest > 0 ? moe_pass_cost(rest) : 0);
-}
 
 template <int DT>
 __device__ __forceinline__ long long code_bytes(long long k) { return DT == 4 ? k / 2 : k; }
@@ -276,11 +269,11 @@ __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) 
     place[k] = i < pairs && chosen[i] >= 0 ? atomicAdd(&count[chosen[i]], 1) : 0;  // the order within an expert changes no result
   }
   __syncthreads();
-  // scan over the experts, THREADS at a time: pairs (low half) and experts in use (high half) before, and their cost
+  // scan over the experts, THREADS at a time: pairs (low half) and experts in use (high half) before, and their passes
   int2 carry = make_int2(0, 0);
   for (int base = 0; base < PER * 32; base += THREADS) {
     const int e = base + threadIdx.x, mine = e < PER * 32 ? count[e] : 0;
-    const int2 here = make_int2(mine + (mine > 0 ? 1 << 16 : 0), mine > 0 ? moe_cost(mine, p.rows_a_pass) : 0);
+    const int2 here = make_int2(mine + (mine > 0 ? 1 << 16 : 0), (mine + p.rows_a_pass - 1) / p.rows_a_pass);
     int2 sum = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -382,16 +375,6 @@ struct MoeSum<true> {
 constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
 
-// What a block knows of its product: columns of weight codes times the codes of some tokens or pairs.
-struct MoeTile {
-  const uint8_t* w;       // the expert's matrix
-  const bf16* w_scale;    // the expert's scales: [N] or [groups, N]
-  const uint8_t* codes;   // of all tokens or pairs
-  const float* scales;
-  int k, n;               // K, and N of the matrix (2 * inner for up/gate)
-  int groups;
-};
-
 // A block works on a range of columns at a time: 32 (K-major weights, NT) or 128 (N-major, NN), for up/gate half of
 // them up columns and half the same columns of the gate.  Its eight warps divide K into shares and, for NN, the
 // columns into halves; a warp has kFrags fragments of 16 columns.
@@ -426,326 +409,6 @@ __device__ __forceinline__ double exact_double(int v) {
 template <int kN>
 __device__ __forceinline__ int sum_place(int frag, int n, int j, int lane) {
   return (((frag * kN + n) * 4 + j) << 5) + (lane ^ ((frag * 4 + j) & 31));
-}
-
-// The column ranges of one expert (and part of K) in the order of work: `run` consecutive positions are every
-// `stride`-th range, so that blocks that work on neighbouring runs at the same time read neighbouring columns: a row of
-// N-major weights is then read in long pieces, not in 64-byte ones a range apart (1.5 times as fast at 14336 columns).
-// Positions whose range does not exist are passed over.
-struct MoeOrder {
-  int ranges, run, stride;
-  __device__ __forceinline__ MoeOrder(int n, int per_block) {
-    ranges = n;
-    run = max(1, min(n, per_block));
-    stride = (n + run - 1) / run;
-  }
-  __device__ __forceinline__ int positions() const { return run * stride; }
-  __device__ __forceinline__ int range(int position) const { return position % run * stride + position / run; }
-};
-
-// Positions [pos0, pos1) and steps [step0, step1) of K of one expert for the `count` <= 8 kN tokens in `rows`.
-// `before_codes` runs between the first weight copies and the first use of `rows` and the codes.  For every range all
-// threads call `begin(range)` before the products, `publish()` between them and a barrier, and then
-// `finish(range, begun, sum)` with the sums at hand: sum(c, t, gate) for its column c and token t.
-template <int DT, bool NN, bool SC, int WORDS, int kN, bool kDown, typename Before, typename Begin, typename Publish, typename Finish>
-__device__ __forceinline__ void moe_pass(const MoeParams& p, const MoeTile& tile, const MoeOrder& order, int pos0, int pos1, int step0,
-                                         int step1, const int* rows, int count, uint8_t* smem, Before&& before_codes, Begin&& begin_range,
-                                         Publish&& publish, Finish&& finish) {
-  using Stage = MoeStage<DT, NN, SC, WORDS, kN>;
-  using Sum = typename Stage::Sum;
-  constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
-  constexpr int kStepBytes = Stage::kStepBytes;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int half = NN ? warp & 1 : 0, share = NN ? warp >> 1 : warp;
-  const int gate = tile.n / 2;  // where the gate columns start
-  // NN: consecutive steps (whole groups of K as far as it goes); NT: every eighth
-  const int steps = step1 - step0, per_share = (steps + kShares - 1) / kShares;
-  const int begin = step0 + (NN ? share * per_share : share), by = NN ? 1 : kShares;
-  const int mine = NN ? max(0, min(steps - share * per_share, per_share)) : max(0, (steps - share + kShares - 1) / kShares);
-  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kStages * Stage::kBytes;
-  const uint8_t* ring = smem + warp * kStages * Stage::kBytes;
-  Sum* sums = reinterpret_cast<Sum*>(smem + Stage::kRingBytes);
-  const long long code_pitch = code_bytes<DT>(tile.k);
-
-  // first column of a fragment of this warp in a range; NN: whether the matrix has it (16 columns at a time)
-  auto column_of = [&](int range, int f) {
-    const int frag = half * kFrags + f;
-    if (kDown) return range * Stage::kCols + frag * 16;
-    return frag < kAllFrags / 2 ? range * (Stage::kCols / 2) + frag * 16 : gate + range * (Stage::kCols / 2) + (frag - kAllFrags / 2) * 16;
-  };
-  auto column_valid = [&](int range, int f) {
-    if (!NN) return true;
-    if (kDown) return column_of(range, f) < tile.n;
-    return range * (Stage::kCols / 2) + (half * kFrags + f) % (kAllFrags / 2) * 16 < gate;
-  };
-
-  // What is copied next: step `i` of `range` into the stage at `to`.  The weight pointer moves on by additions.
-  struct Cursor {
-    int pos, range, i, slot;
-    const uint8_t* w;   // of this lane at step i
-    const bf16* scale;  // of this lane's columns in the first group of K
-    bool valid, scale_valid;
-  } next;
-  const long long w_step = NN ? static_cast<long long>(by) * kStepBytes * tile.n : static_cast<long long>(by) * kStepBytes;
-  const long long w_rows = NN ? 8LL * tile.n : 8 * code_pitch;                                     // to the next of a lane's loads
-  const long long w_frag = NN ? 0 : (kDown ? 16LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its second fragment
-  auto enter_range = [&]() {
-    for (; next.pos < pos1; ++next.pos) {
-      next.range = order.range(next.pos);
-      if (next.range < order.ranges) break;
-    }
-    if (next.pos >= pos1) return;
-    if constexpr (NN) {
-      next.valid = column_valid(next.range, lane & 3);
-      next.w = tile.w + (next.valid ? column_of(next.range, lane & 3) : 0) + (static_cast<long long>(begin) * kStepBytes + (lane >> 2)) * tile.n;
-      if (SC) {
-        next.scale_valid = column_valid(next.range, lane >> 3);
-        next.scale = tile.w_scale + (next.scale_valid ? column_of(next.range, lane >> 3) + (lane & 7) * 2 : 0);
-      }
-    } else {
-      next.w = tile.w + (column_of(next.range, 0) + g) * code_pitch + static_cast<long long>(begin) * kStepBytes + q * 4 * WORDS;
-      if (SC) next.scale = tile.w_scale + column_of(next.range, (lane >> 3) & 1) + (lane & 7) * 2;
-    }
-  };
-  auto start = [&]() {
-    next.pos = pos0;
-    next.i = next.slot = 0;
-    enter_range();
-  };
-  auto advance = [&]() {
-    if (++next.slot == kStages) next.slot = 0;
-    next.w += w_step;
-    if (++next.i == mine) {
-      next.i = 0;
-      ++next.pos;
-      enter_range();
-    }
-  };
-  auto copy_weights = [&]() {
-    const uint32_t at = ring_at + next.slot * Stage::kBytes;
-    if constexpr (NN) {
-      // 16 bytes of row r and fragment f to place r * 4 + (f ^ (r / 2 % 4)): eight rows of a fragment on eight banks
-      const uint8_t* src = next.w;
-      const uint32_t to = at + ((lane >> 2) * 4 + ((lane & 3) ^ ((lane >> 3) & 3))) * 16;
-      // the last step may reach beyond K, which is a multiple of 32: by whole groups of eight rows
-      const int rows_left = static_cast<int>(code_pitch) - (begin + next.i * by) * kStepBytes;
-#pragma unroll
-      for (int l = 0; l < kStepBytes / 8; ++l, src += w_rows) {
-        const bool valid = next.valid && l * 8 < rows_left;
-        copy_async<16>(to + l * 512, valid ? src : tile.w, valid);
-      }
-    } else {
-      const bool valid = (begin + next.i * by) * Stage::kStepK + q * (Stage::kStepK / 4) < tile.k;
-#pragma unroll
-      for (int l = 0; l < 4; ++l)  // fragment l / 2, rows g and g + 8
-        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, valid ? next.w + ((l & 1) ? w_rows : 0) + ((l & 2) ? w_frag : 0) : tile.w, valid);
-    }
-    if constexpr (SC) {
-      const long long group = static_cast<long long>((begin + next.i * by) * Stage::kStepK / p.sub) * tile.n;
-      if (NN || lane < 16) copy_async<4>(at + Stage::kScalesAt + lane * 4, next.scale + group, !NN || next.scale_valid);
-    }
-  };
-  const uint8_t* codes[kN];  // of this lane's tokens, at its first step
-  bool has_token[kN];
-  const float* row_scale = tile.scales;
-  auto enter_rows = [&]() {
-#pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      has_token[n] = n * 8 + g < count;
-      codes[n] = tile.codes + (has_token[n] ? rows[n * 8 + g] * code_pitch : 0) + static_cast<long long>(begin) * kStepBytes + q * 4 * WORDS;
-    }
-    if (SC && lane < count && lane < kN * 8) row_scale = tile.scales + static_cast<long long>(rows[lane]) * tile.groups;
-  };
-  auto copy_codes = [&]() {
-    const uint32_t at = ring_at + next.slot * Stage::kBytes;
-    const int step = begin + next.i * by, offset = next.i * by * kStepBytes;
-    const bool in_k = step * Stage::kStepK + q * (Stage::kStepK / 4) < tile.k;
-#pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const bool valid = in_k && has_token[n];
-      copy_async<4 * WORDS>(at + Stage::kWeights + (n * 32 + lane) * 4 * WORDS, valid ? codes[n] + offset : tile.codes, valid);
-    }
-    if constexpr (SC) {
-      if (lane < kN * 8) copy_async<4>(at + Stage::kRowScalesAt + lane * 4, row_scale + step * Stage::kStepK / p.sub, lane < count);
-    }
-  };
-
-  start();
-#pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (mine > 0 && next.pos < pos1) {
-      copy_weights();
-      advance();
-    }
-  }
-  if constexpr (!SC)  // integers are added to what lies here
-    for (int i = threadIdx.x; i < Stage::kSums; i += kMoeThreads) sums[i] = 0;
-  before_codes();  // holds a barrier
-  enter_rows();
-  start();
-#pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (mine > 0 && next.pos < pos1) {
-      copy_codes();
-      advance();
-    }
-    copy_commit();
-  }
-
-  int slot = 0;
-  for (int pos = pos0; pos < pos1; ++pos) {
-    const int range = order.range(pos);
-    if (range >= order.ranges) continue;
-    const auto begun = begin_range(range);
-    int acc[kFrags][kN][4];
-    double sum[SC ? kFrags : 1][SC ? kN : 1][4];
-#pragma unroll
-    for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-      for (int n = 0; n < kN; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[f][n][i] = 0;
-          if (SC) sum[f][n][i] = 0.0;
-        }
-#pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
-      copy_wait<kStages - 2>();
-      __syncwarp();  // what the other lanes have copied
-      const uint8_t* stage = ring + slot * Stage::kBytes;
-      uint32_t x[kN][4];
-#pragma unroll
-      for (int n = 0; n < kN; ++n) read_words<WORDS>(x[n], stage + Stage::kWeights + (n * 32 + lane) * 4 * WORDS);
-      if constexpr (NN) {
-        const uint32_t at = ring_at + slot * Stage::kBytes;
-        // Row rho = 4 q' + i of a matrix holds byte i of a word of lane q' of each quad, which is row
-        // q' * 4 * WORDS + (4 * word) + i of the stage.  Lanes 0 .. 15 name the rows of the first matrix, the others
-        // those of the second: the same word of two fragments (packed), or two words of one (int8).
-        const int rho = lane & 15, second = lane >> 4;
-        const int row0 = (rho >> 2) * 4 * WORDS + (rho & 3);
-        if constexpr (DT == 4) {
-#pragma unroll
-          for (int word = 0; word < WORDS; ++word) {
-            const int r = row0 + 4 * word;
-            const uint32_t line = at + r * 64;
-            const int flip = (r >> 1) & 3;
-            uint32_t even_x[kN], odd_x[kN];
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-              even_x[n] = even_codes(x[n][word]);
-              odd_x[n] = odd_codes(x[n][word]);
-            }
-#pragma unroll
-            for (int l = 0; l < kFrags / 2; ++l) {
-              uint32_t m[4];
-              load_transposed(m, line + (((2 * l + second) ^ flip) << 4));
-#pragma unroll
-              for (int n = 0; n < kN; ++n) mma_i8(acc[2 * l][n], even_codes(m[0]), even_codes(m[1]), odd_codes(m[0]), odd_codes(m[1]), even_x[n], odd_x[n]);
-#pragma unroll
-              for (int n = 0; n < kN; ++n) mma_i8(acc[2 * l + 1][n], even_codes(m[2]), even_codes(m[3]), odd_codes(m[2]), odd_codes(m[3]), even_x[n], odd_x[n]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int word = 0; word < WORDS; word += 2) {
-            const int r = row0 + 4 * (word + second);
-            const uint32_t line = at + r * 64;
-            const int flip = (r >> 1) & 3;
-#pragma unroll
-            for (int f = 0; f < kFrags; ++f) {
-              uint32_t m[4];
-              load_transposed(m, line + ((f ^ flip) << 4));
-#pragma unroll
-              for (int n = 0; n < kN; ++n) mma_i8(acc[f][n], m[0], m[1], m[2], m[3], x[n][word], x[n][word + 1]);
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int f = 0; f < kFrags; ++f) {
-          uint32_t wa[4], wb[4];
-          read_words<WORDS>(wa, stage + (2 * f * 32 + lane) * 4 * WORDS);
-          read_words<WORDS>(wb, stage + ((2 * f + 1) * 32 + lane) * 4 * WORDS);
-          if constexpr (DT == 4) {
-#pragma unroll
-            for (int j = 0; j < WORDS; ++j)
-#pragma unroll
-              for (int n = 0; n < kN; ++n)
-                mma_i8(acc[f][n], even_codes(wa[j]), even_codes(wb[j]), odd_codes(wa[j]), odd_codes(wb[j]), even_codes(x[n][j]), odd_codes(x[n][j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < WORDS; j += 2)
-#pragma unroll
-              for (int n = 0; n < kN; ++n) mma_i8(acc[f][n], wa[j], wb[j], wa[j + 1], wb[j + 1], x[n][j], x[n][j + 1]);
-          }
-        }
-      }
-      if constexpr (SC) {
-        // the integers of a group of K end here: scaled and added up in fp64 (a step lies in one group)
-        if (i + 1 == mine || !NN || ((begin + i + 1) * Stage::kStepK) % p.sub == 0) {
-          const bf16* w_scales = reinterpret_cast<const bf16*>(stage + Stage::kScalesAt);
-          const float* row_scales = reinterpret_cast<const float*>(stage + Stage::kRowScalesAt);
-#pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            const float2 st = *reinterpret_cast<const float2*>(row_scales + n * 8 + 2 * q);
-            const double st0 = st.x, st1 = st.y;
-#pragma unroll
-            for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const double sw = to_f32(w_scales[f * 16 + g + h * 8]);
-                const int a = acc[f][n][2 * h], b = acc[f][n][2 * h + 1];
-                sum[f][n][2 * h] = fma(exact_double(DT == 4 ? a >> 8 : a), st0 * sw, sum[f][n][2 * h]);
-                sum[f][n][2 * h + 1] = fma(exact_double(DT == 4 ? b >> 8 : b), st1 * sw, sum[f][n][2 * h + 1]);
-                acc[f][n][2 * h] = acc[f][n][2 * h + 1] = 0;
-              }
-          }
-        }
-      }
-      __syncwarp();  // before the stage that was read a step ago is written again
-      if (next.pos < pos1) {
-        copy_weights();
-        copy_codes();
-        advance();
-      }
-      copy_commit();
-      if (++slot == kStages) slot = 0;
-    }
-    publish();
-    if constexpr (!SC) {  // exact integers, in any order
-#pragma unroll
-      for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) atomicAdd(sums + sum_place<kN>(half * kFrags + f, n, j, lane), DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]);
-      __syncthreads();
-    } else {  // one share after the other
-      for (int turn = 0; turn < kShares; ++turn) {
-        if (share == turn) {
-#pragma unroll
-          for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-            for (int n = 0; n < kN; ++n)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                Sum* at = sums + sum_place<kN>(half * kFrags + f, n, j, lane);
-                *at = turn == 0 ? sum[f][n][j] : *at + sum[f][n][j];
-              }
-        }
-        __syncthreads();
-      }
-    }
-    finish(range, begun, [&](int c, int t, bool gate_part) -> Sum {
-      const int column = c + (gate_part ? Stage::kCols / 2 : 0);
-      const int place = sum_place<kN>(column >> 4, t >> 3, ((column >> 3) & 1) * 2 + (t & 1), (column & 7) * 4 + ((t & 7) >> 1));
-      const Sum total = sums[place];
-      if constexpr (!SC) sums[place] = 0;  // for the next range
-      return total;
-    });
-    __syncthreads();
-  }
-  copy_wait<0>();
 }
 
 // Quantises the activations of one pair (fp64 in, as they were computed): what quantize_tokens does, with values that
@@ -866,136 +529,418 @@ __global__ void __launch_bounds__(kMoeQuantThreads) moe_quantize_kernel(const Mo
   }
 }
 
-// The grid is as large as the device holds at once; the units of work, (expert in use, part of K, column range), whose
-// number only the device knows, are divided among its blocks by their cost, consecutive ones to a block.
+// A unit of work: a column range of an expert in use, for one part of K and up to 8 kMaxN of its rows.
+struct MoeUnit {
+  int first, here;    // its pairs: list + first, `here` of them
+  int range, split;
+  int expert;
+  int begin, mine;    // steps of K of this warp: begin, begin + by, ...
+};
+
+// What a lane reads of the weights of a unit, at its warp's first step.
+struct MoeSource {
+  const uint8_t* w;
+  const bf16* scale;  // of its columns in the first group of K
+  bool valid, scale_valid;
+};
+
+// The grid is as large as the device holds at once.  Units are handed out in order, so that blocks that run at the same
+// time read neighbouring columns (a row of N-major weights in long pieces) and light and heavy ones even out: a block's
+// first two by its number, the others by a counter, two units ahead of their use.  When a warp has done the last step
+// of a unit it starts the copies of its weights of the next one, before the sums are finished.
 // kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
 template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
 __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_product_kernel(const MoeParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
+  using Stage = MoeStage<DT, NN, SC, WORDS, kMaxN>;
+  using Sum = typename Stage::Sum;
+  constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
+  constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
   constexpr int kHead = 64;  // slots whose records are read at once
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int4 head[1 + kHead];
-  __shared__ int rows[kMaxN * 8], pair_of[kMaxN * 8];
-  __shared__ float row_scale[kMaxN * 8];
-  using Sum = typename MoeSum<SC>::type;
-  constexpr int kCols = NN ? 128 : 32, out_cols = kDown ? kCols : kCols / 2;
-  constexpr int kStepK = 4 * WORDS * (DT == 4 ? 8 : 4);
+  __shared__ int rows[2][kMaxN * 8], pair_of[2][kMaxN * 8];
+  __shared__ float row_scale[2][kMaxN * 8];
+  __shared__ int unit_after_next;
   if (!kDown) {
     grid_wait();
     grid_release();
   }
-  const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges, splits = kDown ? p.down_splits : 1;
   // written by the select kernel, which had ended before the up/gate product let the next kernels start
   const int4* records = reinterpret_cast<const int4*>(p.active);
   if (threadIdx.x < min(1 + kHead, 1 + p.slots)) head[threadIdx.x] = __ldcg(records + threadIdx.x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+  const int half = NN ? warp & 1 : 0, share = NN ? warp >> 1 : warp;
+  const int k = kDown ? p.inner : p.hidden, columns = kDown ? p.hidden : 2 * p.inner, gate = p.inner;  // gate columns start there
+  const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges, splits = kDown ? p.down_splits : 1;
+  const int groups = SC ? (k + p.sub - 1) / p.sub : 1, steps = (k + kStepK - 1) / kStepK;
+  const long long code_pitch = code_bytes<DT>(k);
+  const uint8_t* all_codes = kDown ? p.aq : p.xq;
+  const float* all_scales = kDown ? p.as : p.xs;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kStages * Stage::kBytes;
+  const uint8_t* ring = smem + warp * kStages * Stage::kBytes;
+  Sum* sums = reinterpret_cast<Sum*>(smem + Stage::kRingBytes);
+  if constexpr (!SC)  // integers are added to what lies here
+    for (int i = threadIdx.x; i < Stage::kSums; i += kMoeThreads) sums[i] = 0;
   __syncthreads();
-  auto record = [&](int slot) { return slot < kHead ? head[1 + slot] : __ldcg(records + 1 + slot); };
-  const int in_use = head[0].x, total_cost = head[0].y;
-  const unsigned units = static_cast<unsigned>(in_use) * splits * ranges;
-  const MoeOrder order(ranges, static_cast<int>(units / gridDim.x));
-  const int slot_units = splits * order.positions();
-  // The unit at which block b starts: the first whose cost lies at or behind b / blocks of the whole.
-  auto start_of = [&](unsigned b, int& slot, int& unit) {
-    const unsigned long long target = static_cast<unsigned long long>(total_cost) * slot_units * b / gridDim.x;
-    const unsigned cost = static_cast<unsigned>(target / slot_units);
-    int low = 0, high = in_use;  // the last slot that starts at or before the target
+  const int in_use = head[0].x, units = head[0].y * splits * ranges;
+  int* counter = p.active + (kDown ? 3 : 2);
+
+  // NN: consecutive steps (whole groups of K as far as it goes); NT: every eighth
+  constexpr bool kConsecutive = NN;
+  const int by = kConsecutive ? 1 : kShares;
+  auto decode = [&](int u) {
+    MoeUnit unit;
+    const int pass = u / (splits * ranges), rest = u - pass * splits * ranges;
+    unit.split = splits == 1 ? 0 : rest / ranges;
+    unit.range = rest - unit.split * ranges;
+    int low = 0, high = in_use;  // the last slot whose passes start at or before this one
+    auto record = [&](int slot) { return slot < kHead ? head[1 + slot] : __ldcg(records + 1 + slot); };
     while (high - low > 1) {
-      const int middle = (low + high) / 2;
-      if (static_cast<unsigned>(record(middle).w) <= cost) low = middle;
+      const int middle = (low + high) >> 1;
+      if (record(middle).w <= pass) low = middle;
       else high = middle;
     }
-    slot = low;
-    if (in_use == 0) {
-      unit = 0;
-      return;
-    }
     const int4 r = record(low);
-    const unsigned each = moe_cost(r.z, kMaxN * 8);
-    unit = static_cast<int>(min(static_cast<unsigned long long>(slot_units), (target - static_cast<unsigned long long>(r.w) * slot_units + each - 1) / each));
+    const int done = (pass - r.w) * kMaxN * 8;
+    unit.expert = r.x;
+    unit.first = r.y + done;
+    unit.here = min(kMaxN * 8, r.z - done);
+    const int step0 = steps * unit.split / splits, count = steps * (unit.split + 1) / splits - step0, per_share = (count + kShares - 1) / kShares;
+    unit.begin = step0 + (kConsecutive ? share * per_share : share);
+    unit.mine = kConsecutive ? max(0, min(count - share * per_share, per_share)) : max(0, (count - share + kShares - 1) / kShares);
+    return unit;
   };
-  int slot, unit, last_slot, last_unit;
-  start_of(blockIdx.x, slot, unit);
-  start_of(blockIdx.x + 1, last_slot, last_unit);
-  if (blockIdx.x + 1 == gridDim.x) {
-    last_slot = in_use;
-    last_unit = 0;
-  }
-  bool waited = !kDown;
-  MoeTile tile;
-  tile.k = kDown ? p.inner : p.hidden;
-  tile.n = kDown ? p.hidden : 2 * p.inner;
-  tile.groups = SC ? (tile.k + p.sub - 1) / p.sub : 1;
-  tile.codes = kDown ? p.aq : p.xq;
-  tile.scales = kDown ? p.as : p.xs;
-  const int steps = (tile.k + kStepK - 1) / kStepK;
-  const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
-  const int c = threadIdx.x % out_cols;  // a thread's outputs are all of one column of a range
-  while (slot < last_slot || (slot == last_slot && unit < last_unit)) {
-    if (unit >= slot_units) {
-      ++slot;
-      unit = 0;
-      continue;
+  // first column of a fragment of this warp in a range; NN: whether the matrix has it (16 columns at a time)
+  auto column_of = [&](int range, int f) {
+    const int frag = half * kFrags + f;
+    if (kDown) return range * kCols + frag * 16;
+    return frag < kAllFrags / 2 ? range * (kCols / 2) + frag * 16 : gate + range * (kCols / 2) + (frag - kAllFrags / 2) * 16;
+  };
+  auto column_valid = [&](int range, int f) {
+    if (!NN) return true;
+    if (kDown) return column_of(range, f) < columns;
+    return range * (kCols / 2) + (half * kFrags + f) % (kAllFrags / 2) * 16 < gate;
+  };
+  const long long w_step = NN ? static_cast<long long>(by) * kStepBytes * columns : static_cast<long long>(by) * kStepBytes;
+  const long long w_rows = NN ? 8LL * columns : 8 * code_pitch;                                    // to the next of a lane's loads
+  const long long w_frag = NN ? 0 : (kDown ? 16LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its second fragment
+  const uint8_t* all_weights = kDown ? p.w_down : p.w_up_gate;
+  const bf16* all_weight_scales = kDown ? p.s_down : p.s_up_gate;
+  auto source_of = [&](const MoeUnit& unit) {
+    MoeSource source;
+    const uint8_t* matrix = all_weights + static_cast<long long>(unit.expert) * columns * code_pitch;
+    const bf16* scales = all_weight_scales + static_cast<long long>(unit.expert) * columns * groups;
+    source.valid = source.scale_valid = true;
+    source.scale = scales;
+    if constexpr (NN) {
+      source.valid = column_valid(unit.range, lane & 3);
+      source.w = matrix + (source.valid ? column_of(unit.range, lane & 3) : 0) + (static_cast<long long>(unit.begin) * kStepBytes + (lane >> 2)) * columns;
+      if (SC) {
+        source.scale_valid = column_valid(unit.range, lane >> 3);
+        source.scale = scales + (source.scale_valid ? column_of(unit.range, lane >> 3) + (lane & 7) * 2 : 0);
+      }
+    } else {
+      source.w = matrix + (column_of(unit.range, 0) + g) * code_pitch + static_cast<long long>(unit.begin) * kStepBytes + q * 4 * WORDS;
+      if (SC) source.scale = scales + column_of(unit.range, (lane >> 3) & 1) + (lane & 7) * 2;
     }
-    const int split = unit / order.positions(), pos0 = unit % order.positions();
-    const int end = min(slot == last_slot ? last_unit : slot_units, (split + 1) * order.positions());
-    const int pos1 = pos0 + end - unit;
-    unit = end;
-    const int step0 = static_cast<int>(static_cast<long long>(steps) * split / splits), step1 = static_cast<int>(static_cast<long long>(steps) * (split + 1) / splits);
-    const int4 r = record(slot);  // {expert, first pair, pairs, ...}
-    const int* list = p.pair_list + r.y;
-    tile.w = (kDown ? p.w_down : p.w_up_gate) + static_cast<long long>(r.x) * tile.n * code_bytes<DT>(tile.k);
-    tile.w_scale = (kDown ? p.s_down : p.s_up_gate) + static_cast<long long>(r.x) * tile.n * tile.groups;
-    for (int done = 0; done < r.z; done += kMaxN * 8) {
-      const int here = min(kMaxN * 8, r.z - done);
-      float my_scale = 1.f;  // of a token; written for the others when a range is finished
-      auto before_codes = [&]() {
-        if (!waited) grid_wait();
-        waited = true;
-        if (threadIdx.x < here) {
-          const int pair = __ldcg(list + done + threadIdx.x), row = kDown ? pair : pair / p.top_k;
-          pair_of[threadIdx.x] = pair;
-          rows[threadIdx.x] = row;
-          if (!SC && !kDown) my_scale = __ldcg(tile.scales + row);
+    return source;
+  };
+  // step `i` of a warp's steps of a unit; source.w moves on with every call
+  auto copy_weights = [&](const MoeUnit& unit, MoeSource& source, int i, int slot) {
+    const uint32_t at = ring_at + slot * Stage::kBytes;
+    const int step = unit.begin + i * by;
+    if constexpr (NN) {
+      // 16 bytes of row r and fragment f to place r * 4 + (f ^ (r / 2 % 4)): eight rows of a fragment on eight banks
+      const uint8_t* src = source.w;
+      const uint32_t to = at + ((lane >> 2) * 4 + ((lane & 3) ^ ((lane >> 3) & 3))) * 16;
+      // the last step may reach beyond K, which is a multiple of 32: by whole groups of eight rows
+      const int rows_left = static_cast<int>(code_pitch) - step * kStepBytes;
+#pragma unroll
+      for (int l = 0; l < kStepBytes / 8; ++l, src += w_rows) {
+        const bool valid = source.valid && l * 8 < rows_left;
+        copy_async<16>(to + l * 512, valid ? src : all_weights, valid);
+      }
+    } else {
+      const bool valid = step * kStepK + q * (kStepK / 4) < k;
+#pragma unroll
+      for (int l = 0; l < 4; ++l)  // fragment l / 2, rows g and g + 8
+        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, valid ? source.w + ((l & 1) ? w_rows : 0) + ((l & 2) ? w_frag : 0) : all_weights, valid);
+    }
+    if constexpr (SC) {
+      const long long group = static_cast<long long>(step * kStepK / p.sub) * columns;
+      if (NN || lane < 16) copy_async<4>(at + Stage::kScalesAt + lane * 4, source.scale + group, source.scale_valid);
+    }
+    source.w += w_step;
+  };
+  // the pairs of a unit: read by its first threads, written down when the buffer is free
+  auto read_pair = [&](const MoeUnit& unit) { return threadIdx.x < unit.here ? __ldcg(p.pair_list + unit.first + threadIdx.x) : 0; };
+  auto write_pair = [&](const MoeUnit& unit, int pair, int buffer) {
+    if (threadIdx.x < unit.here) {
+      const int row = kDown ? pair : pair / p.top_k;
+      pair_of[buffer][threadIdx.x] = pair;
+      rows[buffer][threadIdx.x] = row;
+    }
+  };
+
+  MoeUnit unit, next;
+  MoeSource source{};
+  int slot = 0;        // of the ring: the stage of the step that is worked on
+  int buffer = 0;
+  int number = blockIdx.x, next_number = blockIdx.x + gridDim.x;
+  if (number < units) {
+    unit = decode(number);
+    source = source_of(unit);
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i)
+      if (i < unit.mine) copy_weights(unit, source, i, i);
+  }
+  if (kDown) {
+    grid_wait();
+    grid_release();
+  }
+  if (number >= units) return;
+  write_pair(unit, read_pair(unit), 0);
+  __syncthreads();
+  const int c = threadIdx.x % out_cols;  // a thread's outputs are all of one column of a range
+
+  while (true) {
+    int handed_out = 0;
+    if (threadIdx.x == 0) handed_out = atomicAdd(counter, 1) + 2 * static_cast<int>(gridDim.x);
+    const bool more = next_number < units;
+    if (more) next = decode(next_number);
+    const int next_pair = more ? read_pair(next) : 0;
+    // what the finishing needs besides the sums
+    const int col = unit.range * out_cols + c;
+    float my_scale = 0.f;
+    float2 scale = make_float2(0.f, 0.f);
+    if (!SC && !kDown) {
+      if (threadIdx.x < unit.here) my_scale = __ldcg(all_scales + rows[buffer][threadIdx.x]);
+      if (col < out_n) {
+        const bf16* scales = all_weight_scales + static_cast<long long>(unit.expert) * columns + col;
+        scale = make_float2(to_f32(scales[0]), to_f32(scales[p.inner]));
+      }
+    }
+
+    auto products = [&](auto n_groups) {
+      constexpr int kN = decltype(n_groups)::value;
+      const uint8_t* codes[kN];  // of this lane's tokens, at its first step
+      bool has_token[kN];
+      const float* token_scale = all_scales;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        has_token[n] = n * 8 + g < unit.here;
+        codes[n] = all_codes + (has_token[n] ? rows[buffer][n * 8 + g] * code_pitch : 0) + static_cast<long long>(unit.begin) * kStepBytes + q * 4 * WORDS;
+      }
+      if (SC && lane < unit.here && lane < kN * 8) token_scale = all_scales + static_cast<long long>(rows[buffer][lane]) * groups;
+      auto copy_codes = [&](int i, int to_slot) {
+        const uint32_t at = ring_at + to_slot * Stage::kBytes;
+        const int step = unit.begin + i * by, offset = i * by * kStepBytes;
+        const bool in_k = step * kStepK + q * (kStepK / 4) < k;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          const bool valid = in_k && has_token[n];
+          copy_async<4 * WORDS>(at + Stage::kWeights + (n * 32 + lane) * 4 * WORDS, valid ? codes[n] + offset : all_codes, valid);
         }
-        __syncthreads();
+        if constexpr (SC) {
+          if (lane < kN * 8) copy_async<4>(at + Stage::kRowScalesAt + lane * 4, lane < unit.here ? token_scale + step * kStepK / p.sub : all_scales, lane < unit.here);
+        }
       };
-      // what a range needs besides its sums: read before the products
-      auto begin = [&](int range) {
-        const int col = range * out_cols + c;
-        float2 scale = make_float2(0.f, 0.f);
-        if (!SC && !kDown && col < out_n) scale = make_float2(to_f32(tile.w_scale[col]), to_f32(tile.w_scale[p.inner + col]));
-        return scale;
-      };
-      auto publish = [&]() {
-        if (!SC && !kDown && threadIdx.x < here) row_scale[threadIdx.x] = my_scale;
-      };
-      auto finish = [&](int range, float2 scale, auto sum) {
-        const int col = range * out_cols + c;
-        if (col >= out_n) return;
-        for (int t = threadIdx.x / out_cols; t < here; t += kMoeThreads / out_cols) {
-          if (kDown) {
-            static_cast<Sum*>(p.part)[(split * pairs + rows[t]) * p.hidden + col] = sum(c, t, false);
-          } else {
-            double up = static_cast<double>(sum(c, t, false)), gate = static_cast<double>(sum(c, t, true));
-            if (!SC) {
-              const float s = row_scale[t];
-              up *= static_cast<double>(s * scale.x);  // a product of two bf16 numbers is exact in fp32
-              gate *= static_cast<double>(s * scale.y);
+      int ahead = slot;  // the stage that is copied to next
+#pragma unroll 1
+      for (int i = 0; i < kStages - 1; ++i) {
+        if (i < unit.mine) copy_codes(i, ahead);
+        copy_commit();
+        if (++ahead == kStages) ahead = 0;
+      }
+      int acc[kFrags][kN][4];
+      double sum[SC ? kFrags : 1][SC ? kN : 1][4];
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[f][n][i] = 0;
+            if (SC) sum[f][n][i] = 0.0;
+          }
+#pragma unroll 1
+      for (int i = 0; i < unit.mine; ++i) {
+        copy_wait<kStages - 2>();
+        __syncwarp();  // what the other lanes have copied
+        const uint8_t* stage = ring + slot * Stage::kBytes;
+        uint32_t x[kN][4];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) read_words<WORDS>(x[n], stage + Stage::kWeights + (n * 32 + lane) * 4 * WORDS);
+        if constexpr (NN) {
+          const uint32_t at = ring_at + slot * Stage::kBytes;
+          // Row rho = 4 q' + i of a matrix holds byte i of a word of lane q' of each quad, which is row
+          // q' * 4 * WORDS + (4 * word) + i of the stage.  Lanes 0 .. 15 name the rows of the first matrix, the others
+          // those of the second: the same word of two fragments (packed), or two words of one (int8).
+          const int rho = lane & 15, second = lane >> 4;
+          const int row0 = (rho >> 2) * 4 * WORDS + (rho & 3);
+          if constexpr (DT == 4) {
+#pragma unroll
+            for (int word = 0; word < WORDS; ++word) {
+              const int r = row0 + 4 * word;
+              const uint32_t line = at + r * 64;
+              const int flip = (r >> 1) & 3;
+              uint32_t even_x[kN], odd_x[kN];
+#pragma unroll
+              for (int n = 0; n < kN; ++n) {
+                even_x[n] = even_codes(x[n][word]);
+                odd_x[n] = odd_codes(x[n][word]);
+              }
+#pragma unroll
+              for (int l = 0; l < kFrags / 2; ++l) {
+                uint32_t m[4];
+                load_transposed(m, line + (((2 * l + second) ^ flip) << 4));
+#pragma unroll
+                for (int n = 0; n < kN; ++n) mma_i8(acc[2 * l][n], even_codes(m[0]), even_codes(m[1]), odd_codes(m[0]), odd_codes(m[1]), even_x[n], odd_x[n]);
+#pragma unroll
+                for (int n = 0; n < kN; ++n) mma_i8(acc[2 * l + 1][n], even_codes(m[2]), even_codes(m[3]), odd_codes(m[2]), odd_codes(m[3]), even_x[n], odd_x[n]);
+              }
             }
-            p.act[static_cast<long long>(pair_of[t]) * p.inner + col] = up * gate / (1.0 + exp(-gate));
+          } else {
+#pragma unroll
+            for (int word = 0; word < WORDS; word += 2) {
+              const int r = row0 + 4 * (word + second);
+              const uint32_t line = at + r * 64;
+              const int flip = (r >> 1) & 3;
+#pragma unroll
+              for (int f = 0; f < kFrags; ++f) {
+                uint32_t m[4];
+                load_transposed(m, line + ((f ^ flip) << 4));
+#pragma unroll
+                for (int n = 0; n < kN; ++n) mma_i8(acc[f][n], m[0], m[1], m[2], m[3], x[n][word], x[n][word + 1]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int f = 0; f < kFrags; ++f) {
+            uint32_t wa[4], wb[4];
+            read_words<WORDS>(wa, stage + (2 * f * 32 + lane) * 4 * WORDS);
+            read_words<WORDS>(wb, stage + ((2 * f + 1) * 32 + lane) * 4 * WORDS);
+            if constexpr (DT == 4) {
+#pragma unroll
+              for (int j = 0; j < WORDS; ++j)
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+                  mma_i8(acc[f][n], even_codes(wa[j]), even_codes(wb[j]), odd_codes(wa[j]), odd_codes(wb[j]), even_codes(x[n][j]), odd_codes(x[n][j]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < WORDS; j += 2)
+#pragma unroll
+                for (int n = 0; n < kN; ++n) mma_i8(acc[f][n], wa[j], wb[j], wa[j + 1], wb[j + 1], x[n][j], x[n][j + 1]);
+            }
           }
         }
+        if constexpr (SC) {
+          // the integers of a group of K end here: scaled and added up in fp64 (a step lies in one group)
+          if (i + 1 == unit.mine || !NN || ((unit.begin + i + 1) * kStepK) % p.sub == 0) {
+            const bf16* w_scales = reinterpret_cast<const bf16*>(stage + Stage::kScalesAt);
+            const float* row_scales = reinterpret_cast<const float*>(stage + Stage::kRowScalesAt);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+              const float2 st = *reinterpret_cast<const float2*>(row_scales + n * 8 + 2 * q);
+              const double st0 = st.x, st1 = st.y;
+#pragma unroll
+              for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const double sw = to_f32(w_scales[f * 16 + g + h * 8]);
+                  const int a = acc[f][n][2 * h], b = acc[f][n][2 * h + 1];
+                  sum[f][n][2 * h] = fma(exact_double(DT == 4 ? a >> 8 : a), st0 * sw, sum[f][n][2 * h]);
+                  sum[f][n][2 * h + 1] = fma(exact_double(DT == 4 ? b >> 8 : b), st1 * sw, sum[f][n][2 * h + 1]);
+                  acc[f][n][2 * h] = acc[f][n][2 * h + 1] = 0;
+                }
+            }
+          }
+        }
+        __syncwarp();  // before the stage that was read a step ago is written again
+        if (i + kStages - 1 < unit.mine) {
+          copy_weights(unit, source, i + kStages - 1, ahead);
+          copy_codes(i + kStages - 1, ahead);
+        }
+        copy_commit();
+        if (++ahead == kStages) ahead = 0;
+        if (++slot == kStages) slot = 0;
+      }
+      // the next unit's first weights
+      __syncwarp();
+      if (more) {
+        source = source_of(next);
+        int to_slot = slot;
+#pragma unroll 1
+        for (int i = 0; i < kStages - 1; ++i) {
+          if (i < next.mine) copy_weights(next, source, i, to_slot);
+          if (++to_slot == kStages) to_slot = 0;
+        }
+      }
+      if (!SC && !kDown && threadIdx.x < unit.here) row_scale[buffer][threadIdx.x] = my_scale;
+      if (threadIdx.x == 0) unit_after_next = handed_out;
+      if constexpr (!SC) {  // exact integers, in any order
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) atomicAdd(sums + sum_place<kMaxN>(half * kFrags + f, n, j, lane), DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]);
+        __syncthreads();
+      } else {  // one share after the other
+        for (int turn = 0; turn < kShares; ++turn) {
+          if (share == turn) {
+#pragma unroll
+            for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+              for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  Sum* at = sums + sum_place<kMaxN>(half * kFrags + f, n, j, lane);
+                  *at = turn == 0 ? sum[f][n][j] : *at + sum[f][n][j];
+                }
+          }
+          __syncthreads();
+        }
+      }
+    };
+    if (kMaxN == 1 || unit.here <= 8) products(std::integral_constant<int, 1>());
+    else if (kMaxN == 2 || unit.here <= 16) products(std::integral_constant<int, kMaxN < 2 ? kMaxN : 2>());
+    else if (unit.here <= 24) products(std::integral_constant<int, kMaxN < 3 ? kMaxN : 3>());
+    else products(std::integral_constant<int, kMaxN>());
+
+    if (col < out_n) {
+      auto sum_of = [&](int t, bool gate_part) {
+        const int column = c + (gate_part ? kCols / 2 : 0);
+        const int place = sum_place<kMaxN>(column >> 4, t >> 3, ((column >> 3) & 1) * 2 + (t & 1), (column & 7) * 4 + ((t & 7) >> 1));
+        const Sum total = sums[place];
+        if constexpr (!SC) sums[place] = 0;  // for the next unit
+        return total;
       };
-      auto pass = [&](auto n) {
-        moe_pass<DT, NN, SC, WORDS, decltype(n)::value, kDown>(p, tile, order, pos0, pos1, step0, step1, rows, here, smem, before_codes, begin, publish, finish);
-      };
-      if (kMaxN == 1 || here <= 8) pass(std::integral_constant<int, 1>());
-      else if (kMaxN == 2 || here <= 16) pass(std::integral_constant<int, kMaxN < 2 ? kMaxN : 2>());
-      else if (here <= 24) pass(std::integral_constant<int, kMaxN < 3 ? kMaxN : 3>());
-      else pass(std::integral_constant<int, kMaxN>());
+      for (int t = threadIdx.x / out_cols; t < unit.here; t += kMoeThreads / out_cols) {
+        if (kDown) {
+          const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
+          static_cast<Sum*>(p.part)[(unit.split * pairs + rows[buffer][t]) * p.hidden + col] = sum_of(t, false);
+        } else {
+          double up = static_cast<double>(sum_of(t, false)), gated = static_cast<double>(sum_of(t, true));
+          if (!SC) {
+            const float s = row_scale[buffer][t];
+            up *= static_cast<double>(s * scale.x);  // a product of two bf16 numbers is exact in fp32
+            gated *= static_cast<double>(s * scale.y);
+          }
+          p.act[static_cast<long long>(pair_of[buffer][t]) * p.inner + col] = up * gated / (1.0 + exp(-gated));
+        }
+      }
     }
+    if (!more) break;
+    write_pair(next, next_pair, buffer ^ 1);
+    number = next_number;
+    next_number = unit_after_next;
+    unit = next;
+    buffer ^= 1;
+    __syncthreads();
   }
-  if (!waited) grid_wait();  // no kernel of the call ends before those in front of it
-  if (kDown) grid_release();
+  copy_wait<0>();
 }
 
 // Adds up the parts of K, scales, and adds up the experts' shares of a token in the order of its choices.  A thread has
