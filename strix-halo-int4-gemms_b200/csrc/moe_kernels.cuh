@@ -53,7 +53,7 @@ struct MoeParams {
   float* xs;                // [tokens, groups of hidden]
   double* logits;           // [tokens, experts]
   int* pair_expert;         // [pairs], -1: no expert
-  float* pair_weight;       // [pairs]
+  double* pair_logit;       // [pairs]: of the chosen experts (router != null)
   int* active;              // {experts in use, passes in all, units handed out by the two products}; then slots of
                             // {expert, first pair, pairs, passes of those before}
   int* pair_list;           // [pairs], by expert
@@ -193,7 +193,7 @@ __device__ __forceinline__ double logit_of_key(unsigned long long k) {
 }
 
 // One block of 1024 threads.  A warp picks a token's experts one after the other: the largest logit that is left,
-// ties to the lowest index (a token whose logits are NaN gets the first experts and weights of NaN).  A lane keeps
+// ties to the lowest index (a token whose logits are NaN gets the first experts).  A lane keeps
 // PER logits, of experts lane, lane + 32, ...
 template <int PER, int THREADS>
 __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) {
@@ -213,7 +213,6 @@ __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) 
         const int e = lane + 32 * i;
         key[i] = e < p.experts ? logit_key(__ldcg(p.logits + static_cast<long long>(t) * p.experts + e)) : 0ull;
       }
-      double all = 0.0;
       int mine_id = -1;
       for (int j = 0; j < p.top_k; ++j) {
         unsigned long long best = 0;
@@ -232,32 +231,19 @@ __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) 
           mine = (static_cast<unsigned long long>(top_hi) << 32) | top_lo;
           mine_id = static_cast<int>(id);
         }
-        if (j == 0 && !p.renormalize) {
-          const double top = logit_of_key((static_cast<unsigned long long>(top_hi) << 32) | top_lo);
-#pragma unroll
-          for (int i = 0; i < PER; ++i)
-            if (key[i] != 0) all += exp(logit_of_key(key[i]) - top);
-          all = warp_reduce(all, SumOp());
-        }
 #pragma unroll
         for (int i = 0; i < PER; ++i)
           if (id == static_cast<unsigned>(lane + 32 * i)) key[i] = 0;
       }
-      if (lane < p.top_k) chosen[t * p.top_k + lane] = mine_id;
-      const double logit = logit_of_key(mine), top = __shfl_sync(0xFFFFFFFFu, logit, 0);
-      const double e = lane < p.top_k ? exp(logit - top) : 0.0;
-      const double total = p.renormalize ? warp_reduce(e, SumOp()) : all;
       if (lane < p.top_k) {
-        const float weight = static_cast<float>(e / total);
-        p.pair_weight[t * p.top_k + lane] = weight;
-        if (p.weights_out != nullptr) p.weights_out[t * p.top_k + lane] = weight;
+        chosen[t * p.top_k + lane] = mine_id;
+        p.pair_logit[t * p.top_k + lane] = logit_of_key(mine);
       }
     }
   } else {
     for (int i = threadIdx.x; i < pairs; i += THREADS) {
       const long long id = p.ids_64 ? static_cast<const long long*>(p.ids_in)[i] : static_cast<const int*>(p.ids_in)[i];
       chosen[i] = id >= 0 && id < p.experts ? static_cast<int>(id) : -1;  // any other number: no expert
-      p.pair_weight[i] = p.weights_in[i];
     }
   }
   __syncthreads();
@@ -375,16 +361,16 @@ struct MoeSum<true> {
 constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
 
-// A block works on a range of columns at a time: 32 (K-major weights, NT) or 128 (N-major, NN), for up/gate half of
+// A block works on a range of columns at a time: 64 (K-major weights, NT) or 128 (N-major, NN), for up/gate half of
 // them up columns and half the same columns of the gate.  Its eight warps divide K into shares and, for NN, the
-// columns into halves; a warp has kFrags fragments of 16 columns.
+// columns into halves; a warp has four fragments of 16 columns.
 // A step is 4 * WORDS * (8 or 4) values of K, of which lane q of a quad has WORDS consecutive words of the token codes.
 // NT: and the same words of each column.  NN: rows of 64 columns, which ldmatrix transposes; the row that a lane names
 // for it puts the right values of K into each quad's words.
 // One stage of a warp's ring: weights, token codes, and (SC) the scales of the step's group of K.
 template <int DT, bool NN, bool SC, int WORDS, int kN>
 struct MoeStage {
-  static constexpr int kCols = NN ? 128 : 32, kFrags = NN ? 4 : 2, kHalves = NN ? 2 : 1, kShares = kMoeWarps / kHalves;
+  static constexpr int kCols = NN ? 128 : 64, kFrags = 4, kHalves = NN ? 2 : 1, kShares = kMoeWarps / kHalves;
   static constexpr int kStepK = 4 * WORDS * (DT == 4 ? 8 : 4), kStepBytes = 16 * WORDS;  // of a column
   static constexpr int kWeights = kFrags * 16 * kStepBytes;                              // bytes
   static constexpr int kCodeBytes = 4 * WORDS;                                           // of a token, by a lane
@@ -395,8 +381,10 @@ struct MoeStage {
   static constexpr int kStages = 8448 / kBytes < 3 ? 3 : (8448 / kBytes > 8 ? 8 : 8448 / kBytes);
   using Sum = typename MoeSum<SC>::type;
   static constexpr int kRingBytes = kMoeWarps * kStages * kBytes;
+  // integers are added in place; fp64 numbers by two shares at a time, each pair's first to one half, second to the other
   static constexpr int kSums = kFrags * kHalves * kN * 4 * 32;
-  static constexpr int kSmemBytes = kRingBytes + kSums * static_cast<int>(sizeof(Sum));
+  static constexpr int kSumParts = SC ? 2 : 1;
+  static constexpr int kSmemBytes = kRingBytes + kSums * kSumParts * static_cast<int>(sizeof(Sum));
 };
 
 // int32 -> fp64 without a conversion instruction (16 a clock and SM; the subtraction runs at 64): 2^52 + 2^31 + v, bit
@@ -610,20 +598,19 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     unit.mine = kConsecutive ? max(0, min(count - share * per_share, per_share)) : max(0, (count - share + kShares - 1) / kShares);
     return unit;
   };
-  // first column of a fragment of this warp in a range; NN: whether the matrix has it (16 columns at a time)
+  // first column of a fragment of this warp in a range, and whether the matrix has it (16 columns at a time)
   auto column_of = [&](int range, int f) {
     const int frag = half * kFrags + f;
     if (kDown) return range * kCols + frag * 16;
     return frag < kAllFrags / 2 ? range * (kCols / 2) + frag * 16 : gate + range * (kCols / 2) + (frag - kAllFrags / 2) * 16;
   };
   auto column_valid = [&](int range, int f) {
-    if (!NN) return true;
     if (kDown) return column_of(range, f) < columns;
     return range * (kCols / 2) + (half * kFrags + f) % (kAllFrags / 2) * 16 < gate;
   };
   const long long w_step = NN ? static_cast<long long>(by) * kStepBytes * columns : static_cast<long long>(by) * kStepBytes;
   const long long w_rows = NN ? 8LL * columns : 8 * code_pitch;                                    // to the next of a lane's loads
-  const long long w_frag = NN ? 0 : (kDown ? 16LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its second fragment
+  const long long w_frag = NN ? 0 : (kDown ? 32LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its third fragment
   const uint8_t* all_weights = kDown ? p.w_down : p.w_up_gate;
   const bf16* all_weight_scales = kDown ? p.s_down : p.s_up_gate;
   auto source_of = [&](const MoeUnit& unit) {
@@ -640,8 +627,11 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         source.scale = scales + (source.scale_valid ? column_of(unit.range, lane >> 3) + (lane & 7) * 2 : 0);
       }
     } else {
+      // sizes are multiples of 32: of up/gate every fragment is there, of the down product's last range maybe two
+      source.valid = column_valid(unit.range, 2);
+      source.scale_valid = column_valid(unit.range, lane >> 3);
       source.w = matrix + (column_of(unit.range, 0) + g) * code_pitch + static_cast<long long>(unit.begin) * kStepBytes + q * 4 * WORDS;
-      if (SC) source.scale = scales + column_of(unit.range, (lane >> 3) & 1) + (lane & 7) * 2;
+      source.scale = scales + (source.scale_valid ? column_of(unit.range, lane >> 3) + (lane & 7) * 2 : 0);
     }
     return source;
   };
@@ -661,14 +651,17 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         copy_async<16>(to + l * 512, valid ? src : all_weights, valid);
       }
     } else {
-      const bool valid = step * kStepK + q * (kStepK / 4) < k;
+      const bool in_k = step * kStepK + q * (kStepK / 4) < k;
 #pragma unroll
-      for (int l = 0; l < 4; ++l)  // fragment l / 2, rows g and g + 8
-        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, valid ? source.w + ((l & 1) ? w_rows : 0) + ((l & 2) ? w_frag : 0) : all_weights, valid);
+      for (int l = 0; l < 2 * kFrags; ++l) {
+        const bool valid = in_k && (l < 4 || source.valid);  // columns g and g + 8 of fragment l / 2; the second two follow by w_frag
+        const uint8_t* src = source.w + ((l & 1) ? w_rows : 0) + ((l & 2) ? 2 * w_rows : 0) + ((l & 4) ? w_frag : 0);
+        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, valid ? src : all_weights, valid);
+      }
     }
     if constexpr (SC) {
       const long long group = static_cast<long long>(step * kStepK / p.sub) * columns;
-      if (NN || lane < 16) copy_async<4>(at + Stage::kScalesAt + lane * 4, source.scale + group, source.scale_valid);
+      copy_async<4>(at + Stage::kScalesAt + lane * 4, source.scale + group, source.scale_valid);
     }
     source.w += w_step;
   };
@@ -704,22 +697,26 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   const int c = threadIdx.x % out_cols;  // a thread's outputs are all of one column of a range
 
   while (true) {
-    int handed_out = 0;
-    if (threadIdx.x == 0) handed_out = atomicAdd(counter, 1) + 2 * static_cast<int>(gridDim.x);
     const bool more = next_number < units;
-    if (more) next = decode(next_number);
-    const int next_pair = more ? read_pair(next) : 0;
-    // what the finishing needs besides the sums
     const int col = unit.range * out_cols + c;
+    int handed_out = 0, next_pair = 0;
     float my_scale = 0.f;
     float2 scale = make_float2(0.f, 0.f);
-    if (!SC && !kDown) {
-      if (threadIdx.x < unit.here) my_scale = __ldcg(all_scales + rows[buffer][threadIdx.x]);
-      if (col < out_n) {
-        const bf16* scales = all_weight_scales + static_cast<long long>(unit.expert) * columns + col;
-        scale = make_float2(to_f32(scales[0]), to_f32(scales[p.inner]));
+    // what comes later, asked for while the first copies are on their way
+    auto look_ahead = [&]() {
+      if (threadIdx.x == 0) handed_out = atomicAdd(counter, 1) + 2 * static_cast<int>(gridDim.x);
+      if (!SC && !kDown) {
+        if (threadIdx.x < unit.here) my_scale = __ldcg(all_scales + rows[buffer][threadIdx.x]);
+        if (col < out_n) {
+          const bf16* scales = all_weight_scales + static_cast<long long>(unit.expert) * columns + col;
+          scale = make_float2(to_f32(scales[0]), to_f32(scales[p.inner]));
+        }
       }
-    }
+      if (more) {
+        next = decode(next_number);
+        next_pair = read_pair(next);
+      }
+    };
 
     auto products = [&](auto n_groups) {
       constexpr int kN = decltype(n_groups)::value;
@@ -752,6 +749,7 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         copy_commit();
         if (++ahead == kStages) ahead = 0;
       }
+      look_ahead();
       int acc[kFrags][kN][4];
       double sum[SC ? kFrags : 1][SC ? kN : 1][4];
 #pragma unroll
@@ -887,16 +885,16 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
 #pragma unroll
             for (int j = 0; j < 4; ++j) atomicAdd(sums + sum_place<kMaxN>(half * kFrags + f, n, j, lane), DT == 4 ? acc[f][n][j] >> 8 : acc[f][n][j]);
         __syncthreads();
-      } else {  // one share after the other
-        for (int turn = 0; turn < kShares; ++turn) {
-          if (share == turn) {
+      } else {  // two shares after two others
+        for (int turn = 0; turn < kShares / 2; ++turn) {
+          if (share >> 1 == turn) {
 #pragma unroll
             for (int f = 0; f < kFrags; ++f)
 #pragma unroll
               for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  Sum* at = sums + sum_place<kMaxN>(half * kFrags + f, n, j, lane);
+                  Sum* at = sums + (share & 1) * Stage::kSums + sum_place<kMaxN>(half * kFrags + f, n, j, lane);
                   *at = turn == 0 ? sum[f][n][j] : *at + sum[f][n][j];
                 }
           }
@@ -913,8 +911,9 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
       auto sum_of = [&](int t, bool gate_part) {
         const int column = c + (gate_part ? kCols / 2 : 0);
         const int place = sum_place<kMaxN>(column >> 4, t >> 3, ((column >> 3) & 1) * 2 + (t & 1), (column & 7) * 4 + ((t & 7) >> 1));
-        const Sum total = sums[place];
-        if constexpr (!SC) sums[place] = 0;  // for the next unit
+        Sum total = sums[place];
+        if constexpr (SC) total += sums[Stage::kSums + place];
+        else sums[place] = 0;  // for the next unit
         return total;
       };
       for (int t = threadIdx.x / out_cols; t < unit.here; t += kMoeThreads / out_cols) {
@@ -944,52 +943,77 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
 }
 
 // Adds up the parts of K, scales, and adds up the experts' shares of a token in the order of its choices.  A thread has
-// two columns of one token; what depends on the pair alone is read once a block.
+// two columns of one token; what depends on the pair alone is worked out once a block: the softmax of the chosen logits
+// (or of all) in fp64.  What the select kernel left and the scales are read before the down product has ended.
 template <bool SC>
 __global__ void __launch_bounds__(128) moe_combine_kernel(const MoeParams p) {
   using Sum = typename MoeSum<SC>::type;
   using Sum2 = typename std::conditional<SC, double2, int2>::type;
+  constexpr int kAtOnce = 8;
   __shared__ int expert[kMoeMaxTopK];
   __shared__ float weight[kMoeMaxTopK], scale[kMoeMaxTopK];
-  const int token = blockIdx.y, col = (blockIdx.x * 128 + threadIdx.x) * 2;
-  grid_wait();
-  if (threadIdx.x < p.top_k) {
-    const int pair = token * p.top_k + threadIdx.x;
-    expert[threadIdx.x] = p.pair_expert[pair];
-    weight[threadIdx.x] = p.pair_weight[pair];
-    scale[threadIdx.x] = !SC && p.pair_expert[pair] >= 0 ? p.as[pair] : 1.f;
+  __shared__ double parts[4];
+  const int token = blockIdx.y, col = (blockIdx.x * 128 + threadIdx.x) * 2, lane = threadIdx.x & 31;
+  double others = 0.0;
+  if (p.router != nullptr && !p.renormalize) {
+    const double top = __ldcg(p.pair_logit + token * p.top_k);
+    for (int e = threadIdx.x; e < p.experts; e += 128) others += exp(__ldcg(p.logits + static_cast<long long>(token) * p.experts + e) - top);
+    others = warp_reduce(others, SumOp());
+    if (lane == 0) parts[threadIdx.x >> 5] = others;
+    __syncthreads();
+    others = parts[0] + parts[1] + parts[2] + parts[3];
+  }
+  if (threadIdx.x < 32) {
+    const int pair = token * p.top_k + min(lane, p.top_k - 1);
+    float w;
+    if (p.router != nullptr) {
+      const double logit = __ldcg(p.pair_logit + pair), top = __shfl_sync(0xFFFFFFFFu, logit, 0);
+      const double e = lane < p.top_k ? exp(logit - top) : 0.0;
+      const double total = warp_reduce(e, SumOp());
+      w = static_cast<float>(e / (p.renormalize ? total : others));
+    } else {
+      w = p.weights_in[pair];
+    }
+    if (lane < p.top_k) {
+      expert[lane] = __ldcg(p.pair_expert + pair);
+      weight[lane] = w;
+      if (p.weights_out != nullptr && blockIdx.x == 0) p.weights_out[pair] = w;
+    }
   }
   __syncthreads();
-  if (col >= p.hidden) return;
+  const bool inside = col < p.hidden;
+  uint32_t w[kAtOnce];
+  auto read_scales = [&](int j0) {
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int j = j0 + k;
+      w[k] = !SC && inside && j < p.top_k && expert[j] >= 0 ? *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[j]) * p.hidden + col) : 0u;
+    }
+  };
+  read_scales(0);
+  grid_wait();
+  if (!SC && threadIdx.x < p.top_k) scale[threadIdx.x] = expert[threadIdx.x] >= 0 ? __ldcg(p.as + token * p.top_k + threadIdx.x) : 1.f;
   const long long plane = static_cast<long long>(p.tokens) * p.top_k * p.hidden;
   float total[2] = {0.f, 0.f};
-  for (int j0 = 0; j0 < p.top_k; j0 += 4) {  // four choices at once
-    Sum2 sum[4];
-    uint32_t w[4];
+  for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
+    if (j0 > 0) read_scales(j0);
+    Sum2 sum[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int j = min(j0 + k, p.top_k - 1);
-      const bool valid = j0 + k < p.top_k && expert[j] >= 0;
-      sum[k].x = sum[k].y = 0;
-      w[k] = 0u;
-      if (valid) {
-        sum[k] = *reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + static_cast<long long>(token * p.top_k + j) * p.hidden + col);
-        if (!SC) w[k] = *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[j]) * p.hidden + col);
-      }
-    }
-    for (int s = 1; s < p.down_splits; ++s) {
+    for (int k = 0; k < kAtOnce; ++k) sum[k].x = sum[k].y = 0;
+    for (int s = 0; s < p.down_splits; ++s) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = min(j0 + k, p.top_k - 1);
-        if (j0 + k < p.top_k && expert[j] >= 0) {
-          const Sum2 more = *reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + s * plane + static_cast<long long>(token * p.top_k + j) * p.hidden + col);
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int j = j0 + k;
+        if (inside && j < p.top_k && expert[j] >= 0) {
+          const Sum2 more = __ldcg(reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + s * plane + static_cast<long long>(token * p.top_k + j) * p.hidden + col));
           sum[k].x += more.x;
           sum[k].y += more.y;
         }
       }
     }
+    if (j0 == 0) __syncthreads();  // the scales
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAtOnce; ++k) {
       const int j = j0 + k;
       if (j >= p.top_k || expert[j] < 0) continue;
       double y0 = static_cast<double>(sum[k].x), y1 = static_cast<double>(sum[k].y);
@@ -1001,9 +1025,11 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(const MoeParams p) {
       total[1] += static_cast<float>(y1) * weight[j];
     }
   }
-  bf16* out = p.out + static_cast<long long>(token) * p.hidden + col;
-  out[0] = __float2bfloat16_rn(total[0]);
-  out[1] = __float2bfloat16_rn(total[1]);
+  if (inside) {
+    bf16* out = p.out + static_cast<long long>(token) * p.hidden + col;
+    out[0] = __float2bfloat16_rn(total[0]);
+    out[1] = __float2bfloat16_rn(total[1]);
+  }
 }
 
 }  // namespace b200

@@ -38,13 +38,13 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   const size_t per_byte = m.dtype == B200_DTYPE_INT4 ? 2 : 1;
   const size_t x_groups = m.subchannel ? (m.hidden + m.subchannel - 1) / m.subchannel : 1;
   const size_t a_groups = m.subchannel ? (m.inner + m.subchannel - 1) / m.subchannel : 1;
-  const int down_cols = m.layout == B200_LAYOUT_NN ? 128 : 32;  // of one block
+  const int down_cols = m.layout == B200_LAYOUT_NN ? 128 : 64;  // of one block
   p->slots = static_cast<int>(pairs < static_cast<size_t>(m.experts) ? pairs : m.experts);
   p->up_ranges = (m.inner + down_cols / 2 - 1) / (down_cols / 2);
   p->down_ranges = (m.hidden + down_cols - 1) / down_cols;
   // The down product divides K between blocks where there are fewer (expert, column range) units than would keep the
   // blocks that the device holds (2 or 3 an SM) evenly busy, as long as each of a block's warps has four steps left.
-  const int step = m.layout == B200_LAYOUT_NN ? (m.dtype == B200_DTYPE_INT4 ? 64 : 32) : (m.dtype == B200_DTYPE_INT4 ? 128 : 64);
+  const int step = m.dtype == B200_DTYPE_INT4 ? 64 : 32;
   const int shares = m.layout == B200_LAYOUT_NN ? 4 : 8;
   p->down_splits = 1;
   while (p->down_splits < 8 && static_cast<long long>(p->slots) * p->down_ranges * p->down_splits < 1024 &&
@@ -54,7 +54,7 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->xs = reinterpret_cast<float*>(take(m.tokens * x_groups * 4));
   p->logits = reinterpret_cast<double*>(take(static_cast<size_t>(m.tokens) * m.experts * 8));
   p->pair_expert = reinterpret_cast<int*>(take(pairs * 4));
-  p->pair_weight = reinterpret_cast<float*>(take(pairs * 4));
+  p->pair_logit = reinterpret_cast<double*>(take(pairs * 8));
   p->active = reinterpret_cast<int*>(take((1 + static_cast<size_t>(p->slots)) * 16));
   p->pair_list = reinterpret_cast<int*>(take(pairs * 4));
   p->act = reinterpret_cast<double*>(take(pairs * m.inner * 8));

@@ -96,15 +96,13 @@ int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStr
   // words of token codes that a lane takes at a step: as many as keep a step within a group of K (32 K a word of
   // nibbles, 16 a word of bytes) and the ring's stages small
   constexpr int kWord = kBits == 4 ? 32 : 16, kLeast = kBits == 4 ? 1 : 2;
+  const bool two_words = !p.sub || p.sub >= 2 * kWord;
   if (n_major) {
     if (!p.sub) return launch_for_tokens<true, false, 2>(p, sm_count, stream);
-    if (p.sub >= 2 * kWord) return launch_for_tokens<true, true, 2>(p, sm_count, stream);
-    return launch_for_tokens<true, true, kLeast>(p, sm_count, stream);
+    return two_words ? launch_for_tokens<true, true, 2>(p, sm_count, stream) : launch_for_tokens<true, true, kLeast>(p, sm_count, stream);
   }
-  if (!p.sub) return launch_for_tokens<false, false, 4>(p, sm_count, stream);
-  if (p.sub >= 4 * kWord) return launch_for_tokens<false, true, 4>(p, sm_count, stream);
-  if (p.sub >= 2 * kWord) return launch_for_tokens<false, true, 2>(p, sm_count, stream);
-  return launch_for_tokens<false, true, kLeast>(p, sm_count, stream);
+  if (!p.sub) return launch_for_tokens<false, false, 2>(p, sm_count, stream);
+  return two_words ? launch_for_tokens<false, true, 2>(p, sm_count, stream) : launch_for_tokens<false, true, kLeast>(p, sm_count, stream);
 }
 
 }  // namespace b200
