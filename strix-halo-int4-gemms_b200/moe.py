@@ -10,7 +10,7 @@ from __future__ import annotations
 from typing import Any
 
 from .metadata import GemmLayout, OperandDType, ScaleMode, ScaleSpec
-from .native import DTYPE_CODES, LAYOUT_CODES, OUT_BF16, OUT_F32, MoeProblem, moe_swiglu_on_device
+from .native import DTYPE_CODES, LAYOUT_CODES, OUT_BF16, OUT_F32, moe_swiglu_on_device
 
 MOE_MAX_TOKENS = 64
 MOE_MAX_TOP_K = 16
@@ -27,7 +27,7 @@ def _torch() -> Any:
 
 
 def _check(torch: Any, name: str, tensor: Any, dtypes: tuple[Any, ...], shape: tuple[int, ...] | None, device: Any) -> None:
-    if not torch.is_tensor(tensor):
+    if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
@@ -35,10 +35,15 @@ def _check(torch: Any, name: str, tensor: Any, dtypes: tuple[Any, ...], shape: t
         raise ValueError(f"{name} must be on {device}, the device of x; got {tensor.device}")
     if tensor.dtype not in dtypes:
         raise ValueError(f"{name} must have dtype {' or '.join(str(item) for item in dtypes)}; got {tensor.dtype}")
-    if shape is not None and tuple(tensor.shape) != shape:
+    if shape is not None and tensor.shape != shape:
         raise ValueError(f"{name} must have shape {shape}; got {tuple(tensor.shape)}")
     if not tensor.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+    if tensor.data_ptr() % 16 and name in _WIDE:
+        raise ValueError(f"{name} must start on a multiple of 16 bytes")
+
+
+_WIDE = frozenset(("x", "router_weight", "w_up_gate", "w_down", "up_gate_scale", "down_scale"))  # read 16 bytes at a time
 
 
 def moe_swiglu(
@@ -132,19 +137,14 @@ def moe_swiglu(
         top_k = int(topk_ids.shape[1])
     if not 0 < top_k <= min(MOE_MAX_TOP_K, experts):
         raise ValueError(f"top_k must be in [1, {min(MOE_MAX_TOP_K, experts)}]; got {top_k}")
-    for name, tensor in (("x", x), ("router_weight", router_weight), ("w_up_gate", w_up_gate), ("w_down", w_down),
-                         ("up_gate_scale", up_gate_scale), ("down_scale", down_scale)):
-        if tensor is not None and tensor.data_ptr() % 16:
-            raise ValueError(f"{name} must start on a multiple of 16 bytes")
-
     if tokens == 0:
         out = torch.empty_like(x)
     else:
-        problem = MoeProblem(
+        fields = (
             DTYPE_CODES[dtype], LAYOUT_CODES[layout], sub, tokens, hidden, inner, experts, top_k,
             OUT_F32 if router_weight is not None and router_weight.dtype is torch.float32 else OUT_BF16, int(bool(renormalize)),
             64 if topk_ids is not None and topk_ids.dtype is torch.int64 else 32)
         out = moe_swiglu_on_device(
-            problem, x, router_weight=router_weight, topk_ids=topk_ids, topk_weights=topk_weights, w_up_gate=w_up_gate,
+            fields, x, router_weight=router_weight, topk_ids=topk_ids, topk_weights=topk_weights, w_up_gate=w_up_gate,
             up_gate_scale=up_gate_scale, w_down=w_down, down_scale=down_scale)
     return (out, topk_ids, topk_weights) if return_routing else out

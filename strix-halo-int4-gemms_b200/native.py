@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import threading
 from dataclasses import dataclass
+from functools import lru_cache
 from pathlib import Path
 from typing import Any
 
@@ -305,8 +306,13 @@ def _torch() -> Any:
 
 
 def _stream_handle(torch: Any, tensor: Any, stream: Any | None) -> int:
-    chosen = stream if stream is not None else torch.cuda.current_stream(tensor.device)
-    return int(chosen.cuda_stream)
+    if stream is not None:
+        return int(stream.cuda_stream)
+    # the current stream's handle without building a Stream object, which costs a call 2 us
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is not None and tensor.is_cuda:
+        return int(raw(tensor.get_device()))
+    return int(torch.cuda.current_stream(tensor.device).cuda_stream)
 
 
 def _device_index(tensor: Any) -> int:
@@ -918,26 +924,26 @@ def quantize_tokens_on_device(x: Any, *, bits: int, subchannel: int = 0, library
     torch = _torch()
     if not getattr(x, "is_cuda", False) or x.dtype is not torch.bfloat16:
         raise RuntimeError("quantize_tokens_on_device requires a CUDA bfloat16 tensor")
-    x = _require_contiguous("x", x)
+    if not x.is_contiguous():
+        raise ValueError("x must be contiguous for native dispatch")
     codes, scales, rows, cols = _token_code_outputs(torch, x, bits, subchannel)
     library = load_dispatch_library(library_path)
     rc = library.b200_int4_gemms_quantize_tokens(
-        _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols,
-        int(bits), int(subchannel))
+        x.get_device(), _stream_handle(torch, x, stream), x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols, bits, subchannel)
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
     return codes, scales
 
 
 def _token_code_outputs(torch: Any, x: Any, bits: int, subchannel: int) -> tuple[Any, Any, int, int]:
-    lead, cols = x.shape[:-1], int(x.shape[-1])
-    rows = x.numel() // cols if cols else 0
+    shape = x.shape
+    lead, cols = shape[:-1], shape[-1]
     if bits == 4:
-        codes = torch.empty((*lead, (cols + 1) // 2), device=x.device, dtype=torch.uint8)
+        codes = x.new_empty((*lead, (cols + 1) // 2), dtype=torch.uint8)
     else:
-        codes = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-    scales = torch.empty((*lead, -(-cols // subchannel)) if subchannel else lead, device=x.device, dtype=torch.bfloat16)
-    return codes, scales, rows, cols
+        codes = x.new_empty(shape, dtype=torch.int8)
+    scales = x.new_empty((*lead, -(-cols // subchannel)) if subchannel else lead, dtype=torch.bfloat16)
+    return codes, scales, x.numel() // cols if cols else 0, cols
 
 
 def _type_code(torch: Any, tensor: Any) -> int:
@@ -948,16 +954,18 @@ def layer_norm_on_device(x: Any, weight: Any, bias: Any | None, *, eps: float, l
                          stream: Any | None = None) -> tuple[Any, Any, Any]:
     """(y, mean, rstd) of checked CUDA operands; see :func:`norm.layer_norm`."""
     torch = _torch()
-    cols = int(x.shape[-1])
+    cols = x.shape[-1]
+    rows = x.numel() // cols
     y = torch.empty_like(x)
-    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32)
-    mean, rstd = stats[0], stats[1]
+    stats = x.new_empty((2, *x.shape[:-1]), dtype=torch.float32)  # one allocation for both
+    at = stats.data_ptr()
     library = load_dispatch_library(library_path)
     rc = library.b200_int4_gemms_layer_norm(
-        _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-        y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x.numel() // cols, cols, _type_code(torch, x), _type_code(torch, weight), eps)
+        x.get_device(), _stream_handle(torch, x, stream), x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        y.data_ptr(), at, at + 4 * rows, rows, cols, _type_code(torch, x), _type_code(torch, weight), eps)
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
+    mean, rstd = stats.unbind(0)
     return y, mean, rstd
 
 
@@ -968,8 +976,8 @@ def layer_norm_quantize_on_device(x: Any, weight: Any, bias: Any | None, *, eps:
     codes, scales, rows, cols = _token_code_outputs(torch, x, bits, subchannel)
     library = load_dispatch_library(library_path)
     rc = library.b200_int4_gemms_layer_norm_quantize(
-        _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-        codes.data_ptr(), scales.data_ptr(), rows, cols, _type_code(torch, x), _type_code(torch, weight), eps, int(bits), int(subchannel))
+        x.get_device(), _stream_handle(torch, x, stream), x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        codes.data_ptr(), scales.data_ptr(), rows, cols, _type_code(torch, x), _type_code(torch, weight), eps, bits, subchannel)
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
     return codes, scales
@@ -982,38 +990,46 @@ def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any,
     The scratch is allocated for the call: the caching allocator keeps it apart from other streams' and, under
     capture, inside the graph's own pool."""
     torch = _torch()
-    cols = int(x.shape[-1])
+    cols = x.shape[-1]
     rows = x.numel() // cols
     library = load_dispatch_library(library_path)
-    index = _device_index(x)
-    need = int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(index, rows, cols, _type_code(torch, x)))
+    index, kind = x.get_device(), _type_code(torch, x)
+    need = library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(index, rows, cols, kind)
     dx = torch.empty_like(x)
-    sums = torch.empty((2, cols), device=x.device, dtype=torch.float32)
-    workspace = torch.empty(need // 4, device=x.device, dtype=torch.float32)
+    sums = x.new_empty((2, cols), dtype=torch.float32)
+    workspace = x.new_empty(need // 4, dtype=torch.float32)
+    at = sums.data_ptr()
     rc = library.b200_int4_gemms_layer_norm_bwd(
         index, _stream_handle(torch, x, stream), dy.data_ptr(), x.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-        dx.data_ptr(), sums[0].data_ptr(), sums[1].data_ptr(), workspace.data_ptr(), need, rows, cols, _type_code(torch, x),
-        _type_code(torch, weight))
+        dx.data_ptr(), at, at + 4 * cols, workspace.data_ptr(), need, rows, cols, kind, _type_code(torch, weight))
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
-    return dx, sums[0], sums[1]
+    dweight, dbias = sums.unbind(0)
+    return dx, dweight, dbias
+
+
+@lru_cache(maxsize=256)
+def moe_problem(*fields: int) -> tuple[MoeProblem, int]:
+    """The record of a layer's sizes and kinds, in the order of its fields, and the scratch that it asks for."""
+    problem = MoeProblem(*fields)
+    return problem, int(load_dispatch_library().b200_int4_gemms_moe_swiglu_workspace_bytes(ctypes.byref(problem)))
 
 
 def moe_swiglu_on_device(
-    problem: MoeProblem, x: Any, *, router_weight: Any | None, topk_ids: Any | None, topk_weights: Any | None, w_up_gate: Any,
-    up_gate_scale: Any, w_down: Any, down_scale: Any, library_path: str | Path | None = None, stream: Any | None = None,
+    fields: tuple[int, ...], x: Any, *, router_weight: Any | None, topk_ids: Any | None, topk_weights: Any | None, w_up_gate: Any,
+    up_gate_scale: Any, w_down: Any, down_scale: Any, stream: Any | None = None,
 ) -> Any:
     """The layer's output for checked CUDA operands; see :func:`moe.moe_swiglu`.
 
     The scratch is allocated for the call: the caching allocator keeps it apart from other streams' and, under
     capture, inside the graph's own pool."""
     torch = _torch()
-    library = load_dispatch_library(library_path)
+    library = load_dispatch_library()
+    problem, need = moe_problem(*fields)
     out = torch.empty_like(x)
-    need = int(library.b200_int4_gemms_moe_swiglu_workspace_bytes(ctypes.byref(problem)))
-    workspace = torch.empty(need, device=x.device, dtype=torch.uint8)
+    workspace = x.new_empty(need, dtype=torch.uint8)
     rc = library.b200_int4_gemms_moe_swiglu(
-        ctypes.byref(problem), _device_index(x), _stream_handle(torch, x, stream), x.data_ptr(),
+        ctypes.byref(problem), x.get_device(), _stream_handle(torch, x, stream), x.data_ptr(),
         0 if router_weight is None else router_weight.data_ptr(), 0 if topk_ids is None else topk_ids.data_ptr(),
         0 if topk_weights is None else topk_weights.data_ptr(), w_up_gate.data_ptr(), up_gate_scale.data_ptr(), w_down.data_ptr(),
         down_scale.data_ptr(), out.data_ptr(), workspace.data_ptr(), need)

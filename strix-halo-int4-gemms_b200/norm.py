@@ -26,7 +26,7 @@ def _torch() -> Any:
 
 
 def _check_values(torch: Any, name: str, tensor: Any, dtypes: tuple[Any, ...]) -> None:
-    if not torch.is_tensor(tensor):
+    if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
@@ -47,7 +47,7 @@ def _check_norm_operands(torch: Any, x: Any, weight: Any, bias: Any | None) -> N
         if tensor is None and name == "bias":
             continue
         _check_values(torch, name, tensor, types)
-        if tuple(tensor.shape) != (cols,):
+        if tensor.shape != (cols,):
             raise ValueError(f"{name} must have shape ({cols},); got {tuple(tensor.shape)}")
         if tensor.device != x.device:
             raise ValueError(f"{name} must be on {x.device}, the device of x; got {tensor.device}")
