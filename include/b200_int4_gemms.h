@@ -369,8 +369,8 @@ int b200_int4_gemms_layer_norm_quantize(int device_index, uintptr_t stream_handl
 
 /* Backward pass of b200_int4_gemms_layer_norm.  dy, x, dx [rows, cols] of x_type; mean, rstd as the forward pass
  * wrote them; dweight, dbias f32 [cols] (zero for rows = 0).  Sums over rows in a fixed order: the same bits on
- * every run.  workspace: float32-aligned scratch of ..._workspace_bytes (0 for cols > 16384); calls that may
- * overlap need their own. */
+ * every run.  workspace: 16-byte aligned scratch of ..._workspace_bytes; calls that may overlap need
+ * their own. */
 size_t b200_int4_gemms_layer_norm_bwd_workspace_bytes(int device_index, int64_t rows, int64_t cols, int32_t x_type);
 int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream_handle, const void* dy, const void* x,
                                    const void* weight, const float* mean, const float* rstd, void* dx, float* dweight,

@@ -323,11 +323,6 @@ int host_fail(std::string msg) { return fail(std::move(msg)); }
 int host_fail_cuda(const char* what, cudaError_t err) { return fail_cuda(what, err); }
 void host_clear_error() { g_last_error.clear(); }
 
-volatile int* device_status_word(int device_index) {
-  std::lock_guard<std::mutex> lock(g_device_mutex);
-  return device_index >= 0 && device_index < kMaxDevices && g_devices[device_index].ready ? g_devices[device_index].status_dev : nullptr;
-}
-
 int DeviceScope::enter(int device_index, int* sm_count) {
   if (device_index < 0 || device_index >= kMaxDevices) return fail("device_index out of range");
   static std::mutex mutex;

@@ -14,9 +14,6 @@ int host_fail(std::string msg);
 int host_fail_cuda(const char* what, cudaError_t err);
 void host_clear_error();
 
-// The host-mapped status word of a device that another entry point has set up, else null.
-volatile int* device_status_word(int device_index);
-
 // Selects the device of a call for its duration; the caller's current device is restored at the end.
 class DeviceScope {
  public:

@@ -8,11 +8,8 @@
 // they are too few to fill the device (quantize_tokens of 32768 x 2048: 48 us with 16 values a thread, see below).
 #pragma once
 
-#include <cooperative_groups.h>
-
 #include <cstring>
 
-#include "ptx.cuh"
 #include "row_common.cuh"
 
 namespace b200 {
@@ -118,9 +115,10 @@ quantize_tokens_kernel(const bf16* __restrict__ src, uint8_t* __restrict__ codes
 
 // ---------------------------------------------------------------------------------------------------------------
 // layer norm: y = (x - mean) rstd w + b; mean, then the mean square of the differences, both from registers, in fp32.
+// As many blocks as are resident at once, each for many rows: the next row is on its way while one is worked on.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, typename W, int TPR, int V, bool kAligned>
-__global__ void __launch_bounds__(RowPlace<TPR>::kThreads, 768 / RowPlace<TPR>::kThreads)
+__global__ void __launch_bounds__(RowPlace<TPR>::kThreads, 512 / RowPlace<TPR>::kThreads)
 layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias, T* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, long long cols, float eps) {
   __shared__ float scratch[2][TPR / 32];
@@ -128,13 +126,20 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
   constexpr int G = kAligned ? 16 / sizeof(T) : 1;
   const Columns<TPR, G> column{RowPlace<TPR>::thread(), cols};
   const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
+  constexpr int kHeld = V > 0 ? V : 1;
+  Raw8<T> ahead[kHeld];  // the next row, read while the present one is worked on
+  auto fetch = [&](long long r) {
+    if (V == 0 || r >= rows) return;
+#pragma unroll
+    for (int v = 0; v < kHeld; ++v) ahead[v] = column.load(src + r * cols, v);
+  };
+  fetch(RowPlace<TPR>::first());
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
     const T* row = src + r * cols;
-    Raw8<T> held[V > 0 ? V : 1];
-    if (V > 0) {
+    Raw8<T> held[kHeld];
 #pragma unroll
-      for (int v = 0; v < (V > 0 ? V : 1); ++v) held[v] = column.load(row, v);
-    }
+    for (int v = 0; v < kHeld; ++v) held[v] = ahead[v];
+    fetch(r + RowPlace<TPR>::step());
     auto value = [&](int v) { return V > 0 ? held[V > 0 ? v : 0] : column.load(row, v); };
     float sum = 0.f;
 #pragma unroll
@@ -375,43 +380,13 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
 // A block has several groups of TPR threads, each with rows of its own (and a barrier of its own); the sums of the groups
 // are added up in shared memory, each block leaves one row of partial sums, and column_sums_kernel adds those in a fixed
 // order: no atomics, the same bits on every run.  The next row is read while the present one is reduced.
-// Rows of more than 8192 values belong to a cluster of two blocks, half a row each, which exchange their sums through
-// distributed shared memory.
+// Rows of more than 8192 values are left to two kernels, below.
 // ---------------------------------------------------------------------------------------------------------------
-template <int TPR, int CLUSTER>
+template <int TPR>
 struct BwdShape {
   static constexpr int kThreads = TPR < 512 ? 512 : TPR;
-  static constexpr int kGroups = kThreads / TPR;  // rows at once (by half a row for CLUSTER == 2)
+  static constexpr int kGroups = kThreads / TPR;  // rows at once
 };
-
-// Address of this block's shared memory in another block of the cluster.
-__device__ __forceinline__ uint32_t cluster_address(uint32_t address, int rank) {
-  uint32_t there;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
-  return there;
-}
-
-// Two floats to another block's shared memory, counted there as eight bytes on its barrier.
-__device__ __forceinline__ void store_async(uint32_t address, uint32_t barrier, float a, float b) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(address), "f"(a), "f"(b), "r"(barrier)
-               : "memory");
-}
-
-// Bounded wait for a barrier: false, and the device's status word, when the time runs out.
-__device__ __forceinline__ bool wait_for_peer(uint32_t barrier, uint32_t parity, volatile int* status) {
-  if (mbar_try_wait(barrier, parity)) return true;
-  const unsigned long long begin = global_timer_ns();
-  while (!mbar_try_wait(barrier, parity)) {
-    if (global_timer_ns() - begin > WAIT_LIMIT_NS) {
-      if (status != nullptr && status[0] == STATUS_OK) {
-        status[1] = static_cast<int>(blockIdx.x);
-        status[0] = STATUS_WAIT_TIMEOUT;
-      }
-      return false;
-    }
-  }
-  return true;
-}
 
 // Barrier of one group of a block.
 template <int TPR>
@@ -419,46 +394,24 @@ __device__ __forceinline__ void group_barrier(int group) {
   if (TPR > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
 }
 
-template <typename T, typename W, int TPR, int V, int CLUSTER, bool kAligned>
-__global__ void __launch_bounds__(BwdShape<TPR, CLUSTER>::kThreads)
+template <typename T, typename W, int TPR, int V, bool kAligned>
+__global__ void __launch_bounds__(BwdShape<TPR>::kThreads)
 layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
-                      float* __restrict__ partial, long long rows, long long cols, volatile int* status) {
-  using Shape = BwdShape<TPR, CLUSTER>;
-  constexpr int kWarps = TPR / 32, kGroups = Shape::kGroups, kBlockCols = TPR * V * 8;
+                      float* __restrict__ partial, long long rows, long long cols) {
+  constexpr int kWarps = TPR / 32, kGroups = BwdShape<TPR>::kGroups;
   __shared__ float2 scratch[2][kGroups][kWarps];
-  __shared__ __align__(8) float2 from_peer[2];
-  __shared__ __align__(8) uint64_t arrived[2];
-  __shared__ bool go_on;
-  extern __shared__ float across[];  // [kBlockCols], where there are groups to be added up
+  extern __shared__ float across[];  // [TPR * V * 8], where there are groups to be added up
   const int group = threadIdx.x / TPR, thread = threadIdx.x % TPR;
-  const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
-  const long long unit = blockIdx.x / CLUSTER, step = static_cast<long long>(gridDim.x / CLUSTER) * kGroups;
-  // this block's columns: all, or the half `rank` (the first half is kBlockCols wide)
-  const long long col0 = static_cast<long long>(rank) * kBlockCols;
+  const long long step = static_cast<long long>(gridDim.x) * kGroups;
   constexpr int G = kAligned ? 16 / sizeof(T) : 1;
-  const Columns<TPR, G> column{thread, CLUSTER > 1 ? max(0ll, min(cols - col0, static_cast<long long>(kBlockCols))) : cols};
-  uint32_t peer_value = 0, peer_barrier = 0, my_barrier = 0;
-  if constexpr (CLUSTER > 1) {
-    my_barrier = smem_u32(arrived);
-    if (threadIdx.x == 0) {
-      mbar_init(my_barrier, 1);
-      mbar_init(my_barrier + 8, 1);
-      mbar_fence_init();
-    }
-    peer_value = cluster_address(smem_u32(from_peer), rank ^ 1);
-    peer_barrier = cluster_address(my_barrier, rank ^ 1);
-    cooperative_groups::this_cluster().sync();
-  }
-  src += col0;
-  dy += col0;
-  dx += col0;
+  const Columns<TPR, G> column{thread, cols};
   const float inv_cols = 1.f / static_cast<float>(cols);
   Raw8<W> w[V];
   float dw[V][8], db[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    w[v] = column.load(weight + col0, v);
+    w[v] = column.load(weight, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[v][i] = db[v][i] = 0.f;
   }
@@ -473,10 +426,9 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
     next_mean = __ldg(mean_in + row);
     next_rstd = __ldg(rstd_in + row);
   };
-  long long r = unit * kGroups + group;
+  long long r = static_cast<long long>(blockIdx.x) * kGroups + group;
   if (r < rows) fetch(r);
   int turn = 0;
-  uint32_t phase = 0;
   for (; r < rows; r += step, turn ^= 1) {
     Raw8<T> x[V], d[V];
 #pragma unroll
@@ -512,26 +464,6 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
         sgh += __shfl_xor_sync(0xFFFFFFFFu, sgh, o);
       }
     }
-    if constexpr (CLUSTER > 1) {
-      // One 8-byte store that counts up the other block's barrier; a buffer is written again two rows later, after
-      // the other block has sent its sums of the row between, which it does behind a barrier of all its threads.
-      // (A cluster barrier instead waits for all stores of dx: 517 rows of 14336 took 40 us with it.)
-      if (threadIdx.x == 0) {
-        mbar_arrive_expect_tx(my_barrier + 8 * turn, 8);
-        store_async(peer_value + 8 * turn, peer_barrier + 8 * turn, sg, sgh);
-        go_on = wait_for_peer(my_barrier + 8 * turn, (phase >> turn) & 1u, status);
-      }
-      phase ^= 1u << turn;
-      __syncthreads();
-      if (!go_on) {  // never, unless the device lost the other block: the sums show it
-        dw[0][0] = __int_as_float(0x7FC00000);
-        break;
-      }
-      const float2 other = from_peer[turn];
-      // in the order of the halves, so that both blocks have the same sum
-      sg = rank == 0 ? sg + other.x : other.x + sg;
-      sgh = rank == 0 ? sgh + other.y : other.y + sgh;
-    }
     const float mg = sg * inv_cols, mgh = sgh * inv_cols;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -545,8 +477,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
     }
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // column_sums_kernel, which waits for this one's end
-  if (CLUSTER > 1) cooperative_groups::this_cluster().sync();  // no block ends while the other may still write to it
-  float* mine = partial + unit * 2 * cols + col0;
+  float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * cols;
   if (kGroups == 1) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -585,13 +516,20 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
   }
 }
 
-// Rows of more than 16384 values: dx alone, reading the row twice, and the sums over rows column by column.
+// Rows of more than 8192 values, whose columns do not fit the registers of one block: the means of g and g h of every
+// row, and then dx and the sums over rows with a thread for each chunk of columns, which needs no reduction over the
+// row.  x and dy are read twice, the second time from L2 as far as it holds them.  (517 rows of 14336 fp32 values: a
+// block of 1024 threads a row took 47 us, clusters of two blocks 37 us, both waiting for their reductions.)
+struct __align__(16) RowTerms {
+  float mean, rstd, mean_g, mean_gh;
+};
+
 template <typename T, typename W, bool kAligned>
-__global__ void __launch_bounds__(1024)
-layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
-                           const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
+__global__ void __launch_bounds__(512)
+layer_norm_bwd_rows_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
+                           const float* __restrict__ mean_in, const float* __restrict__ rstd_in, RowTerms* __restrict__ terms,
                            long long rows, long long cols) {
-  constexpr int TPR = 1024, G = kAligned ? 16 / sizeof(T) : 1;
+  constexpr int TPR = 512, G = kAligned ? 16 / sizeof(T) : 1;
   __shared__ float scratch[2][2 * (TPR / 32)];
   const float inv_cols = 1.f / static_cast<float>(cols);
   const Columns<TPR, G> column{static_cast<int>(threadIdx.x), cols};
@@ -602,45 +540,107 @@ layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ src, 
     const T* d_row = dy + r * cols;
     const float mean = __ldg(mean_in + r), rstd = __ldg(rstd_in + r);
     float sg = 0.f, sgh = 0.f;
+#pragma unroll 2
     for (int v = 0; v < count; ++v) {
-      const Raw8<T> xv = column.load(x_row, v), dv = column.load(d_row, v);
+      const Raw8<T> x = column.load(x_row, v), d = column.load(d_row, v);
       const Raw8<W> w = column.load(weight, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float g = dv.get(i) * w.get(i);
+        const float g = d.get(i) * w.get(i);
         sg += g;
-        sgh = __fmaf_rn(g, (xv.get(i) - mean) * rstd, sgh);
+        sgh = __fmaf_rn(g, (x.get(i) - mean) * rstd, sgh);
       }
     }
     row_reduce2<TPR>(sg, sgh, SumOp(), SumOp(), scratch[turn]);
-    const float mg = sg * inv_cols, mgh = sgh * inv_cols;
-    for (int v = 0; v < count; ++v) {
-      const Raw8<T> xv = column.load(x_row, v), dv = column.load(d_row, v);
-      const Raw8<W> w = column.load(weight, v);
-      float out[8];
+    if (threadIdx.x == 0) terms[r] = RowTerms{mean, rstd, sg * inv_cols, sgh * inv_cols};
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// A block has a strip of 32 chunks of G columns and a part of the rows, which its eight warps take in turns; the sums
+// of the warps are added in order and leave one row of partial sums for each part.
+constexpr int kStripWarps = 8;
+
+template <typename T, typename W, int G>
+__global__ void __launch_bounds__(32 * kStripWarps)
+layer_norm_bwd_strips_kernel(const T* __restrict__ dy, const T* __restrict__ src, const W* __restrict__ weight,
+                             const RowTerms* terms, T* __restrict__ dx, float* __restrict__ partial, long long rows, long long cols) {
+  constexpr int kAtOnce = 4;
+  __shared__ float across[2][kStripWarps][32 * G];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long col = (static_cast<long long>(blockIdx.x) * 32 + lane) * G;
+  const bool inside = col < cols;
+  const long long row0 = rows * blockIdx.y / gridDim.y, row1 = rows * (blockIdx.y + 1) / gridDim.y;
+  struct Chunk {
+    T e[G];
+  };
+  auto read = [&](const T* p) {
+    Chunk c;
+    if constexpr (G * sizeof(T) == 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      memcpy(c.e, &v, 16);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = rstd * (dv.get(i) * w.get(i) - mg - (xv.get(i) - mean) * rstd * mgh);
-      column.store(dx + r * cols, v, out);
+      for (int i = 0; i < G; ++i) c.e[i] = p[i];
+    }
+    return c;
+  };
+  float w[G], dw[G], db[G];
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    w[i] = inside ? to_f32(weight[col + i]) : 0.f;
+    dw[i] = db[i] = 0.f;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (inside) {
+    for (long long r0 = row0 + warp; r0 < row1; r0 += kStripWarps * kAtOnce) {
+      Chunk x[kAtOnce], d[kAtOnce];
+      RowTerms t[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const long long r = r0 + k * kStripWarps;
+        if (r >= row1) continue;
+        x[k] = read(src + r * cols + col);
+        d[k] = read(dy + r * cols + col);
+        t[k] = terms[r];
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const long long r = r0 + k * kStripWarps;
+        if (r >= row1) continue;
+        float out[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const float e = to_f32(d[k].e[i]), h = (to_f32(x[k].e[i]) - t[k].mean) * t[k].rstd;
+          dw[i] = __fmaf_rn(e, h, dw[i]);
+          db[i] += e;
+          out[i] = t[k].rstd * (e * w[i] - t[k].mean_g - h * t[k].mean_gh);
+        }
+        T* to = dx + r * cols + col;
+        if constexpr (G == 8) *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3]), pack_bf16x2(out[4], out[5]), pack_bf16x2(out[6], out[7]));
+        else if constexpr (G == 4) *reinterpret_cast<float4*>(to) = make_float4(out[0], out[1], out[2], out[3]);
+        else to[0] = static_cast<T>(out[0]);
+      }
     }
   }
-}
-
-// Block of 32 columns x ROWS rows at a time; the sums of a column are added in a fixed order.
-template <int ROWS>
-__device__ __forceinline__ void column_finish(float sw, float sb, long long col, long long cols, float* dweight, float* dbias) {
-  __shared__ float tile[2][ROWS][33];
-  tile[0][threadIdx.y][threadIdx.x] = sw;
-  tile[1][threadIdx.y][threadIdx.x] = sb;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    across[0][warp][i * 32 + lane] = dw[i];
+    across[1][warp][i * 32 + lane] = db[i];
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
-  // the first warp adds up dw, the second db, a column a lane
-  if (threadIdx.y < 2 && col < cols) {
+  for (int k = threadIdx.x; k < 2 * 32 * G; k += 32 * kStripWarps) {
+    const int half = k / (32 * G), place = k % (32 * G);
+    const long long c = (static_cast<long long>(blockIdx.x) * 32 + place % 32) * G + place / 32;
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) sum += tile[threadIdx.y][k][threadIdx.x];
-    (threadIdx.y == 0 ? dweight : dbias)[col] = sum;
+    for (int j = 0; j < kStripWarps; ++j) sum += across[half][j][place];
+    if (c < cols) partial[(2LL * blockIdx.y + half) * cols + c] = sum;
   }
 }
 
+// Adds up the rows of partial sums: a block for 32 columns, kSumRows rows at a time, in a fixed order.
 constexpr int kSumRows = 16;
 
 static __global__ void __launch_bounds__(32 * kSumRows)
@@ -655,24 +655,17 @@ column_sums_kernel(const float* __restrict__ partial, int parts, long long cols,
       sb += partial[(2LL * p + 1) * cols + col];
     }
   }
-  column_finish<kSumRows>(sw, sb, col, cols, dweight, dbias);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(1024)
-layer_norm_bwd_columns_kernel(const T* __restrict__ dy, const T* __restrict__ src, const float* __restrict__ mean_in,
-                              const float* __restrict__ rstd_in, long long rows, long long cols, float* __restrict__ dweight,
-                              float* __restrict__ dbias) {
-  const long long col = static_cast<long long>(blockIdx.x) * 32 + threadIdx.x;
-  float sw = 0.f, sb = 0.f;
-  if (col < cols) {
-    for (long long r = threadIdx.y; r < rows; r += 32) {
-      const float d = to_f32(dy[r * cols + col]);
-      sw = __fmaf_rn(d, (to_f32(src[r * cols + col]) - __ldg(mean_in + r)) * __ldg(rstd_in + r), sw);
-      sb += d;
-    }
+  __shared__ float tile[2][kSumRows][33];
+  tile[0][threadIdx.y][threadIdx.x] = sw;
+  tile[1][threadIdx.y][threadIdx.x] = sb;
+  __syncthreads();
+  // the first warp adds up dw, the second db, a column a lane
+  if (threadIdx.y < 2 && col < cols) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSumRows; ++k) sum += tile[threadIdx.y][k][threadIdx.x];
+    (threadIdx.y == 0 ? dweight : dbias)[col] = sum;
   }
-  column_finish<32>(sw, sb, col, cols, dweight, dbias);
 }
 
 }  // namespace b200

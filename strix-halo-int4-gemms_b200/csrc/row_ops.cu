@@ -3,6 +3,8 @@
 #include "host_common.h"
 #include "row_launch.h"
 
+#include <algorithm>
+
 namespace {
 
 using namespace b200;
@@ -45,50 +47,48 @@ int check_alignment(const char* name, const void* p, size_t bytes) {
   return 0;
 }
 
-// The backward kernel's shape: threads of a row (of half of it, above 8192 values) and groups of eight values a thread:
-// two of bf16, one of fp32, whose registers are twice as many.
-struct BwdPlan {
-  int threads, vectors, cluster;
-  int groups() const { return threads < 512 ? 512 / threads : 1; }
-};
-BwdPlan bwd_plan(long long cols, int x_type) {
+// The backward pass of rows of up to kBwdHeld values: threads of a row, with two groups of eight bf16 values or one of
+// fp32, whose registers are twice as many.  Wider rows: two kernels, with the rows divided into `parts`.
+constexpr long long kBwdHeld = 8192;
+
+int bwd_threads(long long cols, int x_type) {
   const int v = x_type == B200_OUT_BF16 ? 2 : 1;
-  const int cluster = cols > 8192 ? 2 : 1;
   int threads = 32;
-  while (static_cast<long long>(threads) * v * 8 * cluster < cols) threads *= 2;
-  return {threads, v, cluster};
+  while (static_cast<long long>(threads) * v * 8 < cols) threads *= 2;
+  return threads;
 }
 
-// As many clusters of its blocks as are resident at once, one row of partial sums each.
-long long bwd_units(int sm_count, long long rows, long long cols, int x_type) {
-  if (cols > 16384) return 0;  // no partial sums
-  const BwdPlan plan = bwd_plan(cols, x_type);
-  // 512 threads: two blocks an SM of bf16 (about 64 registers a thread would allow it), 1024: one
-  const long long resident = static_cast<long long>(sm_count) / plan.cluster;
-  const long long needed = (rows + plan.groups() - 1) / plan.groups();
-  return needed < resident ? needed : resident;
+// Rows of partial sums: one for each block that is resident at once (512 threads or more, one an SM), or one for each
+// part of the rows, so many that each SM has about six blocks of strips.
+long long bwd_partials(int sm_count, long long rows, long long cols, int x_type) {
+  if (rows == 0) return 0;
+  if (cols <= kBwdHeld) {
+    const int threads = bwd_threads(cols, x_type), groups = threads < 512 ? 512 / threads : 1;
+    const long long needed = (rows + groups - 1) / groups;
+    return needed < sm_count ? needed : sm_count;
+  }
+  const long long strips = (cols + 127) / 128, wanted = (6LL * sm_count + strips - 1) / strips, most = (rows + 31) / 32;
+  return std::max(1LL, std::min(wanted, most));
 }
 
-template <typename T, typename W, int TPR, int V, int CLUSTER, bool kAligned>
-int launch_bwd(const T* dy, const T* x, const W* weight, const float* mean, const float* rstd, T* dx, float* partial, long long units,
-               long long rows, long long cols, volatile int* status, cudaStream_t stream) {
-  auto kernel = layer_norm_bwd_kernel<T, W, TPR, V, CLUSTER, kAligned>;
-  using Shape = BwdShape<TPR, CLUSTER>;
-  constexpr int smem = Shape::kGroups > 1 ? TPR * V * 8 * 4 : 0;
-  static_assert(smem <= 32 * 1024, "fits without permission");
+size_t bwd_workspace(int sm_count, long long rows, long long cols, int x_type) {
+  const size_t sums = static_cast<size_t>(bwd_partials(sm_count, rows, cols, x_type)) * 2 * cols * sizeof(float);
+  return (sums + 15) / 16 * 16 + (cols > kBwdHeld ? static_cast<size_t>(rows) * sizeof(RowTerms) : 0);
+}
+
+// A launch that may start while the kernel before it on the stream still runs (it waits for it by itself).
+template <typename... Params, typename... Args>
+int launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, bool overlap, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(units * CLUSTER));
-  config.blockDim = dim3(Shape::kThreads);
-  config.dynamicSmemBytes = smem;
+  config.gridDim = grid;
+  config.blockDim = block;
   config.stream = stream;
   cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = CLUSTER;
-  attribute[0].val.clusterDim.y = 1;
-  attribute[0].val.clusterDim.z = 1;
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = overlap ? 1 : 0;
   config.attrs = attribute;
   config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, dy, x, weight, mean, rstd, dx, partial, rows, cols, status);
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
   return err == cudaSuccess ? 0 : host_fail_cuda("layer_norm_bwd launch", err);
 }
 
@@ -146,7 +146,8 @@ extern "C" int b200_int4_gemms_layer_norm(int device_index, uintptr_t stream_han
       using W = decltype(wt);
       for_row_shape<sizeof(T) == 2 ? 8 : 4>(rows, cols, wide, [&](auto tpr, auto v, auto aligned) {
         constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
-        layer_norm_kernel<T, W, TPR, V, decltype(aligned)::value><<<row_blocks<TPR>(rows), RowPlace<TPR>::kThreads, 0, stream>>>(
+        const long long blocks = std::min<long long>(row_blocks<TPR>(rows), 1LL * sms * (512 / RowPlace<TPR>::kThreads));  // its launch bounds
+        layer_norm_kernel<T, W, TPR, V, decltype(aligned)::value><<<static_cast<unsigned>(blocks), RowPlace<TPR>::kThreads, 0, stream>>>(
             static_cast<const T*>(x), static_cast<const W*>(weight), static_cast<const W*>(bias), static_cast<T*>(y), mean, rstd, rows,
             cols, static_cast<float>(eps));
       });
@@ -193,7 +194,7 @@ extern "C" size_t b200_int4_gemms_layer_norm_bwd_workspace_bytes(int device_inde
     DeviceScope device;
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
-    bytes = static_cast<size_t>(bwd_units(sms, rows, cols, x_type)) * 2 * static_cast<size_t>(cols) * sizeof(float);
+    bytes = bwd_workspace(sms, rows, cols, x_type);
     return 0;
   });
   return bytes;
@@ -220,13 +221,13 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
     const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-    const long long units = bwd_units(sms, rows, cols, x_type);
-    if (units > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(units) * 2 * cols * sizeof(float)))
-      return host_fail("workspace must hold b200_int4_gemms_layer_norm_bwd_workspace_bytes bytes");
+    const long long partials = bwd_partials(sms, rows, cols, x_type);
+    const size_t need = bwd_workspace(sms, rows, cols, x_type);
+    if (need > 0 && (workspace == nullptr || !is_aligned(workspace, 16) || workspace_bytes < need))
+      return host_fail("workspace must be 16-byte aligned and hold b200_int4_gemms_layer_norm_bwd_workspace_bytes bytes");
     float* partial = static_cast<float*>(workspace);
-    volatile int* status = device_status_word(device_index);
+    RowTerms* terms = reinterpret_cast<RowTerms*>(static_cast<char*>(workspace) + need - (cols > kBwdHeld ? static_cast<size_t>(rows) * sizeof(RowTerms) : 0));
     const bool wide = cols % 8 == 0 && is_aligned(dy, 16) && is_aligned(x, 16) && is_aligned(dx, 16) && is_aligned(weight, 16);
-    const dim3 column_grid(static_cast<unsigned>((cols + 31) / 32)), column_block(32, 32);
     int rc = 0;
     if (rows > 0) {
       for_types(x_type, weight_type, [&](auto xt, auto wt) {
@@ -239,39 +240,34 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
         for_bool(wide, [&](auto aligned) {
           constexpr bool A = decltype(aligned)::value;
           constexpr int V = sizeof(T) == 2 ? 2 : 1;
+          if (cols > kBwdHeld) {
+            constexpr int G = A ? 16 / static_cast<int>(sizeof(T)) : 1;
+            const long long blocks = std::min<long long>(rows, 4LL * sms);
+            layer_norm_bwd_rows_kernel<T, W, A><<<static_cast<unsigned>(blocks), 512, 0, stream>>>(dy_t, x_t, w_t, mean, rstd, terms, rows, cols);
+            if (rc = launched("layer_norm_bwd launch"); rc != 0) return;
+            const dim3 grid(static_cast<unsigned>((cols + 32 * G - 1) / (32 * G)), static_cast<unsigned>(partials));
+            rc = launch_after(layer_norm_bwd_strips_kernel<T, W, G>, grid, dim3(32 * kStripWarps), true, stream, dy_t, x_t, w_t, terms, dx_t, partial, rows, cols);
+            return;
+          }
           using std::integral_constant;
-          auto rows_of = [&](auto tpr, auto cluster) {
-            rc = launch_bwd<T, W, decltype(tpr)::value, V, decltype(cluster)::value, A>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, units, rows, cols, status, stream);
+          auto rows_of = [&](auto tpr) {
+            constexpr int TPR = decltype(tpr)::value, kThreads = BwdShape<TPR>::kThreads;
+            constexpr int smem = BwdShape<TPR>::kGroups > 1 ? TPR * V * 8 * 4 : 0;
+            layer_norm_bwd_kernel<T, W, TPR, V, A><<<static_cast<unsigned>(partials), kThreads, smem, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, rows, cols);
+            rc = launched("layer_norm_bwd launch");
           };
-          const BwdPlan plan = bwd_plan(cols, x_type);
-          if (cols > 16384) layer_norm_bwd_long_kernel<T, W, A><<<row_blocks<1024>(rows), 1024, 0, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, rows, cols);
-          else if (plan.cluster == 2) rows_of(integral_constant<int, 1024 / V>(), integral_constant<int, 2>());
-          else if (plan.threads == 32) rows_of(integral_constant<int, 32>(), integral_constant<int, 1>());
-          else if (plan.threads == 64) rows_of(integral_constant<int, 64>(), integral_constant<int, 1>());
-          else if (plan.threads == 128) rows_of(integral_constant<int, 128>(), integral_constant<int, 1>());
-          else if (plan.threads == 256) rows_of(integral_constant<int, 256>(), integral_constant<int, 1>());
-          else if (plan.threads == 512) rows_of(integral_constant<int, 512>(), integral_constant<int, 1>());
-          else rows_of(integral_constant<int, V == 1 ? 1024 : 512>(), integral_constant<int, 1>());
+          const int threads = bwd_threads(cols, x_type);
+          if (threads == 32) rows_of(integral_constant<int, 32>());
+          else if (threads == 64) rows_of(integral_constant<int, 64>());
+          else if (threads == 128) rows_of(integral_constant<int, 128>());
+          else if (threads == 256) rows_of(integral_constant<int, 256>());
+          else if (threads == 512) rows_of(integral_constant<int, 512>());
+          else rows_of(integral_constant<int, V == 1 ? 1024 : 512>());
         });
-        if (rc == 0 && cols > 16384)
-          layer_norm_bwd_columns_kernel<T><<<column_grid, column_block, 0, stream>>>(dy_t, x_t, mean, rstd, rows, cols, dweight, dbias);
       });
       if (rc != 0) return rc;
-      if (rc = launched("layer_norm_bwd launch"); rc != 0) return rc;
     }
-    if (rows > 0 && cols > 16384) return launched("layer_norm_bwd columns launch");
-    // may start while the kernel before it ends: it waits for it by itself
-    cudaLaunchConfig_t config{};
-    config.gridDim = column_grid;
-    config.blockDim = dim3(32, kSumRows);
-    config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute[0].val.programmaticStreamSerializationAllowed = rows > 0 ? 1 : 0;
-    config.attrs = attribute;
-    config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, column_sums_kernel, static_cast<const float*>(partial), static_cast<int>(units),
-                                               static_cast<long long>(cols), dweight, dbias);
-    return err == cudaSuccess ? 0 : host_fail_cuda("layer_norm_bwd column sums launch", err);
+    return launch_after(column_sums_kernel, dim3(static_cast<unsigned>((cols + 31) / 32)), dim3(32, kSumRows), rows > 0, stream, partial,
+                        static_cast<int>(partials), cols, dweight, dbias);
   });
 }
