@@ -144,10 +144,9 @@ extern "C" int b200_int4_gemms_layer_norm(int device_index, uintptr_t stream_han
     for_types(x_type, weight_type, [&](auto xt, auto wt) {
       using T = decltype(xt);
       using W = decltype(wt);
-      for_row_shape<sizeof(T) == 2 ? 8 : 4>(rows, cols, wide, [&](auto tpr, auto v, auto aligned) {
+      for_row_shape<4>(rows, cols, wide, [&](auto tpr, auto v, auto aligned) {
         constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
-        const long long blocks = std::min<long long>(row_blocks<TPR>(rows), 1LL * sms * (512 / RowPlace<TPR>::kThreads));  // its launch bounds
-        layer_norm_kernel<T, W, TPR, V, decltype(aligned)::value><<<static_cast<unsigned>(blocks), RowPlace<TPR>::kThreads, 0, stream>>>(
+        layer_norm_kernel<T, W, TPR, V, decltype(aligned)::value><<<row_blocks<TPR>(rows), RowPlace<TPR>::kThreads, 0, stream>>>(
             static_cast<const T*>(x), static_cast<const W*>(weight), static_cast<const W*>(bias), static_cast<T*>(y), mean, rstd, rows,
             cols, static_cast<float>(eps));
       });
