@@ -165,6 +165,18 @@ __device__ __forceinline__ float max_size(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
   return r;
 }
+// The same of three.
+__device__ __forceinline__ float max_size(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The larger of m and two sizes; NaN are passed over.
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+  return r;
+}
 struct MaxSizeOp {
   __device__ __forceinline__ float operator()(float a, float b) const { return max_size(a, b); }
 };
@@ -173,12 +185,48 @@ struct MaxOp {
   __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
 
+// Two fp32 numbers in a register pair: one instruction works on both, each rounded as on its own.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ explicit Pair(float both) : Pair(both, both) {}
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 template <typename V, typename Op>
 __device__ __forceinline__ V warp_reduce(V v, Op op, int width = 32) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     if (o < width) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
   return v;
+}
+
+// Over a whole warp one instruction does it, for whole numbers and for sizes.
+__device__ __forceinline__ uint32_t warp_reduce(uint32_t v, MaxOp op, int width = 32) {
+  if (width == 32) return __reduce_max_sync(0xFFFFFFFFu, v);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < width) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_reduce(float v, MaxSizeOp, int width = 32) {
+  // bit patterns of sizes have the order of the sizes, NaN above infinity
+  return __uint_as_float(warp_reduce(__float_as_uint(v) & 0x7FFFFFFFu, MaxOp(), width));
 }
 
 // Two values at once; every thread of the row gets both results.  `scratch` holds 2 * TPR / 32 values and is not

@@ -197,13 +197,18 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 //
 // A code is decided by the exact value, not by fp32's rounding of it: a value next to the border of two codes
 // would otherwise go to the one or the other with the order of a sum.  The statistics are sums in fp64.  The
-// values are computed in fp32, where they are off by at most E = 2^-21 (|t| + |b|), t = (x - mean) rstd w (four
-// roundings of 2^-24 each, and room); |t| <= amax + |b|, so E <= 2^-21 (amax + 2 max|b|) for a whole group.  A
-// quotient that is further than E/s from every border has its code; otherwise (once in some 10^4 values) the eight
-// values of the thread are computed again in fp64.  The scale is settled in the same way: where amax / top is within its error
-// of a tie of two bf16 numbers, the group's maximum is found again in fp64.  Both are loops that read their values
-// again, out of the way of the code that runs always.
-// The kernel is bound by its instructions, not by HBM.
+// values are computed in fp32, where they are off by at most E = 2^-21 (|t| + |b|), t = (x - mean) rstd w: with the mean
+// in two parts, hi + lo, h = (x - hi) rstd - lo rstd.  Where x - hi is rounded it is far larger than lo; where it is not,
+// it is zero, or at least 2 |lo|, or of the other sign, so that each part is at most 2 |h|.  With rstd's rounding h is off by
+// at most 6 steps of 2^-24 |h|, and t + b by one of its own more.  |t| <= amax + |b|, so E <= 2^-21 (amax + 2 max|b|) for a
+// whole group.  A quotient that is further than E/s from every border has its code; otherwise (once in some 10^4
+// values) the eight values of the thread are computed again in fp64.  The scale is settled in the same way: where
+// amax / top is within its error of a tie of two bf16 numbers, or fp32 has no room for it, the group's maximum is found
+// again in fp64.  Both are loops that read their values again, out of the way of the code that runs always.
+//
+// The kernel is bound by its instructions, not by HBM: 33 a value (two conversions and two sums in fp64 among them),
+// with pairs of fp32 numbers and three-way maxima; 43 without those, 30 us instead of 25 for 4096 x 4096 in bf16 with
+// groups of 256.  More threads an SM with fewer registers change nothing (896 and 1,024: 25 us).
 // ---------------------------------------------------------------------------------------------------------------
 struct NormExact {
   double mean, rstd;
@@ -218,12 +223,15 @@ __device__ __forceinline__ bool near_bf16_tie(float v, float error) {
   return !(fabsf(v - tie) > error);
 }
 
-// The largest size of up to eight exact values from `at` on.
+// The largest size of up to eight exact values from `at` on, as a bit pattern: its order is that of the sizes, with NaN
+// above infinity.
 template <typename T, typename W>
-__device__ __noinline__ double exact_size(const T* row, const W* weight, const W* bias, long long at, long long cols, const NormExact& exact) {
-  double most = 0.0;
-  for (int i = 0; i < 8 && at + i < cols; ++i)
-    most = fmax(most, fabs(exact.value(to_f32(row[at + i]), to_f32(weight[at + i]), bias != nullptr ? to_f32(bias[at + i]) : 0.f)));
+__device__ __noinline__ unsigned long long exact_size(const T* row, const W* weight, const W* bias, long long at, long long cols, const NormExact& exact) {
+  unsigned long long most = 0;
+  for (int i = 0; i < 8 && at + i < cols; ++i) {
+    const double v = exact.value(to_f32(row[at + i]), to_f32(weight[at + i]), bias != nullptr ? to_f32(bias[at + i]) : 0.f);
+    most = MaxOp()(most, static_cast<unsigned long long>(__double_as_longlong(fabs(v))));
+  }
   return most;
 }
 
@@ -249,7 +257,7 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
                            double inv_cols, double eps) {
   __shared__ double scratch_d[2][2 * (TPR / 32)];
   __shared__ float scratch_m[2 * (TPR / 32)];
-  __shared__ double scratch_x[TPR / 32];
+  __shared__ unsigned long long scratch_x[TPR / 32];
   constexpr int kHeld = V > 0 ? V : 1;
   constexpr float kTop = BITS == 4 ? 7.f : 127.f;
   constexpr float kError = 4.76837158203125e-7f;  // 2^-21
@@ -294,23 +302,36 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
     root = root * (1.5 - 0.5 * var * root * root);
     root = root * (1.5 - 0.5 * var * root * root);
     // beyond fp32's range, and for NaN: the library's own
-    if (!(var > 1e-30 && var < 1e30)) root = rsqrt(spread + eps);
+    const bool wild = !(var > 1e-30 && var < 1e30);
+    if (wild) root = rsqrt(spread + eps);
     exact.rstd = root;
     const float mean_hi = static_cast<float>(exact.mean);
     const float mean_lo = static_cast<float>(exact.mean - static_cast<double>(mean_hi));
     const float rstd = static_cast<float>(exact.rstd);
 
-    auto norm8 = [&](int v, float (&out)[8], float& amax, float& bmax) {
+    const Pair minus_hi(-mean_hi), scale(rstd), minus_lo(-mean_lo * rstd);
+    auto norm8 = [&](int v, Pair (&out)[4], float& amax, float& bmax) {
+      if (place(v) >= cols) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = Pair(0.f);
+        return;
+      }
       const Raw8<T> raw = x.get(v);
       Raw8<W> w, b;
       read_affine(v, w, b);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // behind the row w and b are zero, but a row that is not finite would leave NaN there
-        out[i] = __fmaf_rn(((raw.get(i) - mean_hi) - mean_lo) * rstd, w.get(i), b.get(i));
-        if ((kAligned ? place(v) : place(v) + i) >= cols) out[i] = 0.f;
-        amax = max_size(amax, out[i]);
-        bmax = max_size(bmax, b.get(i));
+      for (int i = 0; i < 8; i += 2) {
+        const Pair h = fma2(add2(Pair(raw.get(i), raw.get(i + 1)), minus_hi), scale, minus_lo);
+        out[i / 2] = fma2(h, Pair(w.get(i), w.get(i + 1)), Pair(b.get(i), b.get(i + 1)));
+        float2 f = out[i / 2].get();
+        if (!kAligned) {  // behind the row w and b are zero, but h may be infinite or NaN
+          if (place(v) + i + 1 >= cols) f.y = 0.f;
+          out[i / 2] = Pair(f.x, f.y);
+          if (place(v) + i >= cols) out[i / 2] = Pair(0.f);
+          f = out[i / 2].get();
+        }
+        amax = max_size(amax, f.x, f.y);
+        bmax = max_size(bmax, b.get(i), b.get(i + 1));
       }
     };
     float s = 1.f, delta = 0.f, inv = 1.f;
@@ -320,25 +341,33 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
     auto scale_from = [&](float amax, float bmax) {
       const float error = kError * (amax + 2.f * bmax), quotient = amax * (1.f / kTop);
       s = nonzero_scale(__bfloat162float(__float2bfloat16_rn(quotient)));
-      ordinary = scale_is_ordinary(s);
+      ordinary = !wild && scale_is_ordinary(s);
       inv = about_inverse(s);
       delta = error * inv + kTop * kError;
-      return amax < __int_as_float(0x7F800000) && amax > 0.f && near_bf16_tie(quotient, error * (2.f / kTop));
+      if (!wild && amax == 0.f) return false;
+      // what fp32 has no room for, or too few digits, is settled too
+      return wild || !(amax > 1e-29f && amax < __int_as_float(0x7F800000)) || near_bf16_tie(quotient, error * (2.f / kTop));
     };
-    auto settled = [&](double most) {
-      s = nonzero_scale(bf16_from_double(most / static_cast<double>(kTop)));
+    auto settled = [&](unsigned long long most) {
+      s = nonzero_scale(bf16_from_double(__longlong_as_double(static_cast<long long>(most)) / static_cast<double>(kTop)));
+      ordinary = !wild && scale_is_ordinary(s);
       inv = about_inverse(s);
     };
-    auto put = [&](int v, const float (&out)[8]) {
+    auto put = [&](int v, const Pair (&out)[4]) {
       const long long at = place(v);
       if (at >= cols) return;
       uint32_t c[8];
       float far = 0.f;  // the largest distance of a quotient from its code
+      const Pair inv2(inv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float code = __fmaf_rn(out[i], inv, kRoundMagic);
-        far = fmaxf(far, fabsf(__fmaf_rn(out[i], inv, -__fsub_rn(code, kRoundMagic))));
-        c[i] = __float_as_uint(code);
+      for (int i = 0; i < 8; i += 2) {
+        const Pair code = fma2(out[i / 2], inv2, Pair(kRoundMagic));
+        const float2 word = code.get();
+        c[i] = __float_as_uint(word.x);
+        c[i + 1] = __float_as_uint(word.y);
+        // the code less the quotient
+        const Pair minus = fma2(out[i / 2], Pair(-inv), add2(code, Pair(-kRoundMagic)));
+        far = max_abs(far, minus.get().x, minus.get().y);
       }
       typename CodeWords<BITS>::type packed = CodeWords<BITS>::pack(c);
       if (!(ordinary && far < 0.5f - delta)) {
@@ -348,15 +377,15 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
       store_packed<BITS, kAligned>(codes + r * pitch, at, cols, packed);
     };
 
-    float out[kHeld][8];
+    Pair out[kHeld][4];
     if (!lanes) {
       float amax = 0.f, bmax = 0.f;
 #pragma unroll
       for (int v = 0; v < count; ++v) norm8(v, out[V > 0 ? v : 0], amax, bmax);
       row_reduce2<TPR>(amax, bmax, MaxSizeOp(), MaxSizeOp(), scratch_m);
       if (scale_from(amax, bmax)) {  // the same for all threads of the row
-        double most = 0.0;
-        for (int v = 0; v < count; ++v) most = fmax(most, exact_size<T, W>(row, weight, bias, place(v), cols, exact));
+        unsigned long long most = 0;
+        for (int v = 0; v < count; ++v) most = MaxOp()(most, exact_size<T, W>(row, weight, bias, place(v), cols, exact));
         most = row_reduce<TPR>(most, MaxOp(), scratch_x);
         settled(most);
       }
@@ -376,7 +405,7 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
         bmax = warp_reduce(bmax, MaxSizeOp(), lanes);
         const bool settle = scale_from(amax, bmax);
         if (__any_sync(0xFFFFFFFFu, settle)) {
-          const double most = warp_reduce(exact_size<T, W>(row, weight, bias, place(v), cols, exact), MaxOp(), lanes);
+          const unsigned long long most = warp_reduce(exact_size<T, W>(row, weight, bias, place(v), cols, exact), MaxOp(), lanes);
           if (settle) settled(most);
         }
         if ((threadIdx.x & (lanes - 1)) == 0 && place(v) < cols) scales[r * groups + (place(v) >> sub_bits)] = __float2bfloat16_rn(s);
