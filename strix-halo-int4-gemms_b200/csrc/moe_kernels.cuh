@@ -56,13 +56,19 @@ struct MoeParams {
   double* pair_logit;       // [pairs]: of the chosen experts (router != null)
   int* active;              // {experts in use, passes in all, units handed out by the two products}; then slots of
                             // {expert, first pair, pairs, passes of those before}
-  int* pair_list;           // [pairs], by expert
+  int* pair_list;           // [pairs], by expert; of few tokens [slots, 8]
   double* act;              // [pairs, inner]
   uint8_t* aq;              // [pairs, inner bytes]
   float* as;                // [pairs, groups of inner]
   void* part;               // [down_splits, pairs, hidden]: sums of the codes' products (int32), or scaled ones (fp64)
   int slots, up_ranges, down_ranges, down_splits;
 };
+
+// Up to eight tokens (the products' kMaxN == 1) the time is that of the kernels' starts: every block of the up/gate product
+// picks the experts by itself, and its first one writes them down for the kernels behind.
+constexpr int kMoeFewTokens = 8;
+constexpr int kMoeFewExperts = 256;
+constexpr int kMoeFewPairs = kMoeFewTokens * kMoeMaxTopK;
 
 template <int DT>
 __device__ __forceinline__ long long code_bytes(long long k) { return DT == 4 ? k / 2 : k; }
@@ -172,6 +178,7 @@ template <int DT>
 __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
   grid_release();
   const int b = blockIdx.x;
+  if (b == 0 && threadIdx.x < 2) p.active[2 + threadIdx.x] = 0;  // few tokens; else the select kernel does it
   if (b < p.tokens) {
     route_quantize<DT>(p, b);
   } else if (p.router_f32) {
@@ -192,9 +199,51 @@ __device__ __forceinline__ double logit_of_key(unsigned long long k) {
   return __longlong_as_double(static_cast<long long>((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
 }
 
-// One block of 1024 threads.  A warp picks a token's experts one after the other: the largest logit that is left,
-// ties to the lowest index (a token whose logits are NaN gets the first experts).  A lane keeps
-// PER logits, of experts lane, lane + 32, ...
+// A warp picks a token's experts one after the other: the largest logit that is left, ties to the lowest index (a token
+// whose logits are NaN gets the first experts).  A lane keeps PER logits, of experts lane, lane + 32, ...; lane j
+// hands choice j on.
+template <int PER, typename Take>
+__device__ __forceinline__ void pick_experts(const MoeParams& p, int token, Take&& take) {
+  const int lane = threadIdx.x & 31;
+  unsigned long long key[PER], mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = e < p.experts ? logit_key(__ldcg(p.logits + static_cast<long long>(token) * p.experts + e)) : 0ull;
+  }
+  int mine_id = -1;
+#pragma unroll 1
+  for (int j = 0; j < p.top_k; ++j) {
+    unsigned long long best = 0;
+    unsigned best_id = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        best_id = lane + 32 * i;
+      }
+    const unsigned hi = static_cast<unsigned>(best >> 32), lo = static_cast<unsigned>(best);
+    const unsigned top_hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+    const unsigned top_lo = __reduce_max_sync(0xFFFFFFFFu, hi == top_hi ? lo : 0u);
+    const unsigned id = __reduce_min_sync(0xFFFFFFFFu, hi == top_hi && lo == top_lo ? best_id : 0xFFFFFFFFu);
+    if (lane == j) {
+      mine = (static_cast<unsigned long long>(top_hi) << 32) | top_lo;
+      mine_id = static_cast<int>(id);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (id == static_cast<unsigned>(lane + 32 * i)) key[i] = 0;
+  }
+  if (lane < p.top_k) take(lane, mine_id, logit_of_key(mine));
+}
+
+// The expert that the caller gives a pair; -1 for a number that is none.
+__device__ __forceinline__ int given_expert(const MoeParams& p, int pair) {
+  const long long id = p.ids_64 ? static_cast<const long long*>(p.ids_in)[pair] : static_cast<const int*>(p.ids_in)[pair];
+  return id >= 0 && id < p.experts ? static_cast<int>(id) : -1;
+}
+
+// One block: picks the experts, and lists each one's pairs.
 template <int PER, int THREADS>
 __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) {
   __shared__ int chosen[kMoeMaxPairs];
@@ -207,43 +256,14 @@ __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) 
   grid_release();
   if (p.router != nullptr) {
     for (int t = warp; t < p.tokens; t += THREADS / 32) {
-      unsigned long long key[PER], mine = 0;  // lane j: the key of choice j
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = e < p.experts ? logit_key(__ldcg(p.logits + static_cast<long long>(t) * p.experts + e)) : 0ull;
-      }
-      int mine_id = -1;
-      for (int j = 0; j < p.top_k; ++j) {
-        unsigned long long best = 0;
-        unsigned best_id = 0xFFFFFFFFu;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (key[i] > best) {
-            best = key[i];
-            best_id = lane + 32 * i;
-          }
-        const unsigned hi = static_cast<unsigned>(best >> 32), lo = static_cast<unsigned>(best);
-        const unsigned top_hi = __reduce_max_sync(0xFFFFFFFFu, hi);
-        const unsigned top_lo = __reduce_max_sync(0xFFFFFFFFu, hi == top_hi ? lo : 0u);
-        const unsigned id = __reduce_min_sync(0xFFFFFFFFu, hi == top_hi && lo == top_lo ? best_id : 0xFFFFFFFFu);
-        if (lane == j) {
-          mine = (static_cast<unsigned long long>(top_hi) << 32) | top_lo;
-          mine_id = static_cast<int>(id);
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (id == static_cast<unsigned>(lane + 32 * i)) key[i] = 0;
-      }
-      if (lane < p.top_k) {
-        chosen[t * p.top_k + lane] = mine_id;
-        p.pair_logit[t * p.top_k + lane] = logit_of_key(mine);
-      }
+      pick_experts<PER>(p, t, [&](int choice, int expert, double logit) {
+        chosen[t * p.top_k + choice] = expert;
+        p.pair_logit[t * p.top_k + choice] = logit;
+      });
     }
   } else {
     for (int i = threadIdx.x; i < pairs; i += THREADS) {
-      const long long id = p.ids_64 ? static_cast<const long long*>(p.ids_in)[i] : static_cast<const int*>(p.ids_in)[i];
-      chosen[i] = id >= 0 && id < p.experts ? static_cast<int>(id) : -1;  // any other number: no expert
+      chosen[i] = given_expert(p, i);
     }
   }
   __syncthreads();
@@ -299,6 +319,61 @@ __global__ void __launch_bounds__(THREADS) moe_select_kernel(const MoeParams p) 
     if (chosen[i] >= 0) p.pair_list[first[chosen[i]] + place[k]] = i;
     if (p.ids_out != nullptr) p.ids_out[i] = chosen[i];
   }
+}
+
+// The same within a block of the products of few tokens.  An expert's pairs go into slots of eight, in order, so that
+// every block makes the same ones.
+struct MoeFewChoice {
+  double logit[kMoeFewPairs];
+  int expert[kMoeFewPairs];        // of a pair
+  int slot_expert[kMoeFewPairs];
+  uint8_t slot_pairs[kMoeFewPairs], list[kMoeFewPairs * 8];  // how many, and which
+  uint8_t slot_of[kMoeFewPairs];   // of a pair that begins one
+  int turn[kMoeFewPairs / 32], in_use;
+};
+
+__device__ __forceinline__ void choose_few(const MoeParams& p, MoeFewChoice& few) {
+  const int pairs = p.tokens * p.top_k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (p.router != nullptr) {
+    auto take = [&](int choice, int expert, double logit) {
+      few.expert[warp * p.top_k + choice] = expert;
+      few.logit[warp * p.top_k + choice] = logit;
+    };
+    if (warp < p.tokens) {
+      if (p.experts <= 64) pick_experts<2>(p, warp, take);
+      else pick_experts<kMoeFewExperts / 32>(p, warp, take);
+    }
+  } else if (threadIdx.x < pairs) {
+    few.expert[threadIdx.x] = given_expert(p, threadIdx.x);
+  }
+  __syncthreads();
+  const int i = threadIdx.x, mine = i < pairs ? few.expert[i] : -1;
+  int all = 0, before = 0, leader = i;  // pairs of the same expert; those before this one; the first of its eight
+#pragma unroll 4
+  for (int j = 0; j < pairs; ++j) {
+    if (few.expert[j] != mine) continue;
+    if (j <= i && (all & 7) == 0) leader = j;
+    before += j < i;
+    ++all;
+  }
+  const bool leads = mine >= 0 && leader == i;
+  const unsigned leaders = __ballot_sync(0xFFFFFFFFu, leads);
+  if (lane == 0 && warp < kMoeFewPairs / 32) few.turn[warp] = __popc(leaders);
+  __syncthreads();
+  int slot = __popc(leaders & ((1u << lane) - 1u)), total = 0;
+#pragma unroll
+  for (int w = 0; w < kMoeFewPairs / 32; ++w) {
+    if (w < warp) slot += few.turn[w];
+    total += few.turn[w];
+  }
+  if (leads) {
+    few.slot_expert[slot] = mine;
+    few.slot_pairs[slot] = static_cast<uint8_t>(min(8, all - before));
+    few.slot_of[i] = static_cast<uint8_t>(slot);
+  }
+  if (i == 0) few.in_use = total;
+  __syncthreads();
+  if (mine >= 0) few.list[few.slot_of[leader] * 8 + (before & 7)] = static_cast<uint8_t>(i);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -543,9 +618,11 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   using Sum = typename Stage::Sum;
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
   constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
-  constexpr int kHead = 64;  // slots whose records are read at once
   extern __shared__ __align__(128) uint8_t smem[];
+  constexpr bool kChoose = kMaxN == 1 && !kDown;
+  constexpr int kHead = kChoose ? kMoeFewPairs : 64;  // slots whose records are at hand
   __shared__ int4 head[1 + kHead];
+  __shared__ uint8_t list[kChoose ? kMoeFewPairs * 8 : 1];
   __shared__ int rows[2][kMaxN * 8], pair_of[2][kMaxN * 8];
   __shared__ float row_scale[2][kMaxN * 8];
   __shared__ int unit_after_next;
@@ -553,9 +630,36 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     grid_wait();
     grid_release();
   }
-  // written by the select kernel, which had ended before the up/gate product let the next kernels start
-  const int4* records = reinterpret_cast<const int4*>(p.active);
-  if (threadIdx.x < min(1 + kHead, 1 + p.slots)) head[threadIdx.x] = __ldcg(records + threadIdx.x);
+  // The down product reads before it waits: what the select kernel, or the up/gate product, has written has been there since
+  // before the quantiser let the next kernel start.
+  int4* records = reinterpret_cast<int4*>(p.active);
+  if constexpr (kChoose) {
+    MoeFewChoice& few = *reinterpret_cast<MoeFewChoice*>(smem);  // in the ring, which is not in use yet
+    static_assert(sizeof(MoeFewChoice) <= Stage::kRingBytes, "the choice of experts has to fit the ring");
+    choose_few(p, few);
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i == 0) head[0] = make_int4(few.in_use, few.in_use, 0, 0);
+    if (i < few.in_use) {
+      const int4 record = make_int4(few.slot_expert[i], i * 8, few.slot_pairs[i], i);
+      head[1 + i] = record;
+      if (blockIdx.x == 0) records[1 + i] = record;
+      for (int k = 0; k < record.z; ++k) {
+        list[i * 8 + k] = few.list[i * 8 + k];
+        if (blockIdx.x == 0) p.pair_list[i * 8 + k] = few.list[i * 8 + k];
+      }
+    }
+    if (blockIdx.x == 0) {
+      if (i == 0) p.active[0] = p.active[1] = few.in_use;
+      if (i < p.tokens * p.top_k) {
+        p.pair_expert[i] = few.expert[i];
+        if (p.router != nullptr) p.pair_logit[i] = few.logit[i];
+        if (p.ids_out != nullptr) p.ids_out[i] = few.expert[i];
+      }
+    }
+  } else if (threadIdx.x < min(1 + kHead, 1 + p.tokens * p.top_k)) {
+    head[threadIdx.x] = __ldcg(records + threadIdx.x);
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int half = NN ? warp & 1 : 0, share = NN ? warp >> 1 : warp;
   const int k = kDown ? p.inner : p.hidden, columns = kDown ? p.hidden : 2 * p.inner, gate = p.inner;  // gate columns start there
@@ -666,7 +770,11 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     source.w += w_step;
   };
   // the pairs of a unit: read by its first threads, written down when the buffer is free
-  auto read_pair = [&](const MoeUnit& unit) { return threadIdx.x < unit.here ? __ldcg(p.pair_list + unit.first + threadIdx.x) : 0; };
+  auto read_pair = [&](const MoeUnit& unit) {
+    if (threadIdx.x >= unit.here) return 0;
+    if constexpr (kChoose) return static_cast<int>(list[unit.first + threadIdx.x]);
+    else return __ldcg(p.pair_list + unit.first + threadIdx.x);
+  };
   auto write_pair = [&](const MoeUnit& unit, int pair, int buffer) {
     if (threadIdx.x < unit.here) {
       const int row = kDown ? pair : pair / p.top_k;

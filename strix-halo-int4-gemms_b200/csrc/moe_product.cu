@@ -83,16 +83,15 @@ int launch_moe_int4(const MoeParams& params, bool n_major, int sm_count, cudaStr
 int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStream_t stream) {
 #endif
   MoeParams p = params;
-  p.rows_a_pass = p.tokens <= 8 ? 8 : p.tokens <= 16 || p.sub ? 16 : 32;
+  const bool few = p.tokens <= kMoeFewTokens && p.experts <= kMoeFewExperts;
+  p.rows_a_pass = few ? 8 : p.tokens <= 16 || p.sub ? 16 : 32;
   const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 3) / 4) : 0;
   moe_route_kernel<kBits><<<p.tokens + logit_blocks, 256, 0, stream>>>(p);
   if (const cudaError_t err = cudaGetLastError(); err != cudaSuccess) return host_fail_cuda("moe_swiglu launch", err);
-  // experts <= 64, 256, 1024: logits a lane keeps; a warp for each token, as far as 32 go
-  const bool wide = p.tokens > 8 || p.experts > 256;
-  auto select = p.experts <= 64 ? (wide ? moe_select_kernel<2, 1024> : moe_select_kernel<2, 256>)
-                : p.experts <= 256 ? (wide ? moe_select_kernel<8, 1024> : moe_select_kernel<8, 256>)
-                                   : moe_select_kernel<32, 1024>;
-  if (int rc = launch_dependent(select, dim3(1), wide ? 1024 : 256, 0, stream, p); rc != 0) return rc;
+  if (!few) {  // experts <= 64, 256, 1024: logits a lane keeps
+    auto select = p.experts <= 64 ? moe_select_kernel<2, 1024> : p.experts <= 256 ? moe_select_kernel<8, 1024> : moe_select_kernel<32, 1024>;
+    if (int rc = launch_dependent(select, dim3(1), 1024, 0, stream, p); rc != 0) return rc;
+  }
   // words of token codes that a lane takes at a step: as many as keep a step within a group of K (32 K a word of
   // nibbles, 16 a word of bytes) and the ring's stages small
   constexpr int kWord = kBits == 4 ? 32 : 16, kLeast = kBits == 4 ? 1 : 2;
