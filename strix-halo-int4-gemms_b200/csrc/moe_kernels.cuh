@@ -56,7 +56,7 @@ struct MoeParams {
   double* pair_logit;       // [pairs]: of the chosen experts (router != null)
   int* active;              // {experts in use, passes in all, units handed out by the two products}; then slots of
                             // {expert, first pair, pairs, passes of those before}
-  int* pair_list;           // [pairs], by expert; of few tokens [slots, 8]
+  int* pair_list;           // [pairs], by expert
   double* act;              // [pairs, inner]
   uint8_t* aq;              // [pairs, inner bytes]
   float* as;                // [pairs, groups of inner]
@@ -65,7 +65,7 @@ struct MoeParams {
 };
 
 // Up to eight tokens (the products' kMaxN == 1) the time is that of the kernels' starts: every block of the up/gate product
-// picks the experts by itself, and its first one writes them down for the kernels behind.
+// (and then of the down product) picks the experts by itself.
 constexpr int kMoeFewTokens = 8;
 constexpr int kMoeFewExperts = 256;
 constexpr int kMoeFewPairs = kMoeFewTokens * kMoeMaxTopK;
@@ -327,7 +327,8 @@ struct MoeFewChoice {
   double logit[kMoeFewPairs];
   int expert[kMoeFewPairs];        // of a pair
   int slot_expert[kMoeFewPairs];
-  uint8_t slot_pairs[kMoeFewPairs], list[kMoeFewPairs * 8];  // how many, and which
+  alignas(4) uint8_t list[kMoeFewPairs * 8];  // the pairs of each slot
+  uint8_t slot_pairs[kMoeFewPairs];
   uint8_t slot_of[kMoeFewPairs];   // of a pair that begins one
   int turn[kMoeFewPairs / 32], in_use;
 };
@@ -484,8 +485,8 @@ __global__ void __launch_bounds__(kMoeQuantThreads) moe_quantize_kernel(const Mo
   constexpr double kTop = DT == 4 ? 7.0 : 127.0;
   constexpr int kWarps = kMoeQuantThreads / 32;
   __shared__ unsigned long long warp_max[kWarps];
+  grid_release();  // so that the down product's first weights are on their way while the up/gate product ends
   grid_wait();
-  grid_release();
   const int pair = blockIdx.x;
   if (p.pair_expert[pair] < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -619,10 +620,10 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
   constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr bool kChoose = kMaxN == 1 && !kDown;
+  constexpr bool kChoose = kMaxN == 1;
   constexpr int kHead = kChoose ? kMoeFewPairs : 64;  // slots whose records are at hand
   __shared__ int4 head[1 + kHead];
-  __shared__ uint8_t list[kChoose ? kMoeFewPairs * 8 : 1];
+  __shared__ __align__(4) uint8_t list[kChoose ? kMoeFewPairs * 8 : 4];
   __shared__ int rows[2][kMaxN * 8], pair_of[2][kMaxN * 8];
   __shared__ float row_scale[2][kMaxN * 8];
   __shared__ int unit_after_next;
@@ -630,9 +631,9 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     grid_wait();
     grid_release();
   }
-  // The down product reads before it waits: what the select kernel, or the up/gate product, has written has been there since
-  // before the quantiser let the next kernel start.
-  int4* records = reinterpret_cast<int4*>(p.active);
+  // The down product reads before it waits: the logits, or the select kernel's records, which were there before the up/gate
+  // product let the next kernels start.
+  const int4* records = reinterpret_cast<const int4*>(p.active);
   if constexpr (kChoose) {
     MoeFewChoice& few = *reinterpret_cast<MoeFewChoice*>(smem);  // in the ring, which is not in use yet
     static_assert(sizeof(MoeFewChoice) <= Stage::kRingBytes, "the choice of experts has to fit the ring");
@@ -640,24 +641,14 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     __syncthreads();
     const int i = threadIdx.x;
     if (i == 0) head[0] = make_int4(few.in_use, few.in_use, 0, 0);
-    if (i < few.in_use) {
-      const int4 record = make_int4(few.slot_expert[i], i * 8, few.slot_pairs[i], i);
-      head[1 + i] = record;
-      if (blockIdx.x == 0) records[1 + i] = record;
-      for (int k = 0; k < record.z; ++k) {
-        list[i * 8 + k] = few.list[i * 8 + k];
-        if (blockIdx.x == 0) p.pair_list[i * 8 + k] = few.list[i * 8 + k];
-      }
+    if (i < few.in_use) head[1 + i] = make_int4(few.slot_expert[i], i * 8, few.slot_pairs[i], i);
+    *reinterpret_cast<uint32_t*>(list + i * 4) = *reinterpret_cast<const uint32_t*>(few.list + i * 4);
+    if (!kDown && blockIdx.x == 0 && i < p.tokens * p.top_k) {
+      p.pair_expert[i] = few.expert[i];
+      if (p.router != nullptr) p.pair_logit[i] = few.logit[i];
+      if (p.ids_out != nullptr) p.ids_out[i] = few.expert[i];
     }
-    if (blockIdx.x == 0) {
-      if (i == 0) p.active[0] = p.active[1] = few.in_use;
-      if (i < p.tokens * p.top_k) {
-        p.pair_expert[i] = few.expert[i];
-        if (p.router != nullptr) p.pair_logit[i] = few.logit[i];
-        if (p.ids_out != nullptr) p.ids_out[i] = few.expert[i];
-      }
-    }
-  } else if (threadIdx.x < min(1 + kHead, 1 + p.tokens * p.top_k)) {
+  } else if (threadIdx.x < min(1 + kHead, 1 + p.slots)) {
     head[threadIdx.x] = __ldcg(records + threadIdx.x);
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
@@ -1050,94 +1041,86 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   copy_wait<0>();
 }
 
-// Adds up the parts of K, scales, and adds up the experts' shares of a token in the order of its choices.  A thread has
-// two columns of one token; what depends on the pair alone is worked out once a block: the softmax of the chosen logits
-// (or of all) in fp64.  What the select kernel left and the scales are read before the down product has ended.
+// Adds up the parts of K, scales, and adds up the experts' shares of a token in the order of its choices, for 64 columns
+// of one token.  A thread has two columns of one choice (two choices, beyond eight), whose share it leaves in shared memory:
+// with all choices to a thread the unrolled code took longer to be fetched than to run (3.5 us behind the wait).  What
+// depends on the pair alone is worked out once a block: the softmax of the chosen logits (or of all) in fp64.  What the
+// choice of experts left and the scales are read before the down product has ended.
+constexpr int kCombineLines = 8;
+
 template <bool SC>
-__global__ void __launch_bounds__(128) moe_combine_kernel(const MoeParams p) {
+__global__ void __launch_bounds__(32 * kCombineLines) moe_combine_kernel(const MoeParams p) {
   using Sum = typename MoeSum<SC>::type;
   using Sum2 = typename std::conditional<SC, double2, int2>::type;
-  constexpr int kAtOnce = 8;
-  __shared__ int expert[kMoeMaxTopK];
-  __shared__ float weight[kMoeMaxTopK], scale[kMoeMaxTopK];
-  __shared__ double parts[4];
-  const int token = blockIdx.y, col = (blockIdx.x * 128 + threadIdx.x) * 2, lane = threadIdx.x & 31;
-  double others = 0.0;
-  if (p.router != nullptr && !p.renormalize) {
-    const double top = __ldcg(p.pair_logit + token * p.top_k);
-    for (int e = threadIdx.x; e < p.experts; e += 128) others += exp(__ldcg(p.logits + static_cast<long long>(token) * p.experts + e) - top);
-    others = warp_reduce(others, SumOp());
-    if (lane == 0) parts[threadIdx.x >> 5] = others;
-    __syncthreads();
-    others = parts[0] + parts[1] + parts[2] + parts[3];
+  constexpr int kEach = kMoeMaxTopK / kCombineLines;
+  __shared__ float weight[kMoeMaxTopK];
+  __shared__ bool counts[kMoeMaxTopK];  // a choice without an expert adds nothing, whatever its weight is
+  __shared__ float2 share[kMoeMaxTopK][32];
+  const int token = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5, col = (blockIdx.x * 32 + lane) * 2;
+  const bool inside = col < p.hidden;
+  int expert[kEach];
+  uint32_t w[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = line + i * kCombineLines;
+    expert[i] = j < p.top_k ? __ldcg(p.pair_expert + token * p.top_k + j) : -1;
+    if (lane == 0) counts[j] = expert[i] >= 0;
+    w[i] = !SC && inside && expert[i] >= 0 ? *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[i]) * p.hidden + col) : 0u;
   }
-  if (threadIdx.x < 32) {
+  if (line == 0) {
     const int pair = token * p.top_k + min(lane, p.top_k - 1);
-    float w;
+    float v;
     if (p.router != nullptr) {
       const double logit = __ldcg(p.pair_logit + pair), top = __shfl_sync(0xFFFFFFFFu, logit, 0);
-      const double e = lane < p.top_k ? exp(logit - top) : 0.0;
-      const double total = warp_reduce(e, SumOp());
-      w = static_cast<float>(e / (p.renormalize ? total : others));
+      const double mine = lane < p.top_k ? exp(logit - top) : 0.0;
+      double all = mine;
+      if (!p.renormalize) {
+        all = 0.0;
+        for (int e = lane; e < p.experts; e += 32) all += exp(__ldcg(p.logits + static_cast<long long>(token) * p.experts + e) - top);
+      }
+      v = static_cast<float>(mine / warp_reduce(all, SumOp()));
     } else {
-      w = p.weights_in[pair];
+      v = p.weights_in[pair];
     }
     if (lane < p.top_k) {
-      expert[lane] = __ldcg(p.pair_expert + pair);
-      weight[lane] = w;
-      if (p.weights_out != nullptr && blockIdx.x == 0) p.weights_out[pair] = w;
+      weight[lane] = v;
+      if (p.weights_out != nullptr && blockIdx.x == 0) p.weights_out[pair] = v;
     }
+  }
+  grid_wait();
+  const long long plane = static_cast<long long>(p.tokens) * p.top_k * p.hidden;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = line + i * kCombineLines, pair = token * p.top_k + j;
+    if (!inside || expert[i] < 0) continue;
+    const Sum2* at = reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + static_cast<long long>(pair) * p.hidden + col);
+    const float scale = SC ? 0.f : __ldcg(p.as + pair);
+    Sum2 sum = __ldcg(at);
+#pragma unroll 4
+    for (int s = 1; s < p.down_splits; ++s) {
+      const Sum2 more = __ldcg(at + s * (plane / 2));
+      sum.x += more.x;
+      sum.y += more.y;
+    }
+    double y0 = static_cast<double>(sum.x), y1 = static_cast<double>(sum.y);
+    if (!SC) {
+      y0 *= static_cast<double>(scale * bf16_lo(w[i]));  // a product of two bf16 numbers is exact in fp32
+      y1 *= static_cast<double>(scale * bf16_hi(w[i]));
+    }
+    share[j][lane] = make_float2(static_cast<float>(y0), static_cast<float>(y1));
   }
   __syncthreads();
-  const bool inside = col < p.hidden;
-  uint32_t w[kAtOnce];
-  auto read_scales = [&](int j0) {
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int j = j0 + k;
-      w[k] = !SC && inside && j < p.top_k && expert[j] >= 0 ? *reinterpret_cast<const uint32_t*>(p.s_down + static_cast<long long>(expert[j]) * p.hidden + col) : 0u;
-    }
-  };
-  read_scales(0);
-  grid_wait();
-  if (!SC && threadIdx.x < p.top_k) scale[threadIdx.x] = expert[threadIdx.x] >= 0 ? __ldcg(p.as + token * p.top_k + threadIdx.x) : 1.f;
-  const long long plane = static_cast<long long>(p.tokens) * p.top_k * p.hidden;
-  float total[2] = {0.f, 0.f};
-  for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
-    if (j0 > 0) read_scales(j0);
-    Sum2 sum[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) sum[k].x = sum[k].y = 0;
-    for (int s = 0; s < p.down_splits; ++s) {
-#pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const int j = j0 + k;
-        if (inside && j < p.top_k && expert[j] >= 0) {
-          const Sum2 more = __ldcg(reinterpret_cast<const Sum2*>(static_cast<const Sum*>(p.part) + s * plane + static_cast<long long>(token * p.top_k + j) * p.hidden + col));
-          sum[k].x += more.x;
-          sum[k].y += more.y;
-        }
-      }
-    }
-    if (j0 == 0) __syncthreads();  // the scales
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int j = j0 + k;
-      if (j >= p.top_k || expert[j] < 0) continue;
-      double y0 = static_cast<double>(sum[k].x), y1 = static_cast<double>(sum[k].y);
-      if (!SC) {
-        y0 *= static_cast<double>(scale[j] * bf16_lo(w[k]));  // a product of two bf16 numbers is exact in fp32
-        y1 *= static_cast<double>(scale[j] * bf16_hi(w[k]));
-      }
-      total[0] += static_cast<float>(y0) * weight[j];
-      total[1] += static_cast<float>(y1) * weight[j];
-    }
+  if (line > 0 || !inside) return;
+  float x = 0.f, y = 0.f;
+#pragma unroll 4
+  for (int j = 0; j < p.top_k; ++j) {
+    if (!counts[j]) continue;
+    x = __fmaf_rn(share[j][lane].x, weight[j], x);
+    y = __fmaf_rn(share[j][lane].y, weight[j], y);
   }
-  if (inside) {
-    bf16* out = p.out + static_cast<long long>(token) * p.hidden + col;
-    out[0] = __float2bfloat16_rn(total[0]);
-    out[1] = __float2bfloat16_rn(total[1]);
-  }
+  bf16* out = p.out + static_cast<long long>(token) * p.hidden + col;
+  out[0] = __float2bfloat16_rn(x);
+  out[1] = __float2bfloat16_rn(y);
 }
 
 }  // namespace b200

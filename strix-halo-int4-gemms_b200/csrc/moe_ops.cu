@@ -55,8 +55,8 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->logits = reinterpret_cast<double*>(take(static_cast<size_t>(m.tokens) * m.experts * 8));
   p->pair_expert = reinterpret_cast<int*>(take(pairs * 4));
   p->pair_logit = reinterpret_cast<double*>(take(pairs * 8));
-  p->active = reinterpret_cast<int*>(take((1 + pairs) * 16));
-  p->pair_list = reinterpret_cast<int*>(take((m.tokens <= kMoeFewTokens ? pairs * 8 : pairs) * 4));
+  p->active = reinterpret_cast<int*>(take((1 + static_cast<size_t>(p->slots)) * 16));
+  p->pair_list = reinterpret_cast<int*>(take(pairs * 4));
   p->act = reinterpret_cast<double*>(take(pairs * m.inner * 8));
   p->aq = reinterpret_cast<uint8_t*>(take(pairs * m.inner / per_byte));
   p->as = reinterpret_cast<float*>(take(pairs * a_groups * 4));

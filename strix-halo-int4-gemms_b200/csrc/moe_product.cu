@@ -65,10 +65,11 @@ int launch_for_tokens(const MoeParams& p, int sm_count, cudaStream_t stream) {
     constexpr int kMaxN = decltype(max_n)::value;
     if (int rc = launch_product<NN, SC, WORDS, kMaxN, false>(p, sm_count, stream); rc != 0) return rc;
     constexpr int kRow = kMoeQuantThreads * 2;
-    auto quantize = SC || p.inner <= 2 * kRow ? moe_quantize_kernel<kBits, 2> : p.inner <= 14 * kRow ? moe_quantize_kernel<kBits, 14> : moe_quantize_kernel<kBits, 0>;
+    auto quantize = SC || p.inner <= 4 * kRow ? moe_quantize_kernel<kBits, 4> : p.inner <= 14 * kRow ? moe_quantize_kernel<kBits, 14> : moe_quantize_kernel<kBits, 0>;
     if (int rc = launch_dependent(quantize, dim3(p.tokens * p.top_k), kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
     if (int rc = launch_product<NN, SC, WORDS, kMaxN, true>(p, sm_count, stream); rc != 0) return rc;
-    return launch_dependent(moe_combine_kernel<SC>, dim3((p.hidden + 255) / 256, p.tokens), 128, 0, stream, p);
+    const int lines = p.top_k < kCombineLines ? p.top_k : kCombineLines;
+    return launch_dependent(moe_combine_kernel<SC>, dim3((p.hidden + 63) / 64, p.tokens), 32 * lines, 0, stream, p);
   };
   if (p.rows_a_pass == 8) return products(std::integral_constant<int, 1>());
   if (p.rows_a_pass == 16) return products(std::integral_constant<int, 2>());
