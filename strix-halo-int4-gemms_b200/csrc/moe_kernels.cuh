@@ -46,7 +46,7 @@ struct MoeParams {
   const bf16* s_up_gate;
   const bf16* s_down;
   bf16* out;                // [tokens, hidden]
-  int tokens, hidden, inner, experts, top_k, sub;
+  int tokens, hidden, inner, experts, top_k, sub, sub_bits;  // a group of K: sub = 2^sub_bits values; 0: none
   int router_f32, ids_64, renormalize, rows_a_pass;
   // scratch
   uint8_t* xq;              // [tokens, hidden bytes]
@@ -158,7 +158,7 @@ __device__ __forceinline__ void route_quantize(const MoeParams& p, int token) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = __vmaxu2(m, raw.w[i] & 0x7FFF7FFFu);
       s = scale_of_bf16<DT>(warp_reduce(max(m & 0xFFFFu, m >> 16), MaxOp(), lanes));
-      if ((threadIdx.x & (lanes - 1)) == 0 && at < p.hidden) p.xs[token * groups + at / p.sub] = s;
+      if ((threadIdx.x & (lanes - 1)) == 0 && at < p.hidden) p.xs[token * groups + (at >> p.sub_bits)] = s;
     }
     uint32_t c[8];
     if (scale_is_ordinary(s)) {
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   using Stage = MoeStage<DT, NN, SC, WORDS, kMaxN>;
   using Sum = typename Stage::Sum;
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
-  constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
+  constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kStepBits = kStepK == 64 ? 6 : 5, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr bool kChoose = kMaxN == 1;
   constexpr int kHead = kChoose ? kMoeFewPairs : 64;  // slots whose records are at hand
@@ -668,9 +668,14 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   const int in_use = head[0].x, units = head[0].y * splits * ranges;
   int* counter = p.active + (kDown ? 3 : 2);
 
-  // NN: consecutive steps (whole groups of K as far as it goes); NT: every eighth
-  constexpr bool kConsecutive = NN;
-  const int by = kConsecutive ? 1 : kShares;
+  // A share's steps.  NN: consecutive ones (whole groups of K as far as it goes).  NT: a group's of every eighth group of
+  // K, or every eighth step, so that the eight read a row in one long piece.
+  const int run_bits = SC && !NN ? p.sub_bits - kStepBits : 0;
+  auto step_of = [&](const MoeUnit& unit, int i) {
+    if (NN) return unit.begin + i;
+    return unit.begin + ((i >> run_bits) << run_bits) * kShares + (i & ((1 << run_bits) - 1));
+  };
+  auto group_of = [&](int step) { return (step << kStepBits) >> p.sub_bits; };
   auto decode = [&](int u) {
     MoeUnit unit;
     const int pass = u / (splits * ranges), rest = u - pass * splits * ranges;
@@ -688,9 +693,16 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     unit.expert = r.x;
     unit.first = r.y + done;
     unit.here = min(kMaxN * 8, r.z - done);
-    const int step0 = steps * unit.split / splits, count = steps * (unit.split + 1) / splits - step0, per_share = (count + kShares - 1) / kShares;
-    unit.begin = step0 + (kConsecutive ? share * per_share : share);
-    unit.mine = kConsecutive ? max(0, min(count - share * per_share, per_share)) : max(0, (count - share + kShares - 1) / kShares);
+    const int step0 = steps * unit.split / splits, count = steps * (unit.split + 1) / splits - step0;
+    if (NN) {
+      const int per_share = (count + kShares - 1) / kShares;
+      unit.begin = step0 + share * per_share;
+      unit.mine = max(0, min(count - share * per_share, per_share));
+    } else {
+      const int run = 1 << run_bits, rounds = count >> run_bits, rest = count - (rounds / kShares * kShares << run_bits);
+      unit.begin = step0 + (share << run_bits);
+      unit.mine = (rounds / kShares << run_bits) + max(0, min(rest - (share << run_bits), run));
+    }
     return unit;
   };
   // first column of a fragment of this warp in a range, and whether the matrix has it (16 columns at a time)
@@ -703,7 +715,7 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     if (kDown) return column_of(range, f) < columns;
     return range * (kCols / 2) + (half * kFrags + f) % (kAllFrags / 2) * 16 < gate;
   };
-  const long long w_step = NN ? static_cast<long long>(by) * kStepBytes * columns : static_cast<long long>(by) * kStepBytes;
+  const long long w_step = static_cast<long long>(kStepBytes) * columns;                           // NN: to the next step
   const long long w_rows = NN ? 8LL * columns : 8 * code_pitch;                                    // to the next of a lane's loads
   const long long w_frag = NN ? 0 : (kDown ? 32LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its third fragment
   const uint8_t* all_weights = kDown ? p.w_down : p.w_up_gate;
@@ -730,10 +742,11 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     }
     return source;
   };
-  // step `i` of a warp's steps of a unit; source.w moves on with every call
+  // step `i` of a warp's steps of a unit; for NN source.w moves on with every call.  Nothing is read where `valid` is false
+  // (the copy's size is zero), whatever the address is.
   auto copy_weights = [&](const MoeUnit& unit, MoeSource& source, int i, int slot) {
     const uint32_t at = ring_at + slot * Stage::kBytes;
-    const int step = unit.begin + i * by;
+    const int step = step_of(unit, i);
     if constexpr (NN) {
       // 16 bytes of row r and fragment f to place r * 4 + (f ^ (r / 2 % 4)): eight rows of a fragment on eight banks
       const uint8_t* src = source.w;
@@ -743,22 +756,22 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
 #pragma unroll
       for (int l = 0; l < kStepBytes / 8; ++l, src += w_rows) {
         const bool valid = source.valid && l * 8 < rows_left;
-        copy_async<16>(to + l * 512, valid ? src : all_weights, valid);
+        copy_async<16>(to + l * 512, src, valid);
       }
+      source.w += w_step;
     } else {
       const bool in_k = step * kStepK + q * (kStepK / 4) < k;
 #pragma unroll
       for (int l = 0; l < 2 * kFrags; ++l) {
         const bool valid = in_k && (l < 4 || source.valid);  // columns g and g + 8 of fragment l / 2; the second two follow by w_frag
-        const uint8_t* src = source.w + ((l & 1) ? w_rows : 0) + ((l & 2) ? 2 * w_rows : 0) + ((l & 4) ? w_frag : 0);
-        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, valid ? src : all_weights, valid);
+        const uint8_t* src = source.w + (step - unit.begin) * kStepBytes + ((l & 1) ? w_rows : 0) + ((l & 2) ? 2 * w_rows : 0) + ((l & 4) ? w_frag : 0);
+        copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, src, valid);
       }
     }
     if constexpr (SC) {
-      const long long group = static_cast<long long>(step * kStepK / p.sub) * columns;
+      const long long group = static_cast<long long>(group_of(step)) * columns;
       copy_async<4>(at + Stage::kScalesAt + lane * 4, source.scale + group, source.scale_valid);
     }
-    source.w += w_step;
   };
   // the pairs of a unit: read by its first threads, written down when the buffer is free
   auto read_pair = [&](const MoeUnit& unit) {
@@ -830,15 +843,15 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
       if (SC && lane < unit.here && lane < kN * 8) token_scale = all_scales + static_cast<long long>(rows[buffer][lane]) * groups;
       auto copy_codes = [&](int i, int to_slot) {
         const uint32_t at = ring_at + to_slot * Stage::kBytes;
-        const int step = unit.begin + i * by, offset = i * by * kStepBytes;
+        const int step = step_of(unit, i), offset = (step - unit.begin) * kStepBytes;
         const bool in_k = step * kStepK + q * (kStepK / 4) < k;
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
           const bool valid = in_k && has_token[n];
-          copy_async<4 * WORDS>(at + Stage::kWeights + (n * 32 + lane) * 4 * WORDS, valid ? codes[n] + offset : all_codes, valid);
+          copy_async<4 * WORDS>(at + Stage::kWeights + (n * 32 + lane) * 4 * WORDS, codes[n] + offset, valid);
         }
         if constexpr (SC) {
-          if (lane < kN * 8) copy_async<4>(at + Stage::kRowScalesAt + lane * 4, lane < unit.here ? token_scale + step * kStepK / p.sub : all_scales, lane < unit.here);
+          if (lane < kN * 8) copy_async<4>(at + Stage::kRowScalesAt + lane * 4, token_scale + group_of(step), lane < unit.here);
         }
       };
       int ahead = slot;  // the stage that is copied to next
@@ -849,6 +862,9 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         if (++ahead == kStages) ahead = 0;
       }
       look_ahead();
+      // Packed: a group's sum is below 2^22 in size (256 times 256 products of up to 56), and starts at the bits of 1.5 *
+      // 2^23, so that it is an fp32 number as it stands.
+      constexpr int kAccZero = SC && DT == 4 ? 0x4B400000 : 0;
       int acc[kFrags][kN][4];
       double sum[SC ? kFrags : 1][SC ? kN : 1][4];
 #pragma unroll
@@ -857,7 +873,7 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            acc[f][n][i] = 0;
+            acc[f][n][i] = kAccZero;
             if (SC) sum[f][n][i] = 0.0;
           }
 #pragma unroll 1
@@ -934,22 +950,31 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         }
         if constexpr (SC) {
           // the integers of a group of K end here: scaled and added up in fp64 (a step lies in one group)
-          if (i + 1 == unit.mine || !NN || ((unit.begin + i + 1) * kStepK) % p.sub == 0) {
-            const bf16* w_scales = reinterpret_cast<const bf16*>(stage + Stage::kScalesAt);
+          const int next_step = step_of(unit, i) + 1;
+          if (i + 1 == unit.mine || ((next_step << kStepBits) & (p.sub - 1)) == 0 || (!NN && ((i + 1) & ((1 << run_bits) - 1)) == 0)) {
+            const uint16_t* w_scales = reinterpret_cast<const uint16_t*>(stage + Stage::kScalesAt);
             const float* row_scales = reinterpret_cast<const float*>(stage + Stage::kRowScalesAt);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
               const float2 st = *reinterpret_cast<const float2*>(row_scales + n * 8 + 2 * q);
-              const double st0 = st.x, st1 = st.y;
+              // (packed: the sums are 256 times too large)
+              const double st0 = static_cast<double>(DT == 4 ? st.x * 0.00390625f : st.x), st1 = static_cast<double>(DT == 4 ? st.y * 0.00390625f : st.y);
 #pragma unroll
               for (int f = 0; f < kFrags; ++f)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  const double sw = to_f32(w_scales[f * 16 + g + h * 8]);
-                  const int a = acc[f][n][2 * h], b = acc[f][n][2 * h + 1];
-                  sum[f][n][2 * h] = fma(exact_double(DT == 4 ? a >> 8 : a), st0 * sw, sum[f][n][2 * h]);
-                  sum[f][n][2 * h + 1] = fma(exact_double(DT == 4 ? b >> 8 : b), st1 * sw, sum[f][n][2 * h + 1]);
-                  acc[f][n][2 * h] = acc[f][n][2 * h + 1] = 0;
+                  const float sw = __uint_as_float(static_cast<uint32_t>(w_scales[f * 16 + g + h * 8]) << 16);
+                  int &a = acc[f][n][2 * h], &b = acc[f][n][2 * h + 1];
+                  if (DT == 4) {  // 14 bits of the sum, 8 of the scale: exact in fp32
+                    const Pair whole = add2(Pair(__int_as_float(a), __int_as_float(b)), Pair(-12582912.f));
+                    const float2 scaled = mul2(whole, Pair(sw)).get();
+                    sum[f][n][2 * h] = fma(static_cast<double>(scaled.x), st0, sum[f][n][2 * h]);
+                    sum[f][n][2 * h + 1] = fma(static_cast<double>(scaled.y), st1, sum[f][n][2 * h + 1]);
+                  } else {
+                    sum[f][n][2 * h] = fma(exact_double(a), st0 * static_cast<double>(sw), sum[f][n][2 * h]);
+                    sum[f][n][2 * h + 1] = fma(exact_double(b), st1 * static_cast<double>(sw), sum[f][n][2 * h + 1]);
+                  }
+                  a = b = kAccZero;
                 }
             }
           }

@@ -118,6 +118,7 @@ extern "C" int b200_int4_gemms_moe_swiglu(const b200_moe_problem* problem, int d
     p.experts = m.experts;
     p.top_k = m.top_k;
     p.sub = m.subchannel;
+    while ((1 << p.sub_bits) < p.sub) ++p.sub_bits;
     p.router_f32 = m.router_type == B200_OUT_F32;
     p.ids_64 = m.ids_bits == 64;
     p.renormalize = m.renormalize;
