@@ -438,29 +438,33 @@ constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
 
 // A block works on a range of columns at a time: 64 (K-major weights, NT) or 128 (N-major, NN), for up/gate half of
-// them up columns and half the same columns of the gate.  Its eight warps divide K into shares and, for NN, the
-// columns into halves; a warp has four fragments of 16 columns.
+// them up columns and half the same columns of the gate.  Its eight warps divide K into four shares and the
+// columns into halves; a warp has two or four fragments of 16 columns.  (NT: two, with 64 bytes of each column a step in
+// 16-byte copies.  Four, with 32 bytes in 8-byte copies, kept HBM at a third of its rate.)
 // A step is 4 * WORDS * (8 or 4) values of K, of which lane q of a quad has WORDS consecutive words of the token codes.
 // NT: and the same words of each column.  NN: rows of 64 columns, which ldmatrix transposes; the row that a lane names
 // for it puts the right values of K into each quad's words.
 // One stage of a warp's ring: weights, token codes, and (SC) the scales of the step's group of K.
 template <int DT, bool NN, bool SC, int WORDS, int kN>
 struct MoeStage {
-  static constexpr int kCols = NN ? 128 : 64, kFrags = 4, kHalves = NN ? 2 : 1, kShares = kMoeWarps / kHalves;
+  static constexpr int kFrags = NN ? 4 : 2, kHalves = 2, kCols = kHalves * kFrags * 16, kShares = kMoeWarps / kHalves;
   static constexpr int kStepK = 4 * WORDS * (DT == 4 ? 8 : 4), kStepBytes = 16 * WORDS;  // of a column
   static constexpr int kWeights = kFrags * 16 * kStepBytes;                              // bytes
   static constexpr int kCodeBytes = 4 * WORDS;                                           // of a token, by a lane
   static constexpr int kScalesAt = kWeights + kN * 32 * kCodeBytes;
   static constexpr int kRowScalesAt = kScalesAt + (SC ? kFrags * 32 : 0);
   static constexpr int kBytes = kRowScalesAt + (SC ? kN * 8 * 4 : 0);
-  // about 8 KB a warp, so that three blocks fit an SM where their registers do
-  static constexpr int kStages = 8448 / kBytes < 3 ? 3 : (8448 / kBytes > 8 ? 8 : 8448 / kBytes);
   using Sum = typename MoeSum<SC>::type;
-  static constexpr int kRingBytes = kMoeWarps * kStages * kBytes;
   // integers are added in place; fp64 numbers by two shares at a time, each pair's first to one half, second to the other
   static constexpr int kSums = kFrags * kHalves * kN * 4 * 32;
-  static constexpr int kSumParts = SC ? 2 : 1;
-  static constexpr int kSmemBytes = kRingBytes + kSums * kSumParts * static_cast<int>(sizeof(Sum));
+  static constexpr int kSumParts = SC ? 2 : 1, kSumBytes = kSums * kSumParts * static_cast<int>(sizeof(Sum));
+  // blocks an SM, by registers, and a ring that fills their part of its shared memory
+  static constexpr int kResident = SC || kN == 4 || (!NN && kN == 2) ? 2 : 3;
+  static constexpr int kFit = ((kResident == 3 ? 74 : 110) * 1024 - kSumBytes) / kMoeWarps / kBytes;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  static_assert(kStages >= 3, "two steps have to be on their way while one is worked on");
+  static constexpr int kRingBytes = kMoeWarps * kStages * kBytes;
+  static constexpr int kSmemBytes = kRingBytes + kSumBytes;
 };
 
 // int32 -> fp64 without a conversion instruction (16 a clock and SM; the subtraction runs at 64): 2^52 + 2^31 + v, bit
@@ -614,11 +618,11 @@ struct MoeSource {
 // of a unit it starts the copies of its weights of the next one, before the sums are finished.
 // kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
 template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
-__global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_product_kernel(const MoeParams p) {
+__global__ void __launch_bounds__(kMoeThreads, MoeStage<DT, NN, SC, WORDS, kMaxN>::kResident) moe_product_kernel(const MoeParams p) {
   using Stage = MoeStage<DT, NN, SC, WORDS, kMaxN>;
   using Sum = typename Stage::Sum;
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
-  constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kStepBits = kStepK == 64 ? 6 : 5, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
+  constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kStepBits = kStepK == 128 ? 7 : kStepK == 64 ? 6 : 5, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr bool kChoose = kMaxN == 1;
   constexpr int kHead = kChoose ? kMoeFewPairs : 64;  // slots whose records are at hand
@@ -652,7 +656,7 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
     head[threadIdx.x] = __ldcg(records + threadIdx.x);
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int half = NN ? warp & 1 : 0, share = NN ? warp >> 1 : warp;
+  const int half = warp & 1, share = warp >> 1;
   const int k = kDown ? p.inner : p.hidden, columns = kDown ? p.hidden : 2 * p.inner, gate = p.inner;  // gate columns start there
   const int out_n = kDown ? p.hidden : p.inner, ranges = kDown ? p.down_ranges : p.up_ranges, splits = kDown ? p.down_splits : 1;
   const int groups = SC ? (k + p.sub - 1) / p.sub : 1, steps = (k + kStepK - 1) / kStepK;
@@ -668,8 +672,8 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   const int in_use = head[0].x, units = head[0].y * splits * ranges;
   int* counter = p.active + (kDown ? 3 : 2);
 
-  // A share's steps.  NN: consecutive ones (whole groups of K as far as it goes).  NT: a group's of every eighth group of
-  // K, or every eighth step, so that the eight read a row in one long piece.
+  // A share's steps.  NN: consecutive ones (whole groups of K as far as it goes).  NT: a group's of every fourth group of
+  // K, or every fourth step, so that the four read a row in one long piece.
   const int run_bits = SC && !NN ? p.sub_bits - kStepBits : 0;
   auto step_of = [&](const MoeUnit& unit, int i) {
     if (NN) return unit.begin + i;
@@ -717,7 +721,6 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
   };
   const long long w_step = static_cast<long long>(kStepBytes) * columns;                           // NN: to the next step
   const long long w_rows = NN ? 8LL * columns : 8 * code_pitch;                                    // to the next of a lane's loads
-  const long long w_frag = NN ? 0 : (kDown ? 32LL : static_cast<long long>(gate)) * code_pitch;    // NT: to its third fragment
   const uint8_t* all_weights = kDown ? p.w_down : p.w_up_gate;
   const bf16* all_weight_scales = kDown ? p.s_down : p.s_up_gate;
   auto source_of = [&](const MoeUnit& unit) {
@@ -734,11 +737,10 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
         source.scale = scales + (source.scale_valid ? column_of(unit.range, lane >> 3) + (lane & 7) * 2 : 0);
       }
     } else {
-      // sizes are multiples of 32: of up/gate every fragment is there, of the down product's last range maybe two
-      source.valid = column_valid(unit.range, 2);
-      source.scale_valid = column_valid(unit.range, lane >> 3);
+      // sizes are multiples of 32: both fragments are there, or none
+      source.valid = source.scale_valid = column_valid(unit.range, 0);
       source.w = matrix + (column_of(unit.range, 0) + g) * code_pitch + static_cast<long long>(unit.begin) * kStepBytes + q * 4 * WORDS;
-      source.scale = scales + (source.scale_valid ? column_of(unit.range, lane >> 3) + (lane & 7) * 2 : 0);
+      source.scale = scales + (source.scale_valid ? column_of(unit.range, (lane >> 3) & 1) + (lane & 7) * 2 : 0);
     }
     return source;
   };
@@ -763,14 +765,14 @@ __global__ void __launch_bounds__(kMoeThreads, kMaxN == 4 || SC ? 2 : 3) moe_pro
       const bool in_k = step * kStepK + q * (kStepK / 4) < k;
 #pragma unroll
       for (int l = 0; l < 2 * kFrags; ++l) {
-        const bool valid = in_k && (l < 4 || source.valid);  // columns g and g + 8 of fragment l / 2; the second two follow by w_frag
-        const uint8_t* src = source.w + (step - unit.begin) * kStepBytes + ((l & 1) ? w_rows : 0) + ((l & 2) ? 2 * w_rows : 0) + ((l & 4) ? w_frag : 0);
+        const bool valid = in_k && source.valid;  // columns g and g + 8 of fragment l / 2
+        const uint8_t* src = source.w + (step - unit.begin) * kStepBytes + ((l & 1) ? w_rows : 0) + ((l & 2) ? 2 * w_rows : 0);
         copy_async<4 * WORDS>(at + (l * 32 + lane) * 4 * WORDS, src, valid);
       }
     }
     if constexpr (SC) {
       const long long group = static_cast<long long>(group_of(step)) * columns;
-      copy_async<4>(at + Stage::kScalesAt + lane * 4, source.scale + group, source.scale_valid);
+      if (lane < kFrags * 8) copy_async<4>(at + Stage::kScalesAt + lane * 4, source.scale + group, source.scale_valid);
     }
   };
   // the pairs of a unit: read by its first threads, written down when the buffer is free

@@ -44,8 +44,7 @@ size_t lay_out(const b200_moe_problem& m, char* base, MoeParams* p) {
   p->down_ranges = (m.hidden + down_cols - 1) / down_cols;
   // The down product divides K between blocks where there are fewer (expert, column range) units than would keep the
   // blocks that the device holds (2 or 3 an SM) evenly busy, as long as each of a block's warps has four steps left.
-  const int step = m.dtype == B200_DTYPE_INT4 ? 64 : 32;
-  const int shares = m.layout == B200_LAYOUT_NN ? 4 : 8;
+  const int step = (m.dtype == B200_DTYPE_INT4 ? 64 : 32) * (m.layout == B200_LAYOUT_NN ? 1 : 2), shares = 4;
   p->down_splits = 1;
   while (p->down_splits < 8 && static_cast<long long>(p->slots) * p->down_ranges * p->down_splits < 1024 &&
          m.inner >= static_cast<long long>(step) * shares * p->down_splits * 2 * 4)

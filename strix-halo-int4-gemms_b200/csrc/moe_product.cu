@@ -1,7 +1,6 @@
 // The expert layer's kernels for one code type: compiled with B200_MOE_BITS 4 and 8.
 #include "moe_launch.h"
 
-#include <algorithm>
 #include <atomic>
 
 namespace b200 {
@@ -44,16 +43,11 @@ int launch_dependent(void (*kernel)(Args...), dim3 blocks, int threads, int smem
 template <bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
 int launch_product(const MoeParams& p, int sm_count, cudaStream_t stream) {
   using Stage = MoeStage<kBits, NN, SC, WORDS, kMaxN>;
-  // the most that any number of token groups up to kMaxN asks for
-  using One = MoeStage<kBits, NN, SC, WORDS, 1>;
-  using Two = MoeStage<kBits, NN, SC, WORDS, kMaxN < 2 ? kMaxN : 2>;
-  using Three = MoeStage<kBits, NN, SC, WORDS, kMaxN < 3 ? kMaxN : 3>;
-  constexpr int smem = std::max({Stage::kSmemBytes, One::kSmemBytes, Two::kSmemBytes, Three::kSmemBytes});
+  constexpr int smem = Stage::kSmemBytes;
   constexpr auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kDown>;
   if (int rc = allow_shared_memory<kernel>(smem); rc != 0) return rc;
   const long long units = static_cast<long long>(p.slots) * (kDown ? p.down_ranges * p.down_splits : p.up_ranges);
-  const int resident = smem <= 74 * 1024 && !SC && kMaxN != 4 ? 3 : smem <= 112 * 1024 ? 2 : 1;  // by shared memory and launch bounds
-  const long long blocks = units < static_cast<long long>(resident) * sm_count ? units : static_cast<long long>(resident) * sm_count;
+  const long long resident = static_cast<long long>(Stage::kResident) * sm_count, blocks = units < resident ? units : resident;
   return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), kMoeThreads, smem, stream, p);
 }
 
@@ -101,7 +95,7 @@ int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStr
     if (!p.sub) return launch_for_tokens<true, false, 2>(p, sm_count, stream);
     return two_words ? launch_for_tokens<true, true, 2>(p, sm_count, stream) : launch_for_tokens<true, true, kLeast>(p, sm_count, stream);
   }
-  if (!p.sub) return launch_for_tokens<false, false, 2>(p, sm_count, stream);
+  if (!p.sub || p.sub >= 4 * kWord) return p.sub ? launch_for_tokens<false, true, 4>(p, sm_count, stream) : launch_for_tokens<false, false, 4>(p, sm_count, stream);
   return two_words ? launch_for_tokens<false, true, 2>(p, sm_count, stream) : launch_for_tokens<false, true, kLeast>(p, sm_count, stream);
 }
 
