@@ -64,7 +64,7 @@ struct MoeParams {
   int slots, up_ranges, down_ranges, down_splits;
 };
 
-// Up to eight tokens (the products' kMaxN == 1) the time is that of the kernels' starts: every block of the up/gate product
+// Up to eight tokens (the products' kChoose) the time is that of the kernels' starts: every block of the up/gate product
 // (and then of the down product) picks the experts by itself.
 constexpr int kMoeFewTokens = 8;
 constexpr int kMoeFewExperts = 256;
@@ -459,7 +459,7 @@ struct MoeStage {
   static constexpr int kSums = kFrags * kHalves * kN * 4 * 32;
   static constexpr int kSumParts = SC ? 2 : 1, kSumBytes = kSums * kSumParts * static_cast<int>(sizeof(Sum));
   // blocks an SM, by registers, and a ring that fills their part of its shared memory
-  static constexpr int kResident = SC || kN == 4 || (!NN && kN == 2) ? 2 : 3;
+  static constexpr int kResident = SC || kN >= 3 || (!NN && kN == 2) ? 2 : 3;
   static constexpr int kFit = ((kResident == 3 ? 74 : 110) * 1024 - kSumBytes) / kMoeWarps / kBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static_assert(kStages >= 3, "two steps have to be on their way while one is worked on");
@@ -617,14 +617,14 @@ struct MoeSource {
 // first two by its number, the others by a counter, two units ahead of their use.  When a warp has done the last step
 // of a unit it starts the copies of its weights of the next one, before the sums are finished.
 // kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
-template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
+// kChoose: the blocks pick the experts themselves.
+template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kChoose, bool kDown>
 __global__ void __launch_bounds__(kMoeThreads, MoeStage<DT, NN, SC, WORDS, kMaxN>::kResident) moe_product_kernel(const MoeParams p) {
   using Stage = MoeStage<DT, NN, SC, WORDS, kMaxN>;
   using Sum = typename Stage::Sum;
   constexpr int kFrags = Stage::kFrags, kStages = Stage::kStages, kAllFrags = kFrags * Stage::kHalves, kShares = Stage::kShares;
   constexpr int kStepBytes = Stage::kStepBytes, kStepK = Stage::kStepK, kStepBits = kStepK == 128 ? 7 : kStepK == 64 ? 6 : 5, kCols = Stage::kCols, out_cols = kDown ? kCols : kCols / 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr bool kChoose = kMaxN == 1;
   constexpr int kHead = kChoose ? kMoeFewPairs : 64;  // slots whose records are at hand
   __shared__ int4 head[1 + kHead];
   __shared__ __align__(4) uint8_t list[kChoose ? kMoeFewPairs * 8 : 4];

@@ -40,34 +40,51 @@ int launch_dependent(void (*kernel)(Args...), dim3 blocks, int threads, int smem
   return err == cudaSuccess ? 0 : host_fail_cuda("moe_swiglu launch", err);
 }
 
-template <bool NN, bool SC, int WORDS, int kMaxN, bool kDown>
+template <bool NN, bool SC, int WORDS, int kMaxN, bool kChoose, bool kDown>
 int launch_product(const MoeParams& p, int sm_count, cudaStream_t stream) {
   using Stage = MoeStage<kBits, NN, SC, WORDS, kMaxN>;
   constexpr int smem = Stage::kSmemBytes;
-  constexpr auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kDown>;
+  constexpr auto kernel = moe_product_kernel<kBits, NN, SC, WORDS, kMaxN, kChoose, kDown>;
   if (int rc = allow_shared_memory<kernel>(smem); rc != 0) return rc;
   const long long units = static_cast<long long>(p.slots) * (kDown ? p.down_ranges * p.down_splits : p.up_ranges);
   const long long resident = static_cast<long long>(Stage::kResident) * sm_count, blocks = units < resident ? units : resident;
   return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), kMoeThreads, smem, stream, p);
 }
 
-// An expert can have at most as many rows as there are tokens (times the same expert given twice to a token, which
-// only takes more passes): the fewer rows a pass has to be ready for, the more registers are left for other blocks.
+// Rows of an expert that a pass over its weights can serve.  The fewer it has to be ready for, the more registers and
+// shared memory are left for copies in flight, but a second pass reads the weights again.  As many as the average and
+// two of its square roots: with tokens that choose at random, one expert in some 40 has more.  (64 tokens, two of 8
+// experts of 4096 x 14336: 171 us with 24, 179 with 32.  13 tokens, 6 of 64 experts, K-group scales: 68 us with 8, 75 with 16.)
+int rows_of_a_pass(const MoeParams& p) {
+  const int pairs = p.tokens * p.top_k, most = p.sub ? 16 : 32;  // K-group scales: 24 rows of fp64 sums do not fit the registers
+  int rows = 8;
+  const int mean[] = {4, 9, 16};  // + 2 sqrt: 8, 15, 24
+  for (const int m : mean)
+    if (rows < most && rows < p.tokens && pairs > m * p.experts) rows += 8;
+  return rows;
+}
+
 template <bool NN, bool SC, int WORDS>
-int launch_for_tokens(const MoeParams& p, int sm_count, cudaStream_t stream) {
-  auto products = [&](auto max_n) -> int {
+int launch_for_tokens(const MoeParams& p, bool few, int sm_count, cudaStream_t stream) {
+  auto products = [&](auto max_n, auto choose) -> int {
     constexpr int kMaxN = decltype(max_n)::value;
-    if (int rc = launch_product<NN, SC, WORDS, kMaxN, false>(p, sm_count, stream); rc != 0) return rc;
+    constexpr bool kChoose = decltype(choose)::value;
+    if (int rc = launch_product<NN, SC, WORDS, kMaxN, kChoose, false>(p, sm_count, stream); rc != 0) return rc;
     constexpr int kRow = kMoeQuantThreads * 2;
     auto quantize = SC || p.inner <= 4 * kRow ? moe_quantize_kernel<kBits, 4> : p.inner <= 14 * kRow ? moe_quantize_kernel<kBits, 14> : moe_quantize_kernel<kBits, 0>;
     if (int rc = launch_dependent(quantize, dim3(p.tokens * p.top_k), kMoeQuantThreads, 0, stream, p); rc != 0) return rc;
-    if (int rc = launch_product<NN, SC, WORDS, kMaxN, true>(p, sm_count, stream); rc != 0) return rc;
+    if (int rc = launch_product<NN, SC, WORDS, kMaxN, kChoose, true>(p, sm_count, stream); rc != 0) return rc;
     const int lines = p.top_k < kCombineLines ? p.top_k : kCombineLines;
     return launch_dependent(moe_combine_kernel<SC>, dim3((p.hidden + 63) / 64, p.tokens), 32 * lines, 0, stream, p);
   };
-  if (p.rows_a_pass == 8) return products(std::integral_constant<int, 1>());
-  if (p.rows_a_pass == 16) return products(std::integral_constant<int, 2>());
-  return products(std::integral_constant<int, SC ? 2 : 4>());
+  using std::integral_constant;
+  if (few) return products(integral_constant<int, 1>(), std::true_type());
+  if (p.rows_a_pass == 8) return products(integral_constant<int, 1>(), std::false_type());
+  if constexpr (!SC) {
+    if (p.rows_a_pass == 32) return products(integral_constant<int, 4>(), std::false_type());
+    if (p.rows_a_pass == 24) return products(integral_constant<int, 3>(), std::false_type());
+  }
+  return products(integral_constant<int, 2>(), std::false_type());
 }
 
 }  // namespace
@@ -79,7 +96,7 @@ int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStr
 #endif
   MoeParams p = params;
   const bool few = p.tokens <= kMoeFewTokens && p.experts <= kMoeFewExperts;
-  p.rows_a_pass = few ? 8 : p.tokens <= 16 || p.sub ? 16 : 32;
+  p.rows_a_pass = rows_of_a_pass(p);
   const int logit_blocks = p.router != nullptr ? (p.experts + 3) / 4 * ((p.tokens + 3) / 4) : 0;
   moe_route_kernel<kBits><<<p.tokens + logit_blocks, 256, 0, stream>>>(p);
   if (const cudaError_t err = cudaGetLastError(); err != cudaSuccess) return host_fail_cuda("moe_swiglu launch", err);
@@ -92,11 +109,11 @@ int launch_moe_int8(const MoeParams& params, bool n_major, int sm_count, cudaStr
   constexpr int kWord = kBits == 4 ? 32 : 16, kLeast = kBits == 4 ? 1 : 2;
   const bool two_words = !p.sub || p.sub >= 2 * kWord;
   if (n_major) {
-    if (!p.sub) return launch_for_tokens<true, false, 2>(p, sm_count, stream);
-    return two_words ? launch_for_tokens<true, true, 2>(p, sm_count, stream) : launch_for_tokens<true, true, kLeast>(p, sm_count, stream);
+    if (!p.sub) return launch_for_tokens<true, false, 2>(p, few, sm_count, stream);
+    return two_words ? launch_for_tokens<true, true, 2>(p, few, sm_count, stream) : launch_for_tokens<true, true, kLeast>(p, few, sm_count, stream);
   }
-  if (!p.sub || p.sub >= 4 * kWord) return p.sub ? launch_for_tokens<false, true, 4>(p, sm_count, stream) : launch_for_tokens<false, false, 4>(p, sm_count, stream);
-  return two_words ? launch_for_tokens<false, true, 2>(p, sm_count, stream) : launch_for_tokens<false, true, kLeast>(p, sm_count, stream);
+  if (!p.sub || p.sub >= 4 * kWord) return p.sub ? launch_for_tokens<false, true, 4>(p, few, sm_count, stream) : launch_for_tokens<false, false, 4>(p, few, sm_count, stream);
+  return two_words ? launch_for_tokens<false, true, 2>(p, few, sm_count, stream) : launch_for_tokens<false, true, kLeast>(p, few, sm_count, stream);
 }
 
 }  // namespace b200
