@@ -779,13 +779,13 @@ def unpack_int4_on_device(packed: Any, *, library_path: str | Path | None = None
     if not getattr(packed, "is_cuda", False):
         raise RuntimeError("native kernels require CUDA tensors")
     packed = _require_contiguous("packed", packed)
-    rows = int(packed.numel() // packed.shape[-1]) if packed.numel() else 0
-    out = torch.empty((*packed.shape[:-1], packed.shape[-1] * 2), device=packed.device, dtype=torch.int8)
+    shape = packed.shape
+    row_bytes = shape[-1]
+    rows = packed.numel() // row_bytes if row_bytes else 0
+    out = packed.new_empty((*shape[:-1], row_bytes * 2), dtype=torch.int8)
     library = load_dispatch_library(library_path)
     rc = library.b200_int4_gemms_unpack_int4(
-        _device_index(packed), _stream_handle(torch, packed, stream),
-        ctypes.c_void_p(packed.data_ptr()), ctypes.c_void_p(out.data_ptr()), rows, int(packed.shape[-1]),
-    )
+        packed.get_device(), _stream_handle(torch, packed, stream), packed.data_ptr(), out.data_ptr(), rows, row_bytes)
     if rc != 0:
         raise RuntimeError(_library_last_error(library))
     return out
@@ -983,6 +983,11 @@ def layer_norm_quantize_on_device(x: Any, weight: Any, bias: Any | None, *, eps:
     return codes, scales
 
 
+@lru_cache(maxsize=256)
+def _layer_norm_bwd_workspace(library: Any, *fields: int) -> int:
+    return int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(*fields))
+
+
 def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any, *, library_path: str | Path | None = None,
                              stream: Any | None = None) -> tuple[Any, Any, Any]:
     """(dx, dweight, dbias) of checked CUDA operands; see :func:`norm.layer_norm_bwd`.
@@ -994,7 +999,7 @@ def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any,
     rows = x.numel() // cols
     library = load_dispatch_library(library_path)
     index, kind = x.get_device(), _type_code(torch, x)
-    need = library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(index, rows, cols, kind)
+    need = _layer_norm_bwd_workspace(library, index, rows, cols, kind)
     dx = torch.empty_like(x)
     sums = x.new_empty((2, cols), dtype=torch.float32)
     workspace = x.new_empty(need // 4, dtype=torch.float32)
