@@ -111,6 +111,56 @@ def test_given_routing(pkg, layout, ids_type):
     assert not none.any()
 
 
+@pytest.mark.parametrize("sub", [0, 64])
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("tokens,experts,top_k", [(12, 64, 2), (20, 4, 1), (40, 4, 1), (64, 2, 1), (64, 70, 3)])
+def test_more_rows_than_a_pass(pkg, tokens, experts, top_k, bits, layout, sub):
+    """Routings that are as uneven as can be: an expert has more rows than a pass over its weights is laid out for."""
+    c = _case(pkg, tokens=tokens, experts=experts, hidden=160, inner=96, bits=bits, layout=layout, sub=sub, seed=51)
+    g = torch.Generator().manual_seed(52)
+    ids = torch.randint(0, experts, (tokens, top_k), generator=g)
+    ids[:, 0] = 1
+    share = torch.rand(tokens, top_k, generator=g)
+    out = pkg.moe_swiglu(*c["device"], topk_ids=ids.cuda(), topk_weights=share.cuda(), **c["call"])
+    _check(c, out, ids, share)
+    none = pkg.moe_swiglu(*c["device"], topk_ids=torch.full_like(ids, experts).cuda(), topk_weights=share.cuda(), **c["call"])
+    assert not none.any()
+
+
+@pytest.mark.parametrize("layout,sub", [("nt", 0), ("nn", 0), ("nt", 32), ("nn", 128)])
+def test_an_expert_given_many_times_to_a_token(pkg, layout, sub):
+    c = _case(pkg, tokens=8, experts=20, hidden=96, inner=64, bits=4, layout=layout, sub=sub, seed=53)
+    g = torch.Generator().manual_seed(54)
+    for ids in (torch.full((8, 16), 3), torch.randint(2, 5, (8, 16), generator=g), torch.arange(128).view(8, 16) % 23 - 1):
+        share = torch.rand(8, 16, generator=g)
+        out = pkg.moe_swiglu(*c["device"], topk_ids=ids.int().cuda(), topk_weights=share.cuda(), **c["call"])
+        _check(c, out, torch.where(ids < 20, ids, -1), share)
+
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(8, 256, 16), (3, 257, 8), (9, 1024, 16), (64, 130, 5)])
+def test_many_experts(pkg, tokens, experts, top_k):
+    c = _case(pkg, tokens=tokens, experts=experts, hidden=64, inner=32, bits=4, layout="nn", sub=0, seed=55)
+    for renormalize in (True, False):
+        _routed(pkg, c, top_k, renormalize=renormalize)
+
+
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_that_the_quantiser_reads_twice(pkg, bits, layout):
+    c = _case(pkg, tokens=2, experts=2, hidden=64, inner=14368, bits=bits, layout=layout, sub=0, seed=56)
+    _routed(pkg, c, 2)
+
+
+@pytest.mark.parametrize("sub", [0, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_ends_of_k_inside_a_step(pkg, bits, layout, sub):
+    for tokens, hidden, inner in ((3, 416, 608), (11, 608, 1056), (1, 1056, 32), (18, 32, 2080)):
+        c = _case(pkg, tokens=tokens, experts=3, hidden=hidden, inner=inner, bits=bits, layout=layout, sub=sub, seed=hidden + sub)
+        _routed(pkg, c, 2)
+
+
 @pytest.mark.parametrize("layout", ["nt", "nn"])
 def test_special_tokens(pkg, layout):
     c = _case(pkg, tokens=6, experts=4, hidden=128, inner=64, bits=4, layout=layout, sub=0, seed=15)
@@ -191,9 +241,10 @@ def test_refusals_on_a_gpu(pkg):
         pkg.moe_swiglu(shifted, up, down, **ok)
 
 
-def test_streams_and_graphs(pkg):
+@pytest.mark.parametrize("tokens", [12, 3])
+def test_streams_and_graphs(pkg, tokens):
     """Two calls at once on two streams, and two graphs replayed at once on new inputs: each has its own scratch."""
-    c = _case(pkg, tokens=12, experts=16, hidden=512, inner=256, bits=4, layout="nn", sub=128, seed=21)
+    c = _case(pkg, tokens=tokens, experts=16, hidden=512, inner=256, bits=4, layout="nn", sub=128, seed=21)
     x, up, down = c["device"]
     kw = dict(router_weight=c["router"].cuda(), top_k=4, **c["call"])
     flipped = x.flip(0).contiguous()

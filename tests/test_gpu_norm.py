@@ -230,6 +230,38 @@ def test_layer_norm_quantize_special_rows(pkg, sub):
     assert not codes[2].any() and not codes[3].any() and torch.isnan(scales[2:4]).all() and torch.isfinite(scales[4:]).all()
 
 
+@pytest.mark.parametrize("sub", [0, 32])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_layer_norm_quantize_beyond_float32(pkg, bits, sub):
+    """Differences, products and scales that float32 has no room for, or too few digits: the exact values decide."""
+    g = torch.Generator().manual_seed(61)
+    x = torch.randn(6, 512, generator=g)
+    x[1] = torch.where(torch.rand(512, generator=g) < 0.05, 3.3e38, -3.3e38)    # x - mean is beyond float32
+    x[2] *= 1e-30
+    x[3] *= 1e25
+    x[4] = 1e30 + x[4] * 1e24
+    w = torch.randn(512, generator=g)
+    for weight, bias in ((w, None), (w, w.flip(0)), (w * 1e38, None), (w * 1e-38, None), (w * 1e-42, None), (w * 1e-20, w * 1e18)):
+        weight = torch.where(torch.isfinite(weight), weight, torch.ones(()))
+        for eps in (0.0, 1e-5):
+            _check_norm_codes(pkg, x, weight, bias, bits, sub, eps=eps)
+
+
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [512, 1032, 2040, 4096, 8184, 16384])
+def test_many_rows(pkg, cols, xt):
+    """Rows enough for the launch shapes with many values a thread."""
+    x = _rows(600, cols, xt, cols + 5)
+    w, b = _affine(cols, torch.bfloat16, cols + 6)
+    _check_norm(pkg, x, w, b, 1e-5, x.cuda())
+    _check_norm_codes(pkg, x, w, b, 4, 0)
+    if xt is torch.bfloat16:
+        for bits, sub in ((4, 0), (8, 64)):
+            codes, scales = pkg.quantize_tokens(x.cuda(), dtype=_dtype(pkg, bits), scale=_spec(pkg, sub))
+            want, want_scales, _ = row_oracle.quantize_rows(x, bits, sub)
+            assert torch.equal(scales.cpu().double(), want_scales) and torch.equal(_codes(pkg, codes, bits, cols), want)
+
+
 def test_layer_norm_quantize_shapes_and_alignment(pkg):
     x = _rows(6, 320, torch.bfloat16, 9)
     w, b = _affine(320, torch.bfloat16, 10)
