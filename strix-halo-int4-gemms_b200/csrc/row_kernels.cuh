@@ -5,7 +5,8 @@
 // registers, so that a row is read once.  V == 0 is the form for rows that no block can hold: the same code, reading
 // the row again (from L2) for every pass over it.  What is done once for a row (reductions, scales, addresses) costs some
 // 100 instructions a thread, as much as ten values: many values a thread (V = 8) where rows are many, few (V = 1) where
-// they are too few to fill the device (quantize_tokens of 32768 x 2048: 48 us with 16 values a thread, see below).
+// they are too few to fill the device (quantize_tokens of 32768 x 2048 to int4: 30 us, 5.6 TB/s, with 64 values a
+// thread; 48 us with 16).
 #pragma once
 
 #include <cstring>
@@ -422,6 +423,7 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
 // A block has several groups of TPR threads, each with rows of its own (and a barrier of its own); the sums of the groups
 // are added up in shared memory, each block leaves one row of partial sums, and column_sums_kernel adds those in a fixed
 // order: no atomics, the same bits on every run.  The next row is read while the present one is reduced.
+// 32768 x 2048 in bf16: 75 us, 5.4 TB/s, and 3 us for the partial sums, whose kernel starts while this one ends.
 // Rows of more than 8192 values are left to two kernels, below.
 // ---------------------------------------------------------------------------------------------------------------
 template <int TPR>
@@ -561,7 +563,8 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
 // Rows of more than 8192 values, whose columns do not fit the registers of one block: the means of g and g h of every
 // row, and then dx and the sums over rows with a thread for each chunk of columns, which needs no reduction over the
 // row.  x and dy are read twice, the second time from L2 as far as it holds them.  (517 rows of 14336 fp32 values: a
-// block of 1024 threads a row took 47 us, clusters of two blocks 37 us, both waiting for their reductions.)
+// block of 1024 threads a row took 47 us, clusters of two blocks 37 us, both waiting for their reductions; these take
+// 27 us, 12 to 13 of them for the means.)
 struct __align__(16) RowTerms {
   float mean, rstd, mean_g, mean_gh;
 };
