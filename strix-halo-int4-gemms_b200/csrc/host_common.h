@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -34,6 +35,21 @@ int guarded(Fn&& fn) noexcept {
   } catch (...) {  // std::bad_alloc of a message at most
     return 1;
   }
+}
+
+// Allows a kernel its dynamic shared memory (with the static part it may pass the 48 KB that need no permission), once
+// for each device: the attribute stays with the device's context.
+template <auto Kernel>
+int allow_shared_memory(int smem_bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (const cudaError_t err = cudaGetDevice(&device); err != cudaSuccess) return host_fail_cuda("cudaGetDevice", err);
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return 0;
+  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+  if (err != cudaSuccess) return host_fail_cuda("cudaFuncSetAttribute(max dynamic shared memory)", err);
+  done.fetch_or(bit, std::memory_order_release);
+  return 0;
 }
 
 inline bool is_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -1,27 +1,10 @@
 // The expert layer's kernels for one code type: compiled with B200_MOE_BITS 4 and 8.
 #include "moe_launch.h"
 
-#include <atomic>
-
 namespace b200 {
 namespace {
 
 constexpr int kBits = B200_MOE_BITS;
-
-// Allows a kernel its dynamic shared memory (with the static part it may pass the 48 KB that need no permission), once
-// for each device: the attribute stays with the device's context.
-template <auto Kernel>
-int allow_shared_memory(int smem_bytes) {
-  static std::atomic<uint64_t> done{0};
-  int device = 0;
-  if (const cudaError_t err = cudaGetDevice(&device); err != cudaSuccess) return host_fail_cuda("cudaGetDevice", err);
-  const uint64_t bit = uint64_t{1} << (device & 63);
-  if (done.load(std::memory_order_acquire) & bit) return 0;
-  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
-  if (err != cudaSuccess) return host_fail_cuda("cudaFuncSetAttribute(max dynamic shared memory)", err);
-  done.fetch_or(bit, std::memory_order_release);
-  return 0;
-}
 
 // A launch that may start while the kernel before it on the stream still runs (it waits for it by itself).
 template <typename... Args>

@@ -36,6 +36,11 @@ struct Raw8<bf16> {
       w[i / 2 + 1] = v.y;
     }
   }
+  // eight values in 16 bytes
+  __device__ __forceinline__ void from_chunks(const uint4* at, int) {
+    const uint4 v = *at;
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
   __device__ __forceinline__ void set(const bf16 (&e)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -72,6 +77,14 @@ struct Raw8<float> {
     for (int k = 0; k < G; k += 4) {
       const float4 v = valid ? __ldg(reinterpret_cast<const float4*>(p + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
       f[i + k] = v.x; f[i + k + 1] = v.y; f[i + k + 2] = v.z; f[i + k + 3] = v.w;
+    }
+  }
+  // two times four values, the second `step` chunks behind the first
+  __device__ __forceinline__ void from_chunks(const uint4* at, int step) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(at + k * step);
+      f[4 * k] = v.x; f[4 * k + 1] = v.y; f[4 * k + 2] = v.z; f[4 * k + 3] = v.w;
     }
   }
   __device__ __forceinline__ void set(const float (&e)[8]) {

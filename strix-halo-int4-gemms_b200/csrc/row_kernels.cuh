@@ -422,15 +422,26 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
 // A thread keeps its columns for all of its rows, so the sums over rows stay in registers and x and dy are read once.
 // A block has several groups of TPR threads, each with rows of its own (and a barrier of its own); the sums of the groups
 // are added up in shared memory, each block leaves one row of partial sums, and column_sums_kernel adds those in a fixed
-// order: no atomics, the same bits on every run.  The next row is read while the present one is reduced.
-// 32768 x 2048 in bf16: 75 us, 5.4 TB/s, and 3 us for the partial sums, whose kernel starts while this one ends.
+// order: no atomics, the same bits on every run.  Four rows of a group are on their way (in shared memory: one, in
+// registers, was what bounded the kernel, with 32 KB an SM in flight; two in registers spill).
+// 32768 x 2048 in bf16: 66 us, 6.1 TB/s (75 us with one row ahead), and 3 us for the partial sums, whose kernel starts
+// while this one ends.
 // Rows of more than 8192 values are left to two kernels, below.
 // ---------------------------------------------------------------------------------------------------------------
 template <int TPR>
 struct BwdShape {
   static constexpr int kThreads = TPR < 512 ? 512 : TPR;
   static constexpr int kGroups = kThreads / TPR;  // rows at once
+  // A thread's 64 bytes of x and dy of the rows to come lie in shared memory, copied there asynchronously by the thread
+  // itself: rows of a group on their way, 96 KB in all where a row has its 16 values a thread.
+  static constexpr int kAhead = kThreads == 512 ? 4 : 3;
+  static constexpr int kRingBytes = kAhead * kThreads * 64;
 };
+
+__device__ __forceinline__ void copy_16(void* shared, const void* global, bool valid) {
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(shared));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(global), "r"(valid ? 16 : 0) : "memory");
+}
 
 // Barrier of one group of a block.
 template <int TPR>
@@ -445,57 +456,100 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
                       float* __restrict__ partial, long long rows, long long cols) {
   constexpr int kWarps = TPR / 32, kGroups = BwdShape<TPR>::kGroups;
   __shared__ float2 scratch[2][kGroups][kWarps];
-  extern __shared__ float across[];  // [TPR * V * 8], where there are groups to be added up
+  // the ring of rows to come [kAhead][4][kThreads]; behind the last row [TPR * V * 8] sums, where there are groups to be added up
+  extern __shared__ __align__(16) uint8_t bwd_smem[];
+  float* across = reinterpret_cast<float*>(bwd_smem);
+  uint4* ring = reinterpret_cast<uint4*>(bwd_smem) + threadIdx.x;
   const int group = threadIdx.x / TPR, thread = threadIdx.x % TPR;
   const long long step = static_cast<long long>(gridDim.x) * kGroups;
   constexpr int G = kAligned ? 16 / sizeof(T) : 1;
   const Columns<TPR, G> column{thread, cols};
   const float inv_cols = 1.f / static_cast<float>(cols);
   Raw8<W> w[V];
-  float dw[V][8], db[V][8];
+  Pair dw[V][4], db[V][4];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     w[v] = column.load(weight, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[v][i] = db[v][i] = 0.f;
+    for (int i = 0; i < 4; ++i) dw[v][i] = db[v][i] = Pair(0.f);
   }
-  Raw8<T> next_x[V], next_dy[V];
+  constexpr int kThreads = BwdShape<TPR>::kThreads, kAhead = BwdShape<TPR>::kAhead;
   float next_mean = 0.f, next_rstd = 0.f;
-  auto fetch = [&](long long row) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      next_x[v] = column.load(src + row * cols, v);
-      next_dy[v] = column.load(dy + row * cols, v);
-    }
+  auto read_terms = [&](long long row) {
     next_mean = __ldg(mean_in + row);
     next_rstd = __ldg(rstd_in + row);
   };
-  long long r = static_cast<long long>(blockIdx.x) * kGroups + group;
-  if (r < rows) fetch(r);
-  int turn = 0;
-  for (; r < rows; r += step, turn ^= 1) {
-    Raw8<T> x[V], d[V];
+  Raw8<T> next_x[kAligned ? 1 : V], next_dy[kAligned ? 1 : V];  // where rows cannot be copied 16 bytes at a time: one row in registers
+  auto fetch = [&](long long row, int slot) {
+    if constexpr (kAligned) {
+      if (row < rows) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      x[v] = next_x[v];
-      d[v] = next_dy[v];
-    }
-    const float mean = next_mean, rstd = next_rstd;
-    if (r + step < rows) fetch(r + step);
-    float sg = 0.f, sgh = 0.f;
+        for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+          for (int i = 0; i < 8; i += G) {
+            const int chunk = v * (8 / G) + i / G;
+            const bool has = column.has(v, i);
+            const long long at = row * cols + (has ? column.at(v, i) : 0);
+            copy_16(ring + (slot * 4 + chunk) * kThreads, src + at, has);
+            copy_16(ring + (slot * 4 + 2 + chunk) * kThreads, dy + at, has);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    } else if (row < rows) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = d[v].get(i), h = (x[v].get(i) - mean) * rstd, g = e * w[v].get(i);
-        sg += g;
-        sgh = __fmaf_rn(g, h, sgh);
-        dw[v][i] = __fmaf_rn(e, h, dw[v][i]);
-        db[v][i] += e;
+      for (int v = 0; v < V; ++v) {
+        next_x[v] = column.load(src + row * cols, v);
+        next_dy[v] = column.load(dy + row * cols, v);
       }
     }
+  };
+  static_assert(V * 8 / G <= 2 || !kAligned, "two chunks of x and two of dy a thread");
+  long long r = static_cast<long long>(blockIdx.x) * kGroups + group;
+  if (r < rows) read_terms(r);
+#pragma unroll
+  for (int i = 0; i < (kAligned ? kAhead : 1); ++i) fetch(r + i * step, i);
+  int turn = 0, slot = 0;
+  for (; r < rows; r += step, turn ^= 1) {
+    Raw8<T> x[V], d[V];
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < rows) read_terms(r + step);
+    if constexpr (kAligned) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        x[v].from_chunks(ring + (slot * 4 + v) * kThreads, kThreads);
+        d[v].from_chunks(ring + (slot * 4 + 2 + v) * kThreads, kThreads);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        x[v] = next_x[v];
+        d[v] = next_dy[v];
+      }
+      fetch(r + step, 0);
+    }
+    auto two = [](const auto& raw, int i) { return Pair(raw.get(2 * i), raw.get(2 * i + 1)); };
+    const Pair minus_mean(-mean), scale(rstd);
+    Pair sums(0.f), sums_h(0.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const Pair e = two(d[v], i), h = mul2(add2(two(x[v], i), minus_mean), scale), g = mul2(e, two(w[v], i));
+        sums = add2(sums, g);
+        sums_h = fma2(g, h, sums_h);
+        dw[v][i] = fma2(e, h, dw[v][i]);
+        db[v][i] = add2(db[v][i], e);
+      }
+    }
+    float sg = sums.get().x + sums.get().y, sgh = sums_h.get().x + sums_h.get().y;
     sg = warp_reduce(sg, SumOp());
     sgh = warp_reduce(sgh, SumOp());
+    if constexpr (kAligned) {  // the row has been read: its place is free
+      __syncwarp();
+      fetch(r + kAhead * step, slot);
+      if (++slot == kAhead) slot = 0;
+    }
     if (TPR > 32) {
       if ((thread & 31) == 0) scratch[turn][group][thread >> 5] = make_float2(sg, sgh);
       group_barrier<TPR>(group);
@@ -508,19 +562,30 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
         sgh += __shfl_xor_sync(0xFFFFFFFFu, sgh, o);
       }
     }
-    const float mg = sg * inv_cols, mgh = sgh * inv_cols;
+    const Pair minus_mg(-sg * inv_cols), minus_mgh(-sgh * inv_cols);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float out[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float h = (x[v].get(i) - mean) * rstd;
-        out[i] = rstd * (d[v].get(i) * w[v].get(i) - mg - h * mgh);
+      for (int i = 0; i < 4; ++i) {
+        const Pair h = mul2(add2(two(x[v], i), minus_mean), scale);
+        const float2 f = mul2(fma2(h, minus_mgh, fma2(two(d[v], i), two(w[v], i), minus_mg)), scale).get();
+        out[2 * i] = f.x;
+        out[2 * i + 1] = f.y;
       }
       column.store(dx + r * cols, v, out);
     }
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // column_sums_kernel, which waits for this one's end
+  float dw1[V][8], db1[V][8];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 fw = dw[v][i / 2].get(), fb = db[v][i / 2].get();
+      dw1[v][i] = i % 2 ? fw.y : fw.x;
+      db1[v][i] = i % 2 ? fb.y : fb.x;
+    }
   float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * cols;
   if (kGroups == 1) {
 #pragma unroll
@@ -528,8 +593,8 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (column.has(v, i)) {
-          mine[column.at(v, i)] = dw[v][i];
-          mine[cols + column.at(v, i)] = db[v][i];
+          mine[column.at(v, i)] = dw1[v][i];
+          mine[cols + column.at(v, i)] = db1[v][i];
         }
     return;
   }
@@ -544,7 +609,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float* at = across + (v * 8 + i) * TPR + thread;
-            const float sum = half ? db[v][i] : dw[v][i];
+            const float sum = half ? db1[v][i] : dw1[v][i];
             *at = k == 0 ? sum : *at + sum;
           }
       }

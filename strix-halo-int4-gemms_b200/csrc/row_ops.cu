@@ -251,8 +251,10 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
           using std::integral_constant;
           auto rows_of = [&](auto tpr) {
             constexpr int TPR = decltype(tpr)::value, kThreads = BwdShape<TPR>::kThreads;
-            constexpr int smem = BwdShape<TPR>::kGroups > 1 ? TPR * V * 8 * 4 : 0;
-            layer_norm_bwd_kernel<T, W, TPR, V, A><<<static_cast<unsigned>(partials), kThreads, smem, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, rows, cols);
+            constexpr int sums = BwdShape<TPR>::kGroups > 1 ? TPR * V * 8 * 4 : 0, smem = A ? std::max(sums, BwdShape<TPR>::kRingBytes) : sums;
+            constexpr auto kernel = layer_norm_bwd_kernel<T, W, TPR, V, A>;
+            if (rc = allow_shared_memory<kernel>(smem); rc != 0) return;
+            kernel<<<static_cast<unsigned>(partials), kThreads, smem, stream>>>(dy_t, x_t, w_t, mean, rstd, dx_t, partial, rows, cols);
             rc = launched("layer_norm_bwd launch");
           };
           const int threads = bwd_threads(cols, x_type);

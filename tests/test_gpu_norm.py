@@ -309,6 +309,14 @@ def test_layer_norm_bwd(pkg, cols, xt, wt):
         _check_bwd(pkg, x, dy, _affine(cols, wt, cols + 2)[0])
 
 
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(20001, 64), (20001, 250), (11000, 512), (5003, 1000), (3001, 2048), (1501, 4096), (901, 8192)])
+def test_layer_norm_bwd_rows_that_wait_their_turn(pkg, rows, cols, xt):
+    """Many more rows than are on their way at once."""
+    x, dy = _rows(rows, cols, xt, cols + 7), _rows(rows, cols, xt, cols + 8)
+    _check_bwd(pkg, x, dy, _affine(cols, torch.bfloat16, cols + 9)[0])
+
+
 def test_layer_norm_bwd_many_rows_and_shapes(pkg):
     for rows, cols in ((20011, 48), (5000, 320), (3001, 1000)):
         x = _rows(rows, cols, torch.bfloat16, rows)
