@@ -8,7 +8,7 @@
 //   moe_combine_kernel   softmax; the experts' shares of every token added up
 // Each kernel is launched while the one before it still runs (programmatic dependent launch) and waits for it where
 // it needs its results; the down product's first weights are on their way before the up/gate product has ended.
-// One token, 8 of 64 experts of 2048 x 1408 in int4: 19.5 us on the device, 2 for the router, 3 until the first weights are
+// One token, 8 of 64 experts of 2048 x 1408 in int4: 18.5 us on the device, 2 for the router, 3 until the first weights are
 // on their way, 7 and 3 for the products, 1.5 for the codes, 1 for the shares, the rest between them.  The last block of an expert (of a column
 // range) to finish can make the codes (add up the shares) without a launch; that was slower (26 us), since the
 // counting costs each unit 1 us and what the last block does is not shared.
