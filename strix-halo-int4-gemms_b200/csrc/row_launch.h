@@ -69,7 +69,7 @@ struct NormQuantizeCall {
   void *codes, *scales;
   long long rows, cols;
   bool weight_f32, wide;
-  int bits, subchannel, sm_count;
+  int bits, subchannel;
   double eps;
   cudaStream_t stream;
 };

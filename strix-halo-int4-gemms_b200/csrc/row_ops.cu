@@ -178,7 +178,6 @@ extern "C" int b200_int4_gemms_layer_norm_quantize(int device_index, uintptr_t s
     call.wide = cols % 8 == 0 && is_aligned(x, 16) && is_aligned(codes, 8) && is_aligned(weight, 16) && is_aligned(bias, 16);
     call.bits = bits;
     call.subchannel = subchannel;
-    call.sm_count = sms;
     call.eps = eps;
     call.stream = reinterpret_cast<cudaStream_t>(stream_handle);
     return x_type == B200_OUT_F32 ? launch_norm_quantize_f32(call) : launch_norm_quantize_bf16(call);
