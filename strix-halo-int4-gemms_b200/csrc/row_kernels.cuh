@@ -629,7 +629,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
 // row, and then dx and the sums over rows with a thread for each chunk of columns, which needs no reduction over the
 // row.  x and dy are read twice, the second time from L2 as far as it holds them.  (517 rows of 14336 fp32 values: a
 // block of 1024 threads a row took 47 us, clusters of two blocks 37 us, both waiting for their reductions; these take
-// 27 us, 12 to 13 of them for the means.)
+// 26 us, 12 to 13 of them for the means.)
 struct __align__(16) RowTerms {
   float mean, rstd, mean_g, mean_gh;
 };
