@@ -6,6 +6,9 @@ namespace {
 
 using namespace b200;
 
+static_assert(kMoeMaxTokens == B200_MOE_MAX_TOKENS && kMoeMaxTopK == B200_MOE_MAX_TOP_K && kMoeMaxExperts == B200_MOE_MAX_EXPERTS,
+              "the header states the kernels' limits");
+
 int check_problem(const b200_moe_problem* m) {
   if (m == nullptr) return host_fail("problem must be non-null");
   if (m->dtype != B200_DTYPE_INT4 && m->dtype != B200_DTYPE_INT8) return host_fail("problem.dtype is not INT4 or INT8");
