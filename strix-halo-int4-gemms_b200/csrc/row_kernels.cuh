@@ -115,8 +115,11 @@ quantize_tokens_kernel(const bf16* __restrict__ src, uint8_t* __restrict__ codes
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// layer norm: y = (x - mean) rstd w + b; mean, then the mean square of the differences, both from registers, in fp32.
-// The values are kept as fp32, and as their differences from the mean: bf16 is taken apart once, not in each pass.
+// layer norm: y = (x - mean) rstd w + b, from registers, in fp32.  The first mean m is the row's first value x0 plus the
+// average of x - x0; then d = x - m is summed up beside its square: e = mean(d), what m is off by, corrects the mean, the
+// variance (mean(d^2) - e^2) and every value (d - e).  So the error is the spread's and not the offset's: a row of equal
+// values has exactly that mean, no variance and its bias as its norm, and the rounding of a large mean shifts no row.
+// The values are kept as fp32, and as d: bf16 is taken apart once, not in each pass; pairs of fp32 numbers.
 // 32 values a thread, so that the registers allow 1,024 threads an SM (fp32 holds its words twice for a while: 768).
 // 32768 x 2048 in bf16: 46 us, 5.9 TB/s, where a copy of the same bytes takes 44; 55 us with 64 values a thread and half
 // of the threads, 54 with 16 (the work done once for a row), 56 with resident blocks that read the next row ahead.
@@ -125,61 +128,75 @@ template <typename T, typename W, int TPR, int V, bool kAligned>
 __global__ void __launch_bounds__(RowPlace<TPR>::kThreads, (sizeof(T) == 2 ? 1024 : 768) / RowPlace<TPR>::kThreads)
 layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias, T* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, long long cols, float eps) {
-  __shared__ float scratch[2][TPR / 32];
+  __shared__ float scratch[3 * (TPR / 32)];
   const float inv_cols = 1.f / static_cast<float>(cols);
   constexpr int G = kAligned ? 16 / sizeof(T) : 1;
   const Columns<TPR, G> column{RowPlace<TPR>::thread(), cols};
   const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   constexpr int kHeld = V > 0 ? V : 1;
+  // values behind the row are zero in `f`; this leaves them out of a sum
+  auto kept = [&](Pair f, int v, int i) {
+    if (G > 1) return f;  // whole chunks are left out where they are added up
+    const float2 e = f.get();
+    return Pair(column.has(v, 2 * i) ? e.x : 0.f, column.has(v, 2 * i + 1) ? e.y : 0.f);
+  };
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
     const T* row = src + r * cols;
-    float held[kHeld][8];
-    auto read = [&](int v, float (&f)[8]) {
-      const Raw8<T> raw = column.load(row, v);
+    const float x0 = to_f32(row[0]);
+    Pair held[kHeld][4];
+    auto take = [&](const Raw8<T>& raw, Pair (&f)[4]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = raw.get(i);
+      for (int i = 0; i < 4; ++i) f[i] = Pair(raw.get(2 * i), raw.get(2 * i + 1));
     };
     if (V > 0) {
       Raw8<T> raw[kHeld];
 #pragma unroll
       for (int v = 0; v < kHeld; ++v) raw[v] = column.load(row, v);
 #pragma unroll
-      for (int v = 0; v < kHeld; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) held[v][i] = raw[v].get(i);
+      for (int v = 0; v < kHeld; ++v) take(raw[v], held[v]);
     }
-    float sum = 0.f;
+    const Pair minus_x0(-x0);
+    Pair sum(0.f);
 #pragma unroll
     for (int v = 0; v < count; ++v) {
-      float(&x)[8] = held[V > 0 ? v : 0];
-      if (V == 0) read(v, x);
+      Pair(&x)[4] = held[V > 0 ? v : 0];
+      if (V == 0) take(column.load(row, v), x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[i];
+      for (int i = 0; i < 4; ++i)
+        if (G == 1 || column.has(v, 2 * i)) sum = add2(sum, kept(add2(x[i], minus_x0), v, i));
     }
-    const float mean = row_reduce<TPR>(sum, SumOp(), scratch[0]) * inv_cols;
-    float square = 0.f;
+    const float first = x0 + row_reduce<TPR>(sum.get().x + sum.get().y, SumOp(), scratch) * inv_cols;
+    const Pair minus_first(-first);
+    Pair off(0.f), square(0.f);
 #pragma unroll
     for (int v = 0; v < count; ++v) {
-      float(&x)[8] = held[V > 0 ? v : 0];
-      if (V == 0) read(v, x);
+      Pair(&x)[4] = held[V > 0 ? v : 0];
+      if (V == 0) take(column.load(row, v), x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] -= mean;
-        if (column.has(v, i)) square = __fmaf_rn(x[i], x[i], square);
+      for (int i = 0; i < 4; ++i) {
+        x[i] = kept(add2(x[i], minus_first), v, i);
+        if (G == 1 || column.has(v, 2 * i)) {
+          off = add2(off, x[i]);
+          square = fma2(x[i], x[i], square);
+        }
       }
     }
-    const float rstd = rsqrtf(row_reduce<TPR>(square, SumOp(), scratch[1]) * inv_cols + eps);
+    float d1 = off.get().x + off.get().y, d2 = square.get().x + square.get().y;
+    row_reduce2<TPR>(d1, d2, SumOp(), SumOp(), scratch + TPR / 32);
+    const float e = d1 * inv_cols, spread = __fmaf_rn(-d1, e, d2) * inv_cols;
+    const float rstd = rsqrtf((spread < 0.f ? 0.f : spread) + eps);  // NaN stays NaN
     if (RowPlace<TPR>::thread() == 0) {
-      mean_out[r] = mean;
+      mean_out[r] = first + e;
       rstd_out[r] = rstd;
     }
+    const Pair scale(rstd), minus_e(-(e * rstd));
 #pragma unroll
     for (int v = 0; v < count; ++v) {
-      float(&x)[8] = held[V > 0 ? v : 0];
+      Pair(&x)[4] = held[V > 0 ? v : 0];
       if (V == 0) {
-        read(v, x);
+        take(column.load(row, v), x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] -= mean;
+        for (int i = 0; i < 4; ++i) x[i] = add2(x[i], minus_first);
       }
       const Raw8<W> w = column.load(weight, v);
       Raw8<W> b;
@@ -187,7 +204,11 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
       else b.zero();
       float out[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = __fmaf_rn(x[i] * rstd, w.get(i), b.get(i));
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = fma2(fma2(x[i], scale, minus_e), Pair(w.get(2 * i), w.get(2 * i + 1)), Pair(b.get(2 * i), b.get(2 * i + 1))).get();
+        out[2 * i] = f.x;
+        out[2 * i + 1] = f.y;
+      }
       column.store(y + r * cols, v, out);
     }
   }

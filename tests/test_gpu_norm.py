@@ -379,3 +379,57 @@ def test_row_operators_on_streams_and_in_graphs(pkg):
     torch.cuda.synchronize()
     for result in results:
         assert all(torch.equal(a, c) for a, c in zip(result, other))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [1, 7, 255, 1000, 1405, 2040, 2048, 7168, 10000, 20000, 40001])
+def test_layer_norm_of_equal_values(pkg, cols, xt):
+    """A row of equal values has that value as its mean and no variance: its norm is the bias, or zero without one, and
+    the quantiser behind it gives codes of zero, as the two in one pass do."""
+    values = torch.tensor([0.0, 0.1, 1.0, -3.3, 100.0, 999.0, 29952.0, -1e6, 1e-20, 3e15]).to(xt)
+    w, b = _affine(cols, xt, cols)
+    for rows in (10, 650):                                            # few rows and many have launch shapes of their own
+        x = values.repeat(rows // 10)[:, None].expand(rows, cols).contiguous()
+        y, mean, rstd = pkg.layer_norm(x.cuda(), w.cuda(), b.cuda())
+        assert torch.equal(mean.cpu(), x[:, 0].float())
+        assert torch.equal(y.cpu(), b.expand(rows, cols))
+        assert ((rstd.cpu().double() * 1e-5 ** 0.5 - 1).abs() <= 5 * U).all()      # eps as fp32, the sum, rsqrtf: 2 ulp of 2^-23
+        y = pkg.layer_norm(x.cuda(), w.cuda())[0]
+        assert not y.any()
+        if xt is torch.bfloat16:
+            for codes, scales in (pkg.quantize_tokens(y), pkg.layer_norm_quantize(x.cuda(), w.cuda())):
+                assert not codes.any() and (scales == 1).all()
+
+
+@pytest.mark.parametrize("cols", [255, 1000, 2040, 7168, 20000])
+def test_layer_norm_of_nearly_equal_values(pkg, cols):
+    """The mean's own rounding, and what the sum of large equal parts loses, shift no row: the bound is the spread's, not
+    the offset's.  With S the mean |x - m|, A the mean |x - x0| and d additions in a row: the first mean is off by at most
+    p = U ((d + 4) A + |m|), the correction, a sum of differences that are at most S + p on average, by U (d + 5) (S + p),
+    a difference by its own rounding, and the two products by one of its own each and one of the correction's."""
+    w, b = _affine(cols, torch.float32, cols)
+    g = torch.Generator().manual_seed(cols)
+    for rows in (9, 620):
+        offset = torch.tensor([100.0, 1000.0, -30000.0])[torch.arange(rows) % 3][:, None]
+        spread = torch.tensor([1e-1, 1e-2, 1.0])[torch.arange(rows) // 3 % 3][:, None]
+        x = offset + spread * torch.randn(rows, cols, generator=g)
+        for bias in (b, None):
+            y, mean, rstd = pkg.layer_norm(x.cuda(), w.cuda(), None if bias is None else bias.cuda())
+            want, want_mean, want_rstd = row_oracle.norm(x, w, bias, 1e-5)
+            d, xs, m, r = _depth(cols), x.double(), want_mean[:, None], want_rstd[:, None]
+            apart = (xs - m).abs()
+            s = apart.mean(-1, keepdim=True)
+            p = U * ((d + 4) * (xs - xs[:, :1]).abs().mean(-1, keepdim=True) + m.abs())
+            off_e = U * (d + 5) * (s + p)
+            assert ((mean.cpu().double()[:, None] - m).abs() <= 1.01 * (U * m.abs() + off_e)).all()
+            var = 1 / r ** 2
+            square = (apart ** 2).mean(-1, keepdim=True) + p ** 2                # what is added up, before the correction
+            off_var = U * ((d + 8) * square + 3 * var) + 2 * (p + off_e) * off_e
+            off_r = off_var / var / 2 * 1.01 + 4 * U
+            assert ((rstd.cpu().double()[:, None] / r - 1).abs() <= off_r).all()
+            size = w.double().abs() * r
+            off = size * (U * (apart + p) + off_e + U * (p + off_e) + apart * (off_r + 2 * U))
+            off = 1.01 * (off + U * (size * apart + (0 if bias is None else bias.double().abs())))
+            worst = ((y.cpu().double() - want).abs() / (off + U * (want.abs() + off))).max()
+            assert worst <= 1, float(worst)
