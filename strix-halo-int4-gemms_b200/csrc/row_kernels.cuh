@@ -115,34 +115,49 @@ quantize_tokens_kernel(const bf16* __restrict__ src, uint8_t* __restrict__ codes
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// layer norm: y = (x - mean) rstd w + b, from registers, in fp32.  The first mean m is the row's first value x0 plus the
-// average of x - x0; then d = x - m is summed up beside its square: e = mean(d), what m is off by, corrects the mean, the
-// variance (mean(d^2) - e^2) and every value (d - e).  So the error is the spread's and not the offset's: a row of equal
+// layer norm: y = (x - mean) rstd w + b, from registers, in fp32.  What is added up is x - s, s being the row's first value,
+// and the mean is kept in two parts, hi + lo = s + average, lo being what the rounding of hi loses: it corrects the
+// variance (mean((x - hi)^2) - lo^2) and every value.  So the errors are the spread's and not the offset's: a row of equal
 // values has exactly that mean, no variance and its bias as its norm, and the rounding of a large mean shifts no row.
-// The values are kept as fp32, and as d: bf16 is taken apart once, not in each pass; pairs of fp32 numbers.
+// Where s turns out to be far from the others (more than eight times the spread from the mean), x - hi is added up too
+// and lo is taken from that; always doing so costs the reduction of a second number (2 us of the 46 below).
+// The values are kept as fp32, and as x - hi: bf16 is taken apart once, not in each pass; pairs of fp32 numbers.
 // 32 values a thread, so that the registers allow 1,024 threads an SM (fp32 holds its words twice for a while: 768).
 // 32768 x 2048 in bf16: 46 us, 5.9 TB/s, where a copy of the same bytes takes 44; 55 us with 64 values a thread and half
 // of the threads, 54 with 16 (the work done once for a row), 56 with resident blocks that read the next row ahead.
 // ---------------------------------------------------------------------------------------------------------------
+struct Plus {
+  __device__ __forceinline__ Pair operator()(Pair f, Pair sum) const { return add2(sum, f); }
+  __device__ __forceinline__ float operator()(float f, float sum) const { return sum + f; }
+};
+struct PlusSquare {
+  __device__ __forceinline__ Pair operator()(Pair f, Pair sum) const { return fma2(f, f, sum); }
+  __device__ __forceinline__ float operator()(float f, float sum) const { return __fmaf_rn(f, f, sum); }
+};
+
 template <typename T, typename W, int TPR, int V, bool kAligned>
 __global__ void __launch_bounds__(RowPlace<TPR>::kThreads, (sizeof(T) == 2 ? 1024 : 768) / RowPlace<TPR>::kThreads)
 layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias, T* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, long long cols, float eps) {
-  __shared__ float scratch[3 * (TPR / 32)];
+  __shared__ float scratch[3][TPR / 32];
   const float inv_cols = 1.f / static_cast<float>(cols);
   constexpr int G = kAligned ? 16 / sizeof(T) : 1;
   const Columns<TPR, G> column{RowPlace<TPR>::thread(), cols};
   const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   constexpr int kHeld = V > 0 ? V : 1;
-  // values behind the row are zero in `f`; this leaves them out of a sum
-  auto kept = [&](Pair f, int v, int i) {
-    if (G > 1) return f;  // whole chunks are left out where they are added up
-    const float2 e = f.get();
-    return Pair(column.has(v, 2 * i) ? e.x : 0.f, column.has(v, 2 * i + 1) ? e.y : 0.f);
+  // adds f's two values, of places 2 i and 2 i + 1, as far as they lie in the row (a chunk lies in it or does not)
+  auto add = [&](Pair& sum, float& sum1, Pair f, int v, int i, auto&& term) {
+    if constexpr (G > 1) {
+      if (column.has(v, 2 * i)) sum = term(f, sum);
+    } else {
+      const float2 e = f.get();
+      if (column.has(v, 2 * i)) sum1 = term(e.x, sum1);
+      if (column.has(v, 2 * i + 1)) sum1 = term(e.y, sum1);
+    }
   };
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
     const T* row = src + r * cols;
-    const float x0 = to_f32(row[0]);
+    const float shift = to_f32(row[0]);
     Pair held[kHeld][4];
     auto take = [&](const Raw8<T>& raw, Pair (&f)[4]) {
 #pragma unroll
@@ -155,49 +170,56 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 #pragma unroll
       for (int v = 0; v < kHeld; ++v) take(raw[v], held[v]);
     }
-    const Pair minus_x0(-x0);
+    const Pair minus_shift(-shift);
     Pair sum(0.f);
+    float sum1 = 0.f;
 #pragma unroll
     for (int v = 0; v < count; ++v) {
       Pair(&x)[4] = held[V > 0 ? v : 0];
       if (V == 0) take(column.load(row, v), x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (G == 1 || column.has(v, 2 * i)) sum = add2(sum, kept(add2(x[i], minus_x0), v, i));
+      for (int i = 0; i < 4; ++i) add(sum, sum1, add2(x[i], minus_shift), v, i, Plus());
     }
-    const float first = x0 + row_reduce<TPR>(sum.get().x + sum.get().y, SumOp(), scratch) * inv_cols;
-    const Pair minus_first(-first);
-    Pair off(0.f), square(0.f);
+    const float average = row_reduce<TPR>(sum.get().x + sum.get().y + sum1, SumOp(), scratch[0]) * inv_cols;
+    const float hi = shift + average, moved = hi - shift;
+    float lo = (shift - (hi - moved)) + (average - moved);  // exactly
+    const Pair minus_hi(-hi);
+    auto read_differences = [&](int v, Pair (&x)[4]) {
+      take(column.load(row, v), x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = add2(x[i], minus_hi);
+    };
+    Pair square(0.f);
+    float square1 = 0.f;
 #pragma unroll
     for (int v = 0; v < count; ++v) {
       Pair(&x)[4] = held[V > 0 ? v : 0];
       if (V == 0) take(column.load(row, v), x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = kept(add2(x[i], minus_first), v, i);
-        if (G == 1 || column.has(v, 2 * i)) {
-          off = add2(off, x[i]);
-          square = fma2(x[i], x[i], square);
-        }
+        x[i] = add2(x[i], minus_hi);
+        add(square, square1, x[i], v, i, PlusSquare());
       }
     }
-    float d1 = off.get().x + off.get().y, d2 = square.get().x + square.get().y;
-    row_reduce2<TPR>(d1, d2, SumOp(), SumOp(), scratch + TPR / 32);
-    const float e = d1 * inv_cols, spread = __fmaf_rn(-d1, e, d2) * inv_cols;
+    const float squares = row_reduce<TPR>(square.get().x + square.get().y + square1, SumOp(), scratch[1]) * inv_cols;
+    float spread = __fmaf_rn(-lo, lo, squares);
+    if (average * average > 64.f * spread) {  // the same for all threads of the row
+      float rest = 0.f;  // read again, in a short loop: this code runs for few rows and takes no registers from the others
+#pragma unroll 1
+      for (long long at = RowPlace<TPR>::thread(); at < cols; at += TPR) rest += to_f32(row[at]) - hi;
+      lo = row_reduce<TPR>(rest, SumOp(), scratch[2]) * inv_cols;
+      spread = __fmaf_rn(-lo, lo, squares);
+    }
     const float rstd = rsqrtf((spread < 0.f ? 0.f : spread) + eps);  // NaN stays NaN
     if (RowPlace<TPR>::thread() == 0) {
-      mean_out[r] = first + e;
+      mean_out[r] = hi + lo;
       rstd_out[r] = rstd;
     }
-    const Pair scale(rstd), minus_e(-(e * rstd));
+    const Pair scale(rstd), minus_lo(-(lo * rstd));
 #pragma unroll
     for (int v = 0; v < count; ++v) {
       Pair(&x)[4] = held[V > 0 ? v : 0];
-      if (V == 0) {
-        take(column.load(row, v), x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = add2(x[i], minus_first);
-      }
+      if (V == 0) read_differences(v, x);
       const Raw8<W> w = column.load(weight, v);
       Raw8<W> b;
       if (bias != nullptr) b = column.load(bias, v);
@@ -205,7 +227,7 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
       float out[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = fma2(fma2(x[i], scale, minus_e), Pair(w.get(2 * i), w.get(2 * i + 1)), Pair(b.get(2 * i), b.get(2 * i + 1))).get();
+        const float2 f = fma2(fma2(x[i], scale, minus_lo), Pair(w.get(2 * i), w.get(2 * i + 1)), Pair(b.get(2 * i), b.get(2 * i + 1))).get();
         out[2 * i] = f.x;
         out[2 * i + 1] = f.y;
       }

@@ -402,29 +402,34 @@ def test_layer_norm_of_equal_values(pkg, cols, xt):
                 assert not codes.any() and (scales == 1).all()
 
 
+@pytest.mark.parametrize("first", [0.0, 30.0, 1e4])
 @pytest.mark.parametrize("cols", [255, 1000, 2040, 7168, 20000])
-def test_layer_norm_of_nearly_equal_values(pkg, cols):
-    """The mean's own rounding, and what the sum of large equal parts loses, shift no row: the bound is the spread's, not
-    the offset's.  With S the mean |x - m|, A the mean |x - x0| and d additions in a row: the first mean is off by at most
-    p = U ((d + 4) A + |m|), the correction, a sum of differences that are at most S + p on average, by U (d + 5) (S + p),
-    a difference by its own rounding, and the two products by one of its own each and one of the correction's."""
+def test_layer_norm_of_nearly_equal_values(pkg, cols, first):
+    """The mean's own rounding, and what the sum of large equal parts loses, shift no row: the bound is the spread's, not the
+    offset's.  What is added up are d rounded differences from the row's first value, or, where that is more than eight standard
+    deviations from the mean, from the mean's first part (which is off by p at most): with S the mean |x - m| the mean is
+    off by at most e = U (d + 5) (S + min(|x0 - m|, 8.2 deviations) + p) before it is stored.  A difference has a rounding of
+    its own, the two products one each, and the correction one."""
     w, b = _affine(cols, torch.float32, cols)
     g = torch.Generator().manual_seed(cols)
     for rows in (9, 620):
         offset = torch.tensor([100.0, 1000.0, -30000.0])[torch.arange(rows) % 3][:, None]
         spread = torch.tensor([1e-1, 1e-2, 1.0])[torch.arange(rows) // 3 % 3][:, None]
-        x = offset + spread * torch.randn(rows, cols, generator=g)
+        x = torch.randn(rows, cols, generator=g)
+        x[:, 0] += first
+        x = offset + spread * x
         for bias in (b, None):
             y, mean, rstd = pkg.layer_norm(x.cuda(), w.cuda(), None if bias is None else bias.cuda())
             want, want_mean, want_rstd = row_oracle.norm(x, w, bias, 1e-5)
             d, xs, m, r = _depth(cols), x.double(), want_mean[:, None], want_rstd[:, None]
             apart = (xs - m).abs()
-            s = apart.mean(-1, keepdim=True)
-            p = U * ((d + 4) * (xs - xs[:, :1]).abs().mean(-1, keepdim=True) + m.abs())
-            off_e = U * (d + 5) * (s + p)
+            s, deviation = apart.mean(-1, keepdim=True), (apart ** 2).mean(-1, keepdim=True).sqrt()
+            from_first = apart[:, :1]
+            p = 1.01 * U * ((d + 5) * (s + from_first) + m.abs())
+            off_e = U * (d + 5) * (s + torch.minimum(from_first, 8.2 * deviation) + p)
             assert ((mean.cpu().double()[:, None] - m).abs() <= 1.01 * (U * m.abs() + off_e)).all()
             var = 1 / r ** 2
-            square = (apart ** 2).mean(-1, keepdim=True) + p ** 2                # what is added up, before the correction
+            square = deviation ** 2 + p ** 2                                     # what is added up, before the correction
             off_var = U * ((d + 8) * square + 3 * var) + 2 * (p + off_e) * off_e
             off_r = off_var / var / 2 * 1.01 + 4 * U
             assert ((rstd.cpu().double()[:, None] / r - 1).abs() <= off_r).all()
