@@ -378,24 +378,26 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
         bmax = max_size(bmax, b.get(i), b.get(i + 1));
       }
     };
-    float s = 1.f, delta = 0.f, inv = 1.f;
+    float s = 1.f, error = 0.f, delta = 0.f, inv = 1.f;
     bool ordinary = true;
-    // bf16(amax / top) and the half-width of the border zones in codes; true if the scale has to be found from the
-    // exact maximum
-    auto scale_from = [&](float amax, float bmax) {
-      const float error = kError * (amax + 2.f * bmax), quotient = amax * (1.f / kTop);
-      s = nonzero_scale(__bfloat162float(__float2bfloat16_rn(quotient)));
+    auto take_scale = [&](float scale) {
+      s = nonzero_scale(scale);
       ordinary = !wild && scale_is_ordinary(s);
       inv = about_inverse(s);
       delta = error * inv + kTop * kError;
-      if (!wild && amax == 0.f) return false;
+    };
+    // bf16(amax / top) and the half-width of the border zones in codes; true if the scale has to be found from the
+    // exact maximum
+    auto scale_from = [&](float amax, float bmax) {
+      const float quotient = amax * (1.f / kTop);
+      error = kError * (amax + 2.f * bmax);
+      take_scale(__bfloat162float(__float2bfloat16_rn(quotient)));
+      if (!wild && amax == 0.f && bmax == 0.f) return false;  // with a bias, zeros may be what fp32 left of other numbers
       // what fp32 has no room for, or too few digits, is settled too
       return wild || !(amax > 1e-29f && amax < __int_as_float(0x7F800000)) || near_bf16_tie(quotient, error * (2.f / kTop));
     };
     auto settled = [&](unsigned long long most) {
-      s = nonzero_scale(bf16_from_double(__longlong_as_double(static_cast<long long>(most)) / static_cast<double>(kTop)));
-      ordinary = !wild && scale_is_ordinary(s);
-      inv = about_inverse(s);
+      take_scale(bf16_from_double(__longlong_as_double(static_cast<long long>(most)) / static_cast<double>(kTop)));
     };
     auto put = [&](int v, const Pair (&out)[4]) {
       const long long at = place(v);

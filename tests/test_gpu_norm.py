@@ -438,3 +438,24 @@ def test_layer_norm_of_nearly_equal_values(pkg, cols, first):
             off = 1.01 * (off + U * (size * apart + (0 if bias is None else bias.double().abs())))
             worst = ((y.cpu().double() - want).abs() / (off + U * (want.abs() + off))).max()
             assert worst <= 1, float(worst)
+
+
+@pytest.mark.parametrize("wt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float32])
+def test_layer_norm_quantize_where_the_bias_cancels_the_norm(pkg, xt, bits, wt):
+    """Rows of +-1 with a bias of the opposite fp32 number, or nearly that: float32 sees zeros in the group (or digits of its own
+    rounding alone), the exact norm is what the rounding of rstd leaves.  Whole rows, groups, and a short last group of two values."""
+    for cols, sub in ((2, 0), (64, 0), (2048, 0), (34, 32), (130, 64), (258, 256), (1024, 128), (9002, 0), (20000, 64)):
+        x = torch.ones(1, cols)
+        x[:, 1::2] = -1
+        x = x.to(xt)
+        for eps in (1e-5, 3e-3, 0.37):
+            r = torch.tensor((1 + eps) ** -0.5, dtype=torch.float64).float()
+            if wt is torch.bfloat16:           # the product's weight, so that w r is near a bfloat16 number
+                r = r.bfloat16().float()
+            w = torch.ones(cols).to(wt)
+            for part in (slice(0, cols), slice(cols - 2, cols)):
+                b = torch.linspace(-2, 2, cols)
+                b[part] = -r * x[0, part].float()
+                _check_norm_codes(pkg, x, w, b.to(wt), bits, sub, eps=eps)
