@@ -875,9 +875,9 @@ __global__ void __launch_bounds__(kMoeThreads, MoeStage<DT, NN, SC, WORDS, kMaxN
         if (++ahead == kStages) ahead = 0;
       }
       look_ahead();
-      // Packed: a group's sum is below 2^22 in size (256 times 256 products of up to 56), and starts at the bits of 1.5 *
-      // 2^23, so that it is an fp32 number as it stands.
-      constexpr int kAccZero = SC && DT == 4 ? 0x4B400000 : 0;
+      // Packed: a group's sum is below 2^22 in size (256 times 256 products of up to 56), and starts at the bits of 3, so
+      // that it is an fp32 number as it stands: 3 + 2^-22 times the sum, less than 1 away from 3.
+      constexpr int kAccZero = SC && DT == 4 ? 0x40400000 : 0;
       int acc[kFrags][kN][4];
       double sum[SC ? kFrags : 1][SC ? kN : 1][4];
 #pragma unroll
@@ -981,17 +981,19 @@ __global__ void __launch_bounds__(kMoeThreads, MoeStage<DT, NN, SC, WORDS, kMaxN
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
               const float2 st = *reinterpret_cast<const float2*>(row_scales + n * 8 + 2 * q);
-              // (packed: the sums are 256 times too large)
-              const double st0 = static_cast<double>(DT == 4 ? st.x * 0.00390625f : st.x), st1 = static_cast<double>(DT == 4 ? st.y * 0.00390625f : st.y);
+              // (packed: the sums are 256 times too large, and 2^22 times too small)
+              const double st0 = static_cast<double>(st.x) * (DT == 4 ? 16384.0 : 1.0), st1 = static_cast<double>(st.y) * (DT == 4 ? 16384.0 : 1.0);
 #pragma unroll
               for (int f = 0; f < kFrags; ++f)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   const float sw = __uint_as_float(static_cast<uint32_t>(w_scales[f * 16 + g + h * 8]) << 16);
                   int &a = acc[f][n][2 * h], &b = acc[f][n][2 * h + 1];
-                  if (DT == 4) {  // 14 bits of the sum, 8 of the scale: exact in fp32
-                    const Pair whole = add2(Pair(__int_as_float(a), __int_as_float(b)), Pair(-12582912.f));
-                    const float2 scaled = mul2(whole, Pair(sw)).get();
+                  // 14 bits of the sum, 8 of the scale: exact in fp32.  For every scale: the factor, a multiple of 2^-14 below 1,
+                  // makes no product larger than the scale, and of a multiple of 2^-133 (the least scale) one of 2^-147.
+                  if (DT == 4) {
+                    const Pair part = add2(Pair(__int_as_float(a), __int_as_float(b)), Pair(-3.f));
+                    const float2 scaled = mul2(part, Pair(sw)).get();
                     sum[f][n][2 * h] = fma(static_cast<double>(scaled.x), st0, sum[f][n][2 * h]);
                     sum[f][n][2 * h + 1] = fma(static_cast<double>(scaled.y), st1, sum[f][n][2 * h + 1]);
                   } else {
@@ -1068,9 +1070,9 @@ __global__ void __launch_bounds__(kMoeThreads, MoeStage<DT, NN, SC, WORDS, kMaxN
         } else {
           double up = static_cast<double>(sum_of(t, false)), gated = static_cast<double>(sum_of(t, true));
           if (!SC) {
-            const float s = row_scale[buffer][t];
-            up *= static_cast<double>(s * scale.x);  // a product of two bf16 numbers is exact in fp32
-            gated *= static_cast<double>(s * scale.y);
+            const double s = static_cast<double>(row_scale[buffer][t]);
+            up *= s * static_cast<double>(scale.x);  // exact; in fp32 it could be beyond the range, or below the least number
+            gated *= s * static_cast<double>(scale.y);
           }
           p.act[static_cast<long long>(pair_of[buffer][t]) * p.inner + col] = up * gated / (1.0 + exp(-gated));
         }
@@ -1150,8 +1152,8 @@ __global__ void __launch_bounds__(32 * kCombineLines) moe_combine_kernel(const M
     }
     double y0 = static_cast<double>(sum.x), y1 = static_cast<double>(sum.y);
     if (!SC) {
-      y0 *= static_cast<double>(scale * bf16_lo(w[i]));  // a product of two bf16 numbers is exact in fp32
-      y1 *= static_cast<double>(scale * bf16_hi(w[i]));
+      y0 *= static_cast<double>(scale) * static_cast<double>(bf16_lo(w[i]));  // exact, as above
+      y1 *= static_cast<double>(scale) * static_cast<double>(bf16_hi(w[i]));
     }
     share[j][lane] = make_float2(static_cast<float>(y0), static_cast<float>(y1));
   }

@@ -335,3 +335,79 @@ def test_a_training_step_around_grouped_products(pkg):
     want = row_oracle.norm_bwd(dy.cpu(), x, gamma, mean.cpu(), rstd.cpu())
     assert ((dx.cpu().double() - want[0]).abs() <= 2.0 ** -8 * want[0].abs() + 1e-5 * rstd.cpu()[:, None] * dy.cpu().abs().max()).all()
     assert (dgamma.cpu().double() - want[1]).abs().max() <= 1e-5 * want[1].abs().max() and (dbeta.cpu().double() - want[2]).abs().max() <= 1e-5 * want[2].abs().max()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+def _given(pkg, c, ids, share, **more):
+    call = {**c["call"], "up_gate_scale": c["s_up_gate"].cuda(), "down_scale": c["s_down"].cuda(), **more}
+    return pkg.moe_swiglu(c["x"].cuda(), c["w_up_gate"].cuda(), c["w_down"].cuda(), topk_ids=ids.cuda(), topk_weights=share.cuda(), **call)
+
+
+@pytest.mark.parametrize("sub", [0, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scales_of_any_size(pkg, bits, layout, sub):
+    """Tokens 2^k times smaller and scales of the first product 2^k times larger, and the same with the second product's scales
+    and the experts' weights: powers of two that cancel, so that no bit of the result changes, up to the largest scales that
+    bfloat16 has."""
+    c = _case(pkg, tokens=11, experts=4, hidden=512, inner=768, bits=bits, layout=layout, sub=sub, seed=61)
+    g = torch.Generator().manual_seed(62)
+    ids, share = torch.randint(0, 4, (11, 2), generator=g), torch.rand(11, 2, generator=g) + 0.5
+    small = 2.0 ** -122 if bits == 4 else 2.0 ** -117     # the tokens' scales stay normal bfloat16 numbers
+    c["x"] = (c["x"].double() * small).bfloat16().double().div(small).bfloat16()      # no digits that the small tokens do not have
+    want = _given(pkg, c, ids, share)
+    _check(c, want, ids, share)
+    scaled = {**c, "x": (c["x"].double() * small).bfloat16(), "s_up_gate": (c["s_up_gate"].double() / small).bfloat16()}
+    assert torch.equal(_given(pkg, scaled, ids, share), want)
+    scaled = {**c, "s_down": (c["s_down"].double() / small).bfloat16()}
+    assert torch.equal(_given(pkg, scaled, ids, share * small), want)
+
+
+@pytest.mark.parametrize("sub", [0, 64])
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_columns_of_zeros_with_large_scales(pkg, bits, layout, sub):
+    """A sum of zero is zero, whatever its two scales are: their product may be beyond float32."""
+    c = _case(pkg, tokens=3, experts=2, hidden=128, inner=64, bits=bits, layout=layout, sub=sub, seed=63)
+    nn = layout == "nn"
+    for name, s_name, n in (("w_up_gate", "s_up_gate", 128), ("w_down", "s_down", 128)):
+        empty = torch.arange(n) % 3 == 1
+        w = c[name]
+        if nn:
+            w[:, :, empty] = 0
+        else:
+            w[:, empty] = 0
+        c[s_name][..., empty] = 2.0 ** 100
+    # the other columns: tokens of about 2^40, activations of about 2^60
+    c["x"] = (c["x"].double() * 2.0 ** 40).bfloat16()
+    c["s_up_gate"][..., torch.arange(128) % 3 != 1] *= 2.0 ** -10
+    c["s_down"][..., torch.arange(128) % 3 != 1] *= 2.0 ** -60
+    ids, share = torch.tensor([[0, 1], [1, 0], [0, 0]]), torch.tensor([[0.5, 0.5], [0.25, 0.75], [1.0, 2.0]])
+    out = _given(pkg, c, ids, share)
+    assert torch.isfinite(out).all() and not out[:, torch.arange(128) % 3 == 1].any()
+    _check(c, out, ids, share)
+
+
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("sub", [0, 128])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_products_of_scales_below_float32(pkg, bits, sub, layout):
+    """The product of two scales has sixteen significant bits however small it is; the sum that it multiplies brings the
+    result back into range.  (Tokens of 2^-20, up scales of 2^-117, gate scales of 2^90; then down scales of 2^-100 behind
+    activations of about 2^-35.)"""
+    inner = 1024
+    c = _case(pkg, tokens=5, experts=2, hidden=512, inner=inner, bits=bits, layout=layout, sub=sub, seed=64)
+    c["x"] = (c["x"].double() * 2.0 ** -20).bfloat16()
+    c["s_up_gate"][..., :inner] *= 2.0 ** -112
+    c["s_up_gate"][..., inner:] *= 2.0 ** 96
+    ids, share = torch.tensor([[0, 1], [1, 0], [0, 1], [1, 1], [0, 0]]), torch.ones(5, 2)
+    out = _given(pkg, c, ids, share)
+    assert out.abs().max() > 0
+    _check(c, out, ids, share)
+    c["s_down"] *= 2.0 ** -72
+    out = _given(pkg, c, ids, share)
+    want, size = moe_oracle.layer(c["x"], c["w_up_gate"], c["w_down"], c["s_up_gate"], c["s_down"], ids, share, bits=bits, nn=layout == "nn", sub=sub)
+    assert 2.0 ** -126 < want.abs().max() < 2.0 ** -100
+    # as _check, and the steps of subnormal numbers: half of 2^-149 a share and a sum, half of 2^-133 at the end
+    off = 6 * U * size + 4 * 2.0 ** -150
+    assert ((out.cpu().double() - want).abs() <= 1.01 * off + 2.0 ** -8 * (want.abs() + off) + 2.0 ** -134).all()
