@@ -38,9 +38,10 @@ int guarded(Fn&& fn) noexcept {
 }
 
 // Allows a kernel its dynamic shared memory (with the static part it may pass the 48 KB that need no permission), once
-// for each device: the attribute stays with the device's context.
+// for each device: the attribute stays with the device's context.  Internal linkage: a static of an inline function would be
+// one object for every copy of this library that a process loads, while each copy's kernels need the permission themselves.
 template <auto Kernel>
-int allow_shared_memory(int smem_bytes) {
+static int allow_shared_memory(int smem_bytes) {
   static std::atomic<uint64_t> done{0};
   int device = 0;
   if (const cudaError_t err = cudaGetDevice(&device); err != cudaSuccess) return host_fail_cuda("cudaGetDevice", err);

@@ -459,3 +459,19 @@ def test_layer_norm_quantize_where_the_bias_cancels_the_norm(pkg, xt, bits, wt):
                 b = torch.linspace(-2, 2, cols)
                 b[part] = -r * x[0, part].float()
                 _check_norm_codes(pkg, x, w, b.to(wt), bits, sub, eps=eps)
+
+
+def test_two_copies_of_the_library_in_one_process(pkg, native_lib, tmp_path):
+    """Kernels that need more shared memory than is given unasked get the permission in each copy."""
+    import shutil
+
+    from strix_halo_int4_gemms_b200 import native
+
+    copy = tmp_path / "copy_of_the_library.so"
+    shutil.copy(native_lib, copy)
+    x, dy = [_rows(300, 2048, torch.bfloat16, seed).cuda() for seed in (71, 72)]
+    w = _affine(2048, torch.bfloat16, 73)[0].cuda()
+    _, mean, rstd = pkg.layer_norm(x, w)
+    want = pkg.layer_norm_bwd(dy, x, w, mean, rstd)
+    got = native.layer_norm_bwd_on_device(dy, x, w, mean, rstd, library_path=copy)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))

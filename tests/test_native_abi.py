@@ -3,6 +3,8 @@ reports its status, and rejects bad arguments with rc=1 and a message (no kernel
 Modelled on the reference's tests/test_native.py:34-180."""
 import ctypes
 import re
+import shutil
+import subprocess
 from pathlib import Path
 
 import pytest
@@ -138,3 +140,14 @@ def test_launcher_validation_before_any_device_work(pkg):
     if not torch.cuda.is_available():
         with pytest.raises(RuntimeError, match="require a CUDA torch device"):
             pkg.launch_generated_kernel(a, b, kernel=k, a_scale=torch.ones(128), b_scale=torch.ones(256))
+
+
+def test_two_copies_of_the_library_share_no_state(native_lib):
+    """What a copy of the library remembers (kernels whose attributes it has set, devices) is its own: no symbol of it is one
+    that the loader makes unique in the process ("u"), whatever copy defines it."""
+    nm = shutil.which("nm")
+    if nm is None:
+        pytest.skip("nm is not installed")
+    listed = subprocess.run([nm, "-D", "--defined-only", str(native_lib)], capture_output=True, text=True, check=True).stdout.splitlines()
+    assert len(listed) > 50
+    assert [line for line in listed if line.split()[1] == "u"] == []
