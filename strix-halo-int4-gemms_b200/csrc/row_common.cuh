@@ -126,14 +126,16 @@ struct Columns {
   int thread;
   long long cols;
   __device__ __forceinline__ long long at(int v, int i) const { return (static_cast<long long>(v * (8 / G) + i / G) * TPR + thread) * G + i % G; }
-  __device__ __forceinline__ bool has(int v, int i) const { return at(v, i - i % G) < cols; }  // a chunk is inside or outside
+  // A chunk is inside or outside.  (Rows have less than 2^31 values, and a thread's places end less than 2^31 behind them.)
+  __device__ __forceinline__ bool has(int v, int i) const { return static_cast<unsigned>(at(v, i - i % G)) < static_cast<unsigned>(cols); }
+  // Values behind the row: zero, or (narrow loads) `behind`.
   template <typename T>
-  __device__ __forceinline__ Raw8<T> load(const T* row, int v) const {
+  __device__ __forceinline__ Raw8<T> load(const T* row, int v, T behind = T(0.f)) const {
     Raw8<T> r;
     if constexpr (G == 1) {
       T e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = has(v, i) ? row[at(v, i)] : T(0.f);
+      for (int i = 0; i < 8; ++i) e[i] = has(v, i) ? row[at(v, i)] : behind;
       r.set(e);
     } else {
 #pragma unroll
