@@ -4,6 +4,7 @@
 #include "row_launch.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace {
 
@@ -51,6 +52,10 @@ int check_alignment(const char* name, const void* p, size_t bytes) {
 // fp32, whose registers are twice as many.  Wider rows: two kernels, with the rows divided into `parts`.
 constexpr long long kBwdHeld = 8192;
 
+// Columns of a thread of the strips kernel: 16 bytes of them where rows can be read that way.
+template <typename T, bool kWide>
+constexpr int strip_columns() { return kWide ? 16 / static_cast<int>(sizeof(T)) : 1; }
+
 int bwd_threads(long long cols, int x_type) {
   const int v = x_type == B200_OUT_BF16 ? 2 : 1;
   int threads = 32;
@@ -58,23 +63,79 @@ int bwd_threads(long long cols, int x_type) {
   return threads;
 }
 
-// Rows of partial sums: one for each block that is resident at once (512 threads or more, one an SM), or one for each
-// part of the rows, as many as the device holds at once of their blocks, two an SM (517 x 14336 in bf16: 21 us in all;
-// twice as many blocks 24, three times 27).
-long long bwd_partials(int sm_count, long long rows, long long cols, int x_type) {
+// Blocks of the strips kernel (wide rows) that an SM holds at once, by its registers: one in bf16, two in fp32, three where
+// rows cannot be read 16 bytes at a time.  0 with a message if the device does not say.
+template <typename T, typename W, int G>
+int strip_blocks_an_sm() {
+  static std::atomic<int> known{0};
+  if (int blocks = known.load(std::memory_order_relaxed); blocks > 0) return blocks;
+  int blocks = 0;
+  const cudaError_t err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, layer_norm_bwd_strips_kernel<T, W, G>, 32 * kStripWarps, 0);
+  if (err != cudaSuccess || blocks <= 0) {
+    host_fail_cuda("cudaOccupancyMaxActiveBlocksPerMultiprocessor", err);
+    return 0;
+  }
+  known.store(blocks, std::memory_order_relaxed);
+  return blocks;
+}
+
+// Parts of the rows for the strips kernel: the fewest with which its blocks fill their waves to four fifths, or the best of six.
+// (Measured at 8704 to 131072 columns, 128 to 4096 rows: 1 % above the best number on average.  4096 x 20000 in fp32, 157
+// strips, two blocks an SM: 291 us in one part, 304 in two, 257 in five; 4096 x 40000 in bf16, 157 strips, one block an SM:
+// 451 us in one part, 365 in three.)  A warp adds up at most 512 rows in one chain.
+long long strip_parts(long long strips, long long at_once, long long rows) {
+  const long long least = (rows + 4095) / 4096, most = std::max(least, std::min(least + 5, (rows + 31) / 32));
+  long long best = least;
+  double best_fill = 0.0;
+  for (long long parts = least; parts <= most && best_fill < 0.8; ++parts) {
+    const long long blocks = strips * parts, waves = (blocks + at_once - 1) / at_once;
+    const double fill = static_cast<double>(blocks) / static_cast<double>(waves * at_once);
+    if (fill > best_fill) {
+      best = parts;
+      best_fill = fill;
+    }
+  }
+  return best;
+}
+
+// Rows of partial sums: one for each block that is resident at once (512 threads or more, one an SM), or, for wide rows, one
+// for each part.
+int bwd_partials(int sm_count, long long rows, long long cols, int x_type, int w_type, bool wide, long long* partials) {
+  *partials = 0;
   if (rows == 0) return 0;
   if (cols <= kBwdHeld) {
     const int threads = bwd_threads(cols, x_type), groups = threads < 512 ? 512 / threads : 1;
-    const long long needed = (rows + groups - 1) / groups;
-    return needed < sm_count ? needed : sm_count;
+    *partials = std::min<long long>((rows + groups - 1) / groups, sm_count);
+    return 0;
   }
-  const long long width = x_type == B200_OUT_BF16 ? 256 : 128, strips = (cols + width - 1) / width, wanted = 2LL * sm_count / strips, most = (rows + 31) / 32;
-  return std::max(1LL, std::min(wanted, most));
+  int at_once = 0, width = 0;
+  for_types(x_type, w_type, [&](auto xt, auto wt) {
+    using T = decltype(xt);
+    using W = decltype(wt);
+    for_bool(wide, [&](auto aligned) {
+      constexpr int G = strip_columns<T, decltype(aligned)::value>();
+      at_once = strip_blocks_an_sm<T, W, G>() * sm_count;
+      width = 32 * G;
+    });
+  });
+  if (at_once == 0) return 1;
+  *partials = strip_parts((cols + width - 1) / width, at_once, rows);
+  return 0;
 }
 
-size_t bwd_workspace(int sm_count, long long rows, long long cols, int x_type) {
-  const size_t sums = static_cast<size_t>(bwd_partials(sm_count, rows, cols, x_type)) * 2 * cols * sizeof(float);
-  return (sums + 15) / 16 * 16 + (cols > kBwdHeld ? static_cast<size_t>(rows) * sizeof(RowTerms) : 0);
+size_t bwd_sums_bytes(long long partials, long long cols) { return (static_cast<size_t>(partials) * 2 * cols * sizeof(float) + 15) / 16 * 16; }
+
+// Enough for every type of weight, and whether rows can be read 16 bytes at a time or not.
+int bwd_workspace(int sm_count, long long rows, long long cols, int x_type, size_t* bytes) {
+  long long most = 0;
+  for (const int w_type : {B200_OUT_BF16, B200_OUT_F32})
+    for (const bool wide : {false, true}) {
+      long long partials = 0;
+      if (int rc = bwd_partials(sm_count, rows, cols, x_type, w_type, wide, &partials); rc != 0) return rc;
+      most = std::max(most, partials);
+    }
+  *bytes = bwd_sums_bytes(most, cols) + (cols > kBwdHeld ? static_cast<size_t>(rows) * sizeof(RowTerms) : 0);
+  return 0;
 }
 
 // A launch that may start while the kernel before it on the stream still runs (it waits for it by itself).
@@ -193,8 +254,7 @@ extern "C" size_t b200_int4_gemms_layer_norm_bwd_workspace_bytes(int device_inde
     DeviceScope device;
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
-    bytes = bwd_workspace(sms, rows, cols, x_type);
-    return 0;
+    return bwd_workspace(sms, rows, cols, x_type, &bytes);
   });
   return bytes;
 }
@@ -220,13 +280,15 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
     int sms = 0;
     if (int rc = device.enter(device_index, &sms); rc != 0) return rc;
     const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-    const long long partials = bwd_partials(sms, rows, cols, x_type);
-    const size_t need = bwd_workspace(sms, rows, cols, x_type);
+    const bool wide = cols % 8 == 0 && is_aligned(dy, 16) && is_aligned(x, 16) && is_aligned(dx, 16) && is_aligned(weight, 16);
+    size_t need = 0;
+    if (int rc = bwd_workspace(sms, rows, cols, x_type, &need); rc != 0) return rc;
+    long long partials = 0;
+    if (int rc = bwd_partials(sms, rows, cols, x_type, weight_type, wide, &partials); rc != 0) return rc;
     if (need > 0 && (workspace == nullptr || !is_aligned(workspace, 16) || workspace_bytes < need))
       return host_fail("workspace must be 16-byte aligned and hold b200_int4_gemms_layer_norm_bwd_workspace_bytes bytes");
     float* partial = static_cast<float*>(workspace);
-    RowTerms* terms = reinterpret_cast<RowTerms*>(static_cast<char*>(workspace) + need - (cols > kBwdHeld ? static_cast<size_t>(rows) * sizeof(RowTerms) : 0));
-    const bool wide = cols % 8 == 0 && is_aligned(dy, 16) && is_aligned(x, 16) && is_aligned(dx, 16) && is_aligned(weight, 16);
+    RowTerms* terms = reinterpret_cast<RowTerms*>(static_cast<char*>(workspace) + bwd_sums_bytes(partials, cols));  // wide rows only
     int rc = 0;
     if (rows > 0) {
       for_types(x_type, weight_type, [&](auto xt, auto wt) {
@@ -240,7 +302,7 @@ extern "C" int b200_int4_gemms_layer_norm_bwd(int device_index, uintptr_t stream
           constexpr bool A = decltype(aligned)::value;
           constexpr int V = sizeof(T) == 2 ? 2 : 1;
           if (cols > kBwdHeld) {
-            constexpr int G = A ? 16 / static_cast<int>(sizeof(T)) : 1;
+            constexpr int G = strip_columns<T, A>();
             const long long blocks = std::min<long long>(rows, 4LL * sms);
             layer_norm_bwd_rows_kernel<T, W, A><<<static_cast<unsigned>(blocks), 512, 0, stream>>>(dy_t, x_t, w_t, mean, rstd, terms, rows, cols);
             if (rc = launched("layer_norm_bwd launch"); rc != 0) return;

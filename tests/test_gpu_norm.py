@@ -475,3 +475,42 @@ def test_two_copies_of_the_library_in_one_process(pkg, native_lib, tmp_path):
     want = pkg.layer_norm_bwd(dy, x, w, mean, rstd)
     got = native.layer_norm_bwd_on_device(dy, x, w, mean, rstd, library_path=copy)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(2500, 8712), (1203, 14336), (1500, 16500), (700, 20000), (1029, 40000), (1500, 9001), (1200, 20001)])
+def test_layer_norm_bwd_of_wide_rows(pkg, rows, cols, xt):
+    """Wide rows, read 16 bytes at a time or not, in several parts that the warps of a block share."""
+    x, dy, w = _rows(rows, cols, xt, cols).cuda(), (_rows(rows, cols, xt, cols + 1) / 7).cuda(), _affine(cols, torch.float32, 3)[0].cuda()
+    _, mean, rstd = pkg.layer_norm(x, w)
+    dx, dw, db = pkg.layer_norm_bwd(dy, x, w, mean, rstd)
+    m, r = mean.double(), rstd.double()
+    want_dx, want_dw, want_db = row_oracle.norm_bwd(dy, x, w, m, r)
+    d = _depth(cols)
+    h, g = ((x.double() - m[:, None]) * r[:, None]).abs(), (dy.double() * w.double()).abs()
+    off = r[:, None] * U * (5 * g + (d + 6) * g.mean(-1, keepdim=True) + (d + 12) * h * (g * h).mean(-1, keepdim=True))   # as in _check_bwd
+    assert ((dx.double() - want_dx).abs() <= 1.01 * off + HALF_STEP[xt] * (want_dx.abs() + off)).all()
+    # a thread adds the rows of its warp, one in eight of its part; then the warps' eight sums, and at most six parts
+    path = rows / 8 + 1 + 8 + 6
+    for got, want, terms in ((dw, want_dw, (dy.double().abs() * h).sum(0)), (db, want_db, dy.double().abs().sum(0))):
+        assert ((got.double() - want).abs() <= 1.01 * (path + 4) * U * terms).all()
+
+
+def test_layer_norm_bwd_divides_the_rows_of_wide_rows(pkg):
+    """The number of parts, by the scratch that is asked for (16 bytes a row, and 8 bytes a column for each part): enough blocks for
+    the device at widths whose strips alone fill half of it, and at most 512 rows to a warp however many there are."""
+    from strix_halo_int4_gemms_b200 import native
+
+    size = native.load_dispatch_library().b200_int4_gemms_layer_norm_bwd_workspace_bytes
+
+    def parts(rows, cols, kind):
+        return (size(0, rows, cols, kind) - 16 * rows) // (8 * cols)
+
+    for cols, kind in ((20000, native.OUT_F32), (33000, native.OUT_F32), (40000, native.OUT_BF16)):
+        sms = torch.cuda.get_device_properties(0).multi_processor_count
+        strips = -(-cols // (128 if kind == native.OUT_F32 else 256))
+        if sms < strips <= 1.2 * sms:
+            assert parts(4096, cols, kind) >= 3, cols
+    for cols in (8704, 19200, 65536):
+        for kind in (native.OUT_F32, native.OUT_BF16):
+            assert parts(32768, cols, kind) >= 8 and 1 <= parts(5, cols, kind) <= 2
