@@ -985,7 +985,11 @@ def layer_norm_quantize_on_device(x: Any, weight: Any, bias: Any | None, *, eps:
 
 @lru_cache(maxsize=256)
 def _layer_norm_bwd_workspace(library: Any, *fields: int) -> int:
-    return int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(*fields))
+    """Bytes of scratch for (device, rows, cols, type of x).  0 where it is needed is a failure, which is not kept."""
+    need = int(library.b200_int4_gemms_layer_norm_bwd_workspace_bytes(*fields))
+    if need == 0 and fields[1] > 0:
+        raise RuntimeError(_library_last_error(library))
+    return need
 
 
 def layer_norm_bwd_on_device(dy: Any, x: Any, weight: Any, mean: Any, rstd: Any, *, library_path: str | Path | None = None,

@@ -126,3 +126,29 @@ def test_c_entry_points_check_arguments(pkg, native_lib):
     assert said(b(0, 0, p, p, p, p, p, p, None, p, p, 8, 1, 8, 0, 0)) == "dweight and dbias pointers must be non-null"
     assert said(b(0, 0, None, p, p, p, p, p, p, p, p, 8, 1, 8, 0, 0)) == "dy, x, weight, mean, rstd and dx pointers must be non-null"
     assert lib.b200_int4_gemms_layer_norm_bwd_workspace_bytes(99, 1, 8, 0) == 0
+
+
+def test_a_failed_size_of_the_backward_scratch_is_not_kept(pkg):
+    from strix_halo_int4_gemms_b200 import native
+
+    class Library:
+        """What the library answers while the device cannot be asked, and afterwards."""
+
+        def __init__(self):
+            self.answers, self.calls = [0, 4096], 0
+
+        def b200_int4_gemms_layer_norm_bwd_workspace_bytes(self, *fields):
+            self.calls += 1
+            return self.answers[min(self.calls, 2) - 1]
+
+        @staticmethod
+        def b200_int4_gemms_last_error():
+            return b"the device did not answer"
+
+    library = Library()
+    with pytest.raises(RuntimeError, match="the device did not answer"):
+        native._layer_norm_bwd_workspace(library, 0, 8, 16, native.OUT_F32)
+    assert native._layer_norm_bwd_workspace(library, 0, 8, 16, native.OUT_F32) == 4096
+    assert native._layer_norm_bwd_workspace(library, 0, 8, 16, native.OUT_F32) == 4096 and library.calls == 2
+    library.answers, library.calls = [0, 0], 0
+    assert native._layer_norm_bwd_workspace(library, 0, 0, 16, native.OUT_F32) == 0     # no rows, no scratch
