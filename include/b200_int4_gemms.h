@@ -355,7 +355,8 @@ int b200_int4_gemms_quantize_tokens(int device_index, uintptr_t stream_handle, c
 
 /* Layer norm over the last axis: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(mean((x - mean)^2) + eps).
  *   x, y [rows, cols] of x_type; weight, bias [cols] of weight_type (B200_OUT_BF16 or B200_OUT_F32); bias may be NULL
- *   mean, rstd  f32 [rows], for the backward pass.  Statistics in fp32. */
+ *   mean, rstd  f32 [rows], for the backward pass.  Statistics in fp32, the mean in two parts (rows of equal values give the
+ *   bias).  eps: zero, or a number that fp32 has room for. */
 int b200_int4_gemms_layer_norm(int device_index, uintptr_t stream_handle, const void* x, const void* weight,
                                const void* bias, void* y, float* mean, float* rstd, int64_t rows, int64_t cols,
                                int32_t x_type, int32_t weight_type, double eps);

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 
 namespace {
 
@@ -189,6 +190,8 @@ extern "C" int b200_int4_gemms_layer_norm(int device_index, uintptr_t stream_han
     if (int rc = check_rows(rows, cols); rc != 0) return rc;
     if (int rc = check_types(x_type, weight_type); rc != 0) return rc;
     if (!(eps >= 0.0)) return host_fail("eps must be non-negative");
+    // it is added to a float32 variance: what rounds to zero there would make rows of equal values NaN
+    if (eps != 0.0 && !(eps > 0.5 * FLT_TRUE_MIN && eps <= FLT_MAX)) return host_fail("eps must be zero or within the range of float32");
     if (rows == 0) return 0;
     if (x == nullptr || weight == nullptr || y == nullptr || mean == nullptr || rstd == nullptr)
       return host_fail("x, weight, y, mean and rstd pointers must be non-null");

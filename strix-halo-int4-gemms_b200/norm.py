@@ -15,6 +15,7 @@ from .native import layer_norm_bwd_on_device, layer_norm_on_device, layer_norm_q
 from .quant import _code_bits
 
 DEFAULT_EPS = 1e-5
+FLOAT32_NONE, FLOAT32_MOST = 2.0 ** -150, (2.0 - 2.0 ** -23) * 2.0 ** 127  # what rounds to zero, and the largest
 
 
 def _torch() -> Any:
@@ -68,11 +69,15 @@ def layer_norm(x: Any, weight: Any, bias: Any | None = None, *, eps: float = DEF
 
     ``x``: CUDA bfloat16 or float32 ``[..., N]``, contiguous; ``y`` has its dtype.  ``weight`` and ``bias`` (or
     None) ``[N]``, bfloat16 or float32, whatever ``x`` is.  ``mean`` and ``rstd = 1 / sqrt(var + eps)`` are float32
-    ``[...]``, what :func:`layer_norm_bwd` needs.  Statistics in float32; one rounding of ``y`` at the end.
+    ``[...]``, what :func:`layer_norm_bwd` needs.  Statistics in float32, the mean in two parts, so that its rounding shifts no
+    row (equal values give the bias); one rounding of ``y`` at the end.  ``eps`` is zero or a number that float32 has room for.
     """
     torch = _torch()
     _check_norm_operands(torch, x, weight, bias)
-    return layer_norm_on_device(x, weight, bias, eps=_check_eps(eps))
+    eps = _check_eps(eps)
+    if eps != 0.0 and not FLOAT32_NONE < eps <= FLOAT32_MOST:  # it is added to a float32 variance
+        raise ValueError("eps must be zero or within the range of float32")
+    return layer_norm_on_device(x, weight, bias, eps=eps)
 
 
 def layer_norm_quantize(

@@ -152,3 +152,21 @@ def test_a_failed_size_of_the_backward_scratch_is_not_kept(pkg):
     assert native._layer_norm_bwd_workspace(library, 0, 8, 16, native.OUT_F32) == 4096 and library.calls == 2
     library.answers, library.calls = [0, 0], 0
     assert native._layer_norm_bwd_workspace(library, 0, 0, 16, native.OUT_F32) == 0     # no rows, no scratch
+
+
+def test_layer_norm_refuses_an_eps_that_float32_has_no_room_for(pkg, native_lib):
+    from strix_halo_int4_gemms_b200 import native
+
+    lib = native.load_dispatch_library()
+    for eps in (1e-50, 1e300, float("inf")):
+        assert lib.b200_int4_gemms_layer_norm(0, 0, 4096, 4096, 4096, 4096, 4096, 4096, 1, 8, 0, 0, eps) == 1
+        assert lib.b200_int4_gemms_last_error() == b"eps must be zero or within the range of float32"
+    for eps in (0.0, 1e-45, 1e-38, 3e38):
+        assert lib.b200_int4_gemms_layer_norm(0, 0, None, None, None, None, None, None, 0, 8, 0, 0, eps) == 0
+    if torch.cuda.is_available():
+        x, w = torch.zeros(2, 8, device="cuda"), torch.ones(8, device="cuda")
+        for eps in (1e-50, 1e300):
+            with pytest.raises(ValueError, match="within the range of float32"):
+                pkg.layer_norm(x, w, eps=eps)
+            pkg.layer_norm_quantize(x, w, eps=eps)        # adds it in float64
+        assert not pkg.layer_norm(x, w, eps=1e-45)[0].any()
