@@ -1318,10 +1318,9 @@ extern "C" int b200_int4_gemms_unpack_int4(int device_index, uintptr_t stream_ha
   if (int rc = ensure_device(device_index, &dev); rc != 0) return rc;
   const long long total = rows * cols_packed;
   if (total == 0) return 0;
-  long long blocks = (total / 16 + 255) / 256;
+  long long blocks = ((total + 7) / 8 + 255) / 256;  // a thread takes eight bytes
   const long long cap = static_cast<long long>(dev->sm_count) * 8;
   if (blocks > cap) blocks = cap;
-  if (blocks < 1) blocks = 1;
   unpack_int4_kernel<<<static_cast<unsigned>(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream_handle)>>>(
       static_cast<const uint8_t*>(packed), static_cast<int8_t*>(out_int8), total);
   cudaError_t err = cudaGetLastError();
