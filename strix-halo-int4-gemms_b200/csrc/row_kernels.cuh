@@ -202,17 +202,18 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
       }
     }
     const float squares = row_reduce<TPR>(square.get().x + square.get().y + square1, SumOp(), scratch[1]) * inv_cols;
-    float spread = __fmaf_rn(-lo, lo, squares);
-    if (average * average > 64.f * spread) {  // the same for all threads of the row
+    float spread = __fmaf_rn(-lo, lo, squares), base = hi;
+    if (!(average * average <= 64.f * spread)) {  // the same for all threads of the row; rows that are not finite too
+      base = fabsf(hi) < __int_as_float(0x7F800000) ? hi : 0.f;  // (infinities have their mean)
       float rest = 0.f;  // read again, in a short loop: this code runs for few rows and takes no registers from the others
 #pragma unroll 1
-      for (long long at = RowPlace<TPR>::thread(); at < cols; at += TPR) rest += to_f32(row[at]) - hi;
+      for (long long at = RowPlace<TPR>::thread(); at < cols; at += TPR) rest += to_f32(row[at]) - base;
       lo = row_reduce<TPR>(rest, SumOp(), scratch[2]) * inv_cols;
       spread = __fmaf_rn(-lo, lo, squares);
     }
     const float rstd = rsqrtf((spread < 0.f ? 0.f : spread) + eps);  // NaN stays NaN
     if (RowPlace<TPR>::thread() == 0) {
-      mean_out[r] = hi + lo;
+      mean_out[r] = base + lo;
       rstd_out[r] = rstd;
     }
     const Pair scale(rstd), minus_lo(-(lo * rstd));

@@ -514,3 +514,15 @@ def test_layer_norm_bwd_divides_the_rows_of_wide_rows(pkg):
     for cols in (8704, 19200, 65536):
         for kind in (native.OUT_F32, native.OUT_BF16):
             assert parts(32768, cols, kind) >= 8 and 1 <= parts(5, cols, kind) <= 2
+
+
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [7, 264, 2048, 20000])
+def test_layer_norm_mean_of_rows_that_are_not_finite(pkg, cols, xt):
+    inf, nan = float("inf"), float("nan")
+    x = _rows(7, cols, xt, cols)
+    x[0, 0], x[1, cols - 1], x[2, 0], x[3, 1], x[4, 2] = inf, inf, -inf, -inf, nan
+    x[5, 0], x[5, cols - 1] = inf, -inf
+    y, mean, rstd = pkg.layer_norm(x.cuda(), torch.ones(cols, device="cuda"))
+    assert mean[:4].tolist() == [inf, inf, -inf, -inf] and torch.isnan(mean[4:6]).all()
+    assert torch.isnan(rstd[:6]).all() and torch.isnan(y[:6]).all() and torch.isfinite(y[6]).all() and torch.isfinite(mean[6])
