@@ -153,14 +153,12 @@ struct Columns {
 #pragma unroll
       for (int i = 0; i < 8; i += G) {
         if (!has(v, i)) continue;
+        static_assert(G * sizeof(T) == 16, "a chunk is one store");
         if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int k = 0; k < G; k += 4) *reinterpret_cast<float4*>(row + at(v, i) + k) = make_float4(f[i + k], f[i + k + 1], f[i + k + 2], f[i + k + 3]);
-        } else if constexpr (G == 8) {
+          *reinterpret_cast<float4*>(row + at(v, i)) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        } else {
           *reinterpret_cast<uint4*>(row + at(v, i)) =
               make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-        } else {
-          *reinterpret_cast<uint2*>(row + at(v, i)) = make_uint2(pack_bf16x2(f[i], f[i + 1]), pack_bf16x2(f[i + 2], f[i + 3]));
         }
       }
     }
