@@ -411,3 +411,57 @@ def test_products_of_scales_below_float32(pkg, bits, sub, layout):
     # as _check, and the steps of subnormal numbers: half of 2^-149 a share and a sum, half of 2^-133 at the end
     off = 6 * U * size + 4 * 2.0 ** -150
     assert ((out.cpu().double() - want).abs() <= 1.01 * off + 2.0 ** -8 * (want.abs() + off) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+def test_a_token_alone_and_in_a_batch_where_k_is_divided(pkg, layout):
+    """One scale a column: the down product of one token divides K into more parts than that of the batch, and the integer
+    sums are the same."""
+    from strix_halo_int4_gemms_b200 import native
+
+    tokens, hidden, inner, experts = 40, 2048, 2048, 32
+    nn, kind = layout == "nn", dict(layout=pkg.GemmLayout(layout), dtype=pkg.OperandDType.INT8)
+
+    def parts(count):     # by the scratch that they ask for: all of it but the codes and activations, in shares of [pairs, hidden]
+        fields = (native.DTYPE_CODES[kind["dtype"]], native.LAYOUT_CODES[kind["layout"]], 0, count, hidden, inner, experts, 2, native.OUT_BF16, 1, 32)
+        return (native.moe_problem(*fields)[1] - count * (2 * inner * 9 + hidden)) // (count * 2 * hidden * 4)
+
+    assert parts(1) > parts(tokens) >= 1
+    g = torch.Generator(device="cuda").manual_seed(65)
+    up, down = [torch.randint(-128, 128, (experts, k, n) if nn else (experts, n, k), generator=g, device="cuda", dtype=torch.int8)
+                for k, n in ((hidden, 2 * inner), (inner, hidden))]
+    su, sd = [((torch.rand(experts, n, generator=g, device="cuda") + 0.5) / 3300).bfloat16() for n in (2 * inner, hidden)]
+    x = torch.randn(tokens, hidden, generator=g, device="cuda").bfloat16()
+    router = (torch.randn(experts, hidden, generator=g, device="cuda") / hidden ** 0.5).bfloat16()
+    call = dict(up_gate_scale=su, down_scale=sd, router_weight=router, top_k=2, **kind)
+    whole = pkg.moe_swiglu(x, up, down, **call)
+    assert torch.isfinite(whole).all() and whole.float().abs().max() > 0
+    for t in (0, 17, 39):
+        assert torch.equal(pkg.moe_swiglu(x[t:t + 1], up, down, **call)[0], whole[t])
+
+
+@pytest.mark.parametrize("sub", [32, 64, 128, 256])
+def test_scales_of_k_groups_into_the_products(pkg, sub):
+    """``quantize_tokens`` and ``layer_norm_quantize`` with a scale for each K-group are the A operand and ``a_scale`` of the
+    dense products."""
+    rows, k, n = 256, 512, 256
+    g = torch.Generator().manual_seed(sub)
+    x = torch.randn(rows, k, generator=g).bfloat16()
+    gamma = (1 + 0.2 * torch.randn(k, generator=g)).bfloat16()
+    w = torch.randint(0, 256, (k // 2, 2 * n), generator=g, dtype=torch.uint8)
+    ws = ((torch.rand(k // sub, 2 * n, generator=g) + 0.5) * 0.01).bfloat16()
+    spec = pkg.ScaleSpec(pkg.ScaleMode.SUBCHANNEL, sub)
+    full = moe_oracle.unpack(w, 4, 0)
+    for codes_scales, rows64 in ((pkg.quantize_tokens(x.cuda(), scale=spec), x),
+                                 (pkg.layer_norm_quantize(x.cuda(), gamma.cuda(), scale=spec), row_oracle.norm(x, gamma, None, 1e-5)[0])):
+        codes, scales = codes_scales
+        want_codes, want_scales, _ = row_oracle.quantize_rows(rows64, 4, sub)
+        parts = torch.stack([(want_codes[:, i * sub:(i + 1) * sub].double() @ full[i * sub:(i + 1) * sub]) * want_scales[:, i:i + 1] * ws[i].double() for i in range(k // sub)])
+        exact, size = parts.sum(0), parts.abs().sum(0)
+        out = pkg.mm(codes, w.cuda(), a_scale=scales, b_scale=ws.cuda(), scale=spec)
+        # a group's integer sum, two scales and the sum over at most 16 groups in float32; bfloat16 at the end
+        off = (k // sub + 4) * U * size
+        assert ((out.cpu().double() - exact).abs() <= 1.01 * off + 2.0 ** -8 * (exact.abs() + off)).all()
+        fused = pkg.fused_swiglu_up_gate(codes, w.cuda(), a_scale=scales, b_scale=ws.cuda(), scale=spec)
+        packed = pkg.pack_int4_k_major(want_codes).cuda()
+        assert torch.equal(fused, pkg.fused_swiglu_up_gate(packed, w.cuda(), a_scale=want_scales.bfloat16().cuda(), b_scale=ws.cuda(), scale=spec))
