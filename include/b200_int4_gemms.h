@@ -345,8 +345,9 @@ int b200_int4_gemms_repack_tokens(int device_index, uintptr_t stream_handle, con
 
 /* Quantises every row with a scale of its own (subchannel = 0) or one for each `subchannel` values (32, 64,
  * 128, 256; the last group may be shorter):  scale = bf16(max|x| / top), top = 7 (bits 4) or 127 (bits 8);
- * code = round_half_even(x / scale).  A scale that rounds to zero becomes one (all codes are then zero); a
- * group that is not finite gets that scale (infinity or NaN) and codes of zero.
+ * code = round_half_even(x / scale), at most top in size (a quotient is larger only where a subnormal scale was rounded
+ * down).  A scale that rounds to zero becomes one (all codes are then zero); a group that is not finite gets that
+ * scale (infinity or NaN) and codes of zero.
  *   src    bf16 [rows, cols];   codes  u8 [rows, ceil(cols/2)] packed as everywhere, or int8 [rows, cols]
  *   scales bf16 [rows] or [rows, ceil(cols/subchannel)]: the a_scale of the products
  * No reference counterpart (its quantiser takes one constant scale, quant.py:14-29). */
@@ -400,11 +401,13 @@ typedef struct b200_moe_problem {
 } b200_moe_problem;
 
 /* out[t] = sum_j p_tj down_e(a_tj), e = the token's j-th expert:
- *   logits = x router^T; the top_k largest (ties to the lowest expert) and p = softmax, in fp64;
+ *   logits = x router^T; the top_k largest (ties to the lowest expert, NaN below all others) and p = softmax, in fp64;
  *   x is quantised for each token as b200_int4_gemms_quantize_tokens does; [up | gate] = product with w_up_gate[e],
  *   scaled; a = up * gate / (1 + exp(-gate)), quantised in the same way from its unrounded value; the product with
- *   w_down[e], scaled and weighted with p, is added up in fp32 in the order of j and rounded to bf16 once.
- * Integer sums are exact; the same bits on every run.
+ *   w_down[e], scaled and rounded to fp32, is weighted with p and added up in fp32 in the order of j, and the sum is
+ *   rounded to bf16.  Scales of any size: their products are not rounded.
+ * Integer sums are exact; the same bits on every run.  subchannel = 0: and whatever other tokens are in the call; else the
+ * fp64 sums of the down product are divided by the number of experts in use, and a last bit may hang on that.
  *   x [tokens, hidden] bf16, out [tokens, hidden] bf16
  *   router_weight [experts, hidden], or NULL: then topk_ids [tokens, top_k] and topk_weights f32 [tokens, top_k] are
  *     the routing; an id outside [0, experts) stands for no expert and adds nothing.  With router_weight, topk_ids

@@ -16,10 +16,11 @@
 // At a few tokens each weight is used by a handful of rows, so the layer is bound by reading the weights of the
 // experts in use once from HBM.  The products therefore run on mma.sync.m16n8k32 (int8, exact int32 sums) with the
 // WEIGHTS as the 16-row operand and eight tokens at a time as the other.  Every warp copies its share of the weights
-// into a ring of its own in shared memory (cp.async), several steps ahead and on into the next columns while the sums
-// of the last ones are finished: some 100 KB an SM in flight, which is what HBM's latency asks for.  tcgen05 would
+// into a ring of its own in shared memory (cp.async), several steps ahead: some 100 KB an SM in flight within a unit of
+// work, which is what HBM's latency asks for.  At the end of a unit the ring runs empty: the first weights of the next one
+// are asked for behind its last step, before its sums are finished.  tcgen05 would
 // want 128-row tiles of unpacked weights in shared memory; its rate is of no use here (measured on this part:
-// m16n8k32 every 2 clocks an SM, 256 weights a clock for eight tokens, where HBM delivers 46).
+// m16n8k32 every 2 clocks an SM, 256 weights a clock for eight tokens and 85 for 24, where HBM delivers 46).
 //
 // Operand order.  A lane (g = lane / 4, q = lane % 4) supplies rows g and g + 8 of the 16 x 32 operand and, for
 // each, K values that a quad of lanes divides up.  Which K a lane holds does not matter as long as both operands
@@ -624,9 +625,9 @@ struct MoeSource {
 // of a unit it starts the copies of its weights of the next one, before the sums are finished.
 // kMaxN: groups of eight tokens that a pass over the weights can serve; more tokens of an expert take more passes.
 // kChoose: the blocks pick the experts themselves.
-// 64 tokens, two of 8 experts of 4096 x 14336 in int4: 470 MB of up/gate weights in 103 us (4.6 TB/s), then 235 MB in 51; the
+// 64 tokens, two of 8 experts of 4096 x 14336 in int4: 470 MB of up/gate weights in 102 us (4.6 TB/s), then 235 MB in 54; the
 // blocks issue in half of the cycles and wait for copies in most others: 16 warps an SM is what the sums of 24 rows leave
-// room for.  With K-group scales (13 tokens, 6 of 64 experts of 2048 x 1408, groups of 128): 134 MB in 40 us, with 230
+// room for.  With K-group scales (13 tokens, 6 of 64 experts of 2048 x 1408, groups of 128): 134 MB in 35 us, with 230
 // instructions a step of eight tensor-core products where the plain sums take 145, and half as many again for what a
 // warp does once a unit (eight steps).
 template <int DT, bool NN, bool SC, int WORDS, int kMaxN, bool kChoose, bool kDown>

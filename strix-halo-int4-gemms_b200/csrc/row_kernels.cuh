@@ -251,9 +251,10 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 // amax / top is within its error of a tie of two bf16 numbers, or fp32 has no room for it, the group's maximum is found
 // again in fp64.  Both are loops that read their values again, out of the way of the code that runs always.
 //
-// The kernel is bound by its instructions, not by HBM: 33 a value (two conversions and two sums in fp64 among them),
-// with pairs of fp32 numbers and three-way maxima; 43 without those, 30 us instead of 25 for 4096 x 4096 in bf16 with
-// groups of 256.  More threads an SM with fewer registers change nothing (896 and 1,024: 25 us).
+// 4096 x 4096 in bf16 with groups of 256: 26 us, 7 of them HBM's.  33 instructions a value (two conversions and two sums in
+// fp64 among them) with pairs of fp32 numbers and three-way maxima, which is 15 us of issue; 43 without those, 30 us.  The
+// other ten are the chain of a row (sums and exchanges of doubles, a barrier, the scale, the codes), with six rows an SM
+// at it.  More threads an SM with fewer registers change nothing (896 and 1,024).
 // ---------------------------------------------------------------------------------------------------------------
 struct NormExact {
   double mean, rstd;
@@ -470,7 +471,7 @@ layer_norm_quantize_kernel(const T* __restrict__ src, const W* __restrict__ weig
 // are added up in shared memory, each block leaves one row of partial sums, and column_sums_kernel adds those in a fixed
 // order: no atomics, the same bits on every run.  Four rows of a group are on their way (in shared memory: one, in
 // registers, was what bounded the kernel, with 32 KB an SM in flight; two in registers spill).
-// 32768 x 2048 in bf16: 66 us, 6.1 TB/s (75 us with one row ahead), and 3 us for the partial sums, whose kernel starts
+// 32768 x 2048 in bf16: 66 us, 6.1 TB/s (75 us with one row ahead), and 4 us for the partial sums, whose kernel starts
 // while this one ends.
 // Rows of more than 8192 values are left to two kernels, below.
 // ---------------------------------------------------------------------------------------------------------------
@@ -478,8 +479,8 @@ template <int TPR>
 struct BwdShape {
   static constexpr int kThreads = TPR < 512 ? 512 : TPR;
   static constexpr int kGroups = kThreads / TPR;  // rows at once
-  // A thread's 64 bytes of x and dy of the rows to come lie in shared memory, copied there asynchronously by the thread
-  // itself: rows of a group on their way, 96 KB in all where a row has its 16 values a thread.
+  // A thread's 64 bytes of x and dy of each row to come lie in shared memory, copied there asynchronously by the thread
+  // itself: four rows of a group on their way, 128 KB in all; three with 1,024 threads, 192 KB.
   static constexpr int kAhead = kThreads == 512 ? 4 : 3;
   static constexpr int kRingBytes = kAhead * kThreads * 64;
 };
@@ -673,9 +674,9 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ src, const
 
 // Rows of more than 8192 values, whose columns do not fit the registers of one block: the means of g and g h of every
 // row, and then dx and the sums over rows with a thread for each chunk of columns, which needs no reduction over the
-// row.  x and dy are read twice, the second time from L2 as far as it holds them.  (517 rows of 14336 fp32 values: a
-// block of 1024 threads a row took 47 us, clusters of two blocks 37 us, both waiting for their reductions; these take
-// 26 us, 12 to 13 of them for the means.)
+// row.  x and dy are read twice, the second time from L2 as far as it holds them.  517 rows of 14336 values: 26 us in fp32,
+// 12 to 13 of them for the means, 21 in bf16.  (A block of 1024 threads a row took 47 us in fp32, clusters of two blocks 37,
+// both waiting for their reductions with one row ahead; neither has been tried with the ring of the kernel above.)
 struct __align__(16) RowTerms {
   float mean, rstd, mean_g, mean_gh;
 };

@@ -71,15 +71,18 @@ def moe_swiglu(
     ``down_scale [E, H]``; subchannel ``S``: ``[E, ceil(H/S), 2I]`` and ``[E, ceil(I/S), H]``.  ``H`` and ``I`` are
     multiples of 32.
 
-    Routing: ``router_weight [E, H]`` (bfloat16 or float32) and ``top_k``: the largest logits, ties to the lowest expert,
-    weighted with their softmax (``renormalize=False``: the softmax over all experts).  Or ``topk_ids [T, k]`` (int32 or
-    int64) and ``topk_weights [T, k]`` (float32) from elsewhere; they are not read on the host, and an id outside
-    ``[0, E)``, as -1, stands for no expert.  ``return_routing=True`` returns ``(out, topk_ids, topk_weights)``.
+    Routing: ``router_weight [E, H]`` (bfloat16 or float32) and ``top_k``: the largest logits, ties to the lowest expert and
+    NaN below all others, weighted with their softmax (``renormalize=False``: the softmax over all experts).  Or
+    ``topk_ids [T, k]`` (int32 or int64) and ``topk_weights [T, k]`` (float32) from elsewhere; they are not read on the host,
+    and an id outside ``[0, E)``, as -1, stands for no expert.  ``return_routing=True`` returns
+    ``(out, topk_ids, topk_weights)``.
 
     The tokens, and the activations between the two products, are quantised as ``quantize_tokens`` does (the
     activations without being rounded before).  Integer sums are exact, the choice of experts and the border cases of
-    the quantiser are decided in float64, and each output is rounded to bfloat16 once: the same bits on every run.
-    No autograd.
+    the quantiser are decided in float64, an expert's result is rounded to float32, weighted and added up in the order of
+    the choices, and the sum is rounded to bfloat16: the same bits on every run.  With one scale a column also whatever
+    other tokens are in the call; with K-group scales the float64 sums of the second product are divided by the number of
+    experts in use, and a last bit may hang on that.  No autograd.
     """
     torch = _torch()
     if type(dtype) is not OperandDType:

@@ -112,7 +112,8 @@ def quantize_tokens(
 
     ``x``: CUDA bfloat16 ``[..., K]``, contiguous.  Per-channel: one scale a row, ``scales [...]``; subchannel
     ``S``: one for every ``S`` values along K, ``scales [..., ceil(K/S)]``.  ``scale = bf16(max|x| / top)`` with
-    ``top`` 7 (INT4) or 127 (INT8) and ``code = round_half_even(x / scale)``, both exactly.  Codes are packed uint8
+    ``top`` 7 (INT4) or 127 (INT8) and ``code = round_half_even(x / scale)``, both exactly (at most ``top`` in size, which
+    matters where a subnormal scale was rounded down).  Codes are packed uint8
     ``[..., ceil(K/2)]`` (an odd K is padded with a zero code) or int8 ``[..., K]``.  A scale that rounds to zero is
     stored as one, with codes of zero; values that are not finite give their group that scale and codes of zero, so
     that a product with them is not finite either.  No rows: empty results.  No autograd.
