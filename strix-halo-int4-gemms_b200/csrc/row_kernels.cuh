@@ -116,14 +116,14 @@ quantize_tokens_kernel(const bf16* __restrict__ src, uint8_t* __restrict__ codes
 
 // ---------------------------------------------------------------------------------------------------------------
 // layer norm: y = (x - mean) rstd w + b, from registers, in fp32.  What is added up is x - s, s being the row's first value,
-// and the mean is kept in two parts, hi + lo = s + average, lo being what the rounding of hi loses: it corrects the
-// variance (mean((x - hi)^2) - lo^2) and every value.  So the errors are the spread's and not the offset's: a row of equal
-// values has exactly that mean, no variance and its bias as its norm, and the rounding of a large mean shifts no row.
-// Where s turns out to be far from the others (more than eight times the spread from the mean), x - hi is added up too
-// and lo is taken from that; always doing so costs the reduction of a second number (2 us of the 46 below).
-// In bf16 read 16 bytes at a time s is zero unless the row's next three values are within a quarter of the first: rows
-// around zero, the usual ones, are added up as they are (1 us of 47; in fp32, and in narrow loads of either, choosing
-// costs more than it saves: 32768 x 1024 fp32 44.5 -> 47.6 us, 20000 x 2047 94 -> 104, with fewer instructions).
+// and the mean is kept in two parts, hi + lo, hi = s + average.  lo corrects the variance (mean((x - hi)^2) - lo^2) and
+// every value, so that the errors are the spread's and not the offset's: a row of equal values has exactly that mean, no
+// variance and its bias as its norm, and the rounding of a large mean shifts no row.
+// In fp32 lo is the average of x - hi, summed up beside the squares; a second sum costs nothing there.  In bf16, with twice
+// the values a byte, it costs 2 us of the 46 below: lo is what the rounding of s + average loses, and x - hi is added up
+// only where s turns out to be far from the others (more than eight times the spread from the mean).  And where rows are
+// read 16 bytes at a time s is zero unless the row's next three values are within a quarter of the first: rows around
+// zero, the usual ones, are added up as they are (1 us of 47).
 // The values are kept as fp32, and as x - hi: bf16 is taken apart once, not in each pass; pairs of fp32 numbers.
 // 32 values a thread, so that the registers allow 1,024 threads an SM (fp32 holds its words twice for a while: 768).
 // 32768 x 2048 in bf16: 46 us, 5.9 TB/s, where a copy of the same bytes takes 44; 55 us with 64 values a thread and half
@@ -142,13 +142,13 @@ template <typename T, typename W, int TPR, int V, bool kAligned>
 __global__ void __launch_bounds__(RowPlace<TPR>::kThreads, (sizeof(T) == 2 ? 1024 : 768) / RowPlace<TPR>::kThreads)
 layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const W* __restrict__ bias, T* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, long long cols, float eps) {
-  __shared__ float scratch[3][TPR / 32];
+  __shared__ float scratch[4][TPR / 32];  // of two sums at once in fp32: the second and the third
   const float inv_cols = 1.f / static_cast<float>(cols);
   constexpr int G = kAligned ? 16 / sizeof(T) : 1;
   const Columns<TPR, G> column{RowPlace<TPR>::thread(), cols};
   const int count = V > 0 ? V : static_cast<int>((cols + TPR * 8 - 1) / (TPR * 8));
   constexpr int kHeld = V > 0 ? V : 1;
-  constexpr bool kZeroToo = sizeof(T) == 2 && kAligned;
+  constexpr bool kZeroToo = sizeof(T) == 2 && kAligned, kTwice = sizeof(T) == 4;
   for (long long r = RowPlace<TPR>::first(); r < rows; r += RowPlace<TPR>::step()) {
     const T* row = src + r * cols;
     const T first = row[0], behind = G == 1 && sizeof(T) == 2 ? first : T(0.f);
@@ -206,8 +206,8 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = add2(x[i], minus_hi);
     };
-    Pair square(0.f);
-    float square1 = 0.f;
+    Pair square(0.f), rest(0.f);
+    float square1 = 0.f, rest1 = 0.f;
 #pragma unroll
     for (int v = 0; v < count; ++v) {
       Pair(&x)[4] = held[V > 0 ? v : 0];
@@ -216,22 +216,38 @@ layer_norm_kernel(const T* __restrict__ src, const W* __restrict__ weight, const
       for (int i = 0; i < 4; ++i) {
         x[i] = add2(x[i], minus_hi);
         if constexpr (G > 1) {
-          if (column.has(v, 2 * i)) square = fma2(x[i], x[i], square);
+          if (column.has(v, 2 * i)) {
+            square = fma2(x[i], x[i], square);
+            if (kTwice) rest = add2(rest, x[i]);
+          }
         } else {
           const float2 f = x[i].get();
-          if (column.has(v, 2 * i)) square1 = __fmaf_rn(f.x, f.x, square1);
-          if (column.has(v, 2 * i + 1)) square1 = __fmaf_rn(f.y, f.y, square1);
+          if (column.has(v, 2 * i)) {
+            square1 = __fmaf_rn(f.x, f.x, square1);
+            if (kTwice) rest1 += f.x;
+          }
+          if (column.has(v, 2 * i + 1)) {
+            square1 = __fmaf_rn(f.y, f.y, square1);
+            if (kTwice) rest1 += f.y;
+          }
         }
       }
     }
-    const float squares = row_reduce<TPR>(square.get().x + square.get().y + square1, SumOp(), scratch[1]) * inv_cols;
+    float squares = square.get().x + square.get().y + square1, off = rest.get().x + rest.get().y + rest1;
+    if (kTwice) {
+      row_reduce2<TPR>(squares, off, SumOp(), SumOp(), scratch[1]);
+      lo = off * inv_cols;
+    } else {
+      squares = row_reduce<TPR>(squares, SumOp(), scratch[1]);
+    }
+    squares *= inv_cols;
     float spread = __fmaf_rn(-lo, lo, squares), base = hi;
-    if (!(average * average <= 64.f * spread)) {  // the same for all threads of the row; rows that are not finite too
+    if (kTwice ? !(spread == spread) : !(average * average <= 64.f * spread)) {  // the same for all threads of the row; rows that are not finite too
       base = fabsf(hi) < __int_as_float(0x7F800000) ? hi : 0.f;  // (infinities have their mean)
-      float rest = 0.f;  // read again, in a short loop: this code runs for few rows and takes no registers from the others
+      off = 0.f;  // read again, in a short loop: this code runs for few rows and takes no registers from the others
 #pragma unroll 1
-      for (long long at = RowPlace<TPR>::thread(); at < cols; at += TPR) rest += to_f32(row[at]) - base;
-      lo = row_reduce<TPR>(rest, SumOp(), scratch[2]) * inv_cols;
+      for (long long at = RowPlace<TPR>::thread(); at < cols; at += TPR) off += to_f32(row[at]) - base;
+      lo = row_reduce<TPR>(off, SumOp(), scratch[3]) * inv_cols;
       spread = __fmaf_rn(-lo, lo, squares);
     }
     const float rstd = rsqrtf((spread < 0.f ? 0.f : spread) + eps);  // NaN stays NaN

@@ -406,10 +406,9 @@ def test_layer_norm_of_equal_values(pkg, cols, xt):
 @pytest.mark.parametrize("cols", [255, 1000, 2040, 7168, 20000])
 def test_layer_norm_of_nearly_equal_values(pkg, cols, first):
     """The mean's own rounding, and what the sum of large equal parts loses, shift no row: the bound is the spread's, not the
-    offset's.  What is added up are d rounded differences from the row's first value, or, where that is more than eight standard
-    deviations from the mean, from the mean's first part (which is off by p at most): with S the mean |x - m| the mean is
-    off by at most e = U (d + 5) (S + min(|x0 - m|, 8.2 deviations) + p) before it is stored.  A difference has a rounding of
-    its own, the two products one each, and the correction one."""
+    offset's.  The mean's first part, from d rounded differences from the row's first value x0, is off by at most p =
+    U ((d + 5) (S + |x0 - m|) + |m|), S being the mean |x - m|; the second, from d rounded differences from the first, by
+    e = U (d + 5) (S + p).  A difference has a rounding of its own, the two products one each, and the correction one."""
     w, b = _affine(cols, torch.float32, cols)
     g = torch.Generator().manual_seed(cols)
     for rows in (9, 620):
@@ -426,7 +425,7 @@ def test_layer_norm_of_nearly_equal_values(pkg, cols, first):
             s, deviation = apart.mean(-1, keepdim=True), (apart ** 2).mean(-1, keepdim=True).sqrt()
             from_first = apart[:, :1]
             p = 1.01 * U * ((d + 5) * (s + from_first) + m.abs())
-            off_e = U * (d + 5) * (s + torch.minimum(from_first, 8.2 * deviation) + p)
+            off_e = U * (d + 5) * (s + p)
             assert ((mean.cpu().double()[:, None] - m).abs() <= 1.01 * (U * m.abs() + off_e)).all()
             var = 1 / r ** 2
             square = deviation ** 2 + p ** 2                                     # what is added up, before the correction
