@@ -465,3 +465,29 @@ def test_scales_of_k_groups_into_the_products(pkg, sub):
         fused = pkg.fused_swiglu_up_gate(codes, w.cuda(), a_scale=scales, b_scale=ws.cuda(), scale=spec)
         packed = pkg.pack_int4_k_major(want_codes).cuda()
         assert torch.equal(fused, pkg.fused_swiglu_up_gate(packed, w.cuda(), a_scale=want_scales.bfloat16().cuda(), b_scale=ws.cuda(), scale=spec))
+
+
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+def test_as_many_pairs_as_there_can_be(pkg, layout):
+    c = _case(pkg, tokens=64, experts=1024, hidden=64, inner=32, bits=4, layout=layout, sub=0, seed=71)
+    _routed(pkg, c, 16)
+
+
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hidden,inner", [(131040, 32), (32, 131040)])
+def test_largest_sums(pkg, bits, layout, hidden, inner):
+    """The longest K with the largest codes of one sign on both sides: the integer sums come within 1 % (int8) of 2^31."""
+    c = _case(pkg, tokens=2, experts=2, hidden=hidden, inner=inner, bits=bits, layout=layout, sub=0, seed=72)
+    for name in ("w_up_gate", "w_down"):
+        c[name][0] = 0x88 if bits == 4 else -128
+    c["x"] = torch.full((2, hidden), 1.5).bfloat16()
+    c["x"][1] = -2.0
+    # up and gate of about +-6, activations of one sign each, and results of the size of one
+    lowest = 8.0 if bits == 4 else 128.0
+    c["s_up_gate"][0] = 4.0 / (hidden * lowest)
+    c["s_down"][0] = 1.0 / (inner * lowest)
+    ids, share = torch.tensor([[0], [0]]), torch.ones(2, 1)
+    out = _given(pkg, c, ids, share)
+    assert torch.isfinite(out).all() and (out != 0).all()
+    _check(c, out, ids, share)

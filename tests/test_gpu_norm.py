@@ -525,3 +525,74 @@ def test_layer_norm_mean_of_rows_that_are_not_finite(pkg, cols, xt):
     y, mean, rstd = pkg.layer_norm(x.cuda(), torch.ones(cols, device="cuda"))
     assert mean[:4].tolist() == [inf, inf, -inf, -inf] and torch.isnan(mean[4:6]).all()
     assert torch.isnan(rstd[:6]).all() and torch.isnan(y[:6]).all() and torch.isfinite(y[6]).all() and torch.isfinite(mean[6])
+
+
+def test_row_operators_beyond_2_31_values(pkg):
+    """Rows whose values start more than 2^31 values into the tensor: the same as those rows alone."""
+    rows, cols, some = 1_100_000, 2048, 300
+    g = torch.Generator(device="cuda").manual_seed(81)
+    x, dy = [torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    for t in (x, dy):
+        t[-some:] = torch.randn(some, cols, device="cuda", generator=g).bfloat16()
+    w, b = [t.cuda() for t in _affine(cols, torch.bfloat16, 82)]
+    last = x[-some:].clone()
+    y, mean, rstd = pkg.layer_norm(x, w, b)
+    # 300 rows have another launch shape and order of sums than many: each side is within its bounds of the exact row.  Those of
+    # _check_norm with at most _depth additions, |x - m| below 6 deviations, deviations of about 1 and weights below 3: mean
+    # off by (d + 5) U (2 mean |x|), rstd by (d / 2 + 16) U, y by less than 60 * 6 * 3 U = 2^-13 and half a step of bfloat16.
+    y1, mean1, rstd1 = [t.double() for t in pkg.layer_norm(last, w, b)]
+    d = _depth(cols)
+    assert ((mean[-some:].double() - mean1).abs() <= 2 * (d + 5) * U * 2 * last.double().abs().mean(-1)).all()
+    assert ((rstd[-some:].double() / rstd1 - 1).abs() <= 2 * (d / 2 + 16) * U).all()
+    assert ((y[-some:].double() - y1).abs() <= 2 * (2.0 ** -8 * y1.abs() * 1.01 + 2.0 ** -13)).all()
+    dx, dw, db = pkg.layer_norm_bwd(dy, x, w, mean, rstd)
+    alone = pkg.layer_norm_bwd(dy[-some:].clone(), last, w, mean[-some:].clone(), rstd[-some:].clone())
+    assert torch.equal(dx[-some:], alone[0]) and not dx[:-some].any()
+    # the other rows have no gradient: the same sums but for the order of 300 additions, and a rounding or two of each term
+    tail = dy[-some:].double().abs()
+    h = ((last.double() - mean[-some:, None].double()) * rstd[-some:, None].double()).abs()
+    for got, want, terms in ((dw, alone[1], (tail * h).sum(0)), (db, alone[2], tail.sum(0))):
+        assert ((got.double() - want.double()).abs() <= 2 * 1.01 * (some + 4) * U * terms).all()
+    del y, dx
+    for call in (pkg.quantize_tokens, lambda t, **kw: pkg.layer_norm_quantize(t, w, b, **kw)):
+        for bits, sub in ((4, 0), (8, 64)):
+            kw = dict(dtype=_dtype(pkg, bits), scale=_spec(pkg, sub))
+            for got, want in zip(call(x, **kw), call(last, **kw)):
+                assert torch.equal(got[-some:], want)
+
+
+def test_row_operators_from_two_host_threads(pkg):
+    import threading
+
+    w, b = [t.cuda() for t in _affine(1000, torch.float32, 91)]
+    xs = [_rows(200 + 100 * i, 1000, torch.float32, 92 + i).cuda() for i in range(2)]
+
+    def step(x):
+        y, mean, rstd = pkg.layer_norm(x, w, b)
+        return (y, *pkg.layer_norm_bwd(x, x, w, mean, rstd), *pkg.quantize_tokens(x.bfloat16()), *pkg.layer_norm_quantize(x, w, b))
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                got = step(xs[i])
+                stream.synchronize()
+                if not all(torch.equal(a, c) for a, c in zip(got, want[i])):
+                    failed.append(i)
+                try:                                  # a refusal's message belongs to its thread
+                    pkg.layer_norm(xs[i], w[: 999 - i], b)
+                    failed.append(i)
+                except ValueError as refusal:
+                    if "(1000,)" not in str(refusal) or str(999 - i) not in str(refusal):
+                        failed.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
